@@ -206,6 +206,60 @@ int qr_kv_attention_chunk_step_dev(qr_kv* kv, int seq_id, int layer, int nq, con
                                    const void* q_dev, int q_dtype, float* attn_dev, float scale,
                                    void* stream);
 
+/* ---- chunks of several sequences --------------------------------------
+ * No reference counterpart (the reference runs one sequence, one token at a time): a serving
+ * step's calls for one layer.  A call takes n chunks; chunk i is rows[i] consecutive positions
+ * pos0[i] .. pos0[i] + rows[i] - 1 of sequence seq_ids[i], and the chunks' rows stand one after
+ * another in the row tensors.  rows[i] may be 0 (the chunk takes no part), n may be 0.  The
+ * arrays are host arrays, read before the call returns; everything else is device memory of the
+ * handle's device, aligned to its element size.  Nothing is copied to the device but new
+ * page-table entries, so the calls can be captured (a replay repeats the captured positions;
+ * pages and workspace as for the other *_dev calls).  Any cache type, head size and head count
+ * that qr_kv_create takes. */
+
+/* Append with a norm over each query and key head and the rotation in the same pass, the
+ * RmsNorm (TransformerOps.cs:12) of models with query / key norms before StreamingEngine.cs:245-248.
+ * Each head's row x of q and k: y = x * w / sqrt(mean(x^2) + eps) (w = q_norm / k_norm, head_dim
+ * floats shared by the heads; null: y = x), then the pairs (i, i + rotary_dim/2) of its first
+ * rotary_dim values turn by (rope_pos0[i] + j) * theta^(-2i/rotary_dim) for row j of the chunk.
+ * rope_pos0 null: pos0 (after an eviction a token's slot lies below its position).  The angle is
+ * taken in 64 bits (qr_kv_append_rope* keep the reference's fp32 product, which is off by up to
+ * 2^-8 of a radian at position 131072).  k and v go to the chunk's slots, q to q_out
+ * [rows][heads*head_dim].  q, k, v: rows of `dtype`, q_stride / k_stride / v_stride elements from
+ * one to the next (slices of one fused QKV product).  q and q_out may both be null; q_out may be
+ * q where q's rows stand back to back, and must not overlap q, k or v otherwise.  No sequence
+ * twice.  rotary_dim even, 0 to head_dim.  SeqLen grows as with qr_kv_append. */
+int qr_kv_append_norm_rope_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows,
+                               const int* rope_pos0, const void* q_dev, long long q_stride, const void* k_dev,
+                               long long k_stride, const void* v_dev, long long v_stride, int dtype, void* q_out_dev,
+                               const float* q_norm_dev, const float* k_norm_dev, float eps, float theta, int rotary_dim,
+                               void* stream);
+/* Causal attention of the chunks (appended before): the row at position p attends positions 0..p
+ * of its sequence.  q_dev and attn_dev [rows][heads*head_dim] of `dtype` (attn rounded once).
+ * weights_dev (may be null): fp32 [max_batch][kv_heads][max_seq] of this layer;
+ *   weights[seq][kv head][t] += sum over the chunk's rows and the kv head's query heads of
+ *                               softmax(...)[t],  t = 0 .. pos0 + rows - 1,
+ * the same for every run with the same inputs (no atomics); other elements are left alone.  With
+ * weights no sequence may stand twice. */
+int qr_kv_attention_chunks_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows,
+                               const void* q_dev, int dtype, void* attn_dev, float* weights_dev, float scale, void* stream);
+/* Eviction by accumulated weight, for n sequences of which len[i] positions of this layer are
+ * held.  Where len exceeds the budget first + heavy + recent, every kv head keeps its first `first`
+ * and last `recent` positions and the `heavy` positions between them of the largest weight (ties:
+ * the lower position; NaN counts below every number), in their order: slot j takes what slot
+ * kept[j] held.  kept_dev: int32 [n][kv_heads][first + heavy + recent], ascending, -1 past len.
+ * kept_weights_dev (layout of weights_dev, may be weights_dev itself, else without overlap) takes the kept
+ * positions' weights, then zeros up to len; the rest of it is left alone.  A sequence within the budget
+ * keeps everything.  SeqLen counts all layers and does not change: call qr_kv_truncate when all layers are
+ * done.  Slots behind the kept ones keep what they held.  No sequence twice. */
+int qr_kv_evict_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* len, int first, int heavy, int recent,
+                    const float* weights_dev, float* kept_weights_dev, int* kept_dev, void* stream);
+/* The chunks' cache rows as [rows][kv_dim] in the cache's type (qr_kv_read without the host). */
+int qr_kv_read_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows, void* k_out_dev,
+                   void* v_out_dev, void* stream);
+/* The HIP device that the cache lives on. */
+int qr_kv_device(const qr_kv* kv, int* out);
+
 /* Benchmark instrumentation, no reference counterpart: when `event` (a
  * hipEvent_t) is not NULL, every later attention call records it on its
  * stream right after the split-K kernel and before the combine kernel, so a

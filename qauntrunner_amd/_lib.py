@@ -64,6 +64,7 @@ _ERRORS = {c.status: c for c in (QrInvalidArgument, QrOutOfRange, QrOutOfMemory,
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
+_ll = ctypes.c_longlong
 _ip = ctypes.POINTER(ctypes.c_int)
 _llp = ctypes.POINTER(ctypes.c_longlong)
 _pp = ctypes.POINTER(ctypes.c_void_p)
@@ -94,6 +95,11 @@ SIGNATURES = {
     "qr_kv_attention_dev_noalloc": [_p, _i, _p, _i, _p, _p, _p, _f, _p],
     "qr_kv_attention_chunk": [_p, _i, _i, _i, _i, _p, _i, _p, _f],
     "qr_kv_attention_chunk_dev": [_p, _i, _i, _i, _i, _p, _i, _p, _f, _p],
+    "qr_kv_append_norm_rope_dev": [_p, _i, _p, _i, _p, _p, _p, _p, _ll, _p, _ll, _p, _ll, _i, _p, _p, _p, _f, _f, _i, _p],
+    "qr_kv_attention_chunks_dev": [_p, _i, _p, _i, _p, _p, _p, _i, _p, _p, _f, _p],
+    "qr_kv_evict_dev": [_p, _i, _p, _i, _p, _i, _i, _i, _p, _p, _p, _p],
+    "qr_kv_read_dev": [_p, _i, _p, _i, _p, _p, _p, _p, _p],
+    "qr_kv_device": [_p, _ip],
     "qr_kv_set_split_event": [_p, _p],
     "qr_kv_decode_plan": [_p, _i, _p, _i, _p, _ip, _ip],
     "qr_kv_reset": [_p, _i],

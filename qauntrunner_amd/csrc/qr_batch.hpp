@@ -1,0 +1,144 @@
+// qr_batch.hpp -- launch interfaces of the calls over chunks of several sequences: append with
+// query / key norms and rotation, causal attention with the weight that each cached position
+// received, eviction by that weight, and reading rows back.
+//
+// A call's chunks are described by value (no copy to the device, so a call can be captured), up to
+// kBatch of them per launch; the host drops chunks without rows.  Work is counted in units, the
+// chunks' one after another: unit0 is a chunk's first.
+#pragma once
+
+#include "qr_kernels.hpp"
+
+namespace qr {
+
+constexpr int kBatch = 64;  // one lane each: a unit's chunk is found by one ballot
+
+// Chunk of a unit: the last one whose first unit is not past it.  `first(i)` of i < n ascends.
+template <class F> __device__ __forceinline__ int batch_find(int n, int unit, F first) {
+    const int lane = threadIdx.x & 63;
+    const bool at = lane < n && first(lane < n ? lane : 0) <= unit;
+    return __builtin_amdgcn_readfirstlane(static_cast<int>(__popcll(__builtin_amdgcn_ballot_w64(at))) - 1);
+}
+
+// One element of a dtype at p[i], widened; NaN stays NaN when one is stored.
+__device__ __forceinline__ float load_elem(const void* p, int dtype, long long i) {
+    if (dtype == QR_DTYPE_F32) return static_cast<const float*>(p)[i];
+    const uint16_t u = static_cast<const uint16_t*>(p)[i];
+    return dtype == QR_DTYPE_F16 ? f16_bits_to_f32(u) : bf16_bits_to_f32(u);
+}
+__device__ __forceinline__ uint16_t f32_to_bits16(float x, int dtype) {
+    if (dtype == QR_DTYPE_F16) return f32_to_f16_bits_ref(x);
+    return x == x ? f32_to_bf16_bits_ref(x) : static_cast<uint16_t>((__float_as_uint(x) >> 16) | 0x40u);
+}
+__device__ __forceinline__ void store_elem(void* p, int dtype, long long i, float x) {
+    if (dtype == QR_DTYPE_F32) static_cast<float*>(p)[i] = x;
+    else static_cast<uint16_t*>(p)[i] = f32_to_bits16(x, dtype);
+}
+
+// ------------------------------------------------------------------ append
+struct NormRopeItem {
+    int pt_off;  // page-table row of (sequence, layer)
+    int pos0;    // slot of the first row
+    int rows;
+    int row0;    // first row in q / k / v
+    int rope0;   // position that the first row is rotated by
+    int unit0;
+};
+struct NormRopeArgs {
+    NormRopeItem it[kBatch];
+    int n;
+    int rows;                // rows of all chunks
+    void* pool;
+    const int* page_table;
+    PageGeom geom;
+    int dtype;               // cache
+    int act;                 // q / k / v
+    int heads;
+    const void *q, *k, *v;   // q may be null
+    long long q_stride, k_stride, v_stride;  // elements between rows
+    void* q_out;             // [rows][heads * head_dim]
+    const float *q_norm, *k_norm;            // [head_dim]; null: no norm
+    float eps;
+    int rot;                 // rotated dims, even
+    double turn[kMaxRopeHalf];               // revolutions per position of pair i
+};
+hipError_t launch_norm_rope(const NormRopeArgs& a, hipStream_t stream);
+
+// ------------------------------------------------------------------ rows back
+struct ReadItem {
+    int pt_off, pos0, rows, row0;
+};
+struct ReadArgs {
+    ReadItem it[kBatch];
+    int n;
+    int rows;
+    const void* pool;
+    const int* page_table;
+    PageGeom geom;
+    int dtype;
+    void *k, *v;             // [rows][kv_heads * head_dim] in the cache's type
+};
+hipError_t launch_read(const ReadArgs& a, hipStream_t stream);
+
+// ------------------------------------------------------------------ attention
+struct ChunkItem {
+    int pt_off;
+    int seq;                 // row of the weights
+    int pos0;
+    int rows;
+    int row0;                // first row in q / out
+    int unit0;
+    int blocks;              // row blocks per kv head
+    int splits;              // parts of each block's keys
+    int slot0;               // first split partial: (row * heads + head) * splits + split from here
+    int wunit0;              // first unit of the weights pass
+};
+struct ChunksArgs {
+    ChunkItem it[kBatch];
+    int n;
+    int rows;                // rows of all chunks
+    const void* pool;
+    const int* page_table;
+    PageGeom geom;
+    int dtype;               // cache
+    int act;                 // q and out
+    int heads;
+    const void* q;           // [rows][heads][head_dim]
+    void* out;
+    float* weights;          // [sequences][kv_heads][max_seq], may be null
+    int max_seq;
+    float scale;
+};
+struct ChunksPlan {
+    int units, wunits;
+    long long slots;         // split partials
+    size_t acc_off, part_ml_off, row_ml_off;  // in the workspace
+    size_t workspace_bytes;
+};
+// Fills unit0, blocks, splits, slot0, wunit0 of the chunks.
+ChunksPlan plan_chunks(ChunksArgs& a);
+hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* workspace, hipStream_t stream);
+
+// ------------------------------------------------------------------ eviction
+struct EvictItem {
+    int pt_off;
+    int seq;
+    int len;                 // positions held
+    int entry;               // row of kept
+};
+struct EvictArgs {
+    EvictItem it[kBatch];
+    int n;
+    void* pool;
+    const int* page_table;
+    PageGeom geom;
+    int dtype;
+    int first, heavy, recent;
+    const float* weights;    // [sequences][kv_heads][max_seq]
+    float* kept_weights;     // the same layout; may be weights
+    int max_seq;
+    int* kept;               // [entries][kv_heads][first + heavy + recent]
+};
+hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
+
+}  // namespace qr

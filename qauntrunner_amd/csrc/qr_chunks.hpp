@@ -1,0 +1,48 @@
+// qr_chunks.hpp -- what the kernels of attention over chunks of several sequences share.
+#pragma once
+
+#include <algorithm>
+
+#include "qr_batch.hpp"
+
+namespace qr {
+
+struct ChunksK {
+    ChunkItem it[kBatch];
+    int n;
+    const char* pool;
+    const int* page_table;
+    PageGeom geom;
+    int dtype;               // cache
+    int act;                 // q and out
+    int heads;
+    const void* q;           // [rows][heads][head_dim]
+    void* out;
+    float* weights;          // [sequences][kv_heads][max_seq]
+    int max_seq;
+    float qscale;            // scale log2(e): scores are in log2 units
+    float* part_acc;         // [slots][head_dim]
+    float2* part_ml;         // [slots] (maximum, sum)
+    float2* row_ml;          // [rows * heads] (maximum, sum), null where no weights are wanted
+};
+
+// Query heads h0 .. h0 + g - 1 read kv head kvh (head h reads h * kv_heads / heads).
+__device__ __forceinline__ void chunk_heads(const ChunksK& p, int kvh, int* h0, int* g) {
+    const int kv = p.geom.kv_heads;
+    *h0 = (kvh * p.heads + kv - 1) / kv;
+    *g = ((kvh + 1) * p.heads + kv - 1) / kv - *h0;
+}
+
+// Part `split` of the positions [0, keys) in whole tiles.
+__device__ __forceinline__ void chunk_keys(const ChunkItem& it, int keys, int split, int tile, int* t0, int* t1) {
+    const int tiles = (keys + tile - 1) / tile;
+    *t0 = static_cast<int>(static_cast<long long>(tiles) * split / it.splits) * tile;
+    *t1 = std::min(static_cast<int>(static_cast<long long>(tiles) * (split + 1) / it.splits) * tile, keys);
+}
+
+int chunks_any_rows();
+int chunks_any_tile();
+hipError_t launch_chunks_any(const ChunksK& k, const ChunksPlan& plan, hipStream_t s);
+hipError_t launch_chunks_any_weights(const ChunksK& k, const ChunksPlan& plan, hipStream_t s);
+
+}  // namespace qr

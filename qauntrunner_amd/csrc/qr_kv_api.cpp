@@ -6,7 +6,7 @@
 #include <vector>
 
 #include "qr_chunk.hpp"
-#include "qr_store.hpp"
+#include "qr_kv.hpp"
 
 namespace qr {
 const char* last_error();
@@ -14,92 +14,7 @@ const char* last_error();
 
 using namespace qr;
 
-struct qr_kv {
-    int device = 0;
-    int layers = 0, heads = 0, kv_heads = 0, head_dim = 0, max_seq = 0, dtype = 0, max_batch = 0;
-    int kv_dim = 0;
-    PagedStore store;
-    std::vector<int> seq_len;
-    hipStream_t stream = nullptr;
-    DevBuf stage;      // host <-> device staging of rows, queries and outputs
-    DevBuf workspace;  // split-K partials
-    DevBuf steppos;    // device positions of the queries of a device-position chunk (kMaxDecodeBatch ints)
-    DevBuf counters;   // arrival counters of the in-kernel split merge (kDecodeCounters, zero between calls)
-    hipEvent_t split_event = nullptr;  // benchmark instrumentation (qr_kv_set_split_event)
-    void* scratch = nullptr;           // this device's decode scratch array (no-allocation calls)
-    bool device_steps = false;         // the device copy of the page accounting is in use
-};
-
 namespace {
-
-int check_handle(const qr_kv* kv) {
-    if (!kv) {
-        set_error("null qr_kv handle");
-        return QR_ERR_INVALID_ARGUMENT;
-    }
-    return QR_OK;
-}
-
-int check_seq_layer(const qr_kv* kv, int seq_id, int layer) {
-    QR_CHECK_ARG(seq_id >= 0 && seq_id < kv->max_batch, "seq_id %d outside [0, %d)", seq_id, kv->max_batch);
-    QR_CHECK_ARG(layer >= 0 && layer < kv->layers, "layer %d outside [0, %d)", layer, kv->layers);
-    return QR_OK;
-}
-
-int check_pos(const qr_kv* kv, int pos) {
-    if (pos < 0 || pos >= kv->max_seq) {
-        set_error("position %d outside [0, max_seq=%d)", pos, kv->max_seq);
-        return QR_ERR_OUT_OF_RANGE;
-    }
-    return QR_OK;
-}
-
-int check_resident(const qr_kv* kv, int seq_id, int layer, int pos) {
-    if (!kv->store.resident(seq_id, layer, pos)) {
-        set_error("position %d of sequence %d layer %d was never appended (%d pages resident)", pos,
-                  seq_id, layer, kv->store.pages_held(seq_id, layer));
-        return QR_ERR_NOT_RESIDENT;
-    }
-    return QR_OK;
-}
-
-hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
-
-bool capturing(hipStream_t stream) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    return hipStreamIsCapturing(stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
-}
-
-// Host view of the page accounting and SeqLen, read back from the device after
-// device-side appends (a no-op otherwise).  A device-pointer call enqueued under stream
-// capture skips the read-back (it would wait for the device): its checks then use the
-// host accounting, which never runs ahead of the device's (pages and SeqLen only grow
-// on the device), so they can reject a position the device already holds but never
-// accept one it does not.
-int sync_host(const qr_kv* ckv, hipStream_t stream = nullptr, bool device_call = false) {
-    qr_kv* kv = const_cast<qr_kv*>(ckv);
-    if (!kv->store.device_ahead()) return QR_OK;
-    if (device_call && capturing(stream)) return QR_OK;
-    DeviceGuard dg(kv->device);
-    return kv->store.pull(kv->seq_len);
-}
-
-// A call enqueued under stream capture leaves the addresses of the pool, the split
-// workspace and the position buffer in the graph: from then on the pool never moves
-// (growing it is an error) and a workspace that grows keeps its old allocation alive
-// for the graph's replays until the handle is destroyed.
-void note_capture(qr_kv* kv, hipStream_t stream) {
-    if (!capturing(stream)) return;
-    kv->store.freeze();
-    kv->workspace.keep_retired();
-    kv->steppos.keep_retired();
-}
-
-// Device copy of the accounting after host-side changes (once device-side appends are in use).
-int sync_device(qr_kv* kv, hipStream_t stream) {
-    if (!kv->device_steps) return QR_OK;
-    return kv->store.push(kv->seq_len, stream);
-}
 
 // Appends rows already on the device (src_dtype, row stride kv_dim).
 int append_dev(qr_kv* kv, int seq_id, int layer, int pos0, int n, const void* k, const void* v,
@@ -151,16 +66,6 @@ int rope_append_dev(qr_kv* kv, int seq_id, int layer, int pos0, int n, float* q,
     int& sl = kv->seq_len[seq_id];
     sl = std::max(sl, pos0 + n);  // PagedKvCache.cs:68
     return sync_device(kv, stream);
-}
-
-// The split workspace may only grow outside stream capture.
-int grow_workspace(qr_kv* kv, size_t bytes, hipStream_t st) {
-    const size_t ws = std::max<size_t>(bytes, 256);
-    if (ws > kv->workspace.size()) {
-        QR_CHECK_ARG(!capturing(st), "the split workspace must grow to %zu bytes: make one call outside capture first", ws);
-        QR_TRY(kv->workspace.ensure(ws));
-    }
-    return QR_OK;
 }
 
 // Runs decode entries (seq_ids[i], seq_len[i]) with device q/out rows.

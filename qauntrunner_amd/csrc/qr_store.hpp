@@ -76,6 +76,7 @@ public:
     long long bytes_used() const { return pages_used_ * page_bytes(); }
     int max_pages() const { return max_pages_; }
     long long capacity() const { return pool_cap_; }
+    long long pages_used() const { return pages_used_; }
 
     // Device copy of the page accounting, for appends whose position is read on the
     // device (page_claim_kernel): [0] pages handed out, [1] error bits, then the held
