@@ -87,11 +87,13 @@ struct ChunkItem {
     int pos0;
     int rows;
     int row0;                // first row in q / out
+    // of a launch:
     int unit0;
-    int blocks;              // row blocks per kv head
-    int splits;              // parts of each block's keys
+    int blocks;              // row blocks (weights: position blocks) per kv head
+    int splits;              // parts of each block's keys (weights: rows)
     int slot0;               // first split partial: (row * heads + head) * splits + split from here
-    int wunit0;              // first unit of the weights pass
+    int pad;
+    long long score0;        // first score: (row * heads + head) * chunk_score_len from here
 };
 struct ChunksArgs {
     ChunkItem it[kBatch];
@@ -109,14 +111,21 @@ struct ChunksArgs {
     int max_seq;
     float scale;
 };
+// Which kernel takes a chunk, and how its work is cut.
+struct ChunkPlanItem {
+    int kind, blocks, splits;
+    long long slot0;
+    int wkind, wblocks, wsplits;
+    long long wslot0, score0;
+};
 struct ChunksPlan {
-    int units, wunits;
-    long long slots;         // split partials
-    size_t acc_off, part_ml_off, row_ml_off;  // in the workspace
+    ChunkPlanItem it[kBatch];
+    bool merge;              // some chunk's keys are split
+    bool wmerge;             // some chunk's weights are summed in parts
+    size_t part_ml, row_ml, row_scale, scores, wpart;  // offsets in the workspace; the partials' sums come first
     size_t workspace_bytes;
 };
-// Fills unit0, blocks, splits, slot0, wunit0 of the chunks.
-ChunksPlan plan_chunks(ChunksArgs& a);
+ChunksPlan plan_chunks(const ChunksArgs& a);
 hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* workspace, hipStream_t stream);
 
 // ------------------------------------------------------------------ eviction

@@ -1,4 +1,5 @@
-// qr_chunks.hip -- plan, launch and split merge of the attention of chunks of several sequences.
+// qr_chunks.hip -- plan, launches, split merge and the last step of the weights of the attention of
+// chunks of several sequences.
 #include "qr_chunks.hpp"
 
 namespace qr {
@@ -33,44 +34,132 @@ __global__ void __launch_bounds__(64) chunks_combine_kernel(const ChunksK p) {
     if (p.row_ml && lane == 0) p.row_ml[rh] = make_float2(m, l);
 }
 
+// Weights from the stored scores of a chunk's rows: one thread per position.
+__global__ void __launch_bounds__(256) chunks_scores_kernel(const ChunksK p) {
+    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
+    const ChunkItem it = p.it[e];
+    const int u = blockIdx.x - it.unit0;
+    const int t = u % it.blocks * 256 + threadIdx.x, kvh = u / it.blocks;
+    if (t >= it.pos0 + it.rows) return;
+    const int g = p.heads / p.geom.kv_heads, stride = chunk_score_len(it);
+    float sum = 0.f;
+    for (int j = max(0, t - it.pos0); j < it.rows; ++j)
+        for (int h = kvh * g; h < kvh * g + g; ++h) {
+            const float2 ml = p.row_ml[static_cast<long long>(it.row0 + j) * p.heads + h];
+            sum += fast_exp2(p.scores[it.score0 + (static_cast<long long>(j) * p.heads + h) * stride + t] - ml.x) / ml.y;
+        }
+    p.weights[(static_cast<long long>(it.seq) * p.geom.kv_heads + kvh) * p.max_seq + t] += sum;
+}
+
+// Parts of the weights' sums: one thread per position.
+__global__ void __launch_bounds__(256) chunks_wmerge_kernel(const ChunksK p) {
+    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
+    const ChunkItem it = p.it[e];
+    const int u = blockIdx.x - it.unit0, len = it.pos0 + it.rows;
+    const int t = u % it.blocks * 256 + threadIdx.x, kvh = u / it.blocks;
+    if (t >= len) return;
+    float sum = 0.f;
+    for (int s = 0; s < it.splits; ++s) sum += p.wpart[it.slot0 + (static_cast<long long>(s) * p.geom.kv_heads + kvh) * len + t];
+    p.weights[(static_cast<long long>(it.seq) * p.geom.kv_heads + kvh) * p.max_seq + t] += sum;
+}
+
+struct KindGeom {
+    int rows, tile;   // of a workgroup
+    long long want;   // units that fill the GPU
+};
+constexpr KindGeom kGeom[kChunkKinds] = {{kChunkAnyRows, kChunkAnyTile, 1024}, {32, 128, 256}, {64, 128, 256}, {128, 64, 256}, {256, 64, 256}};
+
+int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
+
 }  // namespace
 
-ChunksPlan plan_chunks(ChunksArgs& a) {
+ChunksPlan plan_chunks(const ChunksArgs& a) {
     ChunksPlan pl{};
-    const int kv = a.geom.kv_heads, gmax = (a.heads + kv - 1) / kv;
-    const int R = chunks_any_rows(), T = chunks_any_tile();
-    // units without splits, and the (block, position) pairs that they read
-    long long base = 0, work = 0;
+    const int kv = a.geom.kv_heads, gmax = cdiv(a.heads, kv);
+    const bool tiles = a.geom.mfma_layout && a.heads % kv == 0;
     for (int i = 0; i < a.n; ++i) {
-        const long long b = (static_cast<long long>(a.it[i].rows) * gmax + R - 1) / R;
-        base += b * kv;
-        work += b * kv * (a.it[i].pos0 + a.it[i].rows);
+        const long long rows = static_cast<long long>(a.it[i].rows) * gmax;
+        pl.it[i].kind = !tiles ? kChunkAny : rows <= 32 ? kChunkStream32 : rows <= 64 ? kChunkStream64 : rows <= 128 ? kChunkStream128 : kChunkTile;
+        pl.it[i].blocks = cdiv(rows, kGeom[pl.it[i].kind].rows);
     }
-    const long long want = 1024;
-    const long long per = base >= want ? (1LL << 40) : std::max<long long>(2 * T, work / want);
-    for (int i = 0; i < a.n; ++i) {
-        ChunkItem& it = a.it[i];
-        const int len = it.pos0 + it.rows;
-        it.blocks = static_cast<int>((static_cast<long long>(it.rows) * gmax + R - 1) / R);
-        it.splits = static_cast<int>(std::min<long long>((len + per - 1) / per, 256));
-        it.unit0 = pl.units;
-        pl.units += it.blocks * it.splits * kv;
-        it.slot0 = static_cast<int>(pl.slots);
-        if (it.splits > 1) pl.slots += static_cast<long long>(it.rows) * a.heads * it.splits;
-        it.wunit0 = pl.wunits;
-        pl.wunits += (len + T - 1) / T * kv;
+    // The keys of a kind's blocks are split while its units do not fill the GPU: as many positions
+    // per unit as leave no more units than that, or one tile.
+    long long slots = 0;
+    for (int kind = 0; kind < kChunkKinds; ++kind) {
+        const KindGeom& g = kGeom[kind];
+        long long base = 0, work = 0;
+        for (int i = 0; i < a.n; ++i)
+            if (pl.it[i].kind == kind) {
+                base += static_cast<long long>(pl.it[i].blocks) * kv;
+                work += static_cast<long long>(pl.it[i].blocks) * kv * cdiv(a.it[i].pos0 + a.it[i].rows, g.tile);
+            }
+        if (!base) continue;
+        long long per = base >= g.want ? 1LL << 40 : std::max<long long>(1, work / g.want);  // tiles of a unit
+        auto units = [&](long long per_) {
+            long long u = 0;
+            for (int i = 0; i < a.n; ++i)
+                if (pl.it[i].kind == kind)
+                    u += static_cast<long long>(pl.it[i].blocks) * kv * cdiv(cdiv(a.it[i].pos0 + a.it[i].rows, g.tile), per_);
+            return u;
+        };
+        if (base < g.want)
+            while (units(per) > g.want && per < (1 << 24)) per += std::max<long long>(1, per / 16);
+        for (int i = 0; i < a.n; ++i) {
+            ChunkPlanItem& it = pl.it[i];
+            if (it.kind != kind) continue;
+            it.splits = std::min(cdiv(cdiv(a.it[i].pos0 + a.it[i].rows, g.tile), per), 256);
+            it.slot0 = slots;
+            if (it.splits > 1) {
+                slots += static_cast<long long>(a.it[i].rows) * a.heads * it.splits;
+                pl.merge = true;
+            }
+        }
     }
-    pl.part_ml_off = static_cast<size_t>(pl.slots) * a.geom.head_dim * sizeof(float);
-    pl.part_ml_off = (pl.part_ml_off + 255) & ~size_t(255);
-    pl.row_ml_off = pl.part_ml_off + ((static_cast<size_t>(pl.slots) * sizeof(float2) + 255) & ~size_t(255));
-    pl.workspace_bytes = pl.row_ml_off + (a.weights ? static_cast<size_t>(a.rows) * a.heads * sizeof(float2) : 0);
+    long long wslots = 0, scores = 0;
+    if (a.weights) {
+        long long units = 0;
+        for (int i = 0; i < a.n; ++i) {
+            ChunkPlanItem& it = pl.it[i];
+            it.wkind = it.kind == kChunkAny ? kWeightsAny : it.kind == kChunkStream32 ? kWeightsScores : kWeightsTile;
+            it.wblocks = cdiv(a.it[i].pos0 + a.it[i].rows, it.kind == kChunkAny ? kChunkAnyTile : 256);
+            it.wsplits = 1;
+            if (it.wkind == kWeightsTile) units += static_cast<long long>(it.wblocks) * kv;
+            if (it.wkind == kWeightsScores) {
+                it.score0 = scores;
+                scores += static_cast<long long>(a.it[i].rows) * a.heads * chunk_score_len(a.it[i]);
+            }
+        }
+        // few position blocks: their rows are split too, 64 rows or more a part
+        for (int i = 0; i < a.n; ++i) {
+            ChunkPlanItem& it = pl.it[i];
+            if (it.wkind != kWeightsTile || units >= 1024) continue;
+            it.wsplits = std::max(1, std::min(cdiv(1024, units), cdiv(static_cast<long long>(a.it[i].rows) * gmax, 64)));
+            it.wslot0 = wslots;
+            if (it.wsplits > 1) {
+                wslots += static_cast<long long>(it.wsplits) * kv * (a.it[i].pos0 + a.it[i].rows);
+                pl.wmerge = true;
+            }
+        }
+    }
+    auto next = [](size_t& at, size_t bytes) {
+        const size_t r = at;
+        at += (bytes + 255) & ~size_t(255);
+        return r;
+    };
+    size_t at = 0;
+    const size_t rh = static_cast<size_t>(a.rows) * a.heads;
+    next(at, static_cast<size_t>(slots) * a.geom.head_dim * sizeof(float));
+    pl.part_ml = next(at, static_cast<size_t>(slots) * sizeof(float2));
+    pl.row_ml = next(at, a.weights ? rh * sizeof(float2) : 0);
+    pl.row_scale = next(at, a.weights ? rh * sizeof(float) : 0);
+    pl.scores = next(at, static_cast<size_t>(scores) * sizeof(float));
+    pl.wpart = next(at, static_cast<size_t>(wslots) * sizeof(float));
+    pl.workspace_bytes = at;
     return pl;
 }
 
 hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* workspace, hipStream_t stream) {
     ChunksK k{};
-    std::copy(a.it, a.it + a.n, k.it);
-    k.n = a.n;
     k.pool = static_cast<const char*>(a.pool);
     k.page_table = a.page_table;
     k.geom = a.geom;
@@ -84,14 +173,62 @@ hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* work
     k.qscale = static_cast<float>(static_cast<double>(a.scale) * 1.4426950408889634);
     char* w = static_cast<char*>(workspace);
     k.part_acc = reinterpret_cast<float*>(w);
-    k.part_ml = reinterpret_cast<float2*>(w + plan.part_ml_off);
-    k.row_ml = a.weights ? reinterpret_cast<float2*>(w + plan.row_ml_off) : nullptr;
-    hipError_t e = launch_chunks_any(k, plan, stream);
-    if (e == hipSuccess && plan.slots) {
+    k.part_ml = reinterpret_cast<float2*>(w + plan.part_ml);
+    if (a.weights) {
+        k.row_ml = reinterpret_cast<float2*>(w + plan.row_ml);
+        if (a.dtype == QR_DTYPE_F16 && a.act != QR_DTYPE_F16) k.row_scale = reinterpret_cast<float*>(w + plan.row_scale);
+        k.wpart = reinterpret_cast<float*>(w + plan.wpart);
+    }
+    const int kv = a.geom.kv_heads;
+    // the chunks that `in` takes, with a launch's blocks and splits
+    auto gather = [&](auto in, bool weights) {
+        k.n = k.units = 0;
+        for (int i = 0; i < a.n; ++i) {
+            const ChunkPlanItem& pi = plan.it[i];
+            if (!in(pi)) continue;
+            ChunkItem& it = k.it[k.n++];
+            it = a.it[i];
+            it.unit0 = k.units;
+            it.blocks = weights ? pi.wblocks : pi.blocks;
+            it.splits = weights ? pi.wsplits : pi.splits;
+            it.slot0 = static_cast<int>(weights ? pi.wslot0 : pi.slot0);
+            it.score0 = pi.score0;
+            k.units += it.blocks * it.splits * kv;
+        }
+        return k.n > 0;
+    };
+    hipError_t e = hipSuccess;
+    for (int kind = 0; kind < kChunkKinds && e == hipSuccess; ++kind) {
+        if (!gather([&](const ChunkPlanItem& p) { return p.kind == kind; }, false)) continue;
+        k.scores = a.weights && kind == kChunkStream32 ? reinterpret_cast<float*>(w + plan.scores) : nullptr;
+        e = kind == kChunkAny ? launch_chunks_any(k, stream) : launch_chunks_tile(k, kind, stream);
+    }
+    if (e == hipSuccess && plan.merge) {
+        gather([](const ChunkPlanItem&) { return true; }, false);
         hipLaunchKernelGGL(chunks_combine_kernel, dim3(a.rows * a.heads), dim3(64), 0, stream, k);
         e = hipGetLastError();
     }
-    if (e == hipSuccess && a.weights) e = launch_chunks_any_weights(k, plan, stream);
+    if (!a.weights) return e;
+    k.scores = reinterpret_cast<float*>(w + plan.scores);
+    for (int kind = 0; kind < kWeightsKinds && e == hipSuccess; ++kind) {
+        if (!gather([&](const ChunkPlanItem& p) { return p.wkind == kind; }, true)) continue;
+        if (kind == kWeightsScores) {
+            hipLaunchKernelGGL(chunks_scores_kernel, dim3(k.units), dim3(256), 0, stream, k);
+            e = hipGetLastError();
+        } else {
+            e = kind == kWeightsAny ? launch_chunks_any_weights(k, stream) : launch_chunks_tile(k, kChunkKinds, stream);
+        }
+    }
+    if (e == hipSuccess && plan.wmerge) {
+        gather([](const ChunkPlanItem& p) { return p.wkind == kWeightsTile && p.wsplits > 1; }, true);
+        k.units = 0;  // one unit per 256 positions and kv head
+        for (int i = 0; i < k.n; ++i) {
+            k.it[i].unit0 = k.units;
+            k.units += k.it[i].blocks * kv;
+        }
+        hipLaunchKernelGGL(chunks_wmerge_kernel, dim3(k.units), dim3(256), 0, stream, k);
+        e = hipGetLastError();
+    }
     return e;
 }
 

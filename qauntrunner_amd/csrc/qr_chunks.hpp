@@ -7,9 +7,17 @@
 
 namespace qr {
 
+// Kernels of a launch; rows (query, query head pairs of a kv head) of a workgroup, positions of a tile.
+enum ChunkKind { kChunkAny, kChunkStream32, kChunkStream64, kChunkStream128, kChunkTile, kChunkKinds };
+// The passes after the attention that add up the weights.
+enum ChunkWeights { kWeightsAny, kWeightsScores, kWeightsTile, kWeightsKinds };
+
+constexpr int kChunkAnyRows = 8, kChunkAnyTile = 32;
+
 struct ChunksK {
     ChunkItem it[kBatch];
     int n;
+    int units;
     const char* pool;
     const int* page_table;
     PageGeom geom;
@@ -24,6 +32,9 @@ struct ChunksK {
     float* part_acc;         // [slots][head_dim]
     float2* part_ml;         // [slots] (maximum, sum)
     float2* row_ml;          // [rows * heads] (maximum, sum), null where no weights are wanted
+    float* row_scale;        // [rows * heads] log2 units per score where q was scaled by a power of two, else null
+    float* scores;           // scaled scores of the chunks whose weights pass reads them, else null
+    float* wpart;            // partial sums of weights: [split][kv head][length] of a chunk from slot0 on
 };
 
 // Query heads h0 .. h0 + g - 1 read kv head kvh (head h reads h * kv_heads / heads).
@@ -40,9 +51,13 @@ __device__ __forceinline__ void chunk_keys(const ChunkItem& it, int keys, int sp
     *t1 = std::min(static_cast<int>(static_cast<long long>(tiles) * (split + 1) / it.splits) * tile, keys);
 }
 
-int chunks_any_rows();
-int chunks_any_tile();
-hipError_t launch_chunks_any(const ChunksK& k, const ChunksPlan& plan, hipStream_t s);
-hipError_t launch_chunks_any_weights(const ChunksK& k, const ChunksPlan& plan, hipStream_t s);
+// Entries of a row of scores: positions of the chunk's last row, whole runs of 8.
+__host__ __device__ inline int chunk_score_len(const ChunkItem& it) { return (it.pos0 + it.rows + 7) & ~7; }
+
+hipError_t launch_chunks_any(const ChunksK& k, hipStream_t s);
+hipError_t launch_chunks_any_weights(const ChunksK& k, hipStream_t s);
+// 16-bit caches in the MFMA page layout, whole groups: kinds kChunkStream32 .. kChunkTile; kChunkKinds:
+// the weights pass.
+hipError_t launch_chunks_tile(const ChunksK& k, int kind, hipStream_t s);
 
 }  // namespace qr

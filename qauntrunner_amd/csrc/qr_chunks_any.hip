@@ -15,8 +15,8 @@ namespace qr {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 8;    // rows of a workgroup
-constexpr int kTile = 32;   // positions of a tile
+constexpr int kRows = kChunkAnyRows;
+constexpr int kTile = kChunkAnyTile;
 
 // Positions t0 .. t0 + 31 (below `end`, one page) of one plane and kv head into LDS as fp32, rows
 // of D + 1 values: a column's 32 reads hit 32 banks.
@@ -149,11 +149,11 @@ __global__ void __launch_bounds__(kThreads) chunks_any_weights_kernel(const Chun
     const int D = p.geom.head_dim;
     float* const q = lds;               // [8][D]
     float* const tile = q + kRows * D;  // [32][D + 1]
-    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].wunit0; });
+    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
     const ChunkItem it = p.it[e];
-    const int len = it.pos0 + it.rows, tiles = (len + kTile - 1) / kTile;
-    const int u = blockIdx.x - it.wunit0;
-    const int t0 = u % tiles * kTile, kvh = u / tiles;
+    const int len = it.pos0 + it.rows;
+    const int u = blockIdx.x - it.unit0;
+    const int t0 = u % it.blocks * kTile, kvh = u / it.blocks;
     int h0, g;
     chunk_heads(p, kvh, &h0, &g);
     load_tile(p, it.pt_off, 0, kvh, t0, len, tile);
@@ -186,15 +186,12 @@ size_t any_lds(int D) { return (kRows * std::max(D, 32) + kTile * (D + 1) + kRow
 
 }  // namespace
 
-int chunks_any_rows() { return kRows; }
-int chunks_any_tile() { return kTile; }
-
-hipError_t launch_chunks_any(const ChunksK& k, const ChunksPlan& plan, hipStream_t s) {
-    hipLaunchKernelGGL(chunks_any_kernel, dim3(plan.units), dim3(kThreads), any_lds(k.geom.head_dim), s, k);
+hipError_t launch_chunks_any(const ChunksK& k, hipStream_t s) {
+    hipLaunchKernelGGL(chunks_any_kernel, dim3(k.units), dim3(kThreads), any_lds(k.geom.head_dim), s, k);
     return hipGetLastError();
 }
-hipError_t launch_chunks_any_weights(const ChunksK& k, const ChunksPlan& plan, hipStream_t s) {
-    hipLaunchKernelGGL(chunks_any_weights_kernel, dim3(plan.wunits), dim3(kThreads), any_lds(k.geom.head_dim), s, k);
+hipError_t launch_chunks_any_weights(const ChunksK& k, hipStream_t s) {
+    hipLaunchKernelGGL(chunks_any_weights_kernel, dim3(k.units), dim3(kThreads), any_lds(k.geom.head_dim), s, k);
     return hipGetLastError();
 }
 

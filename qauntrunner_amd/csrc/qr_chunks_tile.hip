@@ -1,0 +1,745 @@
+// qr_chunks_tile.hip -- causal attention of chunks of several sequences on 32x32x16 MFMA tiles:
+// 16-bit caches of head size 64 or 128 (the MFMA page layout, qr_kernels.hpp), whole groups of
+// query heads, gfx950.
+//
+// A row is one (query, query head) pair of a kv head; a wave owns 32 rows:
+//   QK  S^T[position][row] = K . q^T    (A = K, B = q)
+//   PV  O^T[dim][row]     += V^T . P^T  (A = V, B = P)
+// v_mfma_f32_32x32x16: A[m = lane % 32][k = 8 (lane / 32) + i], B[k = 8 (lane / 32) + i][n = lane % 32],
+// D[m = 8 (r / 4) + 4 (lane / 32) + r % 4][n = lane % 32].  A row's scores lie in two lanes, l and
+// l ^ 32.  QK row m = 16 s + 8 a + 4 h + b stands for position 16 s + 8 h + 4 a + b of its step of 32, so that
+// a lane's scores r = 8 s + i are positions 16 s + 8 (lane / 32) + i: its k-slots of PV step s, and
+// V's operand is 8 consecutive positions of a dim, 16 bytes of the page.
+//
+// Softmax in log2 units with the running maximum held `kHead` above the largest score seen when it
+// last moved: the weights stay at or below 1 (a V near the type's largest value does not overflow)
+// and the accumulators are rescaled only when a score passes it.  Sums are of the fp32 weights.
+// kSplit: queries that are not of the cache's type enter as two parts of it (hi + lo), and so do
+// the weights, which keeps 16 (bf16) or 22 (fp16) bits of both; otherwise the weights are rounded
+// to the type once, as the output is.
+//
+// Tiles are copied into LDS by buffer-load DMA as they lie in the page.
+#include "qr_chunks.hpp"
+#include "qr_mfma.hpp"
+
+namespace qr {
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16_t mfma32(f16x8_t a, f16x8_t b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16_t mfma32(bf16x8_t a, bf16x8_t b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+// (the scores come from MFMAs: fmaxf's quieting of NaNs, one more v_max each, is not needed; a NaN score reaches its
+// row through its weight)
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+template <bool BF16> struct Elem {
+    using T = typename std::conditional<BF16, __bf16, _Float16>::type;
+    typedef T vec8 __attribute__((ext_vector_type(8)));
+};
+
+// One wave's 32 rows.
+template <bool BF16, int D, bool SPLIT>
+struct Rows {
+    using T = typename Elem<BF16>::T;
+    using vec8 = typename Elem<BF16>::vec8;
+    static constexpr int NK = D / 16;   // QK k-steps
+    static constexpr int ND = D / 32;   // PV dim tiles
+    static constexpr float kHead = SPLIT ? 0.f : 4.f;
+
+    int lane, half;
+    int query, head;     // of row lane % 32
+    bool on;
+    int lim;             // last position the row sees
+    vec8 qh[NK], ql[SPLIT ? NK : 1];
+    float sscale;        // log2 units per score
+    float m, l;          // l: this lane's half of the positions
+    f32x16_t acc[ND];
+
+    __device__ __forceinline__ void init(const ChunksK& p, const ChunkItem& it, int kvh, int g, int rho) {
+        lane = threadIdx.x & 63;
+        half = lane >> 5;
+        const int r = rho + (lane & 31);
+        on = r < it.rows * g;
+        const int rr = on ? r : it.rows * g - 1;
+        query = rr / g;
+        head = kvh * g + rr - query * g;
+        lim = it.pos0 + query;
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+    }
+
+    // dims 16 kk + 8 half .. + 7 of the row.  The sign of the scale goes into q: the maximum is
+    // taken before the scores are scaled.
+    __device__ __forceinline__ void load_q(const ChunksK& p, const ChunkItem& it) {
+        const long long at = (static_cast<long long>(it.row0 + query) * p.heads + head) * D + 8 * half;
+        const float sign = p.qscale == 0.f ? 0.f : p.qscale < 0.f ? -1.f : 1.f;
+        sscale = p.qscale == 0.f ? 1.f : fabsf(p.qscale);
+        float x[NK][8];
+        if (p.act == QR_DTYPE_F32) {
+            const float* f = static_cast<const float*>(p.q) + at;
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[kk][i] = f[16 * kk + i];
+        } else {
+            const uint16_t* h = static_cast<const uint16_t*>(p.q) + at;
+            uint16_t u[NK][8];
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) u[kk][i] = h[16 * kk + i];
+            const bool bf = p.act == QR_DTYPE_BF16;
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[kk][i] = bf ? bf16_bits_to_f32(u[kk][i]) : f16_bits_to_f32(u[kk][i]);
+        }
+        float by = sign;
+        if (SPLIT && !BF16) {
+            // fp16 parts: the row's largest value to 2^13 .. 2^14, a power of two that the score scale takes back
+            float a = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(x[kk][i]));
+            a = max_xor32(a);
+            if (a > 1e-30f && a < 3e38f) {
+                const int ex = ilogbf(a) - 13;
+                by = ldexpf(sign, -ex);
+                sscale = ldexpf(sscale, ex);
+            }
+        }
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float v = x[kk][i] * by;
+                qh[kk][i] = static_cast<T>(v);
+                if (SPLIT) ql[kk][i] = static_cast<T>(v - static_cast<float>(qh[kk][i]));
+            }
+    }
+
+    // LDS offset of this lane's part of the K operand of a step (k-step kk: + 512 kk) ...
+    __device__ __forceinline__ int k_off() const {
+        const int m_ = lane & 31, s = m_ >> 4, a = (m_ >> 3) & 1, h = (m_ >> 2) & 1, b = m_ & 3;
+        return 1024 * a * (D / 32) + 16 * (16 * half + 4 * (2 * s + h) + b);
+    }
+    // ... and of the V operand (dim tile md, PV step s: + 2048 md + 512 s)
+    __device__ __forceinline__ int v_off() const { return 1024 * ((lane & 31) >> 4) + 16 * (16 * half + (lane & 15)); }
+
+    // positions t0 + 16 s + 8 half + i past the row's own, or past the end, get no weight
+    __device__ __forceinline__ void mask(f32x16_t& s, int t0, int end) const {
+        const int last = min(lim, end - 1) - t0 - 8 * half;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (16 * (r >> 3) + (r & 7) > last) s[r] = -INFINITY;
+    }
+
+    // Weights of NS steps' scores, as PV operands; rescales what was summed when the maximum moves.
+    template <int NS>
+    __device__ __forceinline__ void softmax(const f32x16_t (&s)[NS], vec8 (&ph)[NS][2], vec8 (&pl)[SPLIT ? NS : 1][2]) {
+        float mx[2 * NS];
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            const float a = max3f(s[n][0], s[n][1], s[n][2]), b = max3f(s[n][3], s[n][4], s[n][5]);
+            const float c = max3f(s[n][6], s[n][7], s[n][8]), d = max3f(s[n][9], s[n][10], s[n][11]);
+            mx[2 * n] = max3f(s[n][12], s[n][13], s[n][14]);
+            mx[2 * n] = max3f(mx[2 * n], s[n][15], a);
+            mx[2 * n + 1] = max3f(b, c, d);
+        }
+        float t = mx[0];
+#pragma unroll
+        for (int n = 1; n < 2 * NS; ++n) t = fmaxf(t, mx[n]);
+        t = max_xor32(t) * sscale;
+        const bool grow = t > m;
+        if (__builtin_amdgcn_ballot_w64(grow)) {
+            const float mn = grow ? t + kHead : m;
+            const float c = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            if (__builtin_amdgcn_ballot_w64(grow && m != -INFINITY)) {
+                const float cc = grow && m != -INFINITY ? c : 1.f;
+                l *= cc;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) acc[d] *= cc;
+            }
+            m = mn;
+        }
+        const float ref = m == -INFINITY ? 0.f : -m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = fast_exp2(fmaf(s[n][r], sscale, ref));
+                sum[r & 3] += e;
+                const T hi = static_cast<T>(e);
+                ph[n][r >> 3][r & 7] = hi;
+                if (SPLIT) pl[n][r >> 3][r & 7] = static_cast<T>(e - static_cast<float>(hi));
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
+
+    // A tile that reaches past what every row sees may hold V elements that are not finite at
+    // positions some rows do not see, where 0 x inf would reach them.  True if the step at `v` has such an element
+    // (the same in every wave that looks).
+    __device__ __forceinline__ bool v_bad(const char* v) const {
+        vec8 zero;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) zero[i] = static_cast<T>(0.f);
+        f32x16_t z;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2 * ND; ++c) z = mfma32(*reinterpret_cast<const vec8*>(v + 1024 * c + 16 * lane), zero, z);
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += z[i];
+        return __builtin_amdgcn_ballot_w64(!(t == 0.f)) != 0;
+    }
+    // Adds the elements of the step at `v` (positions t0 .. t0 + 31) that are not finite to the rows that see them, as they
+    // are: no finite weight changes them.
+    __device__ __forceinline__ void add_bad(const char* v, int t0, int end) {
+#pragma unroll 1
+        for (int k = 0; k < 32; ++k) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int dim = 32 * d + 8 * (r >> 2) + 4 * half + (r & 3);
+                    const float x = static_cast<float>(*reinterpret_cast<const T*>(
+                        v + 1024 * (dim >> 4) + 16 * (16 * (k >> 3) + (dim & 15)) + 2 * (k & 7)));
+                    if (!(fabsf(x) < INFINITY) && t0 + k <= min(lim, end - 1)) acc[d][r] += x;
+                    if ((r & 3) == 3) asm volatile("" ::: "memory");  // no registers for all reads at once
+                }
+        }
+    }
+
+    // Merged (m, l) and the row's output or split partial.  by = 1 / l or 1.
+    __device__ __forceinline__ void store4(const ChunksK& p, const ChunkItem& it, int split, int d, const f32x4_t& a, float lsum) const {
+        if (!on) return;
+        const long long rh = static_cast<long long>(it.row0 + query) * p.heads + head;
+        if (it.splits > 1) {
+            const long long slot = it.slot0 + (static_cast<long long>(query) * p.heads + head) * it.splits + split;
+            *reinterpret_cast<f32x4_t*>(p.part_acc + slot * D + d) = a;
+            return;
+        }
+        const float inv = 1.f / lsum;
+        if (p.act == QR_DTYPE_F32) {
+            float* o = static_cast<float*>(p.out) + rh * D + d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = a[i] * inv;
+        } else {
+            uint16_t b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = f32_to_bits16(a[i] * inv, p.act);
+            __builtin_memcpy(static_cast<uint16_t*>(p.out) + rh * D + d, b, 8);  // one store, element-aligned
+        }
+    }
+    __device__ __forceinline__ void store_ml(const ChunksK& p, const ChunkItem& it, int split, float mm, float lsum) const {
+        if (!on || half) return;
+        if (p.row_scale) p.row_scale[static_cast<long long>(it.row0 + query) * p.heads + head] = sscale;  // the same in every split
+        if (it.splits > 1) p.part_ml[it.slot0 + (static_cast<long long>(query) * p.heads + head) * it.splits + split] = make_float2(mm, lsum);
+        else if (p.row_ml) p.row_ml[static_cast<long long>(it.row0 + query) * p.heads + head] = make_float2(mm, lsum);
+    }
+};
+
+// Clears the elements of `bytes` bytes of V that are not finite.
+template <class T> __device__ __forceinline__ void clear_bad(char* v, int bytes, int threads) {
+    for (int c = threadIdx.x; c < bytes / 2; c += threads) {
+        T* e = reinterpret_cast<T*>(v) + c;
+        if (!(fabsf(static_cast<float>(*e)) < INFINITY)) *e = static_cast<T>(0.f);
+    }
+}
+
+// Page of a position, by a scalar load (no kernel writes the table while this one runs).
+__device__ __forceinline__ int page_of(const ChunksK& p, int pt_off, int t) {
+    return reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p.page_table))[pt_off + (t >> kPageShift)];
+}
+
+// ------------------------------------------------------------------ few rows: HBM-bound
+// RW waves of 32 rows each x PW waves that take one step of 32 positions of every tile.  With
+// RW = 1 a wave copies its own steps and no wave waits for another before the end.
+template <bool BF16, int D, bool SPLIT, int RW, int PW>
+__global__ void __launch_bounds__(64 * RW * PW, 1) chunks_stream_kernel(const ChunksK p) {
+    using R = Rows<BF16, D, SPLIT>;
+    using vec8 = typename R::vec8;
+    constexpr int WAVES = RW * PW;
+    constexpr int TILE = 32 * PW;
+    constexpr int SB = 64 * D;                    // bytes of a step of K (or V)
+    constexpr int STAGE = 2 * SB * PW;            // a tile's steps, each K then V
+    constexpr int NST = STAGE > 32768 ? 2 : STAGE > 16384 ? 3 : 4;
+    constexpr int PER = 2 * SB * PW / 1024 / WAVES;  // DMA loads per wave and tile
+    constexpr int NG = D / 8;                     // f32x4 groups of a row in a lane
+    constexpr int XB = WAVES * 64 * (NG * 16 + 8);   // the waves' (acc, m, l), exchanged at the end
+    constexpr int LDS = NST * STAGE > XB ? NST * STAGE : XB;
+    static_assert(NG % PW == 0 && LDS <= 160 * 1024, "");
+    __shared__ __attribute__((aligned(1024))) char lds[LDS];
+
+    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
+    const ChunkItem it = p.it[e];
+    const int u = blockIdx.x - it.unit0;
+    const int split = u % it.splits, block = u / it.splits % it.blocks, kvh = u / (it.splits * it.blocks);
+    const int g = p.heads / p.geom.kv_heads;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rw = wave % RW, pw = wave / RW;
+    const int rho0 = block * 32 * RW;
+    const int last = min(rho0 + 32 * RW, it.rows * g) - 1;
+    int t0, t1;
+    chunk_keys(it, it.pos0 + last / g + 1, split, TILE, &t0, &t1);
+    const int ntiles = t1 > t0 ? (t1 - t0 + TILE - 1) / TILE : 0;
+    const int seen = it.pos0 + rho0 / g + 1;  // positions below it are seen by every row
+
+    const long long page_bytes = p.geom.page_elems() * 2, plane_bytes = p.geom.plane_elems() * 2;
+    const long long head_bytes = static_cast<long long>(kvh) * kPageTokens * D * 2;
+    const uint32_t lane16 = 16 * (threadIdx.x & 63);
+    auto dma = [&](int i) {
+        // past the last tile: no records, so that zeros are written and no memory is read
+        const int t = t0 + min(i, ntiles - 1) * TILE;
+        char* dst = lds + (i % NST) * STAGE;
+#pragma unroll
+        for (int c = 0; c < PER; ++c) {
+            // RW = 1: the wave's own step; else loads dealt to the waves
+            const int n = RW == 1 ? pw * (2 * SB / 1024) + c : wave + WAVES * c;
+            const int st = n / (2 * SB / 1024), part = n % (2 * SB / 1024);
+            const int ts = t + 32 * st;
+            // a step past the keys' end may lie past the held pages: its page is not looked up
+            const bool in = i < ntiles && ts < t1;
+            const long long phys = in ? page_of(p, it.pt_off, ts) : 0;
+            const char* base = p.pool + phys * page_bytes + head_bytes + (part >= SB / 1024 ? plane_bytes : 0) +
+                               static_cast<long long>(ts & (kPageTokens - 1)) * D * 2;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, in ? SB : 0, kBufferFlags);
+            buffer_load_lds16<kCacheNt>(r, dst + 1024 * n, lane16, 1024 * (part % (SB / 1024)));
+        }
+    };
+    if (ntiles > 0)
+        for (int i = 0; i < NST - 1; ++i) dma(i);
+
+    R w;
+    w.init(p, it, kvh, g, rho0 + 32 * rw);
+    w.load_q(p, it);
+    const int ko = w.k_off(), vo = w.v_off();
+    float* const scores = p.scores ? p.scores + it.score0 + (static_cast<long long>(w.query) * p.heads + w.head) * chunk_score_len(it) : nullptr;
+
+    for (int i = 0; i < ntiles; ++i) {
+        wait_vmcnt<(NST - 2) * PER>();
+        if (RW > 1) lds_barrier_dma_in_flight();  // everyone's part has landed, and the stage filled next was read
+        dma(i + NST - 1);
+        const int ts = t0 + i * TILE + 32 * pw;
+        char* const kt = lds + (i % NST) * STAGE + 2 * SB * pw;
+        char* const vt = kt + SB;
+        const bool edge = t0 + (i + 1) * TILE > seen || t0 + (i + 1) * TILE > t1;
+        if (RW > 1 && edge) {
+            bool bad = false;
+            for (int s = 0; s < PW; ++s) bad |= w.v_bad(lds + (i % NST) * STAGE + 2 * SB * s + SB);
+            if (bad) {
+                w.add_bad(vt, ts, t1);
+                lds_barrier_dma_in_flight();
+                for (int s = 0; s < PW; ++s) clear_bad<typename R::T>(lds + (i % NST) * STAGE + 2 * SB * s + SB, SB, 64 * WAVES);
+                lds_barrier_dma_in_flight();
+            }
+        } else if (edge && w.v_bad(vt)) {
+            w.add_bad(vt, ts, t1);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            for (int c = w.lane; c < SB / 2; c += 64) {
+                typename R::T* x = reinterpret_cast<typename R::T*>(vt) + c;
+                if (!(fabsf(static_cast<float>(*x)) < INFINITY)) *x = static_cast<typename R::T>(0.f);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        f32x16_t s[1];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < R::NK; ++kk) {
+            const vec8 a = *reinterpret_cast<const vec8*>(kt + ko + 512 * kk);
+            s[0] = mfma32(a, w.qh[kk], s[0]);
+            if (SPLIT) s[0] = mfma32(a, w.ql[kk], s[0]);
+        }
+        if (edge) w.mask(s[0], ts, t1);
+        if (scores && w.on) {
+            // for the weights: a row's 8 positions are 32 bytes (whole: a row of scores is whole runs of 8)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                if (ts + 16 * x + 8 * w.half < t1) {
+                    f32x4_t* o = reinterpret_cast<f32x4_t*>(scores + ts + 16 * x + 8 * w.half);
+                    o[0] = f32x4_t{s[0][8 * x], s[0][8 * x + 1], s[0][8 * x + 2], s[0][8 * x + 3]} * w.sscale;
+                    o[1] = f32x4_t{s[0][8 * x + 4], s[0][8 * x + 5], s[0][8 * x + 6], s[0][8 * x + 7]} * w.sscale;
+                }
+        }
+        vec8 ph[1][2], pl[1][2];
+        w.template softmax<1>(s, ph, pl);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int d = 0; d < R::ND; ++d) {
+                const vec8 a = *reinterpret_cast<const vec8*>(vt + vo + 2048 * d + 512 * x);
+                w.acc[d] = mfma32(a, ph[0][x], w.acc[d]);
+                if (SPLIT) w.acc[d] = mfma32(a, pl[0][x], w.acc[d]);
+            }
+    }
+    w.l = sum_xor32(w.l);
+
+    // the PW waves of a row group merge: each adds up NG / PW of the dim groups
+    wait_dma();
+    __syncthreads();
+    f32x4_t* const xa = reinterpret_cast<f32x4_t*>(lds);                        // [wave][group][64]
+    float2* const xm = reinterpret_cast<float2*>(lds + WAVES * 64 * NG * 16);   // [wave][64]
+#pragma unroll
+    for (int d = 0; d < R::ND; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            xa[(wave * NG + 4 * d + q) * 64 + w.lane] = f32x4_t{w.acc[d][4 * q], w.acc[d][4 * q + 1], w.acc[d][4 * q + 2], w.acc[d][4 * q + 3]};
+    xm[wave * 64 + w.lane] = make_float2(w.m, w.l);
+    __syncthreads();
+    float M = -INFINITY, L = 0.f, c[PW];
+#pragma unroll
+    for (int x = 0; x < PW; ++x) M = fmaxf(M, xm[(x * RW + rw) * 64 + w.lane].x);
+#pragma unroll
+    for (int x = 0; x < PW; ++x) {
+        const float2 ml = xm[(x * RW + rw) * 64 + w.lane];
+        c[x] = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
+        L = fmaf(ml.y, c[x], L);
+    }
+    for (int q = pw * (NG / PW); q < (pw + 1) * (NG / PW); ++q) {
+        f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < PW; ++x) a += xa[((x * RW + rw) * NG + q) * 64 + w.lane] * c[x];
+        w.store4(p, it, split, 32 * (q >> 2) + 8 * (q & 3) + 4 * w.half, a, L);
+    }
+    if (pw == 0) w.store_ml(p, it, split, M, L);
+}
+
+// ------------------------------------------------------------------ many rows: MFMA-bound
+// Eight waves of 32 rows share every tile of 64 positions.  Waves 0-3 and 4-7 run half a tile apart: while
+// one group's MFMAs run (scores of tile t, weighted V of tile t - 1), the other group computes its
+// softmax on the same SIMDs; a barrier ends each half.
+template <bool BF16, int D, bool SPLIT>
+__global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
+    using R = Rows<BF16, D, SPLIT>;
+    using vec8 = typename R::vec8;
+    constexpr int TILE = 64, NST = 3;
+    constexpr int SB = 64 * D;           // bytes of a step of K (or V)
+    constexpr int KB = 2 * SB;           // of a tile of K (or V)
+    constexpr int PER = KB / 1024 / 8;   // DMA loads per wave for a tile of K (or V)
+    __shared__ __attribute__((aligned(1024))) char lds[2 * NST * KB];  // K tiles, then V tiles
+
+    // Launch slot b runs on XCD b % 8, which takes contiguous units: the blocks of one kv head
+    // share its K/V in the XCD's L2.  Blocks from the last, which has the most keys, down.
+    const int per_xcd = (p.units + 7) >> 3;
+    const int unit = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if ((static_cast<int>(blockIdx.x) >> 3) >= per_xcd || unit >= p.units) return;
+    const int e = batch_find(p.n, unit, [&](int i) { return p.it[i].unit0; });
+    const ChunkItem it = p.it[e];
+    const int u = unit - it.unit0;
+    const int split = u % it.splits, block = it.blocks - 1 - u / it.splits % it.blocks, kvh = u / (it.splits * it.blocks);
+    const int g = p.heads / p.geom.kv_heads;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rho0 = block * 256;
+    const int last = min(rho0 + 256, it.rows * g) - 1;
+    int t0, t1;
+    chunk_keys(it, it.pos0 + last / g + 1, split, TILE, &t0, &t1);
+    const int ntiles = t1 > t0 ? (t1 - t0 + TILE - 1) / TILE : 0;
+    const int seen = it.pos0 + rho0 / g + 1;  // positions below it are seen by every row
+
+    const long long page_bytes = p.geom.page_elems() * 2, plane_bytes = p.geom.plane_elems() * 2;
+    const long long head_bytes = static_cast<long long>(kvh) * kPageTokens * D * 2;
+    const uint32_t lane16 = 16 * (threadIdx.x & 63);
+    auto dma = [&](int i, int plane) {
+        const bool in = i < ntiles;  // past the last tile: no records, no memory is read
+        const int t = t0 + min(i, ntiles - 1) * TILE;
+        const char* base = p.pool + static_cast<long long>(page_of(p, it.pt_off, t)) * page_bytes + head_bytes + plane * plane_bytes +
+                           static_cast<long long>(t & (kPageTokens - 1)) * D * 2;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, in ? KB : 0, kBufferFlags);
+        char* dst = lds + plane * NST * KB + (i % NST) * KB;
+#pragma unroll
+        for (int c = 0; c < PER; ++c) buffer_load_lds16(r, dst + 1024 * (wave + 8 * c), lane16, 1024 * (wave + 8 * c));
+    };
+    R w;
+    w.init(p, it, kvh, g, rho0 + 32 * wave);
+    if (ntiles > 0) {
+        dma(0, 0);
+        dma(1, 0);
+        dma(0, 1);
+    }
+    w.load_q(p, it);
+    const int ko = w.k_off(), vo = w.v_off();
+    vec8 ph[2][2], pl[SPLIT ? 2 : 1][2];
+    f32x16_t s[2];
+
+    auto barrier = [&]() __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0);
+        lds_barrier_dma_in_flight();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // operand reads run kAhead MFMAs in front of their use
+    constexpr int kAhead = SPLIT ? 3 : 6;
+    auto qk_pv = [&](const char* kt, const char* vt, bool qk, bool pv) __attribute__((always_inline)) {
+        constexpr int NQ = 2 * R::NK, NP = 4 * R::ND;  // operands: K (step, kk), V (step, PV step, dim tile)
+        static_assert(NQ == NP, "one of each in turn");
+        vec8 ring[kAhead];
+        auto read = [&](int i) __attribute__((always_inline)) -> vec8 {
+            const int j = i >> 1;
+            if (i & 1) return *reinterpret_cast<const vec8*>(vt + SB * (j / (2 * R::ND)) + vo + 2048 * (j % R::ND) + 512 * (j / R::ND % 2));
+            return *reinterpret_cast<const vec8*>(kt + SB * (j & 1) + ko + 512 * (j >> 1));
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if ((i & 1) ? pv : qk) ring[i] = read(i);
+#pragma unroll
+        for (int i = 0; i < NQ + NP; ++i) {
+            const int j = i >> 1;
+            if (i & 1) {
+                if (pv) {
+                    const int st = j / (2 * R::ND), x = j / R::ND % 2, d = j % R::ND;
+                    w.acc[d] = mfma32(ring[i % kAhead], ph[st][x], w.acc[d]);
+                    if (SPLIT) w.acc[d] = mfma32(ring[i % kAhead], pl[SPLIT ? st : 0][x], w.acc[d]);
+                }
+            } else if (qk) {
+                const int st = j & 1, kk = j >> 1;
+                s[st] = mfma32(ring[i % kAhead], w.qh[kk], s[st]);
+                if (SPLIT) s[st] = mfma32(ring[i % kAhead], w.ql[SPLIT ? kk : 0], s[st]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + kAhead < NQ + NP && ((i + kAhead) & 1 ? pv : qk)) ring[i % kAhead] = read(i + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    const bool late = wave >= 4;  // half a tile behind
+    // tiles that reach past what every row sees
+    auto edge = [&](int i) { return t0 + (i + 1) * TILE > seen || t0 + (i + 1) * TILE > t1; };
+    // both groups come here with tile i after the same barrier, before either weighs its V
+    auto mend_v = [&](int i) __attribute__((always_inline)) {
+        if (!edge(i)) return;
+        char* v = lds + NST * KB + (i % NST) * KB;
+        const bool b0 = w.v_bad(v), b1 = w.v_bad(v + SB);
+        if (!b0 && !b1) return;
+        w.add_bad(v, t0 + i * TILE, t1);
+        w.add_bad(v + SB, t0 + i * TILE + 32, t1);
+        barrier();
+        clear_bad<typename R::T>(v, KB, 512);
+        barrier();
+    };
+    if (ntiles > 0) {
+        wait_vmcnt<2 * PER>();  // K of tile 0
+        barrier();
+        // Before the early group's tile i: K of tile i + 2 goes over K of tile i - 1 and V of tile i + 1 over V of
+        // tile i - 2, which the late group read for the last time before the barrier just passed.  Both
+        // are awaited two barriers later.
+        if (late) {
+            dma(2, 0);
+            dma(1, 1);
+            barrier();
+        }
+        for (int i = 0; i < ntiles; ++i) {
+            if (!late) {
+                dma(i + 2, 0);
+                dma(i + 1, 1);
+                if (i > 0) mend_v(i - 1);
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[st][r] = 0.f;
+            const char* kt = lds + (i % NST) * KB;
+            const char* vt = lds + NST * KB + ((i + NST - 1) % NST) * KB;
+            if (i == 0) qk_pv(kt, vt, true, false);
+            else qk_pv(kt, vt, true, true);
+            if (late) wait_vmcnt<2 * PER>();
+            barrier();
+            if (late) {
+                dma(i + 3, 0);
+                dma(i + 2, 1);
+                mend_v(i);
+            }
+            const int ts = t0 + i * TILE;
+            if (edge(i)) {
+                w.mask(s[0], ts, t1);
+                w.mask(s[1], ts + 32, t1);
+            }
+            w.template softmax<2>(s, ph, pl);
+            if (!late) wait_vmcnt<2 * PER>();
+            barrier();
+        }
+        const char* vt = lds + NST * KB + ((ntiles - 1) % NST) * KB;
+        if (!late) mend_v(ntiles - 1);
+        qk_pv(vt, vt, false, true);
+        if (!late) barrier();
+    }
+    w.l = sum_xor32(w.l);
+#pragma unroll
+    for (int d = 0; d < R::ND; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            w.store4(p, it, split, 32 * d + 8 * q + 4 * w.half,
+                     f32x4_t{w.acc[d][4 * q], w.acc[d][4 * q + 1], w.acc[d][4 * q + 2], w.acc[d][4 * q + 3]}, w.l);
+    w.store_ml(p, it, split, w.m, w.l);
+}
+
+
+// ------------------------------------------------------------------ weights
+// Weights of 256 positions of one kv head over a part of its rows: a wave keeps the K rows of 32
+// positions as operands and takes the rows 32 at a time from LDS, where each wave puts one k-step's operand of them.
+// Bound by the exponentials (16 cycles per 64 of them, against 16 for the MFMAs of as many scores).
+template <bool BF16, int D, bool SPLIT>
+__global__ void __launch_bounds__(512, 1) chunks_tile_weights_kernel(const ChunksK p) {
+    using T = typename Elem<BF16>::T;
+    using vec8 = typename Elem<BF16>::vec8;
+    constexpr int NK = D / 16;
+    constexpr int RT = 8 / NK;           // 32-row tiles of a round: one operand per wave
+    constexpr int PART = SPLIT ? 2 : 1;
+    __shared__ __attribute__((aligned(1024))) char lds[2][PART * 8 * 1024];
+    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
+    const ChunkItem it = p.it[e];
+    const int u = blockIdx.x - it.unit0;
+    const int split = u % it.splits, block = u / it.splits % it.blocks, kvh = u / (it.splits * it.blocks);
+    const int g = p.heads / p.geom.kv_heads, rows = it.rows * g;
+    const int lane = threadIdx.x & 63, half = lane >> 5, n = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int len = it.pos0 + it.rows;
+    const int b0 = block * 256, t0 = b0 + 32 * wave;
+    // rows that see part of the block, in rounds dealt to the splits
+    const int first = max(0, b0 - it.pos0) * g;
+    const int rounds = (rows - first + 32 * RT - 1) / (32 * RT);
+    const int r0 = first + static_cast<int>(static_cast<long long>(rounds) * split / it.splits) * 32 * RT;
+    const int r1 = min(rows, first + static_cast<int>(static_cast<long long>(rounds) * (split + 1) / it.splits) * 32 * RT);
+
+    vec8 k[NK];
+    {
+        const int s = n >> 4, a = (n >> 3) & 1, h = (n >> 2) & 1, b = n & 3;
+        const int off = 1024 * a * (D / 32) + 16 * (16 * half + 4 * (2 * s + h) + b);
+        const long long phys = t0 < len ? page_of(p, it.pt_off, t0) : 0;
+        const char* src = p.pool + (phys * p.geom.page_elems() + static_cast<long long>(kvh) * kPageTokens * D +
+                                    static_cast<long long>(t0 & (kPageTokens - 1)) * D) * 2 + off;
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+            if (t0 < len) k[kk] = *reinterpret_cast<const vec8*>(src + 512 * kk);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; ++i) k[kk][i] = static_cast<T>(0.f);
+        }
+    }
+    const float sign = p.qscale == 0.f ? 0.f : p.qscale < 0.f ? -1.f : 1.f;
+    const float base = p.qscale == 0.f ? 1.f : fabsf(p.qscale);
+    // this wave's operand of a round: k-step wave % NK of row tile wave / NK
+    float x[8];
+    float scale_x = 1.f;
+    auto fetch = [&](int r) __attribute__((always_inline)) {
+        const int rho = min(r + 32 * (wave / NK) + n, rows - 1);
+        const long long row = static_cast<long long>(it.row0 + rho / g) * p.heads + kvh * g + rho % g;
+        const long long at = row * D + 16 * (wave % NK) + 8 * half;
+        if (p.act == QR_DTYPE_F32) {
+            const float* f = static_cast<const float*>(p.q) + at;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = f[i];
+        } else {
+            const uint16_t* f = static_cast<const uint16_t*>(p.q) + at;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = p.act == QR_DTYPE_BF16 ? bf16_bits_to_f32(f[i]) : f16_bits_to_f32(f[i]);
+        }
+        scale_x = p.row_scale ? base / p.row_scale[row] : 1.f;  // a power of two
+    };
+    auto put = [&](char* to) __attribute__((always_inline)) {
+        vec8 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = x[i] * (sign * scale_x);
+            hi[i] = static_cast<T>(v);
+            lo[i] = static_cast<T>(v - static_cast<float>(hi[i]));
+        }
+        *reinterpret_cast<vec8*>(to + 1024 * wave + 16 * lane) = hi;
+        if (SPLIT) *reinterpret_cast<vec8*>(to + 8192 + 1024 * wave + 16 * lane) = lo;
+    };
+    float sum[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum[r] = 0.f;
+    if (r0 < r1) {
+        fetch(r0);
+        put(lds[0]);
+    }
+    int at = 0;
+    for (int r = r0; r < r1; r += 32 * RT, at ^= 1) {
+        __syncthreads();
+        const bool more = r + 32 * RT < r1;
+        if (more) fetch(r + 32 * RT);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int rho = r + 32 * rt + n;
+            const bool on = rho < r1;
+            const int rr = on ? rho : rows - 1;
+            const int query = rr / g;
+            const long long rh = static_cast<long long>(it.row0 + query) * p.heads + kvh * g + rr - query * g;
+            const float2 ml = p.row_ml[rh];
+            const float sscale = p.row_scale ? p.row_scale[rh] : base;
+            const float inv = on ? 1.f / ml.y : 0.f;
+            f32x16_t s;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) {
+                const char* q = lds[at] + 1024 * (rt * NK + kk) + 16 * lane;
+                s = mfma32(k[kk], *reinterpret_cast<const vec8*>(q), s);
+                if (SPLIT) s = mfma32(k[kk], *reinterpret_cast<const vec8*>(q + 8192), s);
+            }
+            // rows of this tile that do not see every position of the wave's, or stand past the end
+            const int last = on ? it.pos0 + query - t0 - 8 * half : -1;
+            if (__builtin_amdgcn_ballot_w64(last < 24)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (16 * (i >> 3) + (i & 7) <= last) sum[i] = fmaf(fast_exp2(fmaf(s[i], sscale, -ml.x)), inv, sum[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum[i] = fmaf(fast_exp2(fmaf(s[i], sscale, -ml.x)), inv, sum[i]);
+            }
+        }
+        if (more) put(lds[at ^ 1]);
+    }
+    // over the 32 lanes of a half
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] = sum_xor16(group_sum(sum[i], 16));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int t = t0 + 16 * (i >> 3) + 8 * half + (i & 7);
+        if (n == i && t < len) {
+            if (it.splits == 1) p.weights[(static_cast<long long>(it.seq) * p.geom.kv_heads + kvh) * p.max_seq + t] += sum[i];
+            else p.wpart[it.slot0 + (static_cast<long long>(split) * p.geom.kv_heads + kvh) * len + t] = sum[i];
+        }
+    }
+}
+
+template <bool BF16, int D, bool SPLIT>
+hipError_t launch_kind(const ChunksK& k, int kind, hipStream_t s) {
+    switch (kind) {
+        case kChunkStream32: hipLaunchKernelGGL((chunks_stream_kernel<BF16, D, SPLIT, 1, 4>), dim3(k.units), dim3(256), 0, s, k); break;
+        case kChunkStream64: hipLaunchKernelGGL((chunks_stream_kernel<BF16, D, SPLIT, 2, 4>), dim3(k.units), dim3(512), 0, s, k); break;
+        case kChunkStream128: hipLaunchKernelGGL((chunks_stream_kernel<BF16, D, SPLIT, 4, 2>), dim3(k.units), dim3(512), 0, s, k); break;
+        case kChunkTile: hipLaunchKernelGGL((chunks_tile_kernel<BF16, D, SPLIT>), dim3((k.units + 7) / 8 * 8), dim3(512), 0, s, k); break;
+        default: hipLaunchKernelGGL((chunks_tile_weights_kernel<BF16, D, SPLIT>), dim3(k.units), dim3(512), 0, s, k); break;
+    }
+    return hipGetLastError();
+}
+template <bool BF16> hipError_t launch_d(const ChunksK& k, int kind, hipStream_t s) {
+    const bool split = k.act != k.dtype;
+    if (k.geom.head_dim == 128) return split ? launch_kind<BF16, 128, true>(k, kind, s) : launch_kind<BF16, 128, false>(k, kind, s);
+    return split ? launch_kind<BF16, 64, true>(k, kind, s) : launch_kind<BF16, 64, false>(k, kind, s);
+}
+
+}  // namespace
+
+hipError_t launch_chunks_tile(const ChunksK& k, int kind, hipStream_t s) {
+    return k.dtype == QR_DTYPE_BF16 ? launch_d<true>(k, kind, s) : launch_d<false>(k, kind, s);
+}
+
+}  // namespace qr
