@@ -67,7 +67,7 @@ struct KindGeom {
     int rows, tile;   // of a workgroup
     long long want;   // units that fill the GPU
 };
-constexpr KindGeom kGeom[kChunkKinds] = {{kChunkAnyRows, kChunkAnyTile, 1024}, {32, 128, 256}, {64, 128, 256}, {128, 64, 256}, {256, 64, 256}};
+constexpr KindGeom kGeom[kChunkKinds] = {{kChunkAnyRows, kChunkAnyTile, 1024}, {32, 128, 256}, {64, 128, 256}, {128, 64, 256}, {256, 64, 256}, {32, 32, 256}, {64, 32, 256}};
 
 int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
@@ -77,8 +77,15 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
     ChunksPlan pl{};
     const int kv = a.geom.kv_heads, gmax = cdiv(a.heads, kv);
     const bool tiles = a.geom.mfma_layout && a.heads % kv == 0;
+    const bool f32 = !tiles && chunks_f32_takes(a.dtype, a.geom.head_dim, a.heads, kv);
     for (int i = 0; i < a.n; ++i) {
         const long long rows = static_cast<long long>(a.it[i].rows) * gmax;
+        if (f32) {
+            // whole queries per block
+            pl.it[i].kind = rows <= 32 ? kChunkF32Half : kChunkF32;
+            pl.it[i].blocks = cdiv(a.it[i].rows, kGeom[pl.it[i].kind].rows / gmax);
+            continue;
+        }
         pl.it[i].kind = !tiles ? kChunkAny : rows <= 32 ? kChunkStream32 : rows <= 64 ? kChunkStream64 : rows <= 128 ? kChunkStream128 : kChunkTile;
         pl.it[i].blocks = cdiv(rows, kGeom[pl.it[i].kind].rows);
     }
@@ -86,7 +93,8 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
     // per unit as leave no more units than that, or one tile.
     long long slots = 0;
     for (int kind = 0; kind < kChunkKinds; ++kind) {
-        const KindGeom& g = kGeom[kind];
+        KindGeom g = kGeom[kind];
+        if (kind == kChunkF32Half || kind == kChunkF32) g.want *= chunks_f32_per_cu(a.dtype, a.geom.head_dim, kind == kChunkF32Half);
         long long base = 0, work = 0;
         for (int i = 0; i < a.n; ++i)
             if (pl.it[i].kind == kind) {
@@ -120,10 +128,11 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
         long long units = 0;
         for (int i = 0; i < a.n; ++i) {
             ChunkPlanItem& it = pl.it[i];
-            it.wkind = it.kind == kChunkAny ? kWeightsAny : it.kind == kChunkStream32 ? kWeightsScores : kWeightsTile;
-            it.wblocks = cdiv(a.it[i].pos0 + a.it[i].rows, it.kind == kChunkAny ? kChunkAnyTile : 256);
+            it.wkind = it.kind == kChunkAny ? kWeightsAny : it.kind == kChunkStream32 || it.kind == kChunkF32Half ? kWeightsScores
+                     : it.kind == kChunkF32 ? kWeightsF32 : kWeightsTile;
+            it.wblocks = cdiv(a.it[i].pos0 + a.it[i].rows, it.wkind == kWeightsAny ? kChunkAnyTile : it.wkind == kWeightsF32 ? 128 : 256);
             it.wsplits = 1;
-            if (it.wkind == kWeightsTile) units += static_cast<long long>(it.wblocks) * kv;
+            if (it.wkind >= kWeightsTile) units += static_cast<long long>(it.wblocks) * kv;
             if (it.wkind == kWeightsScores) {
                 it.score0 = scores;
                 scores += static_cast<long long>(a.it[i].rows) * a.heads * chunk_score_len(a.it[i]);
@@ -132,7 +141,7 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
         // few position blocks: their rows are split too, 64 rows or more a part
         for (int i = 0; i < a.n; ++i) {
             ChunkPlanItem& it = pl.it[i];
-            if (it.wkind != kWeightsTile || units >= 1024) continue;
+            if (it.wkind < kWeightsTile || units >= 1024) continue;
             it.wsplits = std::max(1, std::min(cdiv(1024, units), cdiv(static_cast<long long>(a.it[i].rows) * gmax, 64)));
             it.wslot0 = wslots;
             if (it.wsplits > 1) {
@@ -200,8 +209,9 @@ hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* work
     hipError_t e = hipSuccess;
     for (int kind = 0; kind < kChunkKinds && e == hipSuccess; ++kind) {
         if (!gather([&](const ChunkPlanItem& p) { return p.kind == kind; }, false)) continue;
-        k.scores = a.weights && kind == kChunkStream32 ? reinterpret_cast<float*>(w + plan.scores) : nullptr;
-        e = kind == kChunkAny ? launch_chunks_any(k, stream) : launch_chunks_tile(k, kind, stream);
+        k.scores = a.weights && (kind == kChunkStream32 || kind == kChunkF32Half) ? reinterpret_cast<float*>(w + plan.scores) : nullptr;
+        e = kind == kChunkAny ? launch_chunks_any(k, stream) : kind >= kChunkF32Half ? launch_chunks_f32(k, kind, stream)
+          : launch_chunks_tile(k, kind, stream);
     }
     if (e == hipSuccess && plan.merge) {
         gather([](const ChunkPlanItem&) { return true; }, false);
@@ -216,14 +226,16 @@ hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* work
             hipLaunchKernelGGL(chunks_scores_kernel, dim3(k.units), dim3(256), 0, stream, k);
             e = hipGetLastError();
         } else {
-            e = kind == kWeightsAny ? launch_chunks_any_weights(k, stream) : launch_chunks_tile(k, kChunkKinds, stream);
+            e = kind == kWeightsAny ? launch_chunks_any_weights(k, stream) : kind == kWeightsF32 ? launch_chunks_f32(k, kChunkKinds, stream)
+              : launch_chunks_tile(k, kChunkKinds, stream);
         }
     }
     if (e == hipSuccess && plan.wmerge) {
-        gather([](const ChunkPlanItem& p) { return p.wkind == kWeightsTile && p.wsplits > 1; }, true);
+        gather([](const ChunkPlanItem& p) { return p.wkind >= kWeightsTile && p.wsplits > 1; }, true);
         k.units = 0;  // one unit per 256 positions and kv head
         for (int i = 0; i < k.n; ++i) {
             k.it[i].unit0 = k.units;
+            k.it[i].blocks = cdiv(k.it[i].pos0 + k.it[i].rows, 256);
             k.units += k.it[i].blocks * kv;
         }
         hipLaunchKernelGGL(chunks_wmerge_kernel, dim3(k.units), dim3(256), 0, stream, k);

@@ -8,9 +8,9 @@
 namespace qr {
 
 // Kernels of a launch; rows (query, query head pairs of a kv head) of a workgroup, positions of a tile.
-enum ChunkKind { kChunkAny, kChunkStream32, kChunkStream64, kChunkStream128, kChunkTile, kChunkKinds };
+enum ChunkKind { kChunkAny, kChunkStream32, kChunkStream64, kChunkStream128, kChunkTile, kChunkF32Half, kChunkF32, kChunkKinds };
 // The passes after the attention that add up the weights.
-enum ChunkWeights { kWeightsAny, kWeightsScores, kWeightsTile, kWeightsKinds };
+enum ChunkWeights { kWeightsAny, kWeightsScores, kWeightsTile, kWeightsF32, kWeightsKinds };
 
 constexpr int kChunkAnyRows = 8, kChunkAnyTile = 32;
 
@@ -59,5 +59,9 @@ hipError_t launch_chunks_any_weights(const ChunksK& k, hipStream_t s);
 // 16-bit caches in the MFMA page layout, whole groups: kinds kChunkStream32 .. kChunkTile; kChunkKinds:
 // the weights pass.
 hipError_t launch_chunks_tile(const ChunksK& k, int kind, hipStream_t s);
+// fp32 tiles: kinds kChunkF32Half (32 rows), kChunkF32 (64 rows); kChunkKinds: the weights pass.
+bool chunks_f32_takes(int dtype, int head_dim, int heads, int kv_heads);
+int chunks_f32_per_cu(int dtype, int head_dim, bool half);  // resident workgroups
+hipError_t launch_chunks_f32(const ChunksK& k, int kind, hipStream_t s);
 
 }  // namespace qr
