@@ -35,6 +35,15 @@ __device__ __forceinline__ void store_elem(void* p, int dtype, long long i, floa
     else static_cast<uint16_t*>(p)[i] = f32_to_bits16(x, dtype);
 }
 
+// An output of attention: rounded to nearest even, NaN stays NaN.
+__device__ __forceinline__ uint16_t f32_to_out16(float x, int dtype) {
+    return dtype == QR_DTYPE_F16 ? __half_as_ushort(__float2half(x)) : f32_to_bits16(x, dtype);
+}
+__device__ __forceinline__ void store_out(void* p, int dtype, long long i, float x) {
+    if (dtype == QR_DTYPE_F32) static_cast<float*>(p)[i] = x;
+    else static_cast<uint16_t*>(p)[i] = f32_to_out16(x, dtype);
+}
+
 // ------------------------------------------------------------------ append
 struct NormRopeItem {
     int pt_off;  // page-table row of (sequence, layer)

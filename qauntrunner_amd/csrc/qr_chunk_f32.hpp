@@ -465,7 +465,7 @@ __device__ __forceinline__ void chunk_f32_tiles(const ChunkF32K& p, int split, i
                 for (int r = 0; r < 4; ++r) {
                     uint16_t b[PE];
 #pragma unroll
-                    for (int e = 0; e < PE; ++e) b[e] = f32_to_bits16(acc[g][e][r] * inv, p.out_dtype);
+                    for (int e = 0; e < PE; ++e) b[e] = f32_to_out16(acc[g][e][r] * inv, p.out_dtype);
                     __builtin_memcpy(o + 16 * PE * g + PE * r, b, sizeof b);
                 }
             return;

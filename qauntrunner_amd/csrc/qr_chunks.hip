@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(64) chunks_combine_kernel(const ChunksK p) {
     const long long rh = blockIdx.x;
 #pragma unroll
     for (int i = 0; i < kGenericMaxDim / 64; ++i)
-        if (lane + 64 * i < D) store_elem(p.out, p.act, rh * D + lane + 64 * i, o[i] / l);
+        if (lane + 64 * i < D) store_out(p.out, p.act, rh * D + lane + 64 * i, o[i] / l);
     if (p.row_ml && lane == 0) p.row_ml[rh] = make_float2(m, l);
 }
 

@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kThreads) chunks_any_kernel(const ChunksK p) {
         for (int c = 0; c < NC; ++c) {
             const int d = threadIdx.x + kThreads * c;
             if (d >= D) continue;
-            if (it.splits == 1) store_elem(p.out, p.act, rh * D + d, acc[i][c] / li);
+            if (it.splits == 1) store_out(p.out, p.act, rh * D + d, acc[i][c] / li);
             else p.part_acc[slot * D + d] = acc[i][c];
         }
         if (threadIdx.x == 0) {

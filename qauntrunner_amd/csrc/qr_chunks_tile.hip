@@ -226,25 +226,42 @@ struct Rows {
         }
     }
 
-    // Merged (m, l) and the row's output or split partial.  by = 1 / l or 1.
-    __device__ __forceinline__ void store4(const ChunksK& p, const ChunkItem& it, int split, int d, const f32x4_t& a, float lsum) const {
+    // The row's output or split partial: N groups of 4 dims from group g0 on, of the weighted sums a.
+    // Group g holds dims 32 (g / 4) + 8 (g % 4) + 4 half .. + 3.
+    template <int N>
+    __device__ __forceinline__ void store(const ChunksK& p, const ChunkItem& it, int split, int g0, float lsum, const f32x4_t (&a)[N]) const {
         if (!on) return;
         const long long rh = static_cast<long long>(it.row0 + query) * p.heads + head;
+        auto dim = [&](int i) { return 32 * ((g0 + i) >> 2) + 8 * ((g0 + i) & 3) + 4 * half; };
         if (it.splits > 1) {
-            const long long slot = it.slot0 + (static_cast<long long>(query) * p.heads + head) * it.splits + split;
-            *reinterpret_cast<f32x4_t*>(p.part_acc + slot * D + d) = a;
+            float* o = p.part_acc + (it.slot0 + (static_cast<long long>(query) * p.heads + head) * it.splits + split) * D;
+#pragma unroll
+            for (int i = 0; i < N; ++i) *reinterpret_cast<f32x4_t*>(o + dim(i)) = a[i];
             return;
         }
         const float inv = 1.f / lsum;
-        if (p.act == QR_DTYPE_F32) {
-            float* o = static_cast<float*>(p.out) + rh * D + d;
+        if (!SPLIT) store16<T>(static_cast<uint16_t*>(p.out) + rh * D, inv, a, dim);
+        else if (p.act == QR_DTYPE_BF16) store16<__bf16>(static_cast<uint16_t*>(p.out) + rh * D, inv, a, dim);
+        else if (p.act == QR_DTYPE_F16) store16<_Float16>(static_cast<uint16_t*>(p.out) + rh * D, inv, a, dim);
+        else {
+            float* o = static_cast<float*>(p.out) + rh * D;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = a[i] * inv;
-        } else {
-            uint16_t b[4];
+            for (int i = 0; i < N; ++i) {
+                const f32x4_t x = a[i] * inv;
+                __builtin_memcpy(o + dim(i), &x, 16);
+            }
+        }
+    }
+    // one store per group, element-aligned
+    template <class O, int N, class G>
+    __device__ static __forceinline__ void store16(uint16_t* o, float inv, const f32x4_t (&a)[N], G dim) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) b[i] = f32_to_bits16(a[i] * inv, p.act);
-            __builtin_memcpy(static_cast<uint16_t*>(p.out) + rh * D + d, b, 8);  // one store, element-aligned
+        for (int i = 0; i < N; ++i) {
+            const f32x4_t x = a[i] * inv;
+            O b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = static_cast<O>(x[j]);
+            __builtin_memcpy(o + dim(i), b, 8);
         }
     }
     __device__ __forceinline__ void store_ml(const ChunksK& p, const ChunkItem& it, int split, float mm, float lsum) const {
@@ -412,12 +429,15 @@ __global__ void __launch_bounds__(64 * RW * PW, 1) chunks_stream_kernel(const Ch
         c[x] = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
         L = fmaf(ml.y, c[x], L);
     }
-    for (int q = pw * (NG / PW); q < (pw + 1) * (NG / PW); ++q) {
-        f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+    constexpr int NP = NG / PW;
+    f32x4_t o[NP];
 #pragma unroll
-        for (int x = 0; x < PW; ++x) a += xa[((x * RW + rw) * NG + q) * 64 + w.lane] * c[x];
-        w.store4(p, it, split, 32 * (q >> 2) + 8 * (q & 3) + 4 * w.half, a, L);
+    for (int q = 0; q < NP; ++q) {
+        o[q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < PW; ++x) o[q] += xa[((x * RW + rw) * NG + pw * NP + q) * 64 + w.lane] * c[x];
     }
+    w.store(p, it, split, pw * NP, L, o);
     if (pw == 0) w.store_ml(p, it, split, M, L);
 }
 
@@ -508,6 +528,9 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
                 }
             } else if (qk) {
                 const int st = j & 1, kk = j >> 1;
+                if (kk == 0)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[st][r] = 0.f;
                 s[st] = mfma32(ring[i % kAhead], w.qh[kk], s[st]);
                 if (SPLIT) s[st] = mfma32(ring[i % kAhead], w.ql[SPLIT ? kk : 0], s[st]);
             }
@@ -517,74 +540,69 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
         }
     };
 
-    const bool late = wave >= 4;  // half a tile behind
-    // tiles that reach past what every row sees
-    auto edge = [&](int i) { return t0 + (i + 1) * TILE > seen || t0 + (i + 1) * TILE > t1; };
-    // both groups come here with tile i after the same barrier, before either weighs its V
-    auto mend_v = [&](int i) __attribute__((always_inline)) {
-        if (!edge(i)) return;
-        char* v = lds + NST * KB + (i % NST) * KB;
-        const bool b0 = w.v_bad(v), b1 = w.v_bad(v + SB);
-        if (!b0 && !b1) return;
-        w.add_bad(v, t0 + i * TILE, t1);
-        w.add_bad(v + SB, t0 + i * TILE + 32, t1);
-        barrier();
-        clear_bad<typename R::T>(v, KB, 512);
-        barrier();
+    auto k_at = [&](int i) { return lds + (i % NST) * KB; };
+    auto v_at = [&](int i) { return lds + NST * KB + (i % NST) * KB; };
+    // K of tile i + 2 over K of tile i - 1, V of tile i + 1 over V of tile i - 2
+    auto request = [&](int i) __attribute__((always_inline)) {
+        dma(i + 2, 0);
+        dma(i + 1, 1);
     };
-    if (ntiles > 0) {
+    // Tiles that every row sees whole.  The early group (waves 0-3) computes scores of tile i and weighs V of tile
+    // i - 1 in half 2i, its softmax of tile i in half 2i + 1; the late group each one half later.  Every wave
+    // makes request(i) at the start of half 2i (the late group read what it replaces for the last time in half
+    // 2i - 1), and awaits it before the barrier that ends half 2i + 3, when request(i + 1) may be in flight.
+    const int nfull = max(0, min(seen, t1) - t0) / TILE;
+    if (nfull > 0) {
+        const bool late = wave >= 4;
         wait_vmcnt<2 * PER>();  // K of tile 0
         barrier();
-        // Before the early group's tile i: K of tile i + 2 goes over K of tile i - 1 and V of tile i + 1 over V of
-        // tile i - 2, which the late group read for the last time before the barrier just passed.  Both
-        // are awaited two barriers later.
-        if (late) {
-            dma(2, 0);
-            dma(1, 1);
-            barrier();
-        }
-        for (int i = 0; i < ntiles; ++i) {
-            if (!late) {
-                dma(i + 2, 0);
-                dma(i + 1, 1);
-                if (i > 0) mend_v(i - 1);
-            }
-#pragma unroll
-            for (int st = 0; st < 2; ++st)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[st][r] = 0.f;
-            const char* kt = lds + (i % NST) * KB;
-            const char* vt = lds + NST * KB + ((i + NST - 1) % NST) * KB;
-            if (i == 0) qk_pv(kt, vt, true, false);
-            else qk_pv(kt, vt, true, true);
-            if (late) wait_vmcnt<2 * PER>();
-            barrier();
-            if (late) {
-                dma(i + 3, 0);
-                dma(i + 2, 1);
-                mend_v(i);
-            }
-            const int ts = t0 + i * TILE;
-            if (edge(i)) {
-                w.mask(s[0], ts, t1);
-                w.mask(s[1], ts + 32, t1);
-            }
+        request(0);
+        if (late) barrier();
+        qk_pv(k_at(0), nullptr, true, false);
+        if (late) wait_vmcnt<2 * PER>();
+        barrier();
+        for (int i = 0; i + 1 < nfull; ++i) {
+            if (late) request(i + 1);
             w.template softmax<2>(s, ph, pl);
             if (!late) wait_vmcnt<2 * PER>();
             barrier();
+            if (!late) request(i + 1);
+            qk_pv(k_at(i + 1), v_at(i), true, true);
+            if (late) wait_vmcnt<2 * PER>();
+            barrier();
         }
-        const char* vt = lds + NST * KB + ((ntiles - 1) % NST) * KB;
-        if (!late) mend_v(ntiles - 1);
-        qk_pv(vt, vt, false, true);
+        w.template softmax<2>(s, ph, pl);
+        if (!late) wait_vmcnt<2 * PER>();
+        barrier();
+        qk_pv(nullptr, v_at(nfull - 1), false, true);
         if (!late) barrier();
     }
+    // The others, masked, all waves together.  K of tiles nfull and nfull + 1 and V of tile nfull are requested.
+    for (int i = nfull; i < ntiles; ++i) {
+        wait_dma();
+        barrier();
+        request(i);
+        char* const v = v_at(i);
+        const bool b0 = w.v_bad(v), b1 = w.v_bad(v + SB);
+        if (b0 || b1) {  // the same in every wave
+            w.add_bad(v, t0 + i * TILE, t1);
+            w.add_bad(v + SB, t0 + i * TILE + 32, t1);
+            barrier();
+            clear_bad<typename R::T>(v, KB, 512);
+            barrier();
+        }
+        qk_pv(k_at(i), nullptr, true, false);
+        w.mask(s[0], t0 + i * TILE, t1);
+        w.mask(s[1], t0 + i * TILE + 32, t1);
+        w.template softmax<2>(s, ph, pl);
+        qk_pv(nullptr, v, false, true);
+    }
     w.l = sum_xor32(w.l);
+    f32x4_t o[4 * R::ND];
 #pragma unroll
-    for (int d = 0; d < R::ND; ++d)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            w.store4(p, it, split, 32 * d + 8 * q + 4 * w.half,
-                     f32x4_t{w.acc[d][4 * q], w.acc[d][4 * q + 1], w.acc[d][4 * q + 2], w.acc[d][4 * q + 3]}, w.l);
+    for (int q = 0; q < 4 * R::ND; ++q)
+        o[q] = f32x4_t{w.acc[q >> 2][4 * (q & 3)], w.acc[q >> 2][4 * (q & 3) + 1], w.acc[q >> 2][4 * (q & 3) + 2], w.acc[q >> 2][4 * (q & 3) + 3]};
+    w.store(p, it, split, 0, w.l, o);
     w.store_ml(p, it, split, w.m, w.l);
 }
 
