@@ -10,6 +10,7 @@ enqueue on torch's current stream.
 from __future__ import annotations
 
 import ctypes
+from array import array
 
 import numpy as np
 
@@ -97,46 +98,59 @@ def _stream_ptr(stream):
 
 
 def _ints(x, what):
-    """A host list of whole numbers as an int32 array (no value is wrapped or rounded)."""
-    a = np.asarray(x)
-    if a.size == 0:
-        return np.zeros(0, np.int32)
-    if a.ndim != 1 or a.dtype.kind not in "iu":
-        raise ValueError(f"{what}: expected a list of whole numbers")
-    if int(a.min()) < -(1 << 31) or int(a.max()) >= 1 << 31:
-        raise ValueError(f"{what}: a number does not fit 32 bits")
-    return np.ascontiguousarray(a, dtype=np.int32)
+    """A host list of whole numbers as a 32-bit array (no value is wrapped or rounded)."""
+    if not isinstance(x, (list, tuple)):
+        x = np.asarray(x)
+        if x.size and (x.ndim != 1 or x.dtype.kind not in "iu"):
+            raise ValueError(f"{what}: expected a list of whole numbers")
+        x = x.ravel().tolist()
+    try:
+        return array("i", x)
+    except (TypeError, OverflowError) as e:
+        raise ValueError(f"{what}: expected whole numbers of 32 bits ({e})") from None
+
+
+def _address(a):
+    return a.buffer_info()[0] if a else None
+
+
+_dtype_codes = {}  # torch dtype -> dtype code
 
 
 def _torch_code(x, what):
-    code = _TORCH_CODES.get(str(getattr(x, "dtype", None)).replace("torch.", ""), -1)
-    if code < 0:
-        raise ValueError(f"{what}: expected a float32, float16 or bfloat16 tensor")
+    dt = getattr(x, "dtype", None)
+    code = _dtype_codes.get(dt)
+    if code is None:
+        code = _TORCH_CODES.get(str(dt).replace("torch.", ""), -1)
+        if code < 0:
+            raise ValueError(f"{what}: expected a float32, float16 or bfloat16 tensor")
+        _dtype_codes[dt] = code
     return code
 
 
 def _on_device(x, device, what):
     if not getattr(x, "is_cuda", False):
         raise ValueError(f"{what}: expected a tensor on the GPU")
-    if x.device.index != device:
-        raise ValueError(f"{what}: the tensor is on device {x.device.index}, the cache on device {device}")
+    if x.get_device() != device:
+        raise ValueError(f"{what}: the tensor is on device {x.get_device()}, the cache on device {device}")
 
 
-def _whole(x, shape, code, device, what):
-    """Address of a contiguous tensor of `shape` (any leading grouping of its elements) and dtype code."""
+def _whole(x, numel, code, device, what):
+    """Addresses [from, to) of a contiguous tensor of `numel` elements and dtype code."""
     _on_device(x, device, what)
     if _torch_code(x, what) != code:
         raise ValueError(f"{what}: dtype {x.dtype} does not match dtype code {code}")
     if not x.is_contiguous():
         raise ValueError(f"{what}: tensor must be contiguous")
-    if x.numel() != int(np.prod(shape, dtype=np.int64)):
-        raise ValueError(f"{what}: expected {' x '.join(map(str, shape))} elements, got {x.numel()}")
-    return ctypes.c_void_p(x.data_ptr())
+    if x.numel() != numel:
+        raise ValueError(f"{what}: expected {numel} elements, got {x.numel()}")
+    p = x.data_ptr()
+    return p, p + numel * (4 if code == _lib.DTYPE_F32 else 2)
 
 
 def _strided(x, rows, width, code, device, what):
-    """(address, elements between rows) of a [rows, width] tensor whose rows are contiguous: a slice of a
-    wider one keeps its stride."""
+    """(addresses [from, to), elements between rows) of a [rows, width] tensor whose rows are contiguous: a slice of
+    a wider one keeps its stride."""
     _on_device(x, device, what)
     if _torch_code(x, what) != code:
         raise ValueError(f"{what}: dtype {x.dtype} does not match the other rows' dtype")
@@ -145,22 +159,15 @@ def _strided(x, rows, width, code, device, what):
     if rows and width > 1 and x.stride(1) != 1:
         raise ValueError(f"{what}: the values of a row must stand next to each other")
     stride = x.stride(0) if rows > 1 else width
-    if rows > 1 and stride < width:
+    if stride < width:
         raise ValueError(f"{what}: rows overlap (stride {stride} for {width} values)")
-    return ctypes.c_void_p(x.data_ptr()), stride
-
-
-def _extent(x):
-    """Addresses [from, to) that a tensor's elements lie in."""
-    if not x.numel():
-        return 0, 0
-    last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
-    return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
+    p = x.data_ptr()
+    size = 4 if code == _lib.DTYPE_F32 else 2
+    return (p, p + ((rows - 1) * stride + width) * size if rows else p), stride
 
 
 def _overlap(x, y):
-    (a, b), (c, d) = _extent(x), _extent(y)
-    return a < d and c < b
+    return x[0] < y[1] and y[0] < x[1]
 
 
 def _stream_of(stream, device):
@@ -168,8 +175,8 @@ def _stream_of(stream, device):
     if stream is None:
         import torch
 
-        return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-    return ctypes.c_void_p(getattr(stream, "cuda_stream", stream))
+        return torch.cuda.current_stream(device).cuda_stream
+    return getattr(stream, "cuda_stream", stream)
 
 
 class PagedKvCache:
@@ -183,6 +190,7 @@ class PagedKvCache:
         check(self._lib.qr_kv_create(ctypes.byref(h), layers, heads, kv_heads, head_dim, max_seq,
                                      dtype_code(kv_dtype), max_batch))
         self._h = h
+        self._device = None
         _lib.track(self)
         self.Layers, self.Heads, self.KvHeads, self.HeadDim = layers, heads, kv_heads, head_dim
         self.MaxSeq, self.MaxBatch = max_seq, max_batch
@@ -419,20 +427,22 @@ class PagedKvCache:
     @property
     def Device(self) -> int:
         """HIP device that the cache lives on."""
-        out = ctypes.c_int()
-        check(self._lib.qr_kv_device(self._h, ctypes.byref(out)))
-        return out.value
+        if self._device is None:
+            out = ctypes.c_int()
+            check(self._lib.qr_kv_device(self._h, ctypes.byref(out)))
+            self._device = out.value
+        return self._device
 
     def _chunks(self, seq_ids, pos0, rows):
         ids, p, n = _ints(seq_ids, "seq_ids"), _ints(pos0, "pos0"), _ints(rows, "rows")
-        if not ids.size == p.size == n.size:
+        if not len(ids) == len(p) == len(n):
             raise ValueError("seq_ids, pos0 and rows must agree")
-        if n.size and int(n.min()) < 0:
+        if n and min(n) < 0:
             raise ValueError("rows: a negative row count")
-        return ids, p, n, int(n.sum(dtype=np.int64))
+        return ids, p, n, sum(n)
 
     def _weights(self, w, device, what):
-        return _whole(w, (self.MaxBatch, self.KvHeads, self.MaxSeq), _lib.DTYPE_F32, device, what)
+        return _whole(w, self.MaxBatch * self.KvHeads * self.MaxSeq, _lib.DTYPE_F32, device, what)
 
     def AppendNormRopeDev(self, layer, seq_ids, pos0, rows, q, k, v, q_out, q_norm, k_norm, eps, theta,
                           rotary_dim=None, rope_pos0=None, stream=None) -> None:
@@ -442,29 +452,26 @@ class PagedKvCache:
         rope_pos0[i] + j (None: pos0[i] + j).  q [rows, heads*head_dim], k and v [rows, kv_heads*head_dim], all of
         one dtype, may be slices of one tensor; q_out (contiguous) takes the queries, q and q_out None: none."""
         ids, p, n, total = self._chunks(seq_ids, pos0, rows)
-        dev, qw = self.Device, self.Heads * self.HeadDim
+        dev, qw, kw = self.Device, self.Heads * self.HeadDim, self.KvDim
         code = _torch_code(k, "k")
-        kp, ks = _strided(k, total, self.KvDim, code, dev, "k")
-        vp, vs = _strided(v, total, self.KvDim, code, dev, "v")
+        ke, ks = _strided(k, total, kw, code, dev, "k")
+        ve, vs = _strided(v, total, kw, code, dev, "v")
         if (q is None) != (q_out is None):
             raise ValueError("q and q_out come together")
-        qp, qs, op = ctypes.c_void_p(), qw, ctypes.c_void_p()
+        qe, qs, oe = (None, None), qw, (None, None)
         if q is not None:
-            qp, qs = _strided(q, total, qw, code, dev, "q")
-            op = _whole(q_out, (total, qw), code, dev, "q_out")
-            same = q_out.data_ptr() == q.data_ptr() and qs == qw
-            if not same and _overlap(q_out, q) or _overlap(q_out, k) or _overlap(q_out, v):
+            qe, qs = _strided(q, total, qw, code, dev, "q")
+            oe = _whole(q_out, total * qw, code, dev, "q_out")
+            if oe != qe and _overlap(oe, qe) or _overlap(oe, ke) or _overlap(oe, ve):
                 raise ValueError("q_out overlaps the rows that are read")
-        norms = [ctypes.c_void_p() if w is None else _whole(w, (self.HeadDim,), _lib.DTYPE_F32, dev, what)
-                 for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm"))]
-        rp = None
-        if rope_pos0 is not None:
-            rp = _ints(rope_pos0, "rope_pos0")
-            if rp.size != ids.size:
-                raise ValueError("rope_pos0 must agree with seq_ids")
+        qn = None if q_norm is None else _whole(q_norm, self.HeadDim, _lib.DTYPE_F32, dev, "q_norm")[0]
+        kn = None if k_norm is None else _whole(k_norm, self.HeadDim, _lib.DTYPE_F32, dev, "k_norm")[0]
+        rp = None if rope_pos0 is None else _ints(rope_pos0, "rope_pos0")
+        if rp is not None and len(rp) != len(ids):
+            raise ValueError("rope_pos0 must agree with seq_ids")
         check(self._lib.qr_kv_append_norm_rope_dev(
-            self._h, ids.size, _ptr(ids), layer, _ptr(p), _ptr(n), None if rp is None else _ptr(rp), qp, qs, kp, ks, vp,
-            vs, code, op, norms[0], norms[1], eps, theta, self.HeadDim if rotary_dim is None else rotary_dim,
+            self._h, len(ids), _address(ids), layer, _address(p), _address(n), _address(rp) if rp else None, qe[0], qs, ke[0], ks,
+            ve[0], vs, code, oe[0], qn, kn, eps, theta, self.HeadDim if rotary_dim is None else rotary_dim,
             _stream_of(stream, dev)))
 
     def AttentionChunksDev(self, layer, seq_ids, pos0, rows, q, out, scale, weights=None, stream=None) -> None:
@@ -475,15 +482,17 @@ class PagedKvCache:
         ids, p, n, total = self._chunks(seq_ids, pos0, rows)
         dev, qw = self.Device, self.Heads * self.HeadDim
         code = _torch_code(q, "q")
-        qp = _whole(q, (total, qw), code, dev, "q")
-        op = _whole(out, (total, qw), code, dev, "out")
-        wp = ctypes.c_void_p()
+        qe = _whole(q, total * qw, code, dev, "q")
+        oe = _whole(out, total * qw, code, dev, "out")
+        we = (None, None)
         if weights is not None:
-            wp = self._weights(weights, dev, "weights")
-        if _overlap(out, q) or weights is not None and (_overlap(weights, q) or _overlap(weights, out)):
-            raise ValueError("out and weights must not overlap each other or q")
-        check(self._lib.qr_kv_attention_chunks_dev(self._h, ids.size, _ptr(ids), layer, _ptr(p), _ptr(n), qp, code, op,
-                                                   wp, scale, _stream_of(stream, dev)))
+            we = self._weights(weights, dev, "weights")
+            if _overlap(we, qe) or _overlap(we, oe):
+                raise ValueError("weights overlap q or out")
+        if _overlap(oe, qe):
+            raise ValueError("out overlaps q")
+        check(self._lib.qr_kv_attention_chunks_dev(self._h, len(ids), _address(ids), layer, _address(p), _address(n), qe[0],
+                                                   code, oe[0], we[0], scale, _stream_of(stream, dev)))
 
     def EvictDev(self, layer, seq_ids, lengths, first, heavy, recent, weights, kept, kept_weights=None, stream=None) -> None:
         """Eviction by accumulated weight: of each sequence's lengths[i] positions every kv head keeps the first
@@ -491,35 +500,37 @@ class PagedKvCache:
         (int32 [n, kv_heads, first+heavy+recent]) takes the positions kept (-1 past the length), kept_weights (None:
         weights itself) their weights and zeros up to the length.  Truncate when every layer is done."""
         ids, ln = _ints(seq_ids, "seq_ids"), _ints(lengths, "lengths")
-        if ids.size != ln.size:
+        if len(ids) != len(ln):
             raise ValueError("seq_ids and lengths must agree")
         dev = self.Device
-        wp = self._weights(weights, dev, "weights")
-        op = wp
+        we = self._weights(weights, dev, "weights")
+        oe = we
         if kept_weights is not None:
-            op = self._weights(kept_weights, dev, "kept_weights")
-            if kept_weights.data_ptr() != weights.data_ptr() and _overlap(weights, kept_weights):
+            oe = self._weights(kept_weights, dev, "kept_weights")
+            if oe != we and _overlap(oe, we):
                 raise ValueError("kept_weights overlaps weights")
         keep = first + heavy + recent
         if min(first, heavy, recent) < 0:
             raise ValueError("negative budget")
         _on_device(kept, dev, "kept")
-        if str(kept.dtype) != "torch.int32" or not kept.is_contiguous() or kept.numel() != ids.size * self.KvHeads * keep:
-            raise ValueError(f"kept: expected a contiguous int32 tensor of {ids.size} x {self.KvHeads} x {keep} elements")
-        if _overlap(kept, weights) or kept_weights is not None and _overlap(kept, kept_weights):
+        if str(kept.dtype) != "torch.int32" or not kept.is_contiguous() or kept.numel() != len(ids) * self.KvHeads * keep:
+            raise ValueError(f"kept: expected a contiguous int32 tensor of {len(ids)} x {self.KvHeads} x {keep} elements")
+        pe = (kept.data_ptr(), kept.data_ptr() + 4 * kept.numel())
+        if _overlap(pe, we) or _overlap(pe, oe):
             raise ValueError("kept overlaps the weights")
-        check(self._lib.qr_kv_evict_dev(self._h, ids.size, _ptr(ids), layer, _ptr(ln), first, heavy, recent, wp, op,
-                                        ctypes.c_void_p(kept.data_ptr()), _stream_of(stream, dev)))
+        check(self._lib.qr_kv_evict_dev(self._h, len(ids), _address(ids), layer, _address(ln), first, heavy, recent, we[0],
+                                        oe[0], pe[0], _stream_of(stream, dev)))
 
     def ReadDev(self, layer, seq_ids, pos0, rows, k_out, v_out, stream=None) -> None:
         """The chunks' cache rows as [rows, kv_dim] tensors of the cache's dtype (Read without the host)."""
         ids, p, n, total = self._chunks(seq_ids, pos0, rows)
         dev = self.Device
-        kp = _whole(k_out, (total, self.KvDim), self.KvDtype, dev, "k_out")
-        vp = _whole(v_out, (total, self.KvDim), self.KvDtype, dev, "v_out")
-        if _overlap(k_out, v_out):
+        ke = _whole(k_out, total * self.KvDim, self.KvDtype, dev, "k_out")
+        ve = _whole(v_out, total * self.KvDim, self.KvDtype, dev, "v_out")
+        if _overlap(ke, ve):
             raise ValueError("k_out and v_out overlap")
-        check(self._lib.qr_kv_read_dev(self._h, ids.size, _ptr(ids), layer, _ptr(p), _ptr(n), kp, vp, _stream_of(stream, dev)))
+        check(self._lib.qr_kv_read_dev(self._h, len(ids), _address(ids), layer, _address(p), _address(n), ke[0], ve[0],
+                                       _stream_of(stream, dev)))
 
     # ---- debug copy-out
     def Read(self, layer, pos0, n, seq_id=0):

@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) chunks_f32_weights_kern
     constexpr int EPC = Gm::EPC, NJ = Gm::NJ, NW = EPC / 4;  // fp32 16-byte chunks per cache chunk
     constexpr int QB = NJ * NW * 1024;                       // bytes of 16 rows
     __shared__ __attribute__((aligned(1024))) char lds[2][QB];
+    __shared__ float4 info[2][16];                           // of the rows: maximum, 1 / sum, last position seen
     const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
     const ChunkItem it = p.it[e];
     const int u = blockIdx.x - it.unit0;
@@ -83,7 +84,13 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) chunks_f32_weights_kern
     // a thread's share of 16 rows: fp32 chunks n = threadIdx.x + 256 c, of which lane n % 64's j = n / 64
     constexpr int CH = NJ * NW * 64, SHARE = (CH + 255) / 256;
     f32x4_t x[SHARE];
+    float4 inf;
     auto fetch = [&](int r) __attribute__((always_inline)) {
+        if (threadIdx.x < 16) {
+            const int rho = r + static_cast<int>(threadIdx.x), rr = rho < r1 ? rho : rows - 1, query = rr / g;
+            const float2 ml = p.row_ml[static_cast<long long>(it.row0 + query) * p.heads + kvh * g + rr - query * g];
+            inf = make_float4(ml.x, 1.f / ml.y, __int_as_float(rho < r1 ? it.pos0 + query : -1), 0.f);
+        }
 #pragma unroll
         for (int c = 0; c < SHARE; ++c) {
             const int n = threadIdx.x + 256 * c, ln = n & 63, jw = n >> 6;
@@ -91,30 +98,34 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) chunks_f32_weights_kern
             const int rho = min(r + (ln & 15), rows - 1);
             const long long row = static_cast<long long>(it.row0 + rho / g) * p.heads + kvh * g + rho % g;
             const long long at = row * D + (4 * (jw / NW) + (ln >> 4)) * EPC + 4 * (jw % NW);
+            if (p.act == QR_DTYPE_F32) {
+                __builtin_memcpy(&x[c], static_cast<const float*>(p.q) + at, 16);
+            } else {
+                uint16_t h[4];
+                __builtin_memcpy(h, static_cast<const uint16_t*>(p.q) + at, 8);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[c][i] = load_elem(p.q, p.act, at + i) * p.qscale;
+                for (int i = 0; i < 4; ++i) x[c][i] = p.act == QR_DTYPE_BF16 ? bf16_bits_to_f32(h[i]) : f16_bits_to_f32(h[i]);
+            }
         }
     };
-    auto put = [&](char* to) __attribute__((always_inline)) {
+    auto put = [&](int b) __attribute__((always_inline)) {
+        char* const to = lds[b];
+        if (threadIdx.x < 16) info[b][threadIdx.x] = inf;
 #pragma unroll
         for (int c = 0; c < SHARE; ++c)
-            if (CH % 256 == 0 || threadIdx.x + 256 * c < CH) *reinterpret_cast<f32x4_t*>(to + 16 * (threadIdx.x + 256 * c)) = x[c];
+            if (CH % 256 == 0 || threadIdx.x + 256 * c < CH) *reinterpret_cast<f32x4_t*>(to + 16 * (threadIdx.x + 256 * c)) = x[c] * p.qscale;
     };
     float sum[2][4] = {};
     if (r0 < r1) {
         fetch(r0);
-        put(lds[0]);
+        put(0);
     }
     int at = 0;
     for (int r = r0; r < r1; r += 16, at ^= 1) {
         __syncthreads();
         const bool more = r + 16 < r1;
         if (more) fetch(r + 16);
-        const int rho = r + l16;
-        const bool on = rho < r1;
-        const int rr = on ? rho : rows - 1, query = rr / g;
-        const float2 ml = p.row_ml[static_cast<long long>(it.row0 + query) * p.heads + kvh * g + rr - query * g];
-        const float inv = 1.f / ml.y;
+        const float4 f = info[at][l16];
         f32x4_t s[2][2] = {};
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -131,13 +142,13 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) chunks_f32_weights_kern
                 for (int mt = 0; mt < 2; ++mt)
                     s[mt][j & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[mt][j][i], q[i], s[mt][j & 1], 0, 0, 0);
         }
-        const int last = on ? it.pos0 + query - t0 - 4 * q4 : -1;  // of this lane's positions, the last the row sees
+        const int last = __float_as_int(f.z) - t0 - 4 * q4;  // of this lane's positions, the last the row sees
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (16 * mt + i <= last) sum[mt][i] = fmaf(fast_exp2(s[mt][0][i] + s[mt][1][i] - ml.x), inv, sum[mt][i]);
-        if (more) put(lds[at ^ 1]);
+                if (16 * mt + i <= last) sum[mt][i] = fmaf(fast_exp2(s[mt][0][i] + s[mt][1][i] - f.x), f.y, sum[mt][i]);
+        if (more) put(at ^ 1);
     }
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)

@@ -148,9 +148,10 @@ struct Rows {
             if (16 * (r >> 3) + (r & 7) > last) s[r] = -INFINITY;
     }
 
-    // Weights of NS steps' scores, as PV operands; rescales what was summed when the maximum moves.
-    template <int NS>
-    __device__ __forceinline__ void softmax(const f32x16_t (&s)[NS], vec8 (&ph)[NS][2], vec8 (&pl)[SPLIT ? NS : 1][2]) {
+    // Weights of NS steps' scores, as PV operands; rescales what was summed when the maximum moves.  `step(k)` is
+    // called after every eighth weight, k = 0 .. 2 NS - 1.
+    template <int NS, class F>
+    __device__ __forceinline__ void softmax(const f32x16_t (&s)[NS], vec8 (&ph)[NS][2], vec8 (&pl)[SPLIT ? NS : 1][2], F step) {
         float mx[2 * NS];
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
@@ -187,6 +188,7 @@ struct Rows {
                 const T hi = static_cast<T>(e);
                 ph[n][r >> 3][r & 7] = hi;
                 if (SPLIT) pl[n][r >> 3][r & 7] = static_cast<T>(e - static_cast<float>(hi));
+                if ((r & 7) == 7) step(2 * n + (r >> 3));
             }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
@@ -396,7 +398,7 @@ __global__ void __launch_bounds__(64 * RW * PW, 1) chunks_stream_kernel(const Ch
                 }
         }
         vec8 ph[1][2], pl[1][2];
-        w.template softmax<1>(s, ph, pl);
+        w.template softmax<1>(s, ph, pl, [](int) {});
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -476,15 +478,20 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
     const long long page_bytes = p.geom.page_elems() * 2, plane_bytes = p.geom.plane_elems() * 2;
     const long long head_bytes = static_cast<long long>(kvh) * kPageTokens * D * 2;
     const uint32_t lane16 = 16 * (threadIdx.x & 63);
-    auto dma = [&](int i, int plane) {
+    auto source = [&](int i, int plane) {
         const bool in = i < ntiles;  // past the last tile: no records, no memory is read
         const int t = t0 + min(i, ntiles - 1) * TILE;
         const char* base = p.pool + static_cast<long long>(page_of(p, it.pt_off, t)) * page_bytes + head_bytes + plane * plane_bytes +
                            static_cast<long long>(t & (kPageTokens - 1)) * D * 2;
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, in ? KB : 0, kBufferFlags);
-        char* dst = lds + plane * NST * KB + (i % NST) * KB;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, in ? KB : 0, kBufferFlags);
+    };
+    auto load = [&](__amdgpu_buffer_rsrc_t r, int i, int plane, int c) {
+        buffer_load_lds16(r, lds + plane * NST * KB + (i % NST) * KB + 1024 * (wave + 8 * c), lane16, 1024 * (wave + 8 * c));
+    };
+    auto dma = [&](int i, int plane) {
+        const __amdgpu_buffer_rsrc_t r = source(i, plane);
 #pragma unroll
-        for (int c = 0; c < PER; ++c) buffer_load_lds16(r, dst + 1024 * (wave + 8 * c), lane16, 1024 * (wave + 8 * c));
+        for (int c = 0; c < PER; ++c) load(r, i, plane, c);
     };
     R w;
     w.init(p, it, kvh, g, rho0 + 32 * wave);
@@ -549,29 +556,45 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
     };
     // Tiles that every row sees whole.  The early group (waves 0-3) computes scores of tile i and weighs V of tile
     // i - 1 in half 2i, its softmax of tile i in half 2i + 1; the late group each one half later.  Every wave
-    // makes request(i) at the start of half 2i (the late group read what it replaces for the last time in half
-    // 2i - 1), and awaits it before the barrier that ends half 2i + 3, when request(i + 1) may be in flight.
+    // makes request(i) during its softmax, the early group in half 2i + 1, the late group in half 2i (it read what that
+    // replaces for the last time in half 2i - 1), and awaits it before the barrier that ends half 2i + 3, when
+    // the next request may be in flight.  The loads stand between the exponentials: a load takes its wave some
+    // hundred cycles to issue when eight waves issue at once, which delayed the MFMAs (271 us a call against 214
+    // without any; 2048 queries after 6144 positions).
     const int nfull = max(0, min(seen, t1) - t0) / TILE;
     if (nfull > 0) {
         const bool late = wave >= 4;
+        auto weigh = [&](int i) __attribute__((always_inline)) {  // with request(i)
+            if (SPLIT) {  // (no registers for both)
+                request(i);
+                w.template softmax<2>(s, ph, pl, [](int) {});
+                return;
+            }
+            const __amdgpu_buffer_rsrc_t rk = source(i + 2, 0), rv = source(i + 1, 1);
+            w.template softmax<2>(s, ph, pl, [&](int c) __attribute__((always_inline)) {
+                if (c < PER) load(rk, i + 2, 0, c);
+                else if (c < 2 * PER) load(rv, i + 1, 1, c - PER);
+            });
+        };
         wait_vmcnt<2 * PER>();  // K of tile 0
         barrier();
-        request(0);
-        if (late) barrier();
+        if (late) {
+            request(0);
+            barrier();
+        }
         qk_pv(k_at(0), nullptr, true, false);
         if (late) wait_vmcnt<2 * PER>();
         barrier();
         for (int i = 0; i + 1 < nfull; ++i) {
-            if (late) request(i + 1);
-            w.template softmax<2>(s, ph, pl);
+            weigh(late ? i + 1 : i);
             if (!late) wait_vmcnt<2 * PER>();
             barrier();
-            if (!late) request(i + 1);
             qk_pv(k_at(i + 1), v_at(i), true, true);
             if (late) wait_vmcnt<2 * PER>();
             barrier();
         }
-        w.template softmax<2>(s, ph, pl);
+        if (late) w.template softmax<2>(s, ph, pl, [](int) {});
+        else weigh(nfull - 1);
         if (!late) wait_vmcnt<2 * PER>();
         barrier();
         qk_pv(nullptr, v_at(nfull - 1), false, true);
@@ -594,7 +617,7 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
         qk_pv(k_at(i), nullptr, true, false);
         w.mask(s[0], t0 + i * TILE, t1);
         w.mask(s[1], t0 + i * TILE + 32, t1);
-        w.template softmax<2>(s, ph, pl);
+        w.template softmax<2>(s, ph, pl, [](int) {});
         qk_pv(nullptr, v, false, true);
     }
     w.l = sum_xor32(w.l);
@@ -609,16 +632,18 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
 
 // ------------------------------------------------------------------ weights
 // Weights of 256 positions of one kv head over a part of its rows: a wave keeps the K rows of 32
-// positions as operands and takes the rows 32 at a time from LDS, where each wave puts one k-step's operand of them.
-// Bound by the exponentials (16 cycles per 64 of them, against 16 for the MFMAs of as many scores).
+// positions as operands; the workgroup puts 128 rows at a time into LDS as operands (each wave its share of the
+// k-steps), with each row's maximum, 1 / sum, last position seen and score scale.  Bound by the exponentials (16 cycles
+// per 64 of them, 8 for the multiply-adds around each, 16 for the MFMAs of as many scores beside them).
 template <bool BF16, int D, bool SPLIT>
-__global__ void __launch_bounds__(512, 1) chunks_tile_weights_kernel(const ChunksK p) {
+__global__ void __launch_bounds__(512, SPLIT && D == 128 ? 1 : 2) chunks_tile_weights_kernel(const ChunksK p) {
     using T = typename Elem<BF16>::T;
     using vec8 = typename Elem<BF16>::vec8;
-    constexpr int NK = D / 16;
-    constexpr int RT = 8 / NK;           // 32-row tiles of a round: one operand per wave
-    constexpr int PART = SPLIT ? 2 : 1;
-    __shared__ __attribute__((aligned(1024))) char lds[2][PART * 8 * 1024];
+    constexpr int NK = D / 16, RT = 4, ROWS = 32 * RT;
+    constexpr int CN = NK * RT / 8;          // operands per wave of a round
+    constexpr int PART = SPLIT ? 2 : 1, QB = NK * RT * 1024;
+    __shared__ __attribute__((aligned(1024))) char lds[2][PART * QB];
+    __shared__ float4 info[2][ROWS];
     const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
     const ChunkItem it = p.it[e];
     const int u = blockIdx.x - it.unit0;
@@ -630,78 +655,99 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_weights_kernel(const Chunk
     const int b0 = block * 256, t0 = b0 + 32 * wave;
     // rows that see part of the block, in rounds dealt to the splits
     const int first = max(0, b0 - it.pos0) * g;
-    const int rounds = (rows - first + 32 * RT - 1) / (32 * RT);
-    const int r0 = first + static_cast<int>(static_cast<long long>(rounds) * split / it.splits) * 32 * RT;
-    const int r1 = min(rows, first + static_cast<int>(static_cast<long long>(rounds) * (split + 1) / it.splits) * 32 * RT);
+    const int rounds = (rows - first + ROWS - 1) / ROWS;
+    const int r0 = first + static_cast<int>(static_cast<long long>(rounds) * split / it.splits) * ROWS;
+    const int r1 = min(rows, first + static_cast<int>(static_cast<long long>(rounds) * (split + 1) / it.splits) * ROWS);
+    const float sign = p.qscale == 0.f ? 0.f : p.qscale < 0.f ? -1.f : 1.f;
+    const float base = p.qscale == 0.f ? 1.f : fabsf(p.qscale);
+    auto row_of = [&](int rho) { return static_cast<long long>(it.row0 + rho / g) * p.heads + kvh * g + rho % g; };
 
+    // a round's share of this thread: operand wave + 8 c is k-step op % NK of row tile op / NK
+    float x[SPLIT ? CN : 1][8];
+    vec8 raw[SPLIT ? 1 : CN];
+    float4 inf;
+    auto fetch = [&](int r) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < CN; ++c) {
+            const int op = wave + 8 * c;
+            const long long row = row_of(min(r + 32 * (op / NK) + n, rows - 1));
+            const long long at = row * D + 16 * (op % NK) + 8 * half;
+            if (!SPLIT) {
+                __builtin_memcpy(&raw[SPLIT ? 0 : c], static_cast<const uint16_t*>(p.q) + at, 16);
+            } else if (p.act == QR_DTYPE_F32) {
+                __builtin_memcpy(x[SPLIT ? c : 0], static_cast<const float*>(p.q) + at, 32);
+            } else {
+                uint16_t h[8];
+                __builtin_memcpy(h, static_cast<const uint16_t*>(p.q) + at, 16);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[SPLIT ? c : 0][i] = p.act == QR_DTYPE_BF16 ? bf16_bits_to_f32(h[i]) : f16_bits_to_f32(h[i]);
+            }
+            if (SPLIT && p.row_scale) {  // a power of two
+                const float by = base / p.row_scale[row];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[SPLIT ? c : 0][i] *= by;
+            }
+        }
+        if (threadIdx.x < ROWS) {
+            const int rho = r + static_cast<int>(threadIdx.x);
+            const bool on = rho < r1;
+            const long long row = row_of(on ? rho : rows - 1);
+            const float2 ml = p.row_ml[row];
+            inf = make_float4(-ml.x, 1.f / ml.y, __int_as_float(on ? it.pos0 + rho / g : -1), p.row_scale ? p.row_scale[row] : base);
+        }
+    };
+    auto put = [&](int to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < CN; ++c) {
+            char* o = lds[to] + 1024 * (wave + 8 * c) + 16 * lane;
+            vec8 hi, lo;
+            if (!SPLIT) {
+                hi = raw[SPLIT ? 0 : c];
+                if (p.qscale <= 0.f)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) hi[i] = static_cast<T>(static_cast<float>(hi[i]) * sign);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = x[SPLIT ? c : 0][i] * sign;
+                    hi[i] = static_cast<T>(v);
+                    lo[i] = static_cast<T>(v - static_cast<float>(hi[i]));
+                }
+                *reinterpret_cast<vec8*>(o + QB) = lo;
+            }
+            *reinterpret_cast<vec8*>(o) = hi;
+        }
+        if (threadIdx.x < ROWS) info[to][threadIdx.x] = inf;
+    };
+    if (r0 < r1) fetch(r0);
     vec8 k[NK];
     {
         const int s = n >> 4, a = (n >> 3) & 1, h = (n >> 2) & 1, b = n & 3;
         const int off = 1024 * a * (D / 32) + 16 * (16 * half + 4 * (2 * s + h) + b);
-        const long long phys = t0 < len ? page_of(p, it.pt_off, t0) : 0;
+        const bool in = t0 < len;  // a block's steps past the end hold no page
+        const long long phys = in ? page_of(p, it.pt_off, t0) : 0;
         const char* src = p.pool + (phys * p.geom.page_elems() + static_cast<long long>(kvh) * kPageTokens * D +
                                     static_cast<long long>(t0 & (kPageTokens - 1)) * D) * 2 + off;
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) {
-            if (t0 < len) k[kk] = *reinterpret_cast<const vec8*>(src + 512 * kk);
-            else
 #pragma unroll
-                for (int i = 0; i < 8; ++i) k[kk][i] = static_cast<T>(0.f);
+            for (int i = 0; i < 8; ++i) k[kk][i] = static_cast<T>(0.f);
+            if (in) k[kk] = *reinterpret_cast<const vec8*>(src + 512 * kk);
         }
     }
-    const float sign = p.qscale == 0.f ? 0.f : p.qscale < 0.f ? -1.f : 1.f;
-    const float base = p.qscale == 0.f ? 1.f : fabsf(p.qscale);
-    // this wave's operand of a round: k-step wave % NK of row tile wave / NK
-    float x[8];
-    float scale_x = 1.f;
-    auto fetch = [&](int r) __attribute__((always_inline)) {
-        const int rho = min(r + 32 * (wave / NK) + n, rows - 1);
-        const long long row = static_cast<long long>(it.row0 + rho / g) * p.heads + kvh * g + rho % g;
-        const long long at = row * D + 16 * (wave % NK) + 8 * half;
-        if (p.act == QR_DTYPE_F32) {
-            const float* f = static_cast<const float*>(p.q) + at;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = f[i];
-        } else {
-            const uint16_t* f = static_cast<const uint16_t*>(p.q) + at;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = p.act == QR_DTYPE_BF16 ? bf16_bits_to_f32(f[i]) : f16_bits_to_f32(f[i]);
-        }
-        scale_x = p.row_scale ? base / p.row_scale[row] : 1.f;  // a power of two
-    };
-    auto put = [&](char* to) __attribute__((always_inline)) {
-        vec8 hi, lo;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float v = x[i] * (sign * scale_x);
-            hi[i] = static_cast<T>(v);
-            lo[i] = static_cast<T>(v - static_cast<float>(hi[i]));
-        }
-        *reinterpret_cast<vec8*>(to + 1024 * wave + 16 * lane) = hi;
-        if (SPLIT) *reinterpret_cast<vec8*>(to + 8192 + 1024 * wave + 16 * lane) = lo;
-    };
     float sum[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) sum[r] = 0.f;
-    if (r0 < r1) {
-        fetch(r0);
-        put(lds[0]);
-    }
+    if (r0 < r1) put(0);
     int at = 0;
-    for (int r = r0; r < r1; r += 32 * RT, at ^= 1) {
+    for (int r = r0; r < r1; r += ROWS, at ^= 1) {
         __syncthreads();
-        const bool more = r + 32 * RT < r1;
-        if (more) fetch(r + 32 * RT);
+        const bool more = r + ROWS < r1;
+        if (more) fetch(r + ROWS);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const int rho = r + 32 * rt + n;
-            const bool on = rho < r1;
-            const int rr = on ? rho : rows - 1;
-            const int query = rr / g;
-            const long long rh = static_cast<long long>(it.row0 + query) * p.heads + kvh * g + rr - query * g;
-            const float2 ml = p.row_ml[rh];
-            const float sscale = p.row_scale ? p.row_scale[rh] : base;
-            const float inv = on ? 1.f / ml.y : 0.f;
+            if (r + 32 * rt >= r1) break;
+            const float4 f = info[at][32 * rt + n];
             f32x16_t s;
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = 0.f;
@@ -709,20 +755,20 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_weights_kernel(const Chunk
             for (int kk = 0; kk < NK; ++kk) {
                 const char* q = lds[at] + 1024 * (rt * NK + kk) + 16 * lane;
                 s = mfma32(k[kk], *reinterpret_cast<const vec8*>(q), s);
-                if (SPLIT) s = mfma32(k[kk], *reinterpret_cast<const vec8*>(q + 8192), s);
+                if (SPLIT) s = mfma32(k[kk], *reinterpret_cast<const vec8*>(q + QB), s);
             }
-            // rows of this tile that do not see every position of the wave's, or stand past the end
-            const int last = on ? it.pos0 + query - t0 - 8 * half : -1;
+            // rows that do not see every position of the wave's, or stand past the end
+            const int last = __float_as_int(f.z) - t0 - 8 * half;
             if (__builtin_amdgcn_ballot_w64(last < 24)) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (16 * (i >> 3) + (i & 7) <= last) sum[i] = fmaf(fast_exp2(fmaf(s[i], sscale, -ml.x)), inv, sum[i]);
+                    if (16 * (i >> 3) + (i & 7) <= last) sum[i] = fmaf(fast_exp2(fmaf(s[i], f.w, f.x)), f.y, sum[i]);
             } else {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sum[i] = fmaf(fast_exp2(fmaf(s[i], sscale, -ml.x)), inv, sum[i]);
+                for (int i = 0; i < 16; ++i) sum[i] = fmaf(fast_exp2(fmaf(s[i], f.w, f.x)), f.y, sum[i]);
             }
         }
-        if (more) put(lds[at ^ 1]);
+        if (more) put(at ^ 1);
     }
     // over the 32 lanes of a half
 #pragma unroll
