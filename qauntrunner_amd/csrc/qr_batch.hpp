@@ -102,7 +102,7 @@ struct ChunkItem {
     int splits;              // parts of each block's keys (weights: rows)
     int slot0;               // first split partial: (row * heads + head) * splits + split from here
     int pad;
-    long long score0;        // first score: (row * heads + head) * chunk_score_len from here
+    long long score0;        // first score: (row * heads + head) * chunk_score_len from here; -1: none are kept
 };
 struct ChunksArgs {
     ChunkItem it[kBatch];

@@ -131,7 +131,7 @@ struct KindGeom {
     int rows, tile;   // of a workgroup
     long long want;   // units that fill the GPU
 };
-constexpr KindGeom kGeom[kChunkKinds] = {{kChunkAnyRows, kChunkAnyTile, 1024}, {32, 128, 256}, {64, 128, 256}, {128, 64, 256}, {256, 64, 256}, {32, 32, 256}, {64, 32, 256}};
+constexpr KindGeom kGeom[kChunkKinds] = {{kChunkAnyRows, kChunkAnyTile, 1024}, {32, 128, 256}, {128, 128, 256}, {256, 64, 256}, {32, 32, 256}, {64, 32, 256}};
 
 int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
@@ -150,16 +150,17 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
             pl.it[i].blocks = cdiv(a.it[i].rows, kGeom[pl.it[i].kind].rows / gmax);
             continue;
         }
-        pl.it[i].kind = !tiles ? kChunkAny : rows <= 32 ? kChunkStream32 : rows <= 64 ? kChunkStream64 : rows <= 128 ? kChunkStream128 : kChunkTile;
+        pl.it[i].kind = !tiles ? kChunkAny : rows <= 32 ? kChunkStream32 : rows <= 128 ? kChunkStream : kChunkTile;
         pl.it[i].blocks = cdiv(rows, kGeom[pl.it[i].kind].rows);
     }
-    // Both of the two wider streaming kinds together: one launch, the wider
-    bool wide = false;
-    for (int i = 0; i < a.n; ++i) wide |= pl.it[i].kind == kChunkStream128;
-    for (int i = 0; i < a.n; ++i)
-        if (wide && pl.it[i].kind == kChunkStream64) pl.it[i].kind = kChunkStream128;
-    // The keys of a kind's blocks are split while its units do not fill the GPU: as many positions
-    // per unit as leave no more units than that, or one tile.
+    // The keys of a kind's blocks are split while its units do not fill the GPU: as many tiles per unit as leave
+    // no more units than that, or one.  (Every tile of a kind takes about the same time: kChunkStream's are of 64 positions
+    // for more than 64 rows, else of 128.)
+    auto tiles_of = [&](int i) {
+        int tile = kGeom[pl.it[i].kind].tile;
+        if (pl.it[i].kind == kChunkStream && static_cast<long long>(a.it[i].rows) * gmax > 64) tile = 64;
+        return cdiv(a.it[i].pos0 + a.it[i].rows, tile);
+    };
     long long slots = 0;
     for (int kind = 0; kind < kChunkKinds; ++kind) {
         KindGeom g = kGeom[kind];
@@ -168,23 +169,22 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
         for (int i = 0; i < a.n; ++i)
             if (pl.it[i].kind == kind) {
                 base += static_cast<long long>(pl.it[i].blocks) * kv;
-                work += static_cast<long long>(pl.it[i].blocks) * kv * cdiv(a.it[i].pos0 + a.it[i].rows, g.tile);
+                work += static_cast<long long>(pl.it[i].blocks) * kv * tiles_of(i);
             }
         if (!base) continue;
         long long per = base >= g.want ? 1LL << 40 : std::max<long long>(1, work / g.want);  // tiles of a unit
         auto units = [&](long long per_) {
             long long u = 0;
             for (int i = 0; i < a.n; ++i)
-                if (pl.it[i].kind == kind)
-                    u += static_cast<long long>(pl.it[i].blocks) * kv * cdiv(cdiv(a.it[i].pos0 + a.it[i].rows, g.tile), per_);
+                if (pl.it[i].kind == kind) u += static_cast<long long>(pl.it[i].blocks) * kv * cdiv(tiles_of(i), per_);
             return u;
         };
         if (base < g.want)
-            while (units(per) > g.want && per < (1 << 24)) per += std::max<long long>(1, per / 16);
+            while (units(per) > g.want && per < (1 << 24)) per += std::max<long long>(1, per / 64);
         for (int i = 0; i < a.n; ++i) {
             ChunkPlanItem& it = pl.it[i];
             if (it.kind != kind) continue;
-            it.splits = std::min(cdiv(cdiv(a.it[i].pos0 + a.it[i].rows, g.tile), per), 256);
+            it.splits = std::min(cdiv(tiles_of(i), per), 256);
             it.slot0 = slots;
             if (it.splits > 1) {
                 slots += static_cast<long long>(a.it[i].rows) * a.heads * it.splits;
@@ -201,6 +201,7 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
                      : it.kind == kChunkF32 ? kWeightsF32 : kWeightsTile;
             it.wblocks = cdiv(a.it[i].pos0 + a.it[i].rows, it.wkind == kWeightsAny ? kChunkAnyTile : it.wkind == kWeightsF32 ? 128 : 256);
             it.wsplits = 1;
+            it.score0 = -1;
             if (it.wkind >= kWeightsTile) units += static_cast<long long>(it.wblocks) * kv;
             if (it.wkind == kWeightsScores) {
                 it.score0 = scores;

@@ -8,12 +8,14 @@
 namespace qr {
 
 // Kernels of a launch; rows (query, query head pairs of a kv head) of a workgroup, positions of a tile.
-enum ChunkKind { kChunkAny, kChunkStream32, kChunkStream64, kChunkStream128, kChunkTile, kChunkF32Half, kChunkF32, kChunkKinds };
+enum ChunkKind { kChunkAny, kChunkStream32, kChunkStream, kChunkTile, kChunkF32Half, kChunkF32, kChunkKinds };
 // The passes after the attention that add up the weights.
 enum ChunkWeights { kWeightsAny, kWeightsScores, kWeightsTile, kWeightsF32, kWeightsKinds };
 
 constexpr int kChunkAnyRows = 8, kChunkAnyTile = 32;
-
+// Parts of the cache's 16-bit type that the streaming kernel takes a query value and a weight as: queries of another type
+// keep 24 bits in three of bf16, 22 in two of fp16.
+constexpr int chunk_parts(int cache, bool other) { return !other ? 1 : cache == QR_DTYPE_BF16 ? 3 : 2; }
 struct ChunksK {
     ChunkItem it[kBatch];
     int n;
@@ -56,7 +58,7 @@ __host__ __device__ inline int chunk_score_len(const ChunkItem& it) { return (it
 
 hipError_t launch_chunks_any(const ChunksK& k, hipStream_t s);
 hipError_t launch_chunks_any_weights(const ChunksK& k, hipStream_t s);
-// 16-bit caches in the MFMA page layout, whole groups: kinds kChunkStream32 .. kChunkTile; kChunkKinds:
+// 16-bit caches in the MFMA page layout, whole groups: kinds kChunkStream32 (up to 32 rows), kChunkStream (up to 128), kChunkTile; kChunkKinds:
 // the weights pass.
 hipError_t launch_chunks_tile(const ChunksK& k, int kind, hipStream_t s);
 // fp32 tiles: kinds kChunkF32Half (32 rows), kChunkF32 (64 rows); kChunkKinds: the weights pass.

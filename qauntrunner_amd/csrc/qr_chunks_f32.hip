@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(256, (F32Geom<ST, D>::wg_per_cu(PG))) chunks_f
     k.queries_per_block = 64 / PG / k.group;
     k.splits = it.splits;
     k.row_ml = p.row_ml ? p.row_ml + row0 : nullptr;
-    k.scores = p.scores ? p.scores + it.score0 : nullptr;
+    k.scores = p.scores && it.score0 >= 0 ? p.scores + it.score0 : nullptr;
     k.score_len = chunk_score_len(it);
     chunk_f32_tiles<ST, D, PG, true>(k, u % it.splits, it.blocks - 1 - u / it.splits % it.blocks, u / (it.splits * it.blocks), lds);
 }

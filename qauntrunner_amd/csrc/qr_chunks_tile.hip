@@ -46,9 +46,10 @@ template <bool BF16> struct Elem {
     typedef T vec8 __attribute__((ext_vector_type(8)));
 };
 
-// One wave's 32 rows.
-template <bool BF16, int D, bool SPLIT>
+// One wave's 32 rows.  PARTS of the cache's type that a query value and a weight enter as.
+template <bool BF16, int D, int PARTS>
 struct Rows {
+    static constexpr bool SPLIT = PARTS > 1;
     using T = typename Elem<BF16>::T;
     using vec8 = typename Elem<BF16>::vec8;
     static constexpr int NK = D / 16;   // QK k-steps
@@ -59,7 +60,7 @@ struct Rows {
     int query, head;     // of row lane % 32
     bool on;
     int lim;             // last position the row sees
-    vec8 qh[NK], ql[SPLIT ? NK : 1];
+    vec8 q[PARTS][NK];
     float sscale;        // log2 units per score
     float m, l;          // l: this lane's half of the positions
     f32x16_t acc[ND];
@@ -126,9 +127,12 @@ struct Rows {
         for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float v = x[kk][i] * by;
-                qh[kk][i] = static_cast<T>(v);
-                if (SPLIT) ql[kk][i] = static_cast<T>(v - static_cast<float>(qh[kk][i]));
+                float v = x[kk][i] * by;
+#pragma unroll
+                for (int c = 0; c < PARTS; ++c) {
+                    q[c][kk][i] = static_cast<T>(v);
+                    v -= static_cast<float>(q[c][kk][i]);
+                }
             }
     }
 
@@ -151,7 +155,7 @@ struct Rows {
     // Weights of NS steps' scores, as PV operands; rescales what was summed when the maximum moves.  `step(k)` is
     // called after every eighth weight, k = 0 .. 2 NS - 1.
     template <int NS, class F>
-    __device__ __forceinline__ void softmax(const f32x16_t (&s)[NS], vec8 (&ph)[NS][2], vec8 (&pl)[SPLIT ? NS : 1][2], F step) {
+    __device__ __forceinline__ void softmax(const f32x16_t (&s)[NS], vec8 (&w)[PARTS][NS][2], F step) {
         float mx[2 * NS];
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
@@ -185,9 +189,12 @@ struct Rows {
             for (int r = 0; r < 16; ++r) {
                 const float e = fast_exp2(fmaf(s[n][r], sscale, ref));
                 sum[r & 3] += e;
-                const T hi = static_cast<T>(e);
-                ph[n][r >> 3][r & 7] = hi;
-                if (SPLIT) pl[n][r >> 3][r & 7] = static_cast<T>(e - static_cast<float>(hi));
+                float v = e;
+#pragma unroll
+                for (int c = 0; c < PARTS; ++c) {
+                    w[c][n][r >> 3][r & 7] = static_cast<T>(v);
+                    v -= static_cast<float>(w[c][n][r >> 3][r & 7]);
+                }
                 if ((r & 7) == 7) step(2 * n + (r >> 3));
             }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -274,9 +281,9 @@ struct Rows {
     }
 };
 
-// Clears the elements of `bytes` bytes of V that are not finite.
-template <class T> __device__ __forceinline__ void clear_bad(char* v, int bytes, int threads) {
-    for (int c = threadIdx.x; c < bytes / 2; c += threads) {
+// Clears the elements of `bytes` bytes of V that are not finite, by `threads` threads.
+template <class T> __device__ __forceinline__ void clear_bad(char* v, int bytes, int thread, int threads) {
+    for (int c = thread; c < bytes / 2; c += threads) {
         T* e = reinterpret_cast<T*>(v) + c;
         if (!(fabsf(static_cast<float>(*e)) < INFINITY)) *e = static_cast<T>(0.f);
     }
@@ -288,27 +295,25 @@ __device__ __forceinline__ int page_of(const ChunksK& p, int pt_off, int t) {
 }
 
 // ------------------------------------------------------------------ few rows: HBM-bound
-// RW waves of 32 rows each x PW waves that take one step of 32 positions of every tile.  With
-// RW = 1 a wave copies its own steps and no wave waits for another before the end.
-template <bool BF16, int D, bool SPLIT, int RW, int PW>
-__global__ void __launch_bounds__(64 * RW * PW, 1) chunks_stream_kernel(const ChunksK p) {
-    using R = Rows<BF16, D, SPLIT>;
+// RW waves of 32 rows each x PW waves that take one step of 32 positions of every tile.  K and V of a tile are
+// units of a ring in LDS that fills it, most of them in flight while one is used.  With RW = 1 a wave copies its own steps
+// and no wave waits for another before the end, where the PW (m, l, o) of a row merge.
+constexpr int kStreamLds = 160 * 1024;
+
+template <bool BF16, int D, int PARTS, int RW, int PW>
+__device__ __forceinline__ void chunk_stream(const ChunksK& p, const ChunkItem& it, int u, char* lds) {
+    using R = Rows<BF16, D, PARTS>;
+    using T = typename R::T;
     using vec8 = typename R::vec8;
     constexpr int WAVES = RW * PW;
     constexpr int TILE = 32 * PW;
     constexpr int SB = 64 * D;                    // bytes of a step of K (or V)
-    constexpr int STAGE = 2 * SB * PW;            // a tile's steps, each K then V
-    constexpr int NST = STAGE > 32768 ? 2 : STAGE > 16384 ? 3 : 4;
-    constexpr int PER = 2 * SB * PW / 1024 / WAVES;  // DMA loads per wave and tile
+    constexpr int UB = SB * PW;                   // of a unit
+    constexpr int UL = UB / 1024 / WAVES;         // DMA loads per wave and unit
+    constexpr int NU = kStreamLds / UB < 10 ? kStreamLds / UB : 10;
     constexpr int NG = D / 8;                     // f32x4 groups of a row in a lane
-    constexpr int XB = WAVES * 64 * (NG * 16 + 8);   // the waves' (acc, m, l), exchanged at the end
-    constexpr int LDS = NST * STAGE > XB ? NST * STAGE : XB;
-    static_assert(NG % PW == 0 && LDS <= 160 * 1024, "");
-    __shared__ __attribute__((aligned(1024))) char lds[LDS];
-
-    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
-    const ChunkItem it = p.it[e];
-    const int u = blockIdx.x - it.unit0;
+    static_assert(NG % PW == 0 && WAVES * 64 * (NG * 16 + 8) <= kStreamLds, "the waves' (acc, m, l) fit");
+    static_assert(UL >= 1 && NU >= 4 && (NU - 2) * UL < 64, "vmcnt");
     const int split = u % it.splits, block = u / it.splits % it.blocks, kvh = u / (it.splits * it.blocks);
     const int g = p.heads / p.geom.kv_heads;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -323,68 +328,64 @@ __global__ void __launch_bounds__(64 * RW * PW, 1) chunks_stream_kernel(const Ch
     const long long page_bytes = p.geom.page_elems() * 2, plane_bytes = p.geom.plane_elems() * 2;
     const long long head_bytes = static_cast<long long>(kvh) * kPageTokens * D * 2;
     const uint32_t lane16 = 16 * (threadIdx.x & 63);
-    auto dma = [&](int i) {
-        // past the last tile: no records, so that zeros are written and no memory is read
-        const int t = t0 + min(i, ntiles - 1) * TILE;
-        char* dst = lds + (i % NST) * STAGE;
-#pragma unroll
-        for (int c = 0; c < PER; ++c) {
-            // RW = 1: the wave's own step; else loads dealt to the waves
-            const int n = RW == 1 ? pw * (2 * SB / 1024) + c : wave + WAVES * c;
-            const int st = n / (2 * SB / 1024), part = n % (2 * SB / 1024);
-            const int ts = t + 32 * st;
-            // a step past the keys' end may lie past the held pages: its page is not looked up
-            const bool in = i < ntiles && ts < t1;
-            const long long phys = in ? page_of(p, it.pt_off, ts) : 0;
-            const char* base = p.pool + phys * page_bytes + head_bytes + (part >= SB / 1024 ? plane_bytes : 0) +
-                               static_cast<long long>(ts & (kPageTokens - 1)) * D * 2;
-            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, in ? SB : 0, kBufferFlags);
-            buffer_load_lds16<kCacheNt>(r, dst + 1024 * n, lane16, 1024 * (part % (SB / 1024)));
-        }
+    // Unit n: K (n even) or V of tile n / 2, load c of this wave.  A step past the keys' end has no records: zeros are
+    // written and no memory is read (it may lie past the held pages, its page is not looked up).
+    // A tile lies in one page, whose entry is looked up a tile ahead (a lookup at its use held the wave for its latency, twice a
+    // tile).
+    auto page = [&](int n) __attribute__((always_inline)) {
+        const int ts = t0 + (n >> 1) * TILE;
+        return ts < t1 ? page_of(p, it.pt_off, ts) : 0;
     };
-    if (ntiles > 0)
-        for (int i = 0; i < NST - 1; ++i) dma(i);
+    auto load = [&](int n, int c, int phys) __attribute__((always_inline)) {
+        const int x = RW == 1 ? pw * (SB / 1024) + c : wave + WAVES * c;  // RW = 1: the wave's own step
+        const int ts = t0 + (n >> 1) * TILE + 32 * (x / (SB / 1024));
+        const bool in = ts < t1;
+        const char* base = p.pool + static_cast<long long>(phys) * page_bytes + head_bytes + (n & 1 ? plane_bytes : 0) +
+                           static_cast<long long>(ts & (kPageTokens - 1)) * D * 2;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, in ? SB : 0, kBufferFlags);
+        buffer_load_lds16<kCacheNt>(r, lds + n % NU * UB + 1024 * x, lane16, 1024 * (x % (SB / 1024)));
+    };
+    auto request = [&](int n, int phys) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < UL; ++c) load(n, c, phys);
+    };
+    // Unit n has landed in every wave, and the one before it was read by every wave.
+    auto turn = [&]() __attribute__((always_inline)) {
+        wait_vmcnt<(NU - 2) * UL>();
+        if (RW > 1) lds_barrier_dma_in_flight();
+    };
+    int phys0 = 0, phys1 = 0;  // of the next request in each half of a tile
+    if (ntiles > 0) {
+        for (int n = 0; n < NU - 1; ++n) request(n, page(n));
+        phys0 = page(NU - 1);
+        phys1 = page(NU);
+    }
 
     R w;
     w.init(p, it, kvh, g, rho0 + 32 * rw);
     w.load_q(p, it);
     const int ko = w.k_off(), vo = w.v_off();
-    float* const scores = p.scores ? p.scores + it.score0 + (static_cast<long long>(w.query) * p.heads + w.head) * chunk_score_len(it) : nullptr;
+    float* const scores = RW == 1 && p.scores ? p.scores + it.score0 + (static_cast<long long>(w.query) * p.heads + w.head) * chunk_score_len(it) : nullptr;
 
     for (int i = 0; i < ntiles; ++i) {
-        wait_vmcnt<(NST - 2) * PER>();
-        if (RW > 1) lds_barrier_dma_in_flight();  // everyone's part has landed, and the stage filled next was read
-        dma(i + NST - 1);
+        turn();
+        request(2 * i + NU - 1, phys0);  // over V of tile i - 1
+        phys0 = page(2 * i + NU + 1);
         const int ts = t0 + i * TILE + 32 * pw;
-        char* const kt = lds + (i % NST) * STAGE + 2 * SB * pw;
-        char* const vt = kt + SB;
+        const char* const kt = lds + 2 * i % NU * UB + SB * pw;
         const bool edge = t0 + (i + 1) * TILE > seen || t0 + (i + 1) * TILE > t1;
-        if (RW > 1 && edge) {
-            bool bad = false;
-            for (int s = 0; s < PW; ++s) bad |= w.v_bad(lds + (i % NST) * STAGE + 2 * SB * s + SB);
-            if (bad) {
-                w.add_bad(vt, ts, t1);
-                lds_barrier_dma_in_flight();
-                for (int s = 0; s < PW; ++s) clear_bad<typename R::T>(lds + (i % NST) * STAGE + 2 * SB * s + SB, SB, 64 * WAVES);
-                lds_barrier_dma_in_flight();
-            }
-        } else if (edge && w.v_bad(vt)) {
-            w.add_bad(vt, ts, t1);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            for (int c = w.lane; c < SB / 2; c += 64) {
-                typename R::T* x = reinterpret_cast<typename R::T*>(vt) + c;
-                if (!(fabsf(static_cast<float>(*x)) < INFINITY)) *x = static_cast<typename R::T>(0.f);
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        }
         f32x16_t s[1];
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+        {
+            vec8 a[R::NK];
 #pragma unroll
-        for (int kk = 0; kk < R::NK; ++kk) {
-            const vec8 a = *reinterpret_cast<const vec8*>(kt + ko + 512 * kk);
-            s[0] = mfma32(a, w.qh[kk], s[0]);
-            if (SPLIT) s[0] = mfma32(a, w.ql[kk], s[0]);
+            for (int kk = 0; kk < R::NK; ++kk) a[kk] = *reinterpret_cast<const vec8*>(kt + ko + 512 * kk);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kk = 0; kk < R::NK; ++kk)
+#pragma unroll
+                for (int c = 0; c < PARTS; ++c) s[0] = mfma32(a[kk], w.q[c][kk], s[0]);
         }
         if (edge) w.mask(s[0], ts, t1);
         if (scores && w.on) {
@@ -397,16 +398,44 @@ __global__ void __launch_bounds__(64 * RW * PW, 1) chunks_stream_kernel(const Ch
                     o[1] = f32x4_t{s[0][8 * x + 4], s[0][8 * x + 5], s[0][8 * x + 6], s[0][8 * x + 7]} * w.sscale;
                 }
         }
-        vec8 ph[1][2], pl[1][2];
-        w.template softmax<1>(s, ph, pl, [](int) {});
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int d = 0; d < R::ND; ++d) {
-                const vec8 a = *reinterpret_cast<const vec8*>(vt + vo + 2048 * d + 512 * x);
-                w.acc[d] = mfma32(a, ph[0][x], w.acc[d]);
-                if (SPLIT) w.acc[d] = mfma32(a, pl[0][x], w.acc[d]);
+        turn();
+        char* const vu = lds + (2 * i + 1) % NU * UB;
+        char* const vt = vu + SB * pw;
+        if (edge) {
+            if (RW > 1) {
+                bool bad = false;
+                for (int x = 0; x < PW; ++x) bad |= w.v_bad(vu + SB * x);
+                if (bad) {  // the same in every wave
+                    w.add_bad(vt, ts, t1);
+                    lds_barrier_dma_in_flight();
+                    clear_bad<T>(vu, UB, threadIdx.x, 64 * WAVES);
+                    lds_barrier_dma_in_flight();
+                }
+            } else if (w.v_bad(vt)) {
+                w.add_bad(vt, ts, t1);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                clear_bad<T>(vt, SB, w.lane, 64);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
+        }
+        request(2 * i + NU, phys1);  // over K of this tile
+        phys1 = page(2 * i + NU + 2);
+        vec8 wt[PARTS][1][2];
+        w.template softmax<1>(s, wt, [](int) {});
+        {
+            vec8 a[2][R::ND];
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int d = 0; d < R::ND; ++d) a[x][d] = *reinterpret_cast<const vec8*>(vt + vo + 2048 * d + 512 * x);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int c = 0; c < PARTS; ++c)
+#pragma unroll
+                    for (int d = 0; d < R::ND; ++d) w.acc[d] = mfma32(a[x][d], wt[c][0][x], w.acc[d]);
+        }
     }
     w.l = sum_xor32(w.l);
 
@@ -443,13 +472,33 @@ __global__ void __launch_bounds__(64 * RW * PW, 1) chunks_stream_kernel(const Ch
     if (pw == 0) w.store_ml(p, it, split, M, L);
 }
 
+// Chunks of up to 32 rows.
+template <bool BF16, int D, int PARTS>
+__global__ void __launch_bounds__(256, 1) chunks_stream32_kernel(const ChunksK p) {
+    __shared__ __attribute__((aligned(1024))) char lds[kStreamLds];
+    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
+    const ChunkItem it = p.it[e];
+    chunk_stream<BF16, D, PARTS, 1, 4>(p, it, blockIdx.x - it.unit0, lds);
+}
+// Chunks of up to 128 rows, each in its own shape.
+template <bool BF16, int D, int PARTS>
+__global__ void __launch_bounds__(512, 1) chunks_stream_kernel(const ChunksK p) {
+    __shared__ __attribute__((aligned(1024))) char lds[kStreamLds];
+    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
+    const ChunkItem it = p.it[e];
+    const int u = blockIdx.x - it.unit0;
+    if (it.rows * (p.heads / p.geom.kv_heads) <= 64) chunk_stream<BF16, D, PARTS, 2, 4>(p, it, u, lds);
+    else chunk_stream<BF16, D, PARTS, 4, 2>(p, it, u, lds);
+}
+
 // ------------------------------------------------------------------ many rows: MFMA-bound
 // Eight waves of 32 rows share every tile of 64 positions.  Waves 0-3 and 4-7 run half a tile apart: while
 // one group's MFMAs run (scores of tile t, weighted V of tile t - 1), the other group computes its
 // softmax on the same SIMDs; a barrier ends each half.
 template <bool BF16, int D, bool SPLIT>
 __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
-    using R = Rows<BF16, D, SPLIT>;
+    constexpr int PARTS = SPLIT ? 2 : 1;
+    using R = Rows<BF16, D, PARTS>;
     using vec8 = typename R::vec8;
     constexpr int TILE = 64, NST = 3;
     constexpr int SB = 64 * D;           // bytes of a step of K (or V)
@@ -478,10 +527,11 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
     const long long page_bytes = p.geom.page_elems() * 2, plane_bytes = p.geom.plane_elems() * 2;
     const long long head_bytes = static_cast<long long>(kvh) * kPageTokens * D * 2;
     const uint32_t lane16 = 16 * (threadIdx.x & 63);
-    auto source = [&](int i, int plane) {
+    auto page = [&](int i) { return page_of(p, it.pt_off, t0 + min(i, ntiles - 1) * TILE); };
+    auto source = [&](int i, int plane, int phys) {
         const bool in = i < ntiles;  // past the last tile: no records, no memory is read
         const int t = t0 + min(i, ntiles - 1) * TILE;
-        const char* base = p.pool + static_cast<long long>(page_of(p, it.pt_off, t)) * page_bytes + head_bytes + plane * plane_bytes +
+        const char* base = p.pool + static_cast<long long>(phys) * page_bytes + head_bytes + plane * plane_bytes +
                            static_cast<long long>(t & (kPageTokens - 1)) * D * 2;
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, in ? KB : 0, kBufferFlags);
     };
@@ -489,7 +539,7 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
         buffer_load_lds16(r, lds + plane * NST * KB + (i % NST) * KB + 1024 * (wave + 8 * c), lane16, 1024 * (wave + 8 * c));
     };
     auto dma = [&](int i, int plane) {
-        const __amdgpu_buffer_rsrc_t r = source(i, plane);
+        const __amdgpu_buffer_rsrc_t r = source(i, plane, page(i));
 #pragma unroll
         for (int c = 0; c < PER; ++c) load(r, i, plane, c);
     };
@@ -502,7 +552,7 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
     }
     w.load_q(p, it);
     const int ko = w.k_off(), vo = w.v_off();
-    vec8 ph[2][2], pl[SPLIT ? 2 : 1][2];
+    vec8 pw[PARTS][2][2];
     f32x16_t s[2];
 
     auto barrier = [&]() __attribute__((always_inline)) {
@@ -530,16 +580,16 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
             if (i & 1) {
                 if (pv) {
                     const int st = j / (2 * R::ND), x = j / R::ND % 2, d = j % R::ND;
-                    w.acc[d] = mfma32(ring[i % kAhead], ph[st][x], w.acc[d]);
-                    if (SPLIT) w.acc[d] = mfma32(ring[i % kAhead], pl[SPLIT ? st : 0][x], w.acc[d]);
+#pragma unroll
+                    for (int c = 0; c < PARTS; ++c) w.acc[d] = mfma32(ring[i % kAhead], pw[c][st][x], w.acc[d]);
                 }
             } else if (qk) {
                 const int st = j & 1, kk = j >> 1;
                 if (kk == 0)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[st][r] = 0.f;
-                s[st] = mfma32(ring[i % kAhead], w.qh[kk], s[st]);
-                if (SPLIT) s[st] = mfma32(ring[i % kAhead], w.ql[SPLIT ? kk : 0], s[st]);
+#pragma unroll
+                for (int c = 0; c < PARTS; ++c) s[st] = mfma32(ring[i % kAhead], w.q[c][kk], s[st]);
             }
             __builtin_amdgcn_sched_barrier(0);
             if (i + kAhead < NQ + NP && ((i + kAhead) & 1 ? pv : qk)) ring[i % kAhead] = read(i + kAhead);
@@ -564,14 +614,20 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
     const int nfull = max(0, min(seen, t1) - t0) / TILE;
     if (nfull > 0) {
         const bool late = wave >= 4;
+        int phys1 = page(late ? 2 : 1), phys2 = page(late ? 3 : 2);  // of tiles i + 1, i + 2 of the next request
         auto weigh = [&](int i) __attribute__((always_inline)) {  // with request(i)
-            if (SPLIT) {  // (no registers for both)
-                request(i);
-                w.template softmax<2>(s, ph, pl, [](int) {});
+            const __amdgpu_buffer_rsrc_t rk = source(i + 2, 0, phys2), rv = source(i + 1, 1, phys1);
+            phys1 = phys2;
+            phys2 = page(i + 3);  // looked up one tile before its use
+            if (SPLIT) {  // (no registers for loads between)
+#pragma unroll
+                for (int c = 0; c < PER; ++c) load(rk, i + 2, 0, c);
+#pragma unroll
+                for (int c = 0; c < PER; ++c) load(rv, i + 1, 1, c);
+                w.template softmax<2>(s, pw, [](int) {});
                 return;
             }
-            const __amdgpu_buffer_rsrc_t rk = source(i + 2, 0), rv = source(i + 1, 1);
-            w.template softmax<2>(s, ph, pl, [&](int c) __attribute__((always_inline)) {
+            w.template softmax<2>(s, pw, [&](int c) __attribute__((always_inline)) {
                 if (c < PER) load(rk, i + 2, 0, c);
                 else if (c < 2 * PER) load(rv, i + 1, 1, c - PER);
             });
@@ -593,7 +649,7 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
             if (late) wait_vmcnt<2 * PER>();
             barrier();
         }
-        if (late) w.template softmax<2>(s, ph, pl, [](int) {});
+        if (late) w.template softmax<2>(s, pw, [](int) {});
         else weigh(nfull - 1);
         if (!late) wait_vmcnt<2 * PER>();
         barrier();
@@ -611,13 +667,13 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
             w.add_bad(v, t0 + i * TILE, t1);
             w.add_bad(v + SB, t0 + i * TILE + 32, t1);
             barrier();
-            clear_bad<typename R::T>(v, KB, 512);
+            clear_bad<typename R::T>(v, KB, threadIdx.x, 512);
             barrier();
         }
         qk_pv(k_at(i), nullptr, true, false);
         w.mask(s[0], t0 + i * TILE, t1);
         w.mask(s[1], t0 + i * TILE + 32, t1);
-        w.template softmax<2>(s, ph, pl, [](int) {});
+        w.template softmax<2>(s, pw, [](int) {});
         qk_pv(nullptr, v, false, true);
     }
     w.l = sum_xor32(w.l);
@@ -785,10 +841,10 @@ __global__ void __launch_bounds__(512, SPLIT && D == 128 ? 1 : 2) chunks_tile_we
 
 template <bool BF16, int D, bool SPLIT>
 hipError_t launch_kind(const ChunksK& k, int kind, hipStream_t s) {
+    constexpr int PARTS = chunk_parts(BF16 ? QR_DTYPE_BF16 : QR_DTYPE_F16, SPLIT);
     switch (kind) {
-        case kChunkStream32: hipLaunchKernelGGL((chunks_stream_kernel<BF16, D, SPLIT, 1, 4>), dim3(k.units), dim3(256), 0, s, k); break;
-        case kChunkStream64: hipLaunchKernelGGL((chunks_stream_kernel<BF16, D, SPLIT, 2, 4>), dim3(k.units), dim3(512), 0, s, k); break;
-        case kChunkStream128: hipLaunchKernelGGL((chunks_stream_kernel<BF16, D, SPLIT, 4, 2>), dim3(k.units), dim3(512), 0, s, k); break;
+        case kChunkStream32: hipLaunchKernelGGL((chunks_stream32_kernel<BF16, D, PARTS>), dim3(k.units), dim3(256), 0, s, k); break;
+        case kChunkStream: hipLaunchKernelGGL((chunks_stream_kernel<BF16, D, PARTS>), dim3(k.units), dim3(512), 0, s, k); break;
         case kChunkTile: hipLaunchKernelGGL((chunks_tile_kernel<BF16, D, SPLIT>), dim3((k.units + 7) / 8 * 8), dim3(512), 0, s, k); break;
         default: hipLaunchKernelGGL((chunks_tile_weights_kernel<BF16, D, SPLIT>), dim3(k.units), dim3(512), 0, s, k); break;
     }
