@@ -131,7 +131,7 @@ struct KindGeom {
     int rows, tile;   // of a workgroup
     long long want;   // units that fill the GPU
 };
-constexpr KindGeom kGeom[kChunkKinds] = {{kChunkAnyRows, kChunkAnyTile, 1024}, {32, 128, 256}, {128, 128, 256}, {256, 64, 256}, {32, 32, 256}, {64, 32, 256}};
+constexpr KindGeom kGeom[kChunkKinds] = {{kChunkAnyRows, kChunkAnyTile, 1024}, {32, 128, 256}, {128, 64, 512}, {256, 64, 256}, {32, 32, 256}, {64, 32, 256}};
 
 int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
@@ -154,11 +154,11 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
         pl.it[i].blocks = cdiv(rows, kGeom[pl.it[i].kind].rows);
     }
     // The keys of a kind's blocks are split while its units do not fill the GPU: as many tiles per unit as leave
-    // no more units than that, or one.  (Every tile of a kind takes about the same time: kChunkStream's are of 64 positions
-    // for more than 64 rows, else of 128.)
+    // no more units than that, or one.  (Every tile of a kind takes about the same time: kChunkStream's are of 32 positions
+    // for more than 64 rows, else of 64.)
     auto tiles_of = [&](int i) {
         int tile = kGeom[pl.it[i].kind].tile;
-        if (pl.it[i].kind == kChunkStream && static_cast<long long>(a.it[i].rows) * gmax > 64) tile = 64;
+        if (pl.it[i].kind == kChunkStream && static_cast<long long>(a.it[i].rows) * gmax > 64) tile = 32;
         return cdiv(a.it[i].pos0 + a.it[i].rows, tile);
     };
     long long slots = 0;

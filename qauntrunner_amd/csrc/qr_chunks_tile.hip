@@ -298,9 +298,8 @@ __device__ __forceinline__ int page_of(const ChunksK& p, int pt_off, int t) {
 // RW waves of 32 rows each x PW waves that take one step of 32 positions of every tile.  K and V of a tile are
 // units of a ring in LDS that fills it, most of them in flight while one is used.  With RW = 1 a wave copies its own steps
 // and no wave waits for another before the end, where the PW (m, l, o) of a row merge.
-constexpr int kStreamLds = 160 * 1024;
 
-template <bool BF16, int D, int PARTS, int RW, int PW>
+template <bool BF16, int D, int PARTS, int RW, int PW, int LDS>
 __device__ __forceinline__ void chunk_stream(const ChunksK& p, const ChunkItem& it, int u, char* lds) {
     using R = Rows<BF16, D, PARTS>;
     using T = typename R::T;
@@ -310,9 +309,9 @@ __device__ __forceinline__ void chunk_stream(const ChunksK& p, const ChunkItem& 
     constexpr int SB = 64 * D;                    // bytes of a step of K (or V)
     constexpr int UB = SB * PW;                   // of a unit
     constexpr int UL = UB / 1024 / WAVES;         // DMA loads per wave and unit
-    constexpr int NU = kStreamLds / UB < 10 ? kStreamLds / UB : 10;
+    constexpr int NU = LDS / UB < 10 ? LDS / UB : 10;
     constexpr int NG = D / 8;                     // f32x4 groups of a row in a lane
-    static_assert(NG % PW == 0 && WAVES * 64 * (NG * 16 + 8) <= kStreamLds, "the waves' (acc, m, l) fit");
+    static_assert(NG % PW == 0 && WAVES * 64 * (NG * 16 + 8) <= LDS, "the waves' (acc, m, l) fit");
     static_assert(UL >= 1 && NU >= 4 && (NU - 2) * UL < 64, "vmcnt");
     const int split = u % it.splits, block = u / it.splits % it.blocks, kvh = u / (it.splits * it.blocks);
     const int g = p.heads / p.geom.kv_heads;
@@ -472,23 +471,26 @@ __device__ __forceinline__ void chunk_stream(const ChunksK& p, const ChunkItem& 
     if (pw == 0) w.store_ml(p, it, split, M, L);
 }
 
-// Chunks of up to 32 rows.
+// Chunks of up to 32 rows: one workgroup per CU, all its LDS.
 template <bool BF16, int D, int PARTS>
 __global__ void __launch_bounds__(256, 1) chunks_stream32_kernel(const ChunksK p) {
-    __shared__ __attribute__((aligned(1024))) char lds[kStreamLds];
+    constexpr int LDS = 160 * 1024;
+    __shared__ __attribute__((aligned(1024))) char lds[LDS];
     const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
     const ChunkItem it = p.it[e];
-    chunk_stream<BF16, D, PARTS, 1, 4>(p, it, blockIdx.x - it.unit0, lds);
+    chunk_stream<BF16, D, PARTS, 1, 4, LDS>(p, it, blockIdx.x - it.unit0, lds);
 }
-// Chunks of up to 128 rows, each in its own shape.
+// Chunks of up to 128 rows, each in its own shape: two workgroups per CU, so that one computes while the other stands
+// at a barrier (one of eight waves: XX).
 template <bool BF16, int D, int PARTS>
-__global__ void __launch_bounds__(512, 1) chunks_stream_kernel(const ChunksK p) {
-    __shared__ __attribute__((aligned(1024))) char lds[kStreamLds];
+__global__ void __launch_bounds__(256, 2) chunks_stream_kernel(const ChunksK p) {
+    constexpr int LDS = 80 * 1024;
+    __shared__ __attribute__((aligned(1024))) char lds[LDS];
     const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
     const ChunkItem it = p.it[e];
     const int u = blockIdx.x - it.unit0;
-    if (it.rows * (p.heads / p.geom.kv_heads) <= 64) chunk_stream<BF16, D, PARTS, 2, 4>(p, it, u, lds);
-    else chunk_stream<BF16, D, PARTS, 4, 2>(p, it, u, lds);
+    if (it.rows * (p.heads / p.geom.kv_heads) <= 64) chunk_stream<BF16, D, PARTS, 2, 2, LDS>(p, it, u, lds);
+    else chunk_stream<BF16, D, PARTS, 4, 1, LDS>(p, it, u, lds);
 }
 
 // ------------------------------------------------------------------ many rows: MFMA-bound
@@ -844,7 +846,7 @@ hipError_t launch_kind(const ChunksK& k, int kind, hipStream_t s) {
     constexpr int PARTS = chunk_parts(BF16 ? QR_DTYPE_BF16 : QR_DTYPE_F16, SPLIT);
     switch (kind) {
         case kChunkStream32: hipLaunchKernelGGL((chunks_stream32_kernel<BF16, D, PARTS>), dim3(k.units), dim3(256), 0, s, k); break;
-        case kChunkStream: hipLaunchKernelGGL((chunks_stream_kernel<BF16, D, PARTS>), dim3(k.units), dim3(512), 0, s, k); break;
+        case kChunkStream: hipLaunchKernelGGL((chunks_stream_kernel<BF16, D, PARTS>), dim3(k.units), dim3(256), 0, s, k); break;
         case kChunkTile: hipLaunchKernelGGL((chunks_tile_kernel<BF16, D, SPLIT>), dim3((k.units + 7) / 8 * 8), dim3(512), 0, s, k); break;
         default: hipLaunchKernelGGL((chunks_tile_weights_kernel<BF16, D, SPLIT>), dim3(k.units), dim3(512), 0, s, k); break;
     }
