@@ -71,11 +71,12 @@ struct NormRopeArgs {
     int rot;                 // rotated dims, even
     double turn[kMaxRopeHalf];               // revolutions per position of pair i
 };
-hipError_t launch_norm_rope(const NormRopeArgs& a, hipStream_t stream);
+hipError_t launch_norm_rope(NormRopeArgs& a, hipStream_t stream);  // sets unit0
 
 // ------------------------------------------------------------------ rows back
 struct ReadItem {
     int pt_off, pos0, rows, row0;
+    int unit0;
 };
 struct ReadArgs {
     ReadItem it[kBatch];
@@ -87,7 +88,7 @@ struct ReadArgs {
     int dtype;
     void *k, *v;             // [rows][kv_heads * head_dim] in the cache's type
 };
-hipError_t launch_read(const ReadArgs& a, hipStream_t stream);
+hipError_t launch_read(ReadArgs& a, hipStream_t stream);  // sets unit0
 
 // ------------------------------------------------------------------ attention
 struct ChunkItem {

@@ -300,7 +300,7 @@ int qr_kv_read_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* p
             a.v = const_cast<char*>(offset_bytes(v_out_dev, done * kv->kv_dim * es));
             for (; i < n && a.n < kBatch; ++i) {
                 if (!rows[i]) continue;
-                a.it[a.n++] = {kv->store.pt_offset(seq_ids[i], layer), pos0[i], rows[i], a.rows};
+                a.it[a.n++] = {kv->store.pt_offset(seq_ids[i], layer), pos0[i], rows[i], a.rows, 0};
                 a.rows += rows[i];
             }
             done += a.rows;

@@ -5,6 +5,8 @@
 // below every number), in their order: slot j takes what slot kept[j] held, kept[j] >= j.
 #include "qr_batch.hpp"
 
+#include <algorithm>
+
 namespace qr {
 namespace {
 
@@ -17,12 +19,31 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// Inclusive sum over a workgroup of 1024 threads; `wsum` holds a value per wave.
+__device__ __forceinline__ int block_scan(int x, int* wsum) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    if (lane == 63) wsum[wave] = x;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) x += wsum[w];
+    __syncthreads();
+    return x;
+}
+
 // One workgroup per (entry, kv head): the key of the last position taken, digit by digit from the
-// top (8 bits a pass), then the kept positions in order.
+// top (11, 11 and 10 bits: counts in LDS, then a scan from the largest digit down), then the kept positions in order.
+// The keys stay in registers, C per thread; C = 0: longer rows, read from L2 in every pass.  A wave whose keys have the
+// same digit counts them with one atomic (whole rows of equal weights would queue 64 on one address).
+template <int C>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
-    constexpr int kWaves = kSelThreads / 64;
-    __shared__ int hist[256];
-    __shared__ int wsum[2][kWaves];
+    constexpr int kWaves = kSelThreads / 64, kBins = 2048;
+    __shared__ int hist[kBins];
+    __shared__ int wsum[kWaves];
+    __shared__ int before[2][C > 0 ? C * kWaves : 1];
     __shared__ uint32_t sh_prefix;
     __shared__ int sh_need;
     const int kvh = blockIdx.x % a.geom.kv_heads;
@@ -40,67 +61,220 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
         return;
     }
     const int lo = a.first, hi = it.len - a.recent;  // candidates
+    const int chunks = C > 0 ? C : (it.len + kSelThreads - 1) / kSelThreads;
+    float x[C > 0 ? C : 1];
+    if (C > 0)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int i = c * kSelThreads + tid;
+            x[c] = i < it.len ? w[i] : 0.f;
+        }
+    auto value = [&](int c, int i) { return C > 0 ? x[C > 0 ? c : 0] : i < it.len ? w[i] : 0.f; };
     uint32_t prefix = 0, mask = 0;
     int need = a.heavy;
     if (need > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+        constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass) {
+            for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
             __syncthreads();
-            for (int i = lo + tid; i < hi; i += kSelThreads) {
-                const uint32_t k = weight_key(w[i]);
-                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+            auto count = [&](int c) __attribute__((always_inline)) {
+                const int i = c * kSelThreads + tid;
+                const uint32_t k = weight_key(value(c, i));
+                const bool in = i >= lo && i < hi && (k & mask) == prefix;
+                const uint64_t act = __builtin_amdgcn_ballot_w64(in);
+                if (!act) return;
+                const int d = (k >> kShift[pass]) & ((1 << kBits[pass]) - 1);
+                const int d0 = __shfl(d, __ffsll(static_cast<unsigned long long>(act)) - 1);
+                const uint64_t same = __builtin_amdgcn_ballot_w64(in && d == d0);
+                if (lane == 0) atomicAdd(&hist[d0], static_cast<int>(__popcll(same)));
+                if (in && d != d0) atomicAdd(&hist[d], 1);
+            };
+            if (C > 0) {
+#pragma unroll
+                for (int c = 0; c < C; ++c) count(c);
+            } else {
+                for (int c = 0; c < chunks; ++c) count(c);
             }
             __syncthreads();
-            if (tid == 0) {  // from the largest digit down, until `need` are passed
-                int left = need, d = 255;
-                while (d > 0 && hist[d] < left) left -= hist[d--];
-                sh_need = left;
-                sh_prefix = prefix | static_cast<uint32_t>(d) << shift;
+            // thread t: the digits kBins - 1 - 2t and the one below; the one where the counts from above reach `need`
+            const int top = kBins - 1 - 2 * tid, h1 = hist[top], h0 = hist[top - 1];
+            const int upto = block_scan(h1 + h0, wsum), above = upto - h1 - h0;
+            if (above < need && need <= upto) {
+                const bool first = need <= above + h1;
+                sh_need = need - above - (first ? 0 : h1);
+                sh_prefix = prefix | static_cast<uint32_t>(first ? top : top - 1) << kShift[pass];
             }
             __syncthreads();
             prefix = sh_prefix;
             need = sh_need;
-            mask |= 255u << shift;
-            __syncthreads();
+            mask |= ((1u << kBits[pass]) - 1) << kShift[pass];
         }
     }
-    // in order: every position above the key, and the first `need` of those that equal it
-    int eq_before = 0, out_before = 0;
-    for (int i0 = 0; i0 < it.len; i0 += kSelThreads) {
-        const int i = i0 + tid;
-        const bool held = i < it.len, cand = i >= lo && i < hi;
-        const float x = held ? w[i] : 0.f;
-        const uint32_t k = weight_key(x);
-        const bool eq = cand && a.heavy > 0 && k == prefix;
-        const uint64_t be = __builtin_amdgcn_ballot_w64(eq);
-        if (lane == 0) wsum[0][wave] = __popcll(be);
-        __syncthreads();  // every weight of the tile is read
-        int eq_at = eq_before + __popcll(be & ((1ull << lane) - 1)), eq_all = 0;
-        for (int j = 0; j < kWaves; ++j) {
-            if (j < wave) eq_at += wsum[0][j];
-            eq_all += wsum[0][j];
+    // in order: the positions outside the candidates, those above the key, and the first `need` of those that equal it.
+    // With A the former two and E the last before a position, it goes to slot A + min(E, need).
+    auto flags = [&](int c, int i, bool* sure, bool* eq) __attribute__((always_inline)) {
+        const uint32_t k = weight_key(value(c, i));
+        const bool cand = i >= lo && i < hi;
+        *sure = i < it.len && (!cand || (a.heavy > 0 && k > prefix));
+        *eq = cand && a.heavy > 0 && k == prefix;
+    };
+    const uint64_t below = (1ull << lane) - 1;
+    if (C > 0) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            bool sure, eq;
+            flags(c, c * kSelThreads + tid, &sure, &eq);
+            const uint64_t bs = __builtin_amdgcn_ballot_w64(sure), be = __builtin_amdgcn_ballot_w64(eq);
+            if (lane == 0) {
+                before[0][C > 0 ? c * kWaves + wave : 0] = __popcll(bs);
+                before[1][C > 0 ? c * kWaves + wave : 0] = __popcll(be);
+            }
         }
-        const bool take = held && (!cand || (a.heavy > 0 && (k > prefix || (eq && eq_at < need))));
-        const uint64_t bt = __builtin_amdgcn_ballot_w64(take);
-        if (lane == 0) wsum[1][wave] = __popcll(bt);
+        __syncthreads();  // every weight is read
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int v = tid < C * kWaves ? before[q][C > 0 ? tid : 0] : 0;
+            const int s = block_scan(v, wsum) - v;
+            if (tid < C * kWaves) before[q][C > 0 ? tid : 0] = s;
+        }
         __syncthreads();
-        int at = out_before + __popcll(bt & ((1ull << lane) - 1)), all = 0;
-        for (int j = 0; j < kWaves; ++j) {
-            if (j < wave) at += wsum[1][j];
-            all += wsum[1][j];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int i = c * kSelThreads + tid;
+            bool sure, eq;
+            flags(c, i, &sure, &eq);
+            const uint64_t bs = __builtin_amdgcn_ballot_w64(sure), be = __builtin_amdgcn_ballot_w64(eq);
+            const int e = before[1][C > 0 ? c * kWaves + wave : 0] + __popcll(be & below);
+            const int at = before[0][C > 0 ? c * kWaves + wave : 0] + __popcll(bs & below) + min(e, need);
+            if (sure || (eq && e < need)) {
+                kept[at] = i;
+                ow[at] = value(c, i);
+            }
         }
-        if (take) {
-            kept[at] = i;
-            ow[at] = x;  // at <= i: its own weight is read, in this tile or an earlier one
+    } else {
+        __shared__ int cnt[2][kWaves];
+        int sure_before = 0, eq_before = 0;
+        for (int c = 0; c < chunks; ++c) {
+            const int i = c * kSelThreads + tid;
+            const float v = value(c, i);
+            bool sure, eq;
+            flags(c, i, &sure, &eq);
+            const uint64_t bs = __builtin_amdgcn_ballot_w64(sure), be = __builtin_amdgcn_ballot_w64(eq);
+            if (lane == 0) {
+                cnt[0][wave] = __popcll(bs);
+                cnt[1][wave] = __popcll(be);
+            }
+            __syncthreads();  // every weight of the chunk is read: slot at <= i, in this chunk or an earlier one
+            int s = sure_before + __popcll(bs & below), e = eq_before + __popcll(be & below);
+            for (int q = 0; q < kWaves; ++q) {
+                if (q < wave) {
+                    s += cnt[0][q];
+                    e += cnt[1][q];
+                }
+                sure_before += cnt[0][q];
+                eq_before += cnt[1][q];
+            }
+            __syncthreads();
+            if (sure || (eq && e < need)) {
+                kept[s + min(e, need)] = i;
+                ow[s + min(e, need)] = v;
+            }
         }
-        eq_before += eq_all;
-        out_before += all;
+        __syncthreads();
     }
-    __syncthreads();
     for (int i = keep + tid; i < it.len; i += kSelThreads) ow[i] = 0.f;
 }
 
 constexpr int kMoveThreads = 256;
+
+// The same for head sizes whose rows are whole 16-byte pieces, 64 bytes of a row (or what is left of it) per workgroup, 512
+// slots at a time; the next 512's positions are looked up ahead.  V of the MFMA page layout: 16 dims per workgroup, a thread
+// gathers 8 slots of a dim (16 bytes of the page).  Bound by HBM for many workgroups, else by the latency of a tile.
+template <int ES, bool MFMA>
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArgs a) {
+    constexpr int N = 16 / ES, TILE = 512;
+    const int D = a.geom.head_dim, pieces = D / N;
+    const int ks = (pieces + 3) / 4, vs = MFMA ? D / 16 : ks;  // workgroups of the K and the V rows of a kv head
+    int u = blockIdx.x;
+    const int part = u % (ks + vs);
+    u /= ks + vs;
+    const int kvh = u % a.geom.kv_heads;
+    const EvictItem it = a.it[u / a.geom.kv_heads];
+    const int keep = a.first + a.heavy + a.recent;
+    if (it.len <= keep) return;
+    const int* const kept = a.kept + (static_cast<long long>(it.entry) * a.geom.kv_heads + kvh) * keep;
+    const int* const pages = a.page_table + it.pt_off;
+    const int plane = part >= ks, s = part - plane * ks;
+    auto moved = [&](int j0) { return kept[min(j0 + TILE, keep) - 1] != min(j0 + TILE, keep) - 1; };
+    int j0 = 0;
+    while (j0 < keep && !moved(j0)) j0 += TILE;  // slots that keep what they hold
+    if (MFMA && plane) {
+        constexpr int IT = 16 * TILE / 8 / kMoveThreads;
+        const int d = 16 * s + (threadIdx.x & 15);
+        for (; j0 < keep; j0 += TILE) {
+            uint16_t x[IT][8];
+#pragma unroll
+            for (int c = 0; c < IT; ++c) {
+                const int j = j0 + 8 * ((threadIdx.x >> 4) + kMoveThreads / 16 * c);
+                int src[8];
+                long long phys[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) src[k] = kept[min(j + k, keep - 1)];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) phys[k] = pages[src[k] >> kPageShift];
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    x[c][k] = static_cast<const uint16_t*>(a.pool)[a.geom.offset(phys[k], 1, kvh, src[k] & (kPageTokens - 1), d)];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < IT; ++c) {
+                const int j = j0 + 8 * ((threadIdx.x >> 4) + kMoveThreads / 16 * c);
+                if (j >= keep) continue;
+                uint16_t* o = static_cast<uint16_t*>(a.pool) + a.geom.offset(pages[j >> kPageShift], 1, kvh, j & (kPageTokens - 1), d);
+                if (j + 8 <= keep) {
+                    uint4 v;
+                    __builtin_memcpy(&v, x[c], 16);
+                    *reinterpret_cast<uint4*>(o) = v;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (j + k < keep) o[k] = x[c][k];
+                }
+            }
+        }
+        return;
+    }
+    constexpr int IT = 4 * TILE / kMoveThreads;
+    // MFMA layout: consecutive lanes take consecutive slots (their pieces lie side by side), else the pieces of a slot
+    const int pc = 4 * s + (MFMA ? static_cast<int>(threadIdx.x) >> 6 : static_cast<int>(threadIdx.x) & 3);
+    const int q0 = MFMA ? threadIdx.x & 63 : threadIdx.x >> 2;
+    const bool in = pc < pieces;
+    int src[IT];
+    auto look = [&](int j1) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < IT; ++c) src[c] = kept[min(j1 + q0 + 64 * c, keep - 1)];
+    };
+    char* const pool = static_cast<char*>(a.pool);
+    if (j0 < keep) look(j0);
+    for (; j0 < keep; j0 += TILE) {
+        U32x4 x[IT];
+        if (in)
+#pragma unroll
+            for (int c = 0; c < IT; ++c)
+                x[c] = load16(pool + ES * a.geom.offset(pages[src[c] >> kPageShift], plane, kvh, src[c] & (kPageTokens - 1), N * pc));
+        if (j0 + TILE < keep) look(j0 + TILE);
+        __syncthreads();
+        if (in)
+#pragma unroll
+            for (int c = 0; c < IT; ++c) {
+                const int j = j0 + q0 + 64 * c;
+                if (j < keep)
+                    *reinterpret_cast<U32x4*>(pool + ES * a.geom.offset(pages[j >> kPageShift], plane, kvh, j & (kPageTokens - 1), N * pc)) = x[c];
+            }
+    }
+}
 
 // K or V rows of one kv head, up to 8 dims of them: slots in ascending order, each tile read whole
 // before it is written (a slot's source lies at or behind it, so a later tile's sources are not
@@ -150,11 +324,23 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_any_kernel(const Evic
 
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
     if (!a.n) return hipSuccess;
-    const int rows = a.n * a.geom.kv_heads;
-    hipLaunchKernelGGL(evict_select_kernel, dim3(rows), dim3(kSelThreads), 0, stream, a);
+    const int rows = a.n * a.geom.kv_heads, keep = a.first + a.heavy + a.recent;
+    int longest = 0;
+    for (int i = 0; i < a.n; ++i)
+        if (a.it[i].len > keep) longest = std::max(longest, a.it[i].len);
+    const dim3 grid(rows), block(kSelThreads);
+    if (longest <= 4 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<4>, grid, block, 0, stream, a);
+    else if (longest <= 16 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<16>, grid, block, 0, stream, a);
+    else if (longest <= 64 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<64>, grid, block, 0, stream, a);
+    else hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, stream, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(evict_move_any_kernel, dim3(rows * 2 * ((a.geom.head_dim + 7) / 8)), dim3(kMoveThreads), 0, stream, a);
+    if (e != hipSuccess || !longest) return e;
+    const int D = a.geom.head_dim, n = 16 / dtype_size(a.dtype), ks = (D / n + 3) / 4;
+    const dim3 mblock(kMoveThreads);
+    if (D % n) hipLaunchKernelGGL(evict_move_any_kernel, dim3(rows * 2 * ((D + 7) / 8)), mblock, 0, stream, a);
+    else if (a.geom.mfma_layout) hipLaunchKernelGGL((evict_move_kernel<2, true>), dim3(rows * (ks + D / 16)), mblock, 0, stream, a);
+    else if (a.dtype == QR_DTYPE_F32) hipLaunchKernelGGL((evict_move_kernel<4, false>), dim3(rows * 2 * ks), mblock, 0, stream, a);
+    else hipLaunchKernelGGL((evict_move_kernel<2, false>), dim3(rows * 2 * ks), mblock, 0, stream, a);
     return hipGetLastError();
 }
 

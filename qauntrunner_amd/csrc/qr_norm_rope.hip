@@ -10,6 +10,8 @@
 // product is off by 2^-8 of a radian.
 #include "qr_batch.hpp"
 
+#include <algorithm>
+
 namespace qr {
 namespace {
 
@@ -78,6 +80,227 @@ __global__ void __launch_bounds__(kThreads) norm_rope_any_kernel(const NormRopeA
     }
 }
 
+// ---- head sizes of whole runs of 8 values (and rotations of as many)
+// An item is 8 values of a head, two runs of 4: item j < R/8 holds the pairs 4j .. 4j + 3 (and R/2 further), the others 8
+// values behind the rotated ones.  The items of a head lie in LPH = 2^n lanes, so that its sum is a lane exchange; a
+// thread's items are the same values of several heads, which share the norm's weights.
+struct Item {
+    int a, b;  // first values of its two runs
+    bool pair;
+};
+__device__ __forceinline__ Item item_of(int j, int rot) {
+    if (8 * j < rot) return {4 * j, 4 * j + rot / 2, true};
+    return {8 * j, 8 * j + 4, false};
+}
+template <bool A32> struct Run;  // 4 consecutive values, element-aligned
+template <> struct Run<true> {
+    float v[4];
+    __device__ __forceinline__ void load(const void* p, long long at) { __builtin_memcpy(v, static_cast<const float*>(p) + at, 16); }
+    __device__ __forceinline__ void widen(int, float (&x)[8], int o) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[o + i] = v[i];
+    }
+};
+template <> struct Run<false> {
+    uint16_t v[4];
+    __device__ __forceinline__ void load(const void* p, long long at) { __builtin_memcpy(v, static_cast<const uint16_t*>(p) + at, 8); }
+    __device__ __forceinline__ void widen(int dtype, float (&x)[8], int o) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[o + i] = dtype == QR_DTYPE_BF16 ? bf16_bits_to_f32(v[i]) : f16_bits_to_f32(v[i]);
+    }
+};
+// 4 values to p[at .. at + 3], element-aligned
+__device__ __forceinline__ void store_run(void* p, int dtype, long long at, const float* x) {
+    if (dtype == QR_DTYPE_F32) {
+        __builtin_memcpy(static_cast<float*>(p) + at, x, 16);
+    } else {
+        uint16_t b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = f32_to_bits16(x[i], dtype);
+        __builtin_memcpy(static_cast<uint16_t*>(p) + at, b, 8);
+    }
+}
+
+// V rows of the MFMA page layout, where 8 aligned slots of a dim are 16 bytes: a thread takes 8 dims of such a run, 8 loads
+// of 8 values and 8 stores of 16 bytes, 128 bytes in a row of the page.  Slots outside the chunk are left alone.
+template <bool A32>
+__global__ void __launch_bounds__(kThreads) v_runs_kernel(const NormRopeArgs a) {
+    const int e = batch_find(a.n, blockIdx.x, [&](int i) { return a.it[i].unit0; });
+    const NormRopeItem it = a.it[e];
+    const int per = a.geom.head_dim / 8, slices = a.geom.kv_heads * per;
+    const int runs = ((it.pos0 + it.rows - 1) >> 3) - (it.pos0 >> 3) + 1;
+    const int u = (static_cast<int>(blockIdx.x) - it.unit0) * kThreads + threadIdx.x;
+    if (u >= runs * slices) return;
+    const int slice = u % slices, kvh = slice / per, d0 = 8 * (slice - kvh * per);
+    const int p0 = ((it.pos0 >> 3) + u / slices) << 3;  // position of the run's first slot
+    Run<A32> x[8][2];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int j = min(max(p0 + k - it.pos0, 0), it.rows - 1);
+        const long long at = static_cast<long long>(it.row0 + j) * a.v_stride + slice * 8;
+        x[k][0].load(a.v, at);
+        x[k][1].load(a.v, at + 4);
+    }
+    const long long phys = a.page_table[it.pt_off + (p0 >> kPageShift)];
+    float y[8][8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        x[k][0].widen(a.act, y[k], 0);
+        x[k][1].widen(a.act, y[k], 4);
+    }
+    const bool whole = p0 >= it.pos0 && p0 + 8 <= it.pos0 + it.rows;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+        uint16_t b[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) b[k] = f32_to_bits16(y[k][d], a.dtype);
+        uint16_t* o = static_cast<uint16_t*>(a.pool) + a.geom.offset(phys, 1, kvh, p0 & (kPageTokens - 1), d0 + d);
+        if (whole) {
+            uint4 w;
+            __builtin_memcpy(&w, b, 16);
+            *reinterpret_cast<uint4*>(o) = w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (p0 + k >= it.pos0 && p0 + k < it.pos0 + it.rows) o[k] = b[k];
+        }
+    }
+}
+
+// One workgroup per row and gridDim.y-th part of its heads (K, then q, then V unless it goes by runs).  The loads of all of a thread's items are
+// issued before the angles are computed.  Bound by HBM, for few rows by the launch.
+template <bool A32, int IPT>
+__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormRopeArgs a, int lph, int v_heads) {
+    __shared__ __attribute__((aligned(16))) float cs[kMaxRopeHalf], sn[kMaxRopeHalf];
+    const int D = a.geom.head_dim, kv = a.geom.kv_heads, per = D / 8;
+    const int row = blockIdx.x;
+    const int e = batch_find(a.n, row, [&](int i) { return a.it[i].row0; });
+    const int j = row - a.it[e].row0, pos = a.it[e].pos0 + j, slot = pos & (kPageTokens - 1);
+    const int qh = a.q ? a.heads : 0, heads = kv + qh + v_heads;
+    const int li = threadIdx.x & (lph - 1);  // item within its head
+    const bool in = li < per;
+    const Item im = item_of(in ? li : 0, a.rot);
+    const int h0 = blockIdx.y * (kThreads / lph * IPT) + threadIdx.x / lph;
+    const int es = A32 ? 4 : 2;
+    const char* const rows[3] = {static_cast<const char*>(a.k) + row * a.k_stride * es, static_cast<const char*>(a.q) + row * a.q_stride * es,
+                                 static_cast<const char*>(a.v) + row * a.v_stride * es};
+    Run<A32> ra[IPT], rb[IPT];
+#pragma unroll
+    for (int k = 0; k < IPT; ++k) {
+        const int h = min(h0 + kThreads / lph * k, heads - 1);
+        const bool is_k = h < kv, is_q = !is_k && h < kv + qh;
+        const long long at = static_cast<long long>(is_k ? h : is_q ? h - kv : h - kv - qh) * D;
+        const char* src = is_k ? rows[0] : is_q ? rows[1] : rows[2];
+        ra[k].load(src, at + im.a);
+        rb[k].load(src, at + im.b);
+    }
+    angles(a, a.it[e].rope0 + j, cs, sn);
+    const long long phys = a.page_table[a.it[e].pt_off + (pos >> kPageShift)];
+    float w[2][8];  // of K heads, of q heads
+    const bool kn = a.k_norm, qn = a.q_norm;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int d = (i < 4 ? im.a : im.b - 4) + i;
+        w[0][i] = kn ? a.k_norm[d] : 1.f;
+        w[1][i] = qn ? a.q_norm[d] : 1.f;
+    }
+    __syncthreads();
+    float c4[4] = {1.f, 1.f, 1.f, 1.f}, s4[4] = {0.f, 0.f, 0.f, 0.f};
+    if (im.pair) {
+        __builtin_memcpy(c4, cs + im.a, 16);
+        __builtin_memcpy(s4, sn + im.a, 16);
+    }
+#pragma unroll
+    for (int k = 0; k < IPT; ++k) {
+        const int h = h0 + kThreads / lph * k;
+        const bool is_k = h < kv, is_q = !is_k && h < kv + qh;
+        float x[8];
+        ra[k].widen(a.act, x, 0);
+        rb[k].widen(a.act, x, 4);
+        if (is_k || is_q) {
+            if (is_k ? kn : qn) {
+                float ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+                ss = group_sum(in ? ss : 0.f, lph);
+                if (lph == 64) ss = sum_xor32(ss);
+                const float r = 1.f / sqrtf(ss / static_cast<float>(D) + a.eps);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = x[i] * r * (is_k ? w[0][i] : w[1][i]);
+            }
+            if (im.pair) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float lo = x[i], hi = x[i + 4];
+                    x[i] = lo * c4[i] - hi * s4[i];
+                    x[i + 4] = lo * s4[i] + hi * c4[i];
+                }
+            }
+        }
+        if (!in || h >= heads) continue;
+        // (q_out may be q: the loads of every item that a workgroup stores stand before the barrier)
+        if (is_q) {
+            const long long at = (static_cast<long long>(row) * a.heads + h - kv) * D;
+            store_run(a.q_out, a.act, at + im.a, x);
+            store_run(a.q_out, a.act, at + im.b, x + 4);
+        } else if (is_k || !a.geom.mfma_layout) {
+            const int hh = is_k ? h : h - kv - qh;
+            store_run(a.pool, a.dtype, a.geom.offset(phys, !is_k, hh, slot, im.a), x);
+            store_run(a.pool, a.dtype, a.geom.offset(phys, !is_k, hh, slot, im.b), x + 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                store_elem(a.pool, a.dtype, a.geom.offset(phys, 1, h - kv - qh, slot, (i < 4 ? im.a : im.b - 4) + i), x[i]);
+        }
+    }
+}
+
+// Rows back, head sizes whose rows are whole 16-byte pieces: a thread per piece; V of the MFMA page layout a thread per 8
+// dims of a run of 8 slots (128 bytes of the page), the first v_groups workgroups.
+__global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a, int v_groups) {
+    const int D = a.geom.head_dim, kv = a.geom.kv_heads;
+    if (static_cast<int>(blockIdx.x) < v_groups) {
+        const int e = batch_find(a.n, blockIdx.x, [&](int i) { return a.it[i].unit0; });
+        const ReadItem it = a.it[e];
+        const int per = D / 8, slices = kv * per, runs = ((it.pos0 + it.rows - 1) >> 3) - (it.pos0 >> 3) + 1;
+        const int u = (static_cast<int>(blockIdx.x) - it.unit0) * kThreads + threadIdx.x;
+        if (u >= runs * slices) return;
+        const int run = u / slices, slice = u % slices;
+        const int p0 = ((it.pos0 >> 3) + run) << 3;
+        const long long phys = a.page_table[it.pt_off + (p0 >> kPageShift)];
+        const uint16_t* src = static_cast<const uint16_t*>(a.pool) + a.geom.offset(phys, 1, slice / per, p0 & (kPageTokens - 1), 8 * (slice % per));
+        uint16_t x[8][8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            const uint4 w = *reinterpret_cast<const uint4*>(src + 8 * d);
+            __builtin_memcpy(x[d], &w, 16);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (p0 + k < it.pos0 || p0 + k >= it.pos0 + it.rows) continue;
+            uint16_t y[8];
+#pragma unroll
+            for (int d = 0; d < 8; ++d) y[d] = x[d][k];
+            __builtin_memcpy(static_cast<uint16_t*>(a.v) + static_cast<long long>(it.row0 + p0 + k - it.pos0) * kv * D + 8 * slice, y, 16);
+        }
+        return;
+    }
+    const int es = dtype_size(a.dtype), n = 16 / es, per = D / n, pieces = kv * per;  // of a row
+    const int planes = v_groups ? 1 : 2;
+    const long long u = (static_cast<long long>(blockIdx.x) - v_groups) * kThreads + threadIdx.x;
+    const int row = min(static_cast<int>(u / (planes * pieces)), a.rows - 1);
+    // the rows of a wave lie in one chunk or a few: each thread looks its own up
+    int e = 0;
+    for (int i = 1; i < a.n; ++i) e += a.it[i].row0 <= row;
+    if (u >= static_cast<long long>(a.rows) * planes * pieces) return;
+    const int c = static_cast<int>(u - static_cast<long long>(row) * planes * pieces), plane = c >= pieces, x = c - plane * pieces;
+    const int pos = a.it[e].pos0 + row - a.it[e].row0;
+    const long long phys = a.page_table[a.it[e].pt_off + (pos >> kPageShift)];
+    const long long from = a.geom.offset(phys, plane, x / per, pos & (kPageTokens - 1), n * (x % per));
+    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.pool) + from * es);
+    __builtin_memcpy(static_cast<char*>(plane ? a.v : a.k) + (static_cast<long long>(row) * pieces + x) * 16, &w, 16);
+}
+
 __global__ void __launch_bounds__(kThreads) read_any_kernel(const ReadArgs a) {
     const int row = blockIdx.x;
     const int e = batch_find(a.n, row, [&](int i) { return a.it[i].row0; });
@@ -94,17 +317,67 @@ __global__ void __launch_bounds__(kThreads) read_any_kernel(const ReadArgs a) {
     }
 }
 
+
+// V of the MFMA layout goes by runs of 8 slots unless the chunks have few rows: 2 bytes per store otherwise, but one
+// launch of one workgroup per row.
+template <class Args> int v_run_groups(Args& a) {
+    if (!a.geom.mfma_layout || a.rows < 4 * a.n) return 0;
+    int groups = 0;
+    for (int i = 0; i < a.n; ++i) {
+        const long long runs = ((a.it[i].pos0 + a.it[i].rows - 1) >> 3) - (a.it[i].pos0 >> 3) + 1;
+        a.it[i].unit0 = groups;
+        groups += static_cast<int>((runs * a.geom.kv_heads * (a.geom.head_dim / 8) + kThreads - 1) / kThreads);
+    }
+    return groups;
+}
+
+template <bool A32> void launch_ipt(const NormRopeArgs& a, int ipt, dim3 grid, int lph, int v_heads, hipStream_t s) {
+    if (ipt == 1) hipLaunchKernelGGL((norm_rope_kernel<A32, 1>), grid, dim3(kThreads), 0, s, a, lph, v_heads);
+    else if (ipt == 2) hipLaunchKernelGGL((norm_rope_kernel<A32, 2>), grid, dim3(kThreads), 0, s, a, lph, v_heads);
+    else if (ipt == 3) hipLaunchKernelGGL((norm_rope_kernel<A32, 3>), grid, dim3(kThreads), 0, s, a, lph, v_heads);
+    else hipLaunchKernelGGL((norm_rope_kernel<A32, 4>), grid, dim3(kThreads), 0, s, a, lph, v_heads);
+}
+
 }  // namespace
 
-hipError_t launch_norm_rope(const NormRopeArgs& a, hipStream_t stream) {
+hipError_t launch_norm_rope(NormRopeArgs& a, hipStream_t stream) {
     if (!a.rows) return hipSuccess;
-    hipLaunchKernelGGL(norm_rope_any_kernel, dim3(a.rows), dim3(kThreads), 0, stream, a);
+    const int D = a.geom.head_dim;
+    if (D % 8 || a.rot % 8) {
+        hipLaunchKernelGGL(norm_rope_any_kernel, dim3(a.rows), dim3(kThreads), 0, stream, a);
+        return hipGetLastError();
+    }
+    int lph = 1;
+    while (lph < D / 8) lph *= 2;
+    const int v_groups = v_run_groups(a);
+    const bool f32 = a.act == QR_DTYPE_F32;
+    if (v_groups) {
+        if (f32) hipLaunchKernelGGL(v_runs_kernel<true>, dim3(v_groups), dim3(kThreads), 0, stream, a);
+        else hipLaunchKernelGGL(v_runs_kernel<false>, dim3(v_groups), dim3(kThreads), 0, stream, a);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    const int v_heads = v_groups ? 0 : a.geom.kv_heads, heads = a.geom.kv_heads + (a.q ? a.heads : 0) + v_heads;
+    const int slots = (heads * lph + kThreads - 1) / kThreads, ipt = std::min(slots, 4);
+    const dim3 grid(a.rows, (slots + ipt - 1) / ipt);
+    if (f32) launch_ipt<true>(a, ipt, grid, lph, v_heads, stream);
+    else launch_ipt<false>(a, ipt, grid, lph, v_heads, stream);
     return hipGetLastError();
 }
 
-hipError_t launch_read(const ReadArgs& a, hipStream_t stream) {
+hipError_t launch_read(ReadArgs& a, hipStream_t stream) {
     if (!a.rows) return hipSuccess;
-    hipLaunchKernelGGL(read_any_kernel, dim3(a.rows), dim3(kThreads), 0, stream, a);
+    const int n = 16 / dtype_size(a.dtype);
+    if (a.geom.head_dim % n) {
+        hipLaunchKernelGGL(read_any_kernel, dim3(a.rows), dim3(kThreads), 0, stream, a);
+        return hipGetLastError();
+    }
+    const int v_groups = v_run_groups(a);
+    if (a.geom.mfma_layout && !v_groups) {
+        hipLaunchKernelGGL(read_any_kernel, dim3(a.rows), dim3(kThreads), 0, stream, a);
+        return hipGetLastError();
+    }
+    const long long pieces = static_cast<long long>(a.rows) * (v_groups ? 1 : 2) * a.geom.kv_heads * (a.geom.head_dim / n);
+    hipLaunchKernelGGL(read_kernel, dim3(v_groups + static_cast<unsigned>((pieces + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, a, v_groups);
     return hipGetLastError();
 }
 
