@@ -172,7 +172,9 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
                 work += static_cast<long long>(pl.it[i].blocks) * kv * tiles_of(i);
             }
         if (!base) continue;
-        long long per = base >= g.want ? 1LL << 40 : std::max<long long>(1, work / g.want);  // tiles of a unit
+        // tiles of a unit.  Enough units already: those with much more than a CU's share are split all the same (six bf16
+        // prompts of 101 to 1501 rows after 3001 to 1 positions, with weights: 139 us, 153 without)
+        long long per = base >= g.want ? std::max<long long>(8, work * 5 / (g.want * 4)) : std::max<long long>(1, work / g.want);
         auto units = [&](long long per_) {
             long long u = 0;
             for (int i = 0; i < a.n; ++i)
@@ -260,9 +262,16 @@ hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* work
     }
     const int kv = a.geom.kv_heads;
     // the chunks that `in` takes, with a launch's blocks and splits
-    auto gather = [&](auto in, bool weights) {
+    // (tile kernels: per kv head, the chunks with the longest units first)
+    int order[kBatch];
+    for (int i = 0; i < a.n; ++i) order[i] = i;
+    std::stable_sort(order, order + a.n, [&](int x, int y) {
+        return static_cast<long long>(a.it[x].pos0 + a.it[x].rows) * plan.it[y].splits > static_cast<long long>(a.it[y].pos0 + a.it[y].rows) * plan.it[x].splits;
+    });
+    auto gather = [&](auto in, bool weights, bool per_head = false) {
         k.n = k.units = 0;
-        for (int i = 0; i < a.n; ++i) {
+        for (int o = 0; o < a.n; ++o) {
+            const int i = per_head ? order[o] : o;
             const ChunkPlanItem& pi = plan.it[i];
             if (!in(pi)) continue;
             ChunkItem& it = k.it[k.n++];
@@ -272,13 +281,13 @@ hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* work
             it.splits = weights ? pi.wsplits : pi.splits;
             it.slot0 = static_cast<int>(weights ? pi.wslot0 : pi.slot0);
             it.score0 = pi.score0;
-            k.units += it.blocks * it.splits * kv;
+            k.units += it.blocks * it.splits * (per_head ? 1 : kv);
         }
         return k.n > 0;
     };
     hipError_t e = hipSuccess;
     for (int kind = 0; kind < kChunkKinds && e == hipSuccess; ++kind) {
-        if (!gather([&](const ChunkPlanItem& p) { return p.kind == kind; }, false)) continue;
+        if (!gather([&](const ChunkPlanItem& p) { return p.kind == kind; }, false, kind >= kChunkTile)) continue;
         k.scores = a.weights && (kind == kChunkStream32 || kind == kChunkF32Half) ? reinterpret_cast<float*>(w + plan.scores) : nullptr;
         e = kind == kChunkAny ? launch_chunks_any(k, stream) : kind >= kChunkF32Half ? launch_chunks_f32(k, kind, stream)
           : launch_chunks_tile(k, kind, stream);

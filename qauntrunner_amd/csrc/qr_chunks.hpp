@@ -46,6 +46,28 @@ __device__ __forceinline__ void chunk_heads(const ChunksK& p, int kvh, int* h0, 
     *g = ((kvh + 1) * p.heads + kv - 1) / kv - *h0;
 }
 
+// Launch slot b of the tile kernels runs on XCD b % 8.  Where the kv heads divide among the XCDs, one takes all units of a
+// kv head (or every 8 / kv_heads-th of them): its K/V stays in one L2 and every XCD has the same share of every chunk.
+// p.units: units of one kv head, the largest chunks' first.
+__device__ __forceinline__ bool chunk_unit(const ChunksK& p, int* kvh, int* unit) {
+    const int kv = p.geom.kv_heads, b = blockIdx.x, x = b & 7, j = b >> 3;
+    if (kv % 8 == 0) {
+        *kvh = x + 8 * (j / p.units);
+        *unit = j % p.units;
+    } else if (8 % kv == 0) {
+        *kvh = x % kv;
+        *unit = j * (8 / kv) + x / kv;
+    } else {
+        *kvh = b % kv;
+        *unit = b / kv;
+    }
+    return *unit < p.units && *kvh < kv;
+}
+inline int chunk_grid(const ChunksK& p) {
+    const int kv = p.geom.kv_heads;
+    return kv % 8 && 8 % kv == 0 ? 8 * ((p.units * kv + 7) / 8) : p.units * kv;
+}
+
 // Part `split` of the positions [0, keys) in whole tiles.
 __device__ __forceinline__ void chunk_keys(const ChunkItem& it, int keys, int split, int tile, int* t0, int* t1) {
     const int tiles = (keys + tile - 1) / tile;

@@ -11,11 +11,8 @@ namespace {
 template <typename ST, int D, int PG>
 __global__ void __launch_bounds__(256, (F32Geom<ST, D>::wg_per_cu(PG))) chunks_f32_kernel(const ChunksK p) {
     __shared__ __attribute__((aligned(1024))) char lds[2][2 * F32Geom<ST, D>::KB];
-    // Launch slot b runs on XCD b % 8, which takes contiguous units: the blocks of one kv head
-    // share its K/V in the XCD's L2.  Blocks from the last, which has the most keys, down.
-    const int per_xcd = (p.units + 7) >> 3;
-    const int unit = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if ((static_cast<int>(blockIdx.x) >> 3) >= per_xcd || unit >= p.units) return;
+    int kvh, unit;
+    if (!chunk_unit(p, &kvh, &unit)) return;
     const int e = batch_find(p.n, unit, [&](int i) { return p.it[i].unit0; });
     const ChunkItem& it = p.it[e];
     const int u = unit - it.unit0;
@@ -40,7 +37,7 @@ __global__ void __launch_bounds__(256, (F32Geom<ST, D>::wg_per_cu(PG))) chunks_f
     k.row_ml = p.row_ml ? p.row_ml + row0 : nullptr;
     k.scores = p.scores && it.score0 >= 0 ? p.scores + it.score0 : nullptr;
     k.score_len = chunk_score_len(it);
-    chunk_f32_tiles<ST, D, PG, true>(k, u % it.splits, it.blocks - 1 - u / it.splits % it.blocks, u / (it.splits * it.blocks), lds);
+    chunk_f32_tiles<ST, D, PG, true>(k, u % it.splits, it.blocks - 1 - u / it.splits, kvh, lds);
 }
 
 // Weights of 128 positions of one kv head over a part of its rows: a wave keeps the K rows of 32
@@ -164,7 +161,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) chunks_f32_weights_kern
 }
 
 template <typename ST, int D> hipError_t launch_st(const ChunksK& k, int kind, hipStream_t s) {
-    const dim3 grid((k.units + 7) / 8 * 8);
+    const dim3 grid(chunk_grid(k));
     if (kind == kChunkF32Half) hipLaunchKernelGGL((chunks_f32_kernel<ST, D, 2>), grid, dim3(256), 0, s, k);
     else if (kind == kChunkF32) hipLaunchKernelGGL((chunks_f32_kernel<ST, D, 1>), grid, dim3(256), 0, s, k);
     else hipLaunchKernelGGL((chunks_f32_weights_kernel<ST, D>), dim3(k.units), dim3(256), 0, s, k);

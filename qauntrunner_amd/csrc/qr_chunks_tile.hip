@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(256, 1) chunks_stream32_kernel(const ChunksK p
     chunk_stream<BF16, D, PARTS, 1, 4, LDS>(p, it, blockIdx.x - it.unit0, lds);
 }
 // Chunks of up to 128 rows, each in its own shape: two workgroups per CU, so that one computes while the other stands
-// at a barrier (one of eight waves: XX).
+// at a barrier (one of eight waves: 111 us where this takes 102).
 template <bool BF16, int D, int PARTS>
 __global__ void __launch_bounds__(256, 2) chunks_stream_kernel(const ChunksK p) {
     constexpr int LDS = 80 * 1024;
@@ -508,15 +508,12 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
     constexpr int PER = KB / 1024 / 8;   // DMA loads per wave for a tile of K (or V)
     __shared__ __attribute__((aligned(1024))) char lds[2 * NST * KB];  // K tiles, then V tiles
 
-    // Launch slot b runs on XCD b % 8, which takes contiguous units: the blocks of one kv head
-    // share its K/V in the XCD's L2.  Blocks from the last, which has the most keys, down.
-    const int per_xcd = (p.units + 7) >> 3;
-    const int unit = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if ((static_cast<int>(blockIdx.x) >> 3) >= per_xcd || unit >= p.units) return;
+    int kvh, unit;
+    if (!chunk_unit(p, &kvh, &unit)) return;
     const int e = batch_find(p.n, unit, [&](int i) { return p.it[i].unit0; });
     const ChunkItem it = p.it[e];
     const int u = unit - it.unit0;
-    const int split = u % it.splits, block = it.blocks - 1 - u / it.splits % it.blocks, kvh = u / (it.splits * it.blocks);
+    const int split = u % it.splits, block = it.blocks - 1 - u / it.splits;  // from the last, which has the most keys, down
     const int g = p.heads / p.geom.kv_heads;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rho0 = block * 256;
@@ -847,7 +844,7 @@ hipError_t launch_kind(const ChunksK& k, int kind, hipStream_t s) {
     switch (kind) {
         case kChunkStream32: hipLaunchKernelGGL((chunks_stream32_kernel<BF16, D, PARTS>), dim3(k.units), dim3(256), 0, s, k); break;
         case kChunkStream: hipLaunchKernelGGL((chunks_stream_kernel<BF16, D, PARTS>), dim3(k.units), dim3(256), 0, s, k); break;
-        case kChunkTile: hipLaunchKernelGGL((chunks_tile_kernel<BF16, D, SPLIT>), dim3((k.units + 7) / 8 * 8), dim3(512), 0, s, k); break;
+        case kChunkTile: hipLaunchKernelGGL((chunks_tile_kernel<BF16, D, SPLIT>), dim3(chunk_grid(k)), dim3(512), 0, s, k); break;
         default: hipLaunchKernelGGL((chunks_tile_weights_kernel<BF16, D, SPLIT>), dim3(k.units), dim3(512), 0, s, k); break;
     }
     return hipGetLastError();

@@ -34,10 +34,13 @@ __device__ __forceinline__ int block_scan(int x, int* wsum) {
     return x;
 }
 
+// The weight of a key (any NaN for 0).
+__device__ __forceinline__ float key_weight(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+
 // One workgroup per (entry, kv head): the key of the last position taken, digit by digit from the
 // top (11, 11 and 10 bits: counts in LDS, then a scan from the largest digit down), then the kept positions in order.
-// The keys stay in registers, C per thread; C = 0: longer rows, read from L2 in every pass.  A wave whose keys have the
-// same digit counts them with one atomic (whole rows of equal weights would queue 64 on one address).
+// The weights stay in registers, C per thread; C = 0: longer rows, read from L2 in every pass.  Bound by the instructions
+// of its one CU.
 template <int C>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
     constexpr int kWaves = kSelThreads / 64, kBins = 2048;
@@ -79,16 +82,11 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
             for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
             __syncthreads();
             auto count = [&](int c) __attribute__((always_inline)) {
+                if (c * kSelThreads >= hi) return;
                 const int i = c * kSelThreads + tid;
                 const uint32_t k = weight_key(value(c, i));
-                const bool in = i >= lo && i < hi && (k & mask) == prefix;
-                const uint64_t act = __builtin_amdgcn_ballot_w64(in);
-                if (!act) return;
-                const int d = (k >> kShift[pass]) & ((1 << kBits[pass]) - 1);
-                const int d0 = __shfl(d, __ffsll(static_cast<unsigned long long>(act)) - 1);
-                const uint64_t same = __builtin_amdgcn_ballot_w64(in && d == d0);
-                if (lane == 0) atomicAdd(&hist[d0], static_cast<int>(__popcll(same)));
-                if (in && d != d0) atomicAdd(&hist[d], 1);
+                if (static_cast<uint32_t>(i - lo) < static_cast<uint32_t>(hi - lo) && (k & mask) == prefix)
+                    atomicAdd(&hist[(k >> kShift[pass]) & ((1 << kBits[pass]) - 1)], 1);
             };
             if (C > 0) {
 #pragma unroll
@@ -113,11 +111,13 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     }
     // in order: the positions outside the candidates, those above the key, and the first `need` of those that equal it.
     // With A the former two and E the last before a position, it goes to slot A + min(E, need).
+    const float T = a.heavy > 0 ? key_weight(prefix) : INFINITY;
+    const bool nan = a.heavy > 0 && prefix == 0;  // even some NaN stay: the numbers do before them
     auto flags = [&](int c, int i, bool* sure, bool* eq) __attribute__((always_inline)) {
-        const uint32_t k = weight_key(value(c, i));
-        const bool cand = i >= lo && i < hi;
-        *sure = i < it.len && (!cand || (a.heavy > 0 && k > prefix));
-        *eq = cand && a.heavy > 0 && k == prefix;
+        const float v = value(c, i);
+        const bool cand = static_cast<uint32_t>(i - lo) < static_cast<uint32_t>(hi - lo);
+        *sure = cand ? (nan ? v == v : v > T) : i < it.len;
+        *eq = a.heavy > 0 && cand && (nan ? v != v : v == T);
     };
     const uint64_t below = (1ull << lane) - 1;
     if (C > 0) {
@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
         __syncthreads();
 #pragma unroll
         for (int c = 0; c < C; ++c) {
+            if (c * kSelThreads >= it.len) break;
             const int i = c * kSelThreads + tid;
             bool sure, eq;
             flags(c, i, &sure, &eq);
@@ -188,14 +189,15 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
 
 constexpr int kMoveThreads = 256;
 
-// The same for head sizes whose rows are whole 16-byte pieces, 64 bytes of a row (or what is left of it) per workgroup, 512
-// slots at a time; the next 512's positions are looked up ahead.  V of the MFMA page layout: 16 dims per workgroup, a thread
-// gathers 8 slots of a dim (16 bytes of the page).  Bound by HBM for many workgroups, else by the latency of a tile.
-template <int ES, bool MFMA>
+// The same for head sizes whose rows are whole 16-byte pieces, P of a row (or what is left of it) per workgroup, 2048 / P
+// slots at a time; the next ones are read before these are written.  V of the MFMA page layout: 16 dims per workgroup, a thread
+// gathers 8 slots of a dim (16 bytes of the page; reading ahead here costs registers and 10 us of 38).  Bound by HBM for
+// many workgroups, else by the latency of a tile.
+template <int ES, bool MFMA, int P>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArgs a) {
-    constexpr int N = 16 / ES, TILE = 512;
+    constexpr int N = 16 / ES, TILE = MFMA ? 512 : 2048 / P;
     const int D = a.geom.head_dim, pieces = D / N;
-    const int ks = (pieces + 3) / 4, vs = MFMA ? D / 16 : ks;  // workgroups of the K and the V rows of a kv head
+    const int ks = (pieces + P - 1) / P, vs = MFMA ? D / 16 : ks;  // workgroups of the K and the V rows of a kv head
     int u = blockIdx.x;
     const int part = u % (ks + vs);
     u /= ks + vs;
@@ -205,10 +207,12 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
     if (it.len <= keep) return;
     const int* const kept = a.kept + (static_cast<long long>(it.entry) * a.geom.kv_heads + kvh) * keep;
     const int* const pages = a.page_table + it.pt_off;
+    auto page = [&](int j) { return static_cast<long long>(pages[j >> kPageShift]); };
     const int plane = part >= ks, s = part - plane * ks;
     auto moved = [&](int j0) { return kept[min(j0 + TILE, keep) - 1] != min(j0 + TILE, keep) - 1; };
     int j0 = 0;
     while (j0 < keep && !moved(j0)) j0 += TILE;  // slots that keep what they hold
+    if (j0 >= keep) return;
     if (MFMA && plane) {
         constexpr int IT = 16 * TILE / 8 / kMoveThreads;
         const int d = 16 * s + (threadIdx.x & 15);
@@ -222,7 +226,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
 #pragma unroll
                 for (int k = 0; k < 8; ++k) src[k] = kept[min(j + k, keep - 1)];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) phys[k] = pages[src[k] >> kPageShift];
+                for (int k = 0; k < 8; ++k) phys[k] = page(src[k]);
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     x[c][k] = static_cast<const uint16_t*>(a.pool)[a.geom.offset(phys[k], 1, kvh, src[k] & (kPageTokens - 1), d)];
@@ -246,33 +250,42 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
         }
         return;
     }
-    constexpr int IT = 4 * TILE / kMoveThreads;
+    constexpr int IT = 8, STEP = kMoveThreads / P;
+    static_assert(IT * STEP == TILE, "whole tiles");
     // MFMA layout: consecutive lanes take consecutive slots (their pieces lie side by side), else the pieces of a slot
-    const int pc = 4 * s + (MFMA ? static_cast<int>(threadIdx.x) >> 6 : static_cast<int>(threadIdx.x) & 3);
-    const int q0 = MFMA ? threadIdx.x & 63 : threadIdx.x >> 2;
+    const int pc = P * s + static_cast<int>(MFMA ? threadIdx.x / STEP : threadIdx.x % P);
+    const int q0 = MFMA ? threadIdx.x % STEP : threadIdx.x / P;
     const bool in = pc < pieces;
+    const int piece = in ? pc : pieces - 1;  // (an idle thread reads a piece that it does not write)
     int src[IT];
+    U32x4 x[IT], y[IT];
+    char* const pool = static_cast<char*>(a.pool);
     auto look = [&](int j1) __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < IT; ++c) src[c] = kept[min(j1 + q0 + 64 * c, keep - 1)];
+        for (int c = 0; c < IT; ++c) src[c] = kept[min(j1 + q0 + STEP * c, keep - 1)];
     };
-    char* const pool = static_cast<char*>(a.pool);
-    if (j0 < keep) look(j0);
+    auto load = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < IT; ++c)
+            y[c] = load16(pool + ES * a.geom.offset(page(src[c]), plane, kvh, src[c] & (kPageTokens - 1), N * piece));
+    };
+    look(j0);
+    load();
+    look(j0 + TILE);
     for (; j0 < keep; j0 += TILE) {
-        U32x4 x[IT];
-        if (in)
 #pragma unroll
-            for (int c = 0; c < IT; ++c)
-                x[c] = load16(pool + ES * a.geom.offset(pages[src[c] >> kPageShift], plane, kvh, src[c] & (kPageTokens - 1), N * pc));
-        if (j0 + TILE < keep) look(j0 + TILE);
+        for (int c = 0; c < IT; ++c) x[c] = y[c];
+        if (j0 + TILE < keep) {
+            load();
+            look(j0 + 2 * TILE);
+        }
         __syncthreads();
-        if (in)
 #pragma unroll
-            for (int c = 0; c < IT; ++c) {
-                const int j = j0 + q0 + 64 * c;
-                if (j < keep)
-                    *reinterpret_cast<U32x4*>(pool + ES * a.geom.offset(pages[j >> kPageShift], plane, kvh, j & (kPageTokens - 1), N * pc)) = x[c];
-            }
+        for (int c = 0; c < IT; ++c) {
+            const int j = j0 + q0 + STEP * c;
+            if (in && j < keep)
+                *reinterpret_cast<U32x4*>(pool + ES * a.geom.offset(page(j), plane, kvh, j & (kPageTokens - 1), N * pc)) = x[c];
+        }
     }
 }
 
@@ -331,16 +344,22 @@ hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
     const dim3 grid(rows), block(kSelThreads);
     if (longest <= 4 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<4>, grid, block, 0, stream, a);
     else if (longest <= 16 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<16>, grid, block, 0, stream, a);
+    else if (longest <= 32 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<32>, grid, block, 0, stream, a);
     else if (longest <= 64 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<64>, grid, block, 0, stream, a);
     else hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !longest) return e;
-    const int D = a.geom.head_dim, n = 16 / dtype_size(a.dtype), ks = (D / n + 3) / 4;
+    // four pieces of a row per workgroup, two where that leaves CUs idle (8192 of 65536 fp32 positions
+    // kept: 74 us, 103 with four)
+    const int D = a.geom.head_dim, n = 16 / dtype_size(a.dtype), ks4 = (D / n + 3) / 4, ks2 = (D / n + 1) / 2;
     const dim3 mblock(kMoveThreads);
+    const bool two = rows * 2 * ks4 < 512;
     if (D % n) hipLaunchKernelGGL(evict_move_any_kernel, dim3(rows * 2 * ((D + 7) / 8)), mblock, 0, stream, a);
-    else if (a.geom.mfma_layout) hipLaunchKernelGGL((evict_move_kernel<2, true>), dim3(rows * (ks + D / 16)), mblock, 0, stream, a);
-    else if (a.dtype == QR_DTYPE_F32) hipLaunchKernelGGL((evict_move_kernel<4, false>), dim3(rows * 2 * ks), mblock, 0, stream, a);
-    else hipLaunchKernelGGL((evict_move_kernel<2, false>), dim3(rows * 2 * ks), mblock, 0, stream, a);
+    else if (a.geom.mfma_layout) hipLaunchKernelGGL((evict_move_kernel<2, true, 4>), dim3(rows * (ks4 + D / 16)), mblock, 0, stream, a);
+    else if (a.dtype == QR_DTYPE_F32 && two) hipLaunchKernelGGL((evict_move_kernel<4, false, 2>), dim3(rows * 2 * ks2), mblock, 0, stream, a);
+    else if (a.dtype == QR_DTYPE_F32) hipLaunchKernelGGL((evict_move_kernel<4, false, 4>), dim3(rows * 2 * ks4), mblock, 0, stream, a);
+    else if (two) hipLaunchKernelGGL((evict_move_kernel<2, false, 2>), dim3(rows * 2 * ks2), mblock, 0, stream, a);
+    else hipLaunchKernelGGL((evict_move_kernel<2, false, 4>), dim3(rows * 2 * ks4), mblock, 0, stream, a);
     return hipGetLastError();
 }
 
