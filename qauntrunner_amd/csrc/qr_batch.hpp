@@ -158,6 +158,8 @@ struct EvictArgs {
     int max_seq;
     int* kept;               // [entries][kv_heads][first + heavy + recent]
 };
-hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
+size_t evict_workspace_bytes(const EvictArgs& a);  // 0: it takes none
+// workspace null: each row by one workgroup
+hipError_t launch_evict(const EvictArgs& a, void* workspace, hipStream_t stream);
 
 }  // namespace qr

@@ -265,7 +265,11 @@ int qr_kv_evict_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* 
         a.kept = kept_dev;
         for (int i = 0; i < n;) {
             for (a.n = 0; i < n && a.n < kBatch; ++i) a.it[a.n++] = {kv->store.pt_offset(seq_ids[i], layer), seq_ids[i], len[i], i};
-            QR_HIP(launch_evict(a, st));
+            // a captured call cannot grow the workspace: without room for it, each row is selected by one workgroup
+            const size_t bytes = evict_workspace_bytes(a);
+            const bool room = !capturing(st) || kv->workspace.size() >= bytes;
+            if (room && bytes) QR_TRY(grow_workspace(kv, bytes, st));
+            QR_HIP(launch_evict(a, room && bytes ? kv->workspace.get() : nullptr, st));
         }
         return QR_OK;
     });

@@ -37,16 +37,77 @@ __device__ __forceinline__ int block_scan(int x, int* wsum) {
 // The weight of a key (any NaN for 0).
 __device__ __forceinline__ float key_weight(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
+// The digits of a key, from the top.
+constexpr int kBins = 2048;
+__device__ constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
+__device__ __forceinline__ uint32_t digits_above(int pass) { return pass ? ~0u << kShift[pass - 1] : 0u; }
+
+// Which positions stay: `sure` those outside the candidates and those above the key, and the first `need` of `eq`, that
+// equal it.  With A of the former and E of the latter before a position, it goes to slot A + min(E, need).
+struct Stay {
+    int lo, hi, len, heavy;
+    uint32_t key;
+    __device__ __forceinline__ bool candidate(int i) const { return static_cast<uint32_t>(i - lo) < static_cast<uint32_t>(hi - lo); }
+    __device__ __forceinline__ void operator()(int i, float v, bool* sure, bool* eq) const {
+        const float T = heavy > 0 ? key_weight(key) : INFINITY;
+        const bool nan = heavy > 0 && key == 0;  // even some NaN stay: the numbers do before them
+        const bool cand = candidate(i);
+        *sure = cand ? (nan ? v == v : v > T) : i < len;
+        *eq = heavy > 0 && cand && (nan ? v != v : v == T);
+    }
+};
+
+// In order: x holds the weights of positions c * 1024 + thread + p0, A and E stand before p0.  out may hold the weights read.
+template <int C>
+__device__ __forceinline__ void place(const Stay& stay, const float (&x)[C], int p0, int A, int E, int need, int (&before)[2][C * kSelThreads / 64],
+                                      int* wsum, int* kept, float* out) {
+    constexpr int kWaves = kSelThreads / 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        bool sure, eq;
+        stay(p0 + c * kSelThreads + tid, x[c], &sure, &eq);
+        const uint64_t bs = __builtin_amdgcn_ballot_w64(sure), be = __builtin_amdgcn_ballot_w64(eq);
+        if (lane == 0) {
+            before[0][c * kWaves + wave] = __popcll(bs);
+            before[1][c * kWaves + wave] = __popcll(be);
+        }
+    }
+    __syncthreads();  // every weight is read
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int v = tid < C * kWaves ? before[q][tid] : 0;
+        const int s = block_scan(v, wsum) - v;
+        if (tid < C * kWaves) before[q][tid] = s;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int i = p0 + c * kSelThreads + tid;
+        if (p0 + c * kSelThreads >= stay.len) break;
+        bool sure, eq;
+        stay(i, x[c], &sure, &eq);
+        const uint64_t bs = __builtin_amdgcn_ballot_w64(sure), be = __builtin_amdgcn_ballot_w64(eq);
+        const int e = E + before[1][c * kWaves + wave] + __popcll(be & below);
+        const int at = A + before[0][c * kWaves + wave] + __popcll(bs & below) + min(e, need);
+        if (sure || (eq && e < need)) {
+            kept[at] = i;
+            out[at] = x[c];
+        }
+    }
+}
+
 // One workgroup per (entry, kv head): the key of the last position taken, digit by digit from the
 // top (11, 11 and 10 bits: counts in LDS, then a scan from the largest digit down), then the kept positions in order.
 // The weights stay in registers, C per thread; C = 0: longer rows, read from L2 in every pass.  Bound by the instructions
 // of its one CU.
 template <int C>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictArgs a) {
-    constexpr int kWaves = kSelThreads / 64, kBins = 2048;
+    constexpr int kWaves = kSelThreads / 64;
     __shared__ int hist[kBins];
     __shared__ int wsum[kWaves];
-    __shared__ int before[2][C > 0 ? C * kWaves : 1];
+    __shared__ int before[2][(C > 0 ? C : 1) * kWaves];
     __shared__ uint32_t sh_prefix;
     __shared__ int sh_need;
     const int kvh = blockIdx.x % a.geom.kv_heads;
@@ -73,10 +134,9 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
             x[c] = i < it.len ? w[i] : 0.f;
         }
     auto value = [&](int c, int i) { return C > 0 ? x[C > 0 ? c : 0] : i < it.len ? w[i] : 0.f; };
-    uint32_t prefix = 0, mask = 0;
+    uint32_t prefix = 0;
     int need = a.heavy;
     if (need > 0) {
-        constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
 #pragma unroll
         for (int pass = 0; pass < 3; ++pass) {
             for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
@@ -85,7 +145,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
                 if (c * kSelThreads >= hi) return;
                 const int i = c * kSelThreads + tid;
                 const uint32_t k = weight_key(value(c, i));
-                if (static_cast<uint32_t>(i - lo) < static_cast<uint32_t>(hi - lo) && (k & mask) == prefix)
+                if (static_cast<uint32_t>(i - lo) < static_cast<uint32_t>(hi - lo) && (k & digits_above(pass)) == prefix)
                     atomicAdd(&hist[(k >> kShift[pass]) & ((1 << kBits[pass]) - 1)], 1);
             };
             if (C > 0) {
@@ -106,61 +166,20 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
             __syncthreads();
             prefix = sh_prefix;
             need = sh_need;
-            mask |= ((1u << kBits[pass]) - 1) << kShift[pass];
         }
     }
-    // in order: the positions outside the candidates, those above the key, and the first `need` of those that equal it.
-    // With A the former two and E the last before a position, it goes to slot A + min(E, need).
-    const float T = a.heavy > 0 ? key_weight(prefix) : INFINITY;
-    const bool nan = a.heavy > 0 && prefix == 0;  // even some NaN stay: the numbers do before them
-    auto flags = [&](int c, int i, bool* sure, bool* eq) __attribute__((always_inline)) {
-        const float v = value(c, i);
-        const bool cand = static_cast<uint32_t>(i - lo) < static_cast<uint32_t>(hi - lo);
-        *sure = cand ? (nan ? v == v : v > T) : i < it.len;
-        *eq = a.heavy > 0 && cand && (nan ? v != v : v == T);
-    };
-    const uint64_t below = (1ull << lane) - 1;
+    const Stay stay{lo, hi, it.len, a.heavy, prefix};
     if (C > 0) {
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            bool sure, eq;
-            flags(c, c * kSelThreads + tid, &sure, &eq);
-            const uint64_t bs = __builtin_amdgcn_ballot_w64(sure), be = __builtin_amdgcn_ballot_w64(eq);
-            if (lane == 0) {
-                before[0][C > 0 ? c * kWaves + wave : 0] = __popcll(bs);
-                before[1][C > 0 ? c * kWaves + wave : 0] = __popcll(be);
-            }
-        }
-        __syncthreads();  // every weight is read
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const int v = tid < C * kWaves ? before[q][C > 0 ? tid : 0] : 0;
-            const int s = block_scan(v, wsum) - v;
-            if (tid < C * kWaves) before[q][C > 0 ? tid : 0] = s;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (c * kSelThreads >= it.len) break;
-            const int i = c * kSelThreads + tid;
-            bool sure, eq;
-            flags(c, i, &sure, &eq);
-            const uint64_t bs = __builtin_amdgcn_ballot_w64(sure), be = __builtin_amdgcn_ballot_w64(eq);
-            const int e = before[1][C > 0 ? c * kWaves + wave : 0] + __popcll(be & below);
-            const int at = before[0][C > 0 ? c * kWaves + wave : 0] + __popcll(bs & below) + min(e, need);
-            if (sure || (eq && e < need)) {
-                kept[at] = i;
-                ow[at] = value(c, i);
-            }
-        }
+        place(stay, x, 0, 0, 0, need, before, wsum, kept, ow);
     } else {
         __shared__ int cnt[2][kWaves];
+        const uint64_t below = (1ull << lane) - 1;
         int sure_before = 0, eq_before = 0;
         for (int c = 0; c < chunks; ++c) {
             const int i = c * kSelThreads + tid;
             const float v = value(c, i);
             bool sure, eq;
-            flags(c, i, &sure, &eq);
+            stay(i, v, &sure, &eq);
             const uint64_t bs = __builtin_amdgcn_ballot_w64(sure), be = __builtin_amdgcn_ballot_w64(eq);
             if (lane == 0) {
                 cnt[0][wave] = __popcll(bs);
@@ -187,6 +206,133 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictAr
     for (int i = keep + tid; i < it.len; i += kSelThreads) ow[i] = 0.f;
 }
 
+// ---- long rows: one workgroup per kPart positions of a row, the digits counted by a launch each
+constexpr int kPartC = 8, kPart = kPartC * kSelThreads;
+
+// The workspace: digit counts of [row][digit][part], per (row, digit) the key's digits up to there and what is
+// still to be taken, per (row, digit, part) the candidates before the part that lie above it, and the kept weights.
+struct Parts {
+    int n;  // of the longest row
+    int* counts;
+    int2* state;
+    int* above;
+    float* staged;
+    __device__ __forceinline__ int* at(int row, int pass, int part) const { return counts + ((static_cast<long long>(row) * 3 + pass) * n + part) * kBins; }
+};
+
+// From the counts of all parts: the digit of `pass`, what is still to be taken, the candidates in the parts before this
+// one that lie above the digit, and (`equal`) those that have it.
+struct Digit {
+    uint32_t prefix;
+    int need, above, equal;
+};
+__device__ __forceinline__ Digit find_digit(const Parts& w, int row, int parts, int part, int pass, uint32_t prefix, int need, int* wsum) {
+    __shared__ Digit found;
+    const int tid = threadIdx.x, top = kBins - 1 - 2 * tid;
+    int h1 = 0, h0 = 0, b1 = 0, b0 = 0;
+#pragma unroll 8
+    for (int g = 0; g < parts; ++g) {
+        const int2 h = *reinterpret_cast<const int2*>(w.at(row, pass, g) + top - 1);
+        h0 += h.x;
+        h1 += h.y;
+        if (g < part) {
+            b0 += h.x;
+            b1 += h.y;
+        }
+    }
+    const int upto = block_scan(h1 + h0, wsum), above = upto - h1 - h0;
+    const int bupto = block_scan(b1 + b0, wsum);
+    if (above < need && need <= upto) {
+        const bool first = need <= above + h1;
+        found = {prefix | static_cast<uint32_t>(first ? top : top - 1) << kShift[pass], need - above - (first ? 0 : h1),
+                 bupto - b0 - (first ? b1 : 0), first ? b1 : b0};
+    }
+    __syncthreads();
+    return found;
+}
+
+template <int PASS>
+__global__ void __launch_bounds__(kSelThreads) evict_count_kernel(const EvictArgs a, const Parts w) {
+    __shared__ int hist[kBins];
+    __shared__ int wsum[kSelThreads / 64];
+    const int part = blockIdx.x % w.n, row = blockIdx.x / w.n, kvh = row % a.geom.kv_heads;
+    const EvictItem it = a.it[row / a.geom.kv_heads];
+    const int keep = a.first + a.heavy + a.recent, parts = (it.len + kPart - 1) / kPart;
+    if (it.len <= keep || part >= parts) return;
+    const float* const wt = a.weights + (static_cast<long long>(it.seq) * a.geom.kv_heads + kvh) * a.max_seq;
+    const int tid = threadIdx.x, lo = a.first, hi = it.len - a.recent;
+    float x[kPartC];
+#pragma unroll
+    for (int c = 0; c < kPartC; ++c) {
+        const int i = part * kPart + c * kSelThreads + tid;
+        x[c] = i < it.len ? wt[i] : 0.f;
+    }
+    uint32_t prefix = 0;
+    if (PASS > 0) {
+        const int2 s = PASS > 1 ? w.state[row * 2] : make_int2(0, a.heavy);
+        const Digit d = find_digit(w, row, parts, part, PASS - 1, static_cast<uint32_t>(s.x), s.y, wsum);
+        prefix = d.prefix;
+        if (tid == 0) {
+            if (part == 0) w.state[row * 2 + PASS - 1] = make_int2(static_cast<int>(d.prefix), d.need);
+            w.above[(row * 2 + PASS - 1) * w.n + part] = d.above;
+        }
+    }
+    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kPartC; ++c) {
+        const int i = part * kPart + c * kSelThreads + tid;
+        const uint32_t k = weight_key(x[c]);
+        if (static_cast<uint32_t>(i - lo) < static_cast<uint32_t>(hi - lo) && (k & digits_above(PASS)) == prefix)
+            atomicAdd(&hist[(k >> kShift[PASS]) & ((1 << kBits[PASS]) - 1)], 1);
+    }
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kSelThreads) w.at(row, PASS, part)[i] = hist[i];
+}
+
+__global__ void __launch_bounds__(kSelThreads) evict_place_kernel(const EvictArgs a, const Parts w) {
+    __shared__ int wsum[kSelThreads / 64];
+    __shared__ int before[2][kPartC * kSelThreads / 64];
+    const int part = blockIdx.x % w.n, row = blockIdx.x / w.n, kvh = row % a.geom.kv_heads;
+    const EvictItem it = a.it[row / a.geom.kv_heads];
+    const int keep = a.first + a.heavy + a.recent, parts = (it.len + kPart - 1) / kPart;
+    int* const kept = a.kept + (static_cast<long long>(it.entry) * a.geom.kv_heads + kvh) * keep;
+    const int tid = threadIdx.x, p0 = part * kPart;
+    if (it.len <= keep) {  // nothing leaves
+        if (part == 0)
+            for (int i = tid; i < keep; i += kSelThreads) kept[i] = i < it.len ? i : -1;
+        return;
+    }
+    if (part >= parts) return;
+    const float* const wt = a.weights + (static_cast<long long>(it.seq) * a.geom.kv_heads + kvh) * a.max_seq;
+    const int lo = a.first, hi = it.len - a.recent;
+    float x[kPartC];
+#pragma unroll
+    for (int c = 0; c < kPartC; ++c) {
+        const int i = p0 + c * kSelThreads + tid;
+        x[c] = i < it.len ? wt[i] : 0.f;
+    }
+    Digit d{0, 0, 0, 0};
+    if (a.heavy > 0) {
+        const int2 s = w.state[row * 2 + 1];
+        d = find_digit(w, row, parts, part, 2, static_cast<uint32_t>(s.x), s.y, wsum);
+        d.above += w.above[row * 2 * w.n + part] + w.above[(row * 2 + 1) * w.n + part];
+    }
+    place(Stay{lo, hi, it.len, a.heavy, d.prefix}, x, p0, min(p0, lo) + max(p0 - hi, 0) + d.above, d.equal, d.need, before, wsum, kept,
+          w.staged + static_cast<long long>(row) * keep);
+}
+
+// kept_weights may be weights: written once all are read
+__global__ void __launch_bounds__(256) evict_weights_kernel(const EvictArgs a, const Parts w) {
+    const int blocks = kPart / 256 * w.n, row = blockIdx.x / blocks, kvh = row % a.geom.kv_heads;
+    const EvictItem it = a.it[row / a.geom.kv_heads];
+    const int keep = a.first + a.heavy + a.recent, i = blockIdx.x % blocks * 256 + threadIdx.x;
+    if (i >= it.len) return;
+    const long long at = (static_cast<long long>(it.seq) * a.geom.kv_heads + kvh) * a.max_seq + i;
+    if (it.len > keep) a.kept_weights[at] = i < keep ? w.staged[static_cast<long long>(row) * keep + i] : 0.f;
+    else if (a.kept_weights != a.weights) a.kept_weights[at] = a.weights[at];
+}
+
 constexpr int kMoveThreads = 256;
 
 // The same for head sizes whose rows are whole 16-byte pieces, P of a row (or what is left of it) per workgroup, 2048 / P
@@ -198,9 +344,9 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArg
     constexpr int N = 16 / ES, TILE = MFMA ? 512 : 2048 / P;
     const int D = a.geom.head_dim, pieces = D / N;
     const int ks = (pieces + P - 1) / P, vs = MFMA ? D / 16 : ks;  // workgroups of the K and the V rows of a kv head
-    int u = blockIdx.x;
-    const int part = u % (ks + vs);
-    u /= ks + vs;
+    // plain pages: the parts of a row run on one XCD where the rows are whole eights, whose L2 joins their pieces to lines
+    const int rows = gridDim.x / (ks + vs);
+    const int part = MFMA ? blockIdx.x % (ks + vs) : blockIdx.x / rows, u = MFMA ? blockIdx.x / (ks + vs) : blockIdx.x % rows;
     const int kvh = u % a.geom.kv_heads;
     const EvictItem it = a.it[u / a.geom.kv_heads];
     const int keep = a.first + a.heavy + a.recent;
@@ -335,22 +481,61 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_any_kernel(const Evic
 
 }  // namespace
 
-hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
-    if (!a.n) return hipSuccess;
-    const int rows = a.n * a.geom.kv_heads, keep = a.first + a.heavy + a.recent;
-    int longest = 0;
+namespace {
+struct EvictShape {
+    int rows, keep, longest;  // of the entries that give positions up
+    int parts;                // workgroups per row, 0: one
+};
+// Rows of more than 32768 positions are shared by workgroups while the counts stay in L2 (8 rows of 65536: 34 us, one
+// workgroup each 93; 128 rows of up to 17000: 40 us, 27)
+EvictShape evict_shape(const EvictArgs& a) {
+    EvictShape s{a.n * a.geom.kv_heads, a.first + a.heavy + a.recent, 0, 0};
     for (int i = 0; i < a.n; ++i)
-        if (a.it[i].len > keep) longest = std::max(longest, a.it[i].len);
+        if (a.it[i].len > s.keep) s.longest = std::max(s.longest, a.it[i].len);
+    const long long parts = (s.longest + kPart - 1) / kPart;
+    if (parts > 4 && s.rows * parts <= 512) s.parts = static_cast<int>(parts);
+    return s;
+}
+}  // namespace
+
+size_t evict_workspace_bytes(const EvictArgs& a) {
+    const EvictShape s = evict_shape(a);
+    return 4 * static_cast<size_t>(s.rows) * (s.parts ? static_cast<size_t>(s.parts) * (3 * kBins + 2) + 4 + s.keep : 0);
+}
+
+hipError_t launch_evict(const EvictArgs& a, void* workspace, hipStream_t stream) {
+    if (!a.n) return hipSuccess;
+    const EvictShape sh = evict_shape(a);
+    const int rows = sh.rows, longest = sh.longest;
     const dim3 grid(rows), block(kSelThreads);
-    if (longest <= 4 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<4>, grid, block, 0, stream, a);
-    else if (longest <= 16 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<16>, grid, block, 0, stream, a);
-    else if (longest <= 32 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<32>, grid, block, 0, stream, a);
-    else if (longest <= 64 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<64>, grid, block, 0, stream, a);
-    else hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, stream, a);
+    if (sh.parts && workspace) {
+        Parts w{sh.parts, static_cast<int*>(workspace), nullptr, nullptr, nullptr};
+        w.state = reinterpret_cast<int2*>(w.counts + static_cast<size_t>(rows) * 3 * w.n * kBins);
+        w.above = reinterpret_cast<int*>(w.state + 2 * rows);
+        w.staged = reinterpret_cast<float*>(w.above + 2 * rows * w.n);
+        const dim3 pgrid(rows * w.n);
+        if (a.heavy > 0) {
+            hipLaunchKernelGGL(evict_count_kernel<0>, pgrid, block, 0, stream, a, w);
+            hipLaunchKernelGGL(evict_count_kernel<1>, pgrid, block, 0, stream, a, w);
+            hipLaunchKernelGGL(evict_count_kernel<2>, pgrid, block, 0, stream, a, w);
+        }
+        hipLaunchKernelGGL(evict_place_kernel, pgrid, block, 0, stream, a, w);
+        hipLaunchKernelGGL(evict_weights_kernel, dim3(rows * w.n * (kPart / 256)), dim3(256), 0, stream, a, w);
+    } else if (longest <= 4 * kSelThreads) {
+        hipLaunchKernelGGL(evict_select_kernel<4>, grid, block, 0, stream, a);
+    } else if (longest <= 16 * kSelThreads) {
+        hipLaunchKernelGGL(evict_select_kernel<16>, grid, block, 0, stream, a);
+    } else if (longest <= 32 * kSelThreads) {
+        hipLaunchKernelGGL(evict_select_kernel<32>, grid, block, 0, stream, a);
+    } else if (longest <= 64 * kSelThreads) {
+        hipLaunchKernelGGL(evict_select_kernel<64>, grid, block, 0, stream, a);
+    } else {
+        hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, stream, a);
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !longest) return e;
     // four pieces of a row per workgroup, two where that leaves CUs idle (8192 of 65536 fp32 positions
-    // kept: 74 us, 103 with four)
+    // kept: 59 us, 96 with four)
     const int D = a.geom.head_dim, n = 16 / dtype_size(a.dtype), ks4 = (D / n + 3) / 4, ks2 = (D / n + 1) / 2;
     const dim3 mblock(kMoveThreads);
     const bool two = rows * 2 * ks4 < 512;

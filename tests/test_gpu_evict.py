@@ -93,6 +93,49 @@ def test_long(gpu, dtype, D):
         check(kv, rows, [1, 0], [9000, n], 4, 5000, 1000, randn(4, 2, 2, n).exp())
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("kind", ["plain", "equal", "special"])
+@pytest.mark.parametrize("first,heavy,recent", [(4, 9000, 1000), (0, 20000, 0), (9000, 0, 100), (0, 1, 9000), (1, 1, 20000)])
+def test_rows_of_several_workgroups(gpu, kind, first, heavy, recent, in_place):
+    n = 40007
+    kv, rows = filled(3, 2, 8, "f32", [n, 17000, 900])
+    with kv:
+        w = randn(4, 3, 2, n).exp()
+        if kind == "equal":
+            w = (w * 0).add_(0.25)
+            w[0, 0, 30000:] = 0.5
+        elif kind == "special":
+            w[0, 0, ::2] = float("nan")
+            w[0, 0, 1::7] = float("inf")
+            w[0, 1] = float("nan")
+            w[1, 0, ::3] *= -1
+        check(kv, rows, [1, 2, 0], [17000, 900, n], first, heavy, recent, w, in_place)
+
+
+@pytest.mark.parametrize("first,heavy,recent", [(4, 9000, 1000), (0, 69998, 1)])
+def test_captured_first(gpu, first, heavy, recent):
+    """Captured with no call before: no workspace to share rows with."""
+    n = 70001
+    kv, rows = filled(1, 1, 8, "f32", [n])
+    with kv:
+        w, out, w0 = randn(4, 1, 1, n).exp(), randn(5, 1, 1, n), randn(6, 1, 1, n)
+        keep = first + heavy + recent
+        kept = torch.zeros(1, 1, keep, dtype=torch.int32, device="cuda")
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            kv.EvictDev(0, [0], [n], first, heavy, recent, w0, kept, kept_weights=out)
+        w0.copy_(w)
+        g.replay()
+        want = kept_of(w[0, 0].tolist(), n, first, heavy, recent)
+        assert kept[0, 0].tolist() == want
+        idx = torch.tensor(want, device="cuda")
+        assert torch.equal(out[0, 0, :keep], w[0, 0, idx]) and not out[0, 0, keep:].any()
+        ko, vo = (torch.empty(keep, 8, device="cuda") for _ in range(2))
+        kv.ReadDev(0, [0], [0], [keep], ko, vo)
+        assert torch.equal(ko, rows[0][0][idx, 0]) and torch.equal(vo, rows[0][1][idx, 0])
+
+
 def test_more_sequences_than_one_launch_takes(gpu):
     n = 70
     lengths = [20 + (i * 13) % 90 for i in range(n)]
