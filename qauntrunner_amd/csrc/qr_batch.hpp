@@ -26,9 +26,17 @@ __device__ __forceinline__ float load_elem(const void* p, int dtype, long long i
     const uint16_t u = static_cast<const uint16_t*>(p)[i];
     return dtype == QR_DTYPE_F16 ? f16_bits_to_f32(u) : bf16_bits_to_f32(u);
 }
+// (fp16: f32_to_f16_bits_ref without its branches; below 2^-14 both round to nearest even)
 __device__ __forceinline__ uint16_t f32_to_bits16(float x, int dtype) {
-    if (dtype == QR_DTYPE_F16) return f32_to_f16_bits_ref(x);
-    return x == x ? f32_to_bf16_bits_ref(x) : static_cast<uint16_t>((__float_as_uint(x) >> 16) | 0x40u);
+    if (dtype == QR_DTYPE_F16) {
+        const uint32_t b = __float_as_uint(x), a = b & 0x7FFFFFFFu;
+        const uint32_t normal = min((a - 0x37FFF000u) >> 13, 0x7C00u), small = __half_as_ushort(__float2half(__uint_as_float(a)));
+        return static_cast<uint16_t>((b >> 16 & 0x8000u) | (a > 0x7F800000u ? 0x7E00u : a < 0x38800000u ? small : normal));
+    }
+    uint16_t u;
+    const __bf16 y = static_cast<__bf16>(x);  // (nearest even)
+    __builtin_memcpy(&u, &y, 2);
+    return u;
 }
 __device__ __forceinline__ void store_elem(void* p, int dtype, long long i, float x) {
     if (dtype == QR_DTYPE_F32) static_cast<float*>(p)[i] = x;

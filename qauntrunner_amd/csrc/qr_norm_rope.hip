@@ -11,6 +11,7 @@
 #include "qr_batch.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace qr {
 namespace {
@@ -92,38 +93,30 @@ __device__ __forceinline__ Item item_of(int j, int rot) {
     if (8 * j < rot) return {4 * j, 4 * j + rot / 2, true};
     return {8 * j, 8 * j + 4, false};
 }
-template <bool A32> struct Run;  // 4 consecutive values, element-aligned
-template <> struct Run<true> {
-    float v[4];
-    __device__ __forceinline__ void load(const void* p, long long at) { __builtin_memcpy(v, static_cast<const float*>(p) + at, 16); }
-    __device__ __forceinline__ void widen(int, float (&x)[8], int o) const {
+template <int T> struct Run {  // 4 consecutive values of dtype T, element-aligned
+    typedef typename std::conditional<T == QR_DTYPE_F32, float, uint16_t>::type E;
+    E v[4];
+    __device__ __forceinline__ void load(const void* p, long long at) { __builtin_memcpy(v, static_cast<const E*>(p) + at, sizeof(v)); }
+    __device__ __forceinline__ void widen(float (&x)[8], int o) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[o + i] = v[i];
-    }
-};
-template <> struct Run<false> {
-    uint16_t v[4];
-    __device__ __forceinline__ void load(const void* p, long long at) { __builtin_memcpy(v, static_cast<const uint16_t*>(p) + at, 8); }
-    __device__ __forceinline__ void widen(int dtype, float (&x)[8], int o) const {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[o + i] = dtype == QR_DTYPE_BF16 ? bf16_bits_to_f32(v[i]) : f16_bits_to_f32(v[i]);
+        for (int i = 0; i < 4; ++i) x[o + i] = T == QR_DTYPE_F32 ? v[i] : T == QR_DTYPE_BF16 ? bf16_bits_to_f32(v[i]) : f16_bits_to_f32(v[i]);
     }
 };
 // 4 values to p[at .. at + 3], element-aligned
-__device__ __forceinline__ void store_run(void* p, int dtype, long long at, const float* x) {
-    if (dtype == QR_DTYPE_F32) {
+template <int T> __device__ __forceinline__ void store_run(void* p, long long at, const float* x) {
+    if (T == QR_DTYPE_F32) {
         __builtin_memcpy(static_cast<float*>(p) + at, x, 16);
     } else {
         uint16_t b[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = f32_to_bits16(x[i], dtype);
+        for (int i = 0; i < 4; ++i) b[i] = f32_to_bits16(x[i], T);
         __builtin_memcpy(static_cast<uint16_t*>(p) + at, b, 8);
     }
 }
 
 // V rows of the MFMA page layout, where 8 aligned slots of a dim are 16 bytes: a thread takes 8 dims of such a run, 8 loads
 // of 8 values and 8 stores of 16 bytes, 128 bytes in a row of the page.  Slots outside the chunk are left alone.
-template <bool A32>
+template <int ACT, int DT>
 __global__ void __launch_bounds__(kThreads) v_runs_kernel(const NormRopeArgs a) {
     const int e = batch_find(a.n, blockIdx.x, [&](int i) { return a.it[i].unit0; });
     const NormRopeItem it = a.it[e];
@@ -133,7 +126,7 @@ __global__ void __launch_bounds__(kThreads) v_runs_kernel(const NormRopeArgs a) 
     if (u >= runs * slices) return;
     const int slice = u % slices, kvh = slice / per, d0 = 8 * (slice - kvh * per);
     const int p0 = ((it.pos0 >> 3) + u / slices) << 3;  // position of the run's first slot
-    Run<A32> x[8][2];
+    Run<ACT> x[8][2];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         const int j = min(max(p0 + k - it.pos0, 0), it.rows - 1);
@@ -145,15 +138,15 @@ __global__ void __launch_bounds__(kThreads) v_runs_kernel(const NormRopeArgs a) 
     float y[8][8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        x[k][0].widen(a.act, y[k], 0);
-        x[k][1].widen(a.act, y[k], 4);
+        x[k][0].widen(y[k], 0);
+        x[k][1].widen(y[k], 4);
     }
     const bool whole = p0 >= it.pos0 && p0 + 8 <= it.pos0 + it.rows;
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
         uint16_t b[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) b[k] = f32_to_bits16(y[k][d], a.dtype);
+        for (int k = 0; k < 8; ++k) b[k] = f32_to_bits16(y[k][d], DT);
         uint16_t* o = static_cast<uint16_t*>(a.pool) + a.geom.offset(phys, 1, kvh, p0 & (kPageTokens - 1), d0 + d);
         if (whole) {
             uint4 w;
@@ -167,9 +160,11 @@ __global__ void __launch_bounds__(kThreads) v_runs_kernel(const NormRopeArgs a) 
     }
 }
 
-// One workgroup per row and gridDim.y-th part of its heads (K, then q, then V unless it goes by runs).  The loads of all of a thread's items are
-// issued before the angles are computed.  Bound by HBM, for few rows by the launch.
-template <bool A32, int IPT>
+// One workgroup per row and gridDim.y-th part of its heads (K, then q, then V unless it goes by runs).  The loads of all of
+// a thread's items are issued before the angles are computed.  Bound by HBM, for few rows by the launch: four bf16 prompts
+// of 32 / 8 heads (123 MB read and written) 31 us, of which the norms take 2 and the 16-byte pieces of K 6; runs of 8
+// values or workgroups of several rows are no faster, 16-bit types that the kernel is not compiled for cost 8.
+template <int ACT, int DT, int IPT>
 __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormRopeArgs a, int lph, int v_heads) {
     __shared__ __attribute__((aligned(16))) float cs[kMaxRopeHalf], sn[kMaxRopeHalf];
     const int D = a.geom.head_dim, kv = a.geom.kv_heads, per = D / 8;
@@ -181,10 +176,10 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormRopeArgs 
     const bool in = li < per;
     const Item im = item_of(in ? li : 0, a.rot);
     const int h0 = blockIdx.y * (kThreads / lph * IPT) + threadIdx.x / lph;
-    const int es = A32 ? 4 : 2;
+    constexpr int es = ACT == QR_DTYPE_F32 ? 4 : 2;
     const char* const rows[3] = {static_cast<const char*>(a.k) + row * a.k_stride * es, static_cast<const char*>(a.q) + row * a.q_stride * es,
                                  static_cast<const char*>(a.v) + row * a.v_stride * es};
-    Run<A32> ra[IPT], rb[IPT];
+    Run<ACT> ra[IPT], rb[IPT];
 #pragma unroll
     for (int k = 0; k < IPT; ++k) {
         const int h = min(h0 + kThreads / lph * k, heads - 1);
@@ -198,11 +193,13 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormRopeArgs 
     const long long phys = a.page_table[a.it[e].pt_off + (pos >> kPageShift)];
     float w[2][8];  // of K heads, of q heads
     const bool kn = a.k_norm, qn = a.q_norm;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = (i < 4 ? im.a : im.b - 4) + i;
-        w[0][i] = kn ? a.k_norm[d] : 1.f;
-        w[1][i] = qn ? a.q_norm[d] : 1.f;
+    if (kn) {
+        __builtin_memcpy(w[0], a.k_norm + im.a, 16);
+        __builtin_memcpy(w[0] + 4, a.k_norm + im.b, 16);
+    }
+    if (qn) {
+        __builtin_memcpy(w[1], a.q_norm + im.a, 16);
+        __builtin_memcpy(w[1] + 4, a.q_norm + im.b, 16);
     }
     __syncthreads();
     float c4[4] = {1.f, 1.f, 1.f, 1.f}, s4[4] = {0.f, 0.f, 0.f, 0.f};
@@ -215,8 +212,8 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormRopeArgs 
         const int h = h0 + kThreads / lph * k;
         const bool is_k = h < kv, is_q = !is_k && h < kv + qh;
         float x[8];
-        ra[k].widen(a.act, x, 0);
-        rb[k].widen(a.act, x, 4);
+        ra[k].widen(x, 0);
+        rb[k].widen(x, 4);
         if (is_k || is_q) {
             if (is_k ? kn : qn) {
                 float ss = 0.f;
@@ -241,16 +238,16 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormRopeArgs 
         // (q_out may be q: the loads of every item that a workgroup stores stand before the barrier)
         if (is_q) {
             const long long at = (static_cast<long long>(row) * a.heads + h - kv) * D;
-            store_run(a.q_out, a.act, at + im.a, x);
-            store_run(a.q_out, a.act, at + im.b, x + 4);
+            store_run<ACT>(a.q_out, at + im.a, x);
+            store_run<ACT>(a.q_out, at + im.b, x + 4);
         } else if (is_k || !a.geom.mfma_layout) {
             const int hh = is_k ? h : h - kv - qh;
-            store_run(a.pool, a.dtype, a.geom.offset(phys, !is_k, hh, slot, im.a), x);
-            store_run(a.pool, a.dtype, a.geom.offset(phys, !is_k, hh, slot, im.b), x + 4);
+            store_run<DT>(a.pool, a.geom.offset(phys, !is_k, hh, slot, im.a), x);
+            store_run<DT>(a.pool, a.geom.offset(phys, !is_k, hh, slot, im.b), x + 4);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                store_elem(a.pool, a.dtype, a.geom.offset(phys, 1, h - kv - qh, slot, (i < 4 ? im.a : im.b - 4) + i), x[i]);
+                store_elem(a.pool, DT, a.geom.offset(phys, 1, h - kv - qh, slot, (i < 4 ? im.a : im.b - 4) + i), x[i]);
         }
     }
 }
@@ -331,11 +328,20 @@ template <class Args> int v_run_groups(Args& a) {
     return groups;
 }
 
-template <bool A32> void launch_ipt(const NormRopeArgs& a, int ipt, dim3 grid, int lph, int v_heads, hipStream_t s) {
-    if (ipt == 1) hipLaunchKernelGGL((norm_rope_kernel<A32, 1>), grid, dim3(kThreads), 0, s, a, lph, v_heads);
-    else if (ipt == 2) hipLaunchKernelGGL((norm_rope_kernel<A32, 2>), grid, dim3(kThreads), 0, s, a, lph, v_heads);
-    else if (ipt == 3) hipLaunchKernelGGL((norm_rope_kernel<A32, 3>), grid, dim3(kThreads), 0, s, a, lph, v_heads);
-    else hipLaunchKernelGGL((norm_rope_kernel<A32, 4>), grid, dim3(kThreads), 0, s, a, lph, v_heads);
+template <int ACT, int DT> void launch_runs(const NormRopeArgs& a, int v_groups, int lph, hipStream_t s) {
+    if (DT != QR_DTYPE_F32 && v_groups) hipLaunchKernelGGL((v_runs_kernel<ACT, DT == QR_DTYPE_F32 ? QR_DTYPE_F16 : DT>), dim3(v_groups), dim3(kThreads), 0, s, a);
+    const int v_heads = v_groups ? 0 : a.geom.kv_heads, heads = a.geom.kv_heads + (a.q ? a.heads : 0) + v_heads;
+    const int slots = (heads * lph + kThreads - 1) / kThreads, ipt = std::min(slots, 4);
+    const dim3 grid(a.rows, (slots + ipt - 1) / ipt);
+    if (ipt == 1) hipLaunchKernelGGL((norm_rope_kernel<ACT, DT, 1>), grid, dim3(kThreads), 0, s, a, lph, v_heads);
+    else if (ipt == 2) hipLaunchKernelGGL((norm_rope_kernel<ACT, DT, 2>), grid, dim3(kThreads), 0, s, a, lph, v_heads);
+    else if (ipt == 3) hipLaunchKernelGGL((norm_rope_kernel<ACT, DT, 3>), grid, dim3(kThreads), 0, s, a, lph, v_heads);
+    else hipLaunchKernelGGL((norm_rope_kernel<ACT, DT, 4>), grid, dim3(kThreads), 0, s, a, lph, v_heads);
+}
+template <int ACT> void launch_dtype(const NormRopeArgs& a, int v_groups, int lph, hipStream_t s) {
+    if (a.dtype == QR_DTYPE_F32) launch_runs<ACT, QR_DTYPE_F32>(a, v_groups, lph, s);
+    else if (a.dtype == QR_DTYPE_F16) launch_runs<ACT, QR_DTYPE_F16>(a, v_groups, lph, s);
+    else launch_runs<ACT, QR_DTYPE_BF16>(a, v_groups, lph, s);
 }
 
 }  // namespace
@@ -350,17 +356,9 @@ hipError_t launch_norm_rope(NormRopeArgs& a, hipStream_t stream) {
     int lph = 1;
     while (lph < D / 8) lph *= 2;
     const int v_groups = v_run_groups(a);
-    const bool f32 = a.act == QR_DTYPE_F32;
-    if (v_groups) {
-        if (f32) hipLaunchKernelGGL(v_runs_kernel<true>, dim3(v_groups), dim3(kThreads), 0, stream, a);
-        else hipLaunchKernelGGL(v_runs_kernel<false>, dim3(v_groups), dim3(kThreads), 0, stream, a);
-        if (hipError_t e = hipGetLastError()) return e;
-    }
-    const int v_heads = v_groups ? 0 : a.geom.kv_heads, heads = a.geom.kv_heads + (a.q ? a.heads : 0) + v_heads;
-    const int slots = (heads * lph + kThreads - 1) / kThreads, ipt = std::min(slots, 4);
-    const dim3 grid(a.rows, (slots + ipt - 1) / ipt);
-    if (f32) launch_ipt<true>(a, ipt, grid, lph, v_heads, stream);
-    else launch_ipt<false>(a, ipt, grid, lph, v_heads, stream);
+    if (a.act == QR_DTYPE_F32) launch_dtype<QR_DTYPE_F32>(a, v_groups, lph, stream);
+    else if (a.act == QR_DTYPE_F16) launch_dtype<QR_DTYPE_F16>(a, v_groups, lph, stream);
+    else launch_dtype<QR_DTYPE_BF16>(a, v_groups, lph, stream);
     return hipGetLastError();
 }
 

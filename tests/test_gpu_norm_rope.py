@@ -162,6 +162,27 @@ def test_read_equals_the_host_copy(gpu):
             assert torch.equal(ko, k[want]) and torch.equal(vo, v[want])
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_every_rounding(gpu, dtype):
+    """Every upper half of an fp32 value with lower halves at, below and above the places where it rounds: the bits that
+    the append without norms and rotation stores, and NaN for NaN."""
+    hi = torch.arange(65536, dtype=torch.int32, device="cuda") << 16
+    low = torch.tensor([0, 1, 0x0FFF, 0x1000, 0x1001, 0x7FFF, 0x8000, 0x8001, 0xFFFF], dtype=torch.int32, device="cuda")
+    x = (hi[:, None] | low).view(torch.float32).reshape(-1, 256).contiguous()
+    n = x.shape[0]
+    with qr.PagedKvCache(1, 2, 2, 128, n, dtype, 1) as kv:
+        def rows():
+            out = [torch.empty(n, 256, dtype=TORCH[dtype], device="cuda") for _ in range(2)]
+            kv.ReadDev(0, [0], [0], [n], *out)
+            return out
+        kv.AppendRangeDev(0, 0, x, x, "f32")
+        want = rows()
+        kv.AppendNormRopeDev(0, [0], [0], [n], None, x, x, None, None, None, EPS, THETA, rotary_dim=0)
+        for got, ref in zip(rows(), want):
+            assert torch.equal(got.isnan(), x.isnan())
+            assert torch.equal(got.view(torch.int16)[~x.isnan()], ref.view(torch.int16)[~x.isnan()])
+
+
 def test_zero_rows_and_infinities(gpu):
     """A row of zeros stays zero (eps > 0); an infinite value makes its own head NaN, not its neighbours."""
     with qr.PagedKvCache(1, 2, 2, 64, 16, "f32", 1) as kv:
