@@ -107,10 +107,10 @@ struct ChunkItem {
     int row0;                // first row in q / out
     // of a launch:
     int unit0;
-    int blocks;              // row blocks (weights: position blocks) per kv head
-    int splits;              // parts of each block's keys (weights: rows)
+    int blocks;              // row blocks per kv head (weights: position blocks; by tiles: units)
+    int splits;              // parts of each block's keys
     int slot0;               // first split partial: (row * heads + head) * splits + split from here
-    int pad;
+    int per;                 // weights by tiles: rounds of rows of a unit
     long long score0;        // first score: (row * heads + head) * chunk_score_len from here; -1: none are kept
 };
 struct ChunksArgs {
@@ -133,7 +133,7 @@ struct ChunksArgs {
 struct ChunkPlanItem {
     int kind, blocks, splits;
     long long slot0;
-    int wkind, wblocks, wsplits;
+    int wkind, wblocks, wper, wparts;
     long long wslot0, score0;
 };
 struct ChunksPlan {

@@ -122,8 +122,19 @@ __global__ void __launch_bounds__(256) chunks_wmerge_kernel(const ChunksK p) {
     const int u = blockIdx.x - it.unit0, len = it.pos0 + it.rows;
     const int t = u % it.blocks * 256 + threadIdx.x, kvh = u / it.blocks;
     if (t >= len) return;
+    const WeightTiles w = p.geom.mfma_layout ? kWeightTiles16 : kWeightTiles32;
+    const int parts = w.parts(it, p.heads / p.geom.kv_heads, t / w.positions, it.per);
+    if (parts == 1) return;  // added by its unit
+    const float* const from = p.wpart + it.slot0 + static_cast<long long>(kvh) * len + t;
+    const long long stride = static_cast<long long>(p.geom.kv_heads) * len;
     float sum = 0.f;
-    for (int s = 0; s < it.splits; ++s) sum += p.wpart[it.slot0 + (static_cast<long long>(s) * p.geom.kv_heads + kvh) * len + t];
+    for (int s0 = 0; s0 < parts; s0 += 8) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = from[min(s0 + i, parts - 1) * stride];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += s0 + i < parts ? x[i] : 0.f;
+    }
     p.weights[(static_cast<long long>(it.seq) * p.geom.kv_heads + kvh) * p.max_seq + t] += sum;
 }
 
@@ -196,28 +207,32 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
     }
     long long wslots = 0, scores = 0;
     if (a.weights) {
-        long long units = 0;
+        const WeightTiles wt = tiles ? kWeightTiles16 : kWeightTiles32;
+        long long rounds = 0;
         for (int i = 0; i < a.n; ++i) {
             ChunkPlanItem& it = pl.it[i];
             it.wkind = it.kind == kChunkAny ? kWeightsAny : it.kind == kChunkStream32 || it.kind == kChunkF32Half ? kWeightsScores
                      : it.kind == kChunkF32 ? kWeightsF32 : kWeightsTile;
-            it.wblocks = cdiv(a.it[i].pos0 + a.it[i].rows, it.wkind == kWeightsAny ? kChunkAnyTile : it.wkind == kWeightsF32 ? 128 : 256);
-            it.wsplits = 1;
+            it.wblocks = cdiv(a.it[i].pos0 + a.it[i].rows, it.wkind == kWeightsAny ? kChunkAnyTile : 256);
             it.score0 = -1;
-            if (it.wkind >= kWeightsTile) units += static_cast<long long>(it.wblocks) * kv;
+            if (it.wkind >= kWeightsTile) rounds += kv * wt.units(a.it[i], gmax, 1);
             if (it.wkind == kWeightsScores) {
                 it.score0 = scores;
                 scores += static_cast<long long>(a.it[i].rows) * a.heads * chunk_score_len(a.it[i]);
             }
         }
-        // few position blocks: their rows are split too, 64 rows or more a part
+        // units of an equal share of the rounds
+        const long long want = tiles ? 1024 : 512;
+        const int per = static_cast<int>(std::max<long long>(tiles ? 1 : 4, (rounds + want - 1) / want));
         for (int i = 0; i < a.n; ++i) {
             ChunkPlanItem& it = pl.it[i];
-            if (it.wkind < kWeightsTile || units >= 1024) continue;
-            it.wsplits = std::max(1, std::min(cdiv(1024, units), cdiv(static_cast<long long>(a.it[i].rows) * gmax, 64)));
+            if (it.wkind < kWeightsTile) continue;
+            it.wper = per;
+            it.wblocks = static_cast<int>(wt.units(a.it[i], gmax, per));
+            it.wparts = wt.parts(a.it[i], gmax, 0, per);
             it.wslot0 = wslots;
-            if (it.wsplits > 1) {
-                wslots += static_cast<long long>(it.wsplits) * kv * (a.it[i].pos0 + a.it[i].rows);
+            if (it.wparts > 1) {
+                wslots += static_cast<long long>(it.wparts) * kv * (a.it[i].pos0 + a.it[i].rows);
                 pl.wmerge = true;
             }
         }
@@ -278,7 +293,8 @@ hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* work
             it = a.it[i];
             it.unit0 = k.units;
             it.blocks = weights ? pi.wblocks : pi.blocks;
-            it.splits = weights ? pi.wsplits : pi.splits;
+            it.splits = weights ? 1 : pi.splits;
+            it.per = pi.wper;
             it.slot0 = static_cast<int>(weights ? pi.wslot0 : pi.slot0);
             it.score0 = pi.score0;
             k.units += it.blocks * it.splits * (per_head ? 1 : kv);
@@ -322,7 +338,7 @@ hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* work
         }
     }
     if (e == hipSuccess && plan.wmerge) {
-        gather([](const ChunkPlanItem& p) { return p.wkind >= kWeightsTile && p.wsplits > 1; }, true);
+        gather([](const ChunkPlanItem& p) { return p.wkind >= kWeightsTile && p.wparts > 1; }, true);
         k.units = 0;  // one unit per 256 positions and kv head
         for (int i = 0; i < k.n; ++i) {
             k.it[i].unit0 = k.units;

@@ -68,6 +68,48 @@ inline int chunk_grid(const ChunksK& p) {
     return kv % 8 && 8 % kv == 0 ? 8 * ((p.units * kv + 7) / 8) : p.units * kv;
 }
 
+// The weights passes by tiles: a unit takes the rows of a block of positions that see part of it, in rounds, up to `per`
+// of them.  Rows before the block see none of it, so later blocks have fewer units.
+struct WeightTiles {
+    int positions, rows;  // of a block, of a round
+    __host__ __device__ int first(const ChunkItem& it, int g, int block) const {
+        const int b0 = block * positions;
+        return b0 > it.pos0 ? (b0 - it.pos0) * g : 0;
+    }
+    __host__ __device__ int rounds(const ChunkItem& it, int g, int block) const { return (it.rows * g - first(it, g, block) + rows - 1) / rows; }
+    __host__ __device__ int parts(const ChunkItem& it, int g, int block, int per) const { return (rounds(it, g, block) + per - 1) / per; }
+    __host__ __device__ int blocks(const ChunkItem& it) const { return (it.pos0 + it.rows + positions - 1) / positions; }
+    __host__ __device__ int whole(const ChunkItem& it) const {  // blocks that every row sees
+        const int n = it.pos0 / positions + 1, m = blocks(it);
+        return n < m ? n : m;
+    }
+    // units of a kv head
+    long long units(const ChunkItem& it, int g, int per) const {
+        long long u = static_cast<long long>(whole(it)) * parts(it, g, 0, per);
+        for (int b = whole(it); b < blocks(it); ++b) u += parts(it, g, b, per);
+        return u;
+    }
+    __device__ __forceinline__ void find(const ChunkItem& it, int g, int unit, int* block, int* part, int* n) const {
+        const int s0 = parts(it, g, 0, it.per), n0 = whole(it);
+        if (unit < n0 * s0) {
+            *block = unit / s0;
+            *part = unit - *block * s0;
+            *n = s0;
+            return;
+        }
+        unit -= n0 * s0;
+        int b = n0, s = parts(it, g, b, it.per);
+        for (; unit >= s; s = parts(it, g, b, it.per)) {
+            unit -= s;
+            ++b;
+        }
+        *block = b;
+        *part = unit;
+        *n = s;
+    }
+};
+constexpr WeightTiles kWeightTiles16{256, 128}, kWeightTiles32{128, 16};
+
 // Part `split` of the positions [0, keys) in whole tiles.
 __device__ __forceinline__ void chunk_keys(const ChunkItem& it, int keys, int split, int tile, int* t0, int* t1) {
     const int tiles = (keys + tile - 1) / tile;

@@ -54,16 +54,16 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) chunks_f32_weights_kern
     const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
     const ChunkItem it = p.it[e];
     const int u = blockIdx.x - it.unit0;
-    const int split = u % it.splits, block = u / it.splits % it.blocks, kvh = u / (it.splits * it.blocks);
-    const int g = p.heads / p.geom.kv_heads, rows = it.rows * g;
+    const int kvh = u / it.blocks, g = p.heads / p.geom.kv_heads, rows = it.rows * g;
+    int split, block, splits;
+    kWeightTiles32.find(it, g, u - kvh * it.blocks, &block, &split, &splits);
     const int lane = threadIdx.x & 63, q4 = lane >> 4, l16 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int len = it.pos0 + it.rows;
-    const int b0 = block * 128, t0 = b0 + 32 * wave;
-    const int first = max(0, b0 - it.pos0) * g;  // rows before it see none of the block
-    const int rounds = (rows - first + 15) / 16;
-    const int r0 = first + static_cast<int>(static_cast<long long>(rounds) * split / it.splits) * 16;
-    const int r1 = min(rows, first + static_cast<int>(static_cast<long long>(rounds) * (split + 1) / it.splits) * 16);
+    const int b0 = block * kWeightTiles32.positions, t0 = b0 + 32 * wave;
+    const int first = kWeightTiles32.first(it, g, block), rounds = kWeightTiles32.rounds(it, g, block);
+    const int r0 = first + static_cast<int>(static_cast<long long>(rounds) * split / splits) * 16;
+    const int r1 = min(rows, first + static_cast<int>(static_cast<long long>(rounds) * (split + 1) / splits) * 16);
 
     float kv[2][NJ][EPC];
 #pragma unroll
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) chunks_f32_weights_kern
             const float s = group_sum(sum[mt][i], 16);  // over the rows
             const int t = t0 + 16 * mt + 4 * q4 + i;
             if (l16 == 4 * mt + i && t < len) {
-                if (it.splits == 1) p.weights[(static_cast<long long>(it.seq) * p.geom.kv_heads + kvh) * p.max_seq + t] += s;
+                if (splits == 1) p.weights[(static_cast<long long>(it.seq) * p.geom.kv_heads + kvh) * p.max_seq + t] += s;
                 else p.wpart[it.slot0 + (static_cast<long long>(split) * p.geom.kv_heads + kvh) * len + t] = s;
             }
         }

@@ -702,17 +702,17 @@ __global__ void __launch_bounds__(512, SPLIT && D == 128 ? 1 : 2) chunks_tile_we
     const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
     const ChunkItem it = p.it[e];
     const int u = blockIdx.x - it.unit0;
-    const int split = u % it.splits, block = u / it.splits % it.blocks, kvh = u / (it.splits * it.blocks);
-    const int g = p.heads / p.geom.kv_heads, rows = it.rows * g;
+    const int kvh = u / it.blocks, g = p.heads / p.geom.kv_heads, rows = it.rows * g;
+    static_assert(ROWS == kWeightTiles16.rows, "rows of a round");
+    int split, block, splits;
+    kWeightTiles16.find(it, g, u - kvh * it.blocks, &block, &split, &splits);
     const int lane = threadIdx.x & 63, half = lane >> 5, n = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int len = it.pos0 + it.rows;
-    const int b0 = block * 256, t0 = b0 + 32 * wave;
-    // rows that see part of the block, in rounds dealt to the splits
-    const int first = max(0, b0 - it.pos0) * g;
-    const int rounds = (rows - first + ROWS - 1) / ROWS;
-    const int r0 = first + static_cast<int>(static_cast<long long>(rounds) * split / it.splits) * ROWS;
-    const int r1 = min(rows, first + static_cast<int>(static_cast<long long>(rounds) * (split + 1) / it.splits) * ROWS);
+    const int b0 = block * kWeightTiles16.positions, t0 = b0 + 32 * wave;
+    const int first = kWeightTiles16.first(it, g, block), rounds = kWeightTiles16.rounds(it, g, block);
+    const int r0 = first + static_cast<int>(static_cast<long long>(rounds) * split / splits) * ROWS;
+    const int r1 = min(rows, first + static_cast<int>(static_cast<long long>(rounds) * (split + 1) / splits) * ROWS);
     const float sign = p.qscale == 0.f ? 0.f : p.qscale < 0.f ? -1.f : 1.f;
     const float base = p.qscale == 0.f ? 1.f : fabsf(p.qscale);
     auto row_of = [&](int rho) { return static_cast<long long>(it.row0 + rho / g) * p.heads + kvh * g + rho % g; };
@@ -721,12 +721,23 @@ __global__ void __launch_bounds__(512, SPLIT && D == 128 ? 1 : 2) chunks_tile_we
     float x[SPLIT ? CN : 1][8];
     vec8 raw[SPLIT ? 1 : CN];
     float4 inf;
+    // its row as (query, head), from one operand to the next and on to the next round without divisions
+    constexpr int STEP = 32 * 8 / NK;
+    static_assert(STEP * CN == ROWS, "a round");
+    const int step_q = STEP / g, step_h = STEP % g;
+    int fq = (r0 + 32 * (wave / NK) + n) / g, fh = (r0 + 32 * (wave / NK) + n) % g;
     auto fetch = [&](int r) __attribute__((always_inline)) {
 #pragma unroll
         for (int c = 0; c < CN; ++c) {
             const int op = wave + 8 * c;
-            const long long row = row_of(min(r + 32 * (op / NK) + n, rows - 1));
+            const long long row = static_cast<long long>(it.row0 + min(fq, it.rows - 1)) * p.heads + kvh * g + fh;
             const long long at = row * D + 16 * (op % NK) + 8 * half;
+            fq += step_q;
+            fh += step_h;
+            if (fh >= g) {
+                fh -= g;
+                ++fq;
+            }
             if (!SPLIT) {
                 __builtin_memcpy(&raw[SPLIT ? 0 : c], static_cast<const uint16_t*>(p.q) + at, 16);
             } else if (p.act == QR_DTYPE_F32) {
@@ -832,7 +843,7 @@ __global__ void __launch_bounds__(512, SPLIT && D == 128 ? 1 : 2) chunks_tile_we
     for (int i = 0; i < 16; ++i) {
         const int t = t0 + 16 * (i >> 3) + 8 * half + (i & 7);
         if (n == i && t < len) {
-            if (it.splits == 1) p.weights[(static_cast<long long>(it.seq) * p.geom.kv_heads + kvh) * p.max_seq + t] += sum[i];
+            if (splits == 1) p.weights[(static_cast<long long>(it.seq) * p.geom.kv_heads + kvh) * p.max_seq + t] += sum[i];
             else p.wpart[it.slot0 + (static_cast<long long>(split) * p.geom.kv_heads + kvh) * len + t] = sum[i];
         }
     }
