@@ -176,13 +176,17 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
     for (int kind = 0; kind < kChunkKinds; ++kind) {
         KindGeom g = kGeom[kind];
         if (kind == kChunkF32Half || kind == kChunkF32) g.want *= chunks_f32_per_cu(a.dtype, a.geom.head_dim, kind == kChunkF32Half);
-        long long base = 0, work = 0;
+        long long base = 0, work = 0, chunks = 0;
         for (int i = 0; i < a.n; ++i)
             if (pl.it[i].kind == kind) {
+                ++chunks;
                 base += static_cast<long long>(pl.it[i].blocks) * kv;
                 work += static_cast<long long>(pl.it[i].blocks) * kv * tiles_of(i);
             }
         if (!base) continue;
+        // fp32 blocks of several chunks differ most, and a tile takes long: two rounds of units (three prompts of 61 to 501
+        // rows after 1501 to 11: 71 us, 78 in one round; the first alone 37 and 33)
+        if (kind == kChunkF32 && chunks > 1) g.want *= 2;
         // tiles of a unit.  Enough units already: those with much more than a CU's share are split all the same (six bf16
         // prompts of 101 to 1501 rows after 3001 to 1 positions, with weights: 139 us, 153 without)
         long long per = base >= g.want ? std::max<long long>(8, work * 5 / (g.want * 4)) : std::max<long long>(1, work / g.want);
