@@ -308,6 +308,7 @@ hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* work
     hipError_t e = hipSuccess;
     for (int kind = 0; kind < kChunkKinds && e == hipSuccess; ++kind) {
         if (!gather([&](const ChunkPlanItem& p) { return p.kind == kind; }, false, kind >= kChunkTile)) continue;
+        k.paired = kind >= kChunkF32Half && static_cast<long long>(k.units) * kv <= 256LL * chunks_f32_per_cu(a.dtype, a.geom.head_dim, kind == kChunkF32Half);
         k.scores = a.weights && (kind == kChunkStream32 || kind == kChunkF32Half) ? reinterpret_cast<float*>(w + plan.scores) : nullptr;
         e = kind == kChunkAny ? launch_chunks_any(k, stream) : kind >= kChunkF32Half ? launch_chunks_f32(k, kind, stream)
           : launch_chunks_tile(k, kind, stream);

@@ -20,6 +20,7 @@ struct ChunksK {
     ChunkItem it[kBatch];
     int n;
     int units;
+    bool paired;             // (tile kernels) fewer units than run at once
     const char* pool;
     const int* page_table;
     PageGeom geom;
@@ -61,7 +62,12 @@ __device__ __forceinline__ bool chunk_unit(const ChunksK& p, int* kvh, int* unit
         *kvh = b % kv;
         *unit = b / kv;
     }
-    return *unit < p.units && *kvh < kv;
+    if (*unit >= p.units || *kvh >= kv) return false;
+    // all units run at once, several on a CU: the long ones share it with short ones (512 fp32 rows after 1536: 161 us, 166
+    // from the longest down)
+    const int h = (p.units + 1) >> 1;
+    if (p.paired && *unit >= h) *unit = p.units - 1 - (*unit - h);
+    return true;
 }
 inline int chunk_grid(const ChunksK& p) {
     const int kv = p.geom.kv_heads;
