@@ -333,15 +333,17 @@ __global__ void __launch_bounds__(256) evict_weights_kernel(const EvictArgs a, c
     else if (a.kept_weights != a.weights) a.kept_weights[at] = a.weights[at];
 }
 
-constexpr int kMoveThreads = 256;
+constexpr int kMoveThreads = 1024;
 
-// The same for head sizes whose rows are whole 16-byte pieces, P of a row (or what is left of it) per workgroup, 2048 / P
-// slots at a time; the next ones are read before these are written.  V of the MFMA page layout: 16 dims per workgroup, a thread
-// gathers 8 slots of a dim (16 bytes of the page; reading ahead here costs registers and 10 us of 38).  Bound by HBM for
-// many workgroups, else by the latency of a tile.
+// K and V rows to the slots that keep them, head sizes whose rows are whole 16-byte pieces: P pieces of a row (or what is left
+// of it) per workgroup, 8192 / P slots at a time, since a tile is read before it is written; the next ones are read
+// before these are written.  V of the MFMA page layout: 16 dims per workgroup, a thread gathers 8 slots of a dim (16 bytes
+// of the page; reading ahead here costs registers and a third of the time).  Bound by HBM for many workgroups (16
+// sequences of 3000 to 17000 bf16 positions, whose gaps share lines with what stays: 167 us), else by the latency of a tile:
+// 1024 threads 14 us for one sequence of 2304, 256 threads with tiles of a quarter 22.
 template <int ES, bool MFMA, int P>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArgs a) {
-    constexpr int N = 16 / ES, TILE = MFMA ? 512 : 2048 / P;
+    constexpr int N = 16 / ES, TILE = MFMA ? 2 * kMoveThreads : 8 * kMoveThreads / P;
     const int D = a.geom.head_dim, pieces = D / N;
     const int ks = (pieces + P - 1) / P, vs = MFMA ? D / 16 : ks;  // workgroups of the K and the V rows of a kv head
     // plain pages: the parts of a row run on one XCD where the rows are whole eights, whose L2 joins their pieces to lines
@@ -535,7 +537,7 @@ hipError_t launch_evict(const EvictArgs& a, void* workspace, hipStream_t stream)
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !longest) return e;
     // four pieces of a row per workgroup, two where that leaves CUs idle (8192 of 65536 fp32 positions
-    // kept: 59 us, 96 with four)
+    // kept: 43 us, 49 with four, 60 with one)
     const int D = a.geom.head_dim, n = 16 / dtype_size(a.dtype), ks4 = (D / n + 3) / 4, ks2 = (D / n + 1) / 2;
     const dim3 mblock(kMoveThreads);
     const bool two = rows * 2 * ks4 < 512;

@@ -201,6 +201,29 @@ def test_the_same_sequence_twice_without_weights(gpu):
         kv.AttentionChunksDev(0, [0, 0], [3, 4], [1, 0], q[:1].contiguous(), torch.empty_like(q[:1]), 1.0, weights=w)
 
 
+@pytest.mark.parametrize("dtype,act,D", [("bf16", "bf16", 128), ("f16", "f32", 64), ("f32", "f32", 128), ("f32", "bf16", 64), ("f32", "f32", 40),
+                                         ("bf16", "f32", 96)])
+def test_tensors_off_vector_alignment(gpu, dtype, act, D):
+    """q, out and weights whose addresses are aligned to their element only give what aligned ones give."""
+    kv, rows = filled(8, 2, D, dtype, [700, 300, 130, 9])
+    chunks = ([0, 1, 2, 3], [400, 299, 110, 0], [300, 1, 20, 9])
+    n = sum(chunks[2])
+    with kv:
+        q = randn(3, n, 8 * D, dtype=act)
+        out, w = torch.zeros_like(q), torch.zeros(4, 2, 700, device="cuda")
+        kv.AttentionChunksDev(0, *chunks, q, out, D ** -0.5, weights=w)
+        for off in (1, 2):
+            def moved(x):
+                y = torch.full((x.numel() + 8,), 5.0, dtype=x.dtype, device="cuda")
+                y[off:off + x.numel()] = x.flatten()
+                return y, y[off:off + x.numel()].view_as(x)
+            (_, q1), (oe, o1), (we, w1) = moved(q), moved(torch.zeros_like(q)), moved(torch.zeros_like(w))
+            kv.AttentionChunksDev(0, *chunks, q1, o1, D ** -0.5, weights=w1)
+            assert torch.equal(o1, out) and torch.equal(w1, w)
+            for e, x in ((oe, out), (we, w)):
+                assert (e[:off] == 5).all() and (e[off + x.numel():] == 5).all()
+
+
 def test_nothing_to_do(gpu):
     kv, _ = filled(8, 2, 64, "f32", [4, 4])
     with kv:
