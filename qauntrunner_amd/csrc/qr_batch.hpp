@@ -107,10 +107,11 @@ struct ChunkItem {
     int row0;                // first row in q / out
     // of a launch:
     int unit0;
-    int blocks;              // row blocks per kv head (weights: position blocks; by tiles: units)
-    int splits;              // parts of each block's keys
+    int blocks;              // row blocks per kv head (weights: position blocks); of the tile kernels units
+    int splits;              // parts of a block's keys, of the tile kernels of the block that has the most
     int slot0;               // first split partial: (row * heads + head) * splits + split from here
-    int per;                 // weights by tiles: rounds of rows of a unit
+    int per;                 // tile kernels: tiles of keys (weights: rounds of rows) of a unit, up to; else 0
+    int parts;               // (within a kernel) of this block's keys; splits where all blocks have as many
     long long score0;        // first score: (row * heads + head) * chunk_score_len from here; -1: none are kept
 };
 struct ChunksArgs {
@@ -131,7 +132,7 @@ struct ChunksArgs {
 };
 // Which kernel takes a chunk, and how its work is cut.
 struct ChunkPlanItem {
-    int kind, blocks, splits;
+    int kind, blocks, splits, per;
     long long slot0;
     int wkind, wblocks, wper, wparts;
     long long wslot0, score0;

@@ -36,6 +36,7 @@ struct ChunkF32K {
     float2* row_ml;          // [nq*heads] (maximum, sum), may be null
     float* scores;           // [nq*heads][score_len] scaled scores, may be null
     int score_len;
+    int stride;              // partials of a row, splits or more
 };
 
 template <typename ST, int D>
@@ -453,7 +454,7 @@ __device__ __forceinline__ void chunk_f32_tiles(const ChunkF32K& p, int split, i
     // lane (q4, l16) holds dims 16 PE g + PE (4q4 + r) + e of row l16 in acc[g][e][r]
     if (!row_on) return;
     const size_t r0 = static_cast<size_t>(row_q) * p.heads + row_h;
-    const size_t slot = r0 * p.splits + split;
+    const size_t slot = r0 * (BATCH ? p.stride : p.splits) + split;
     if constexpr (BATCH) {
         if (p.row_ml && p.splits == 1 && q4 == 0) p.row_ml[r0] = make_float2(m, l);
         if (p.splits == 1 && p.out_dtype != QR_DTYPE_F32) {

@@ -43,21 +43,28 @@ __global__ void __launch_bounds__(256) chunks_merge_kernel(const ChunksK p) {
     const long long r = static_cast<long long>(blockIdx.x - it.unit0) * RPB + rr;
     if (rr >= RPB || r >= static_cast<long long>(it.rows) * p.heads) return;
     const long long base = it.slot0 + r * it.splits;
+    int parts = it.splits;
+    if (it.per) {
+        const KeyTiles t = p.geom.mfma_layout ? kKeyTiles16 : key_tiles32(p.heads / p.geom.kv_heads);
+        const int g = p.heads / p.geom.kv_heads, q = static_cast<int>(r / p.heads), h = static_cast<int>(r - static_cast<long long>(q) * p.heads);
+        parts = t.parts(it, g, (q * g + h % g) / t.rows, it.per);
+        if (parts == 1) return;  // written by its unit
+    }
     const float4* part = reinterpret_cast<const float4*>(p.part_acc) + base * TPR + c;
     float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < it.splits; s0 += kB) {
+    for (int s0 = 0; s0 < parts; s0 += kB) {
         float4 a[kB];
         float2 ml[kB];
 #pragma unroll
         for (int i = 0; i < kB; ++i) {
-            const int s = min(s0 + i, it.splits - 1);
+            const int s = min(s0 + i, parts - 1);
             a[i] = part[static_cast<long long>(s) * TPR];
             ml[i] = p.part_ml[base + s];
         }
         float mb = m;
 #pragma unroll
         for (int i = 0; i < kB; ++i) {
-            if (s0 + i >= it.splits) ml[i].x = -INFINITY;  // a repeated split
+            if (s0 + i >= parts) ml[i].x = -INFINITY;  // a repeated split
             mb = fmaxf(mb, ml[i].x);
         }
         const float cm = m == -INFINITY ? 0.f : fast_exp2(m - mb);
@@ -66,7 +73,7 @@ __global__ void __launch_bounds__(256) chunks_merge_kernel(const ChunksK p) {
         for (int x = 0; x < 4; ++x) o[x] *= cm;
 #pragma unroll
         for (int i = 0; i < kB; ++i) {
-            if (s0 + i >= it.splits) continue;
+            if (s0 + i >= parts) continue;
             const float w = ml[i].x == -INFINITY ? 0.f : fast_exp2(ml[i].x - mb);
             l = fmaf(ml[i].y, w, l);
             o[0] = fmaf(a[i].x, w, o[0]);
@@ -176,24 +183,24 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
     for (int kind = 0; kind < kChunkKinds; ++kind) {
         KindGeom g = kGeom[kind];
         if (kind == kChunkF32Half || kind == kChunkF32) g.want *= chunks_f32_per_cu(a.dtype, a.geom.head_dim, kind == kChunkF32Half);
-        long long base = 0, work = 0, chunks = 0;
+        const bool by_block = kind == kChunkTile || kind == kChunkF32;
+        const KeyTiles kt = kind == kChunkTile ? kKeyTiles16 : key_tiles32(std::min(gmax, 64));
+        long long base = 0, work = 0;
         for (int i = 0; i < a.n; ++i)
             if (pl.it[i].kind == kind) {
-                ++chunks;
                 base += static_cast<long long>(pl.it[i].blocks) * kv;
-                work += static_cast<long long>(pl.it[i].blocks) * kv * tiles_of(i);
+                work += kv * (by_block ? kt.units(a.it[i], gmax, 1) : static_cast<long long>(pl.it[i].blocks) * tiles_of(i));
             }
         if (!base) continue;
-        // fp32 blocks of several chunks differ most, and a tile takes long: two rounds of units (three prompts of 61 to 501
-        // rows after 1501 to 11: 71 us, 78 in one round; the first alone 37 and 33)
-        if (kind == kChunkF32 && chunks > 1) g.want *= 2;
         // tiles of a unit.  Enough units already: those with much more than a CU's share are split all the same (six bf16
-        // prompts of 101 to 1501 rows after 3001 to 1 positions, with weights: 139 us, 153 without)
+        // prompts of 101 to 1501 rows after 3001 to 1 positions, with weights: 119 us, 130 without, 127 where fewer tiles than
+        // a quarter more than the share are split too)
         long long per = base >= g.want ? std::max<long long>(8, work * 5 / (g.want * 4)) : std::max<long long>(1, work / g.want);
         auto units = [&](long long per_) {
             long long u = 0;
             for (int i = 0; i < a.n; ++i)
-                if (pl.it[i].kind == kind) u += static_cast<long long>(pl.it[i].blocks) * kv * cdiv(tiles_of(i), per_);
+                if (pl.it[i].kind == kind)
+                    u += kv * (by_block ? kt.units(a.it[i], gmax, static_cast<int>(per_)) : static_cast<long long>(pl.it[i].blocks) * cdiv(tiles_of(i), per_));
             return u;
         };
         if (base < g.want)
@@ -203,6 +210,11 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
             if (it.kind != kind) continue;
             it.splits = std::min(cdiv(tiles_of(i), per), 256);
             it.slot0 = slots;
+            if (by_block) {
+                it.per = std::max(static_cast<int>(per), cdiv(tiles_of(i), 256));
+                it.blocks = static_cast<int>(kt.units(a.it[i], gmax, it.per));
+                it.splits = cdiv(tiles_of(i), it.per);
+            }
             if (it.splits > 1) {
                 slots += static_cast<long long>(a.it[i].rows) * a.heads * it.splits;
                 pl.merge = true;
@@ -298,10 +310,11 @@ hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* work
             it.unit0 = k.units;
             it.blocks = weights ? pi.wblocks : pi.blocks;
             it.splits = weights ? 1 : pi.splits;
-            it.per = pi.wper;
+            it.parts = it.splits;
+            it.per = weights ? pi.wper : pi.per;
             it.slot0 = static_cast<int>(weights ? pi.wslot0 : pi.slot0);
             it.score0 = pi.score0;
-            k.units += it.blocks * it.splits * (per_head ? 1 : kv);
+            k.units += it.blocks * (it.per ? 1 : it.splits) * (per_head ? 1 : kv);
         }
         return k.n > 0;
     };

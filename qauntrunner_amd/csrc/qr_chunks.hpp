@@ -74,6 +74,53 @@ inline int chunk_grid(const ChunksK& p) {
     return kv % 8 && 8 % kv == 0 ? 8 * ((p.units * kv + 7) / 8) : p.units * kv;
 }
 
+// The tile kernels' row blocks: a block's keys are split into parts of up to `per` tiles, so that late blocks, which see
+// more keys, have more units.
+struct KeyTiles {
+    int rows, tile;  // (query, head) rows of a block, positions of a tile
+    __host__ __device__ int blocks(const ChunkItem& it, int g) const { return (it.rows * g + rows - 1) / rows; }
+    __host__ __device__ int tiles(const ChunkItem& it, int g, int block) const {
+        const int r0 = block * rows, left = it.rows * g - r0, last = r0 + (left < rows ? left : rows) - 1;
+        return (it.pos0 + last / g + tile) / tile;
+    }
+    __host__ __device__ int parts(const ChunkItem& it, int g, int block, int per) const { return (tiles(it, g, block) + per - 1) / per; }
+    long long units(const ChunkItem& it, int g, int per) const {  // of a kv head
+        long long u = 0;
+        for (int b = 0; b < blocks(it, g); ++b) u += parts(it, g, b, per);
+        return u;
+    }
+    // from the last block, which has the most keys, down; sets it.parts.  (Without divisions in the loop: 40 blocks
+    // would cost a unit several microseconds.)
+    __device__ __forceinline__ void find(ChunkItem& it, int g, int unit, int* block, int* part) const {
+        int b = blocks(it, g) - 1, s = it.splits;
+        if (s == 1) {
+            b -= unit;
+            unit = 0;
+        } else if (unit >= s) {
+            unit -= s;
+            const int end = b * rows - 1, step = rows / g, over = rows - step * g;
+            int query = end / g, head = end - query * g;  // of the last row of block b - 1
+            for (--b;; --b) {
+                const int n = (it.pos0 + query + tile) / tile;
+                while ((s - 1) * it.per >= n) --s;
+                if (unit < s) break;
+                unit -= s;
+                query -= step;
+                head -= over;
+                if (head < 0) {
+                    head += g;
+                    --query;
+                }
+            }
+        }
+        *block = b;
+        *part = unit;
+        it.parts = s;
+    }
+};
+constexpr KeyTiles kKeyTiles16{256, 64};
+__host__ __device__ constexpr KeyTiles key_tiles32(int g) { return {64 / g * g, 32}; }  // whole queries
+
 // The weights passes by tiles: a unit takes the rows of a block of positions that see part of it, in rounds, up to `per`
 // of them.  Rows before the block see none of it, so later blocks have fewer units.
 struct WeightTiles {
@@ -104,10 +151,12 @@ struct WeightTiles {
             return;
         }
         unit -= n0 * s0;
-        int b = n0, s = parts(it, g, b, it.per);
-        for (; unit >= s; s = parts(it, g, b, it.per)) {
+        int b = n0, s = s0;
+        for (;; ++b) {
+            const int n = rounds(it, g, b);
+            while ((s - 1) * it.per >= n) --s;
+            if (unit < s) break;
             unit -= s;
-            ++b;
         }
         *block = b;
         *part = unit;
@@ -119,8 +168,8 @@ constexpr WeightTiles kWeightTiles16{256, 128}, kWeightTiles32{128, 16};
 // Part `split` of the positions [0, keys) in whole tiles.
 __device__ __forceinline__ void chunk_keys(const ChunkItem& it, int keys, int split, int tile, int* t0, int* t1) {
     const int tiles = (keys + tile - 1) / tile;
-    *t0 = static_cast<int>(static_cast<long long>(tiles) * split / it.splits) * tile;
-    *t1 = std::min(static_cast<int>(static_cast<long long>(tiles) * (split + 1) / it.splits) * tile, keys);
+    *t0 = static_cast<int>(static_cast<long long>(tiles) * split / it.parts) * tile;
+    *t1 = std::min(static_cast<int>(static_cast<long long>(tiles) * (split + 1) / it.parts) * tile, keys);
 }
 
 // Entries of a row of scores: positions of the chunk's last row, whole runs of 8.

@@ -14,8 +14,16 @@ __global__ void __launch_bounds__(256, (F32Geom<ST, D>::wg_per_cu(PG))) chunks_f
     int kvh, unit;
     if (!chunk_unit(p, &kvh, &unit)) return;
     const int e = batch_find(p.n, unit, [&](int i) { return p.it[i].unit0; });
-    const ChunkItem& it = p.it[e];
-    const int u = unit - it.unit0;
+    ChunkItem it = p.it[e];
+    const int g = p.heads / p.geom.kv_heads;
+    int block, split;
+    if (PG == 1) {
+        key_tiles32(g).find(it, g, unit - it.unit0, &block, &split);
+    } else {
+        const int u = unit - it.unit0;
+        split = u % it.splits;
+        block = it.blocks - 1 - u / it.splits;
+    }
     const long long row0 = static_cast<long long>(it.row0) * p.heads;
     ChunkF32K k{};
     k.pool = p.pool;
@@ -23,7 +31,7 @@ __global__ void __launch_bounds__(256, (F32Geom<ST, D>::wg_per_cu(PG))) chunks_f
     k.page_elems = p.geom.page_elems();
     k.plane_elems = p.geom.plane_elems();
     k.heads = p.heads;
-    k.group = p.heads / p.geom.kv_heads;
+    k.group = g;
     k.pos0 = it.pos0;
     k.nq = it.rows;
     k.q_dtype = k.out_dtype = p.act;
@@ -33,11 +41,12 @@ __global__ void __launch_bounds__(256, (F32Geom<ST, D>::wg_per_cu(PG))) chunks_f
     k.part_ml = p.part_ml + it.slot0;
     k.qscale = p.qscale;
     k.queries_per_block = 64 / PG / k.group;
-    k.splits = it.splits;
+    k.splits = it.parts;
+    k.stride = it.splits;
     k.row_ml = p.row_ml ? p.row_ml + row0 : nullptr;
     k.scores = p.scores && it.score0 >= 0 ? p.scores + it.score0 : nullptr;
     k.score_len = chunk_score_len(it);
-    chunk_f32_tiles<ST, D, PG, true>(k, u % it.splits, it.blocks - 1 - u / it.splits, kvh, lds);
+    chunk_f32_tiles<ST, D, PG, true>(k, split, block, kvh, lds);
 }
 
 // Weights of 128 positions of one kv head over a part of its rows: a wave keeps the K rows of 32

@@ -242,7 +242,7 @@ struct Rows {
         if (!on) return;
         const long long rh = static_cast<long long>(it.row0 + query) * p.heads + head;
         auto dim = [&](int i) { return 32 * ((g0 + i) >> 2) + 8 * ((g0 + i) & 3) + 4 * half; };
-        if (it.splits > 1) {
+        if (it.parts > 1) {
             float* o = p.part_acc + (it.slot0 + (static_cast<long long>(query) * p.heads + head) * it.splits + split) * D;
 #pragma unroll
             for (int i = 0; i < N; ++i) *reinterpret_cast<f32x4_t*>(o + dim(i)) = a[i];
@@ -276,7 +276,7 @@ struct Rows {
     __device__ __forceinline__ void store_ml(const ChunksK& p, const ChunkItem& it, int split, float mm, float lsum) const {
         if (!on || half) return;
         if (p.row_scale) p.row_scale[static_cast<long long>(it.row0 + query) * p.heads + head] = sscale;  // the same in every split
-        if (it.splits > 1) p.part_ml[it.slot0 + (static_cast<long long>(query) * p.heads + head) * it.splits + split] = make_float2(mm, lsum);
+        if (it.parts > 1) p.part_ml[it.slot0 + (static_cast<long long>(query) * p.heads + head) * it.splits + split] = make_float2(mm, lsum);
         else if (p.row_ml) p.row_ml[static_cast<long long>(it.row0 + query) * p.heads + head] = make_float2(mm, lsum);
     }
 };
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
     constexpr int PARTS = SPLIT ? 2 : 1;
     using R = Rows<BF16, D, PARTS>;
     using vec8 = typename R::vec8;
-    constexpr int TILE = 64, NST = 3;
+    constexpr int TILE = kKeyTiles16.tile, NST = 3;
     constexpr int SB = 64 * D;           // bytes of a step of K (or V)
     constexpr int KB = 2 * SB;           // of a tile of K (or V)
     constexpr int PER = KB / 1024 / 8;   // DMA loads per wave for a tile of K (or V)
@@ -511,11 +511,12 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
     int kvh, unit;
     if (!chunk_unit(p, &kvh, &unit)) return;
     const int e = batch_find(p.n, unit, [&](int i) { return p.it[i].unit0; });
-    const ChunkItem it = p.it[e];
-    const int u = unit - it.unit0;
-    const int split = u % it.splits, block = it.blocks - 1 - u / it.splits;  // from the last, which has the most keys, down
+    ChunkItem it = p.it[e];
     const int g = p.heads / p.geom.kv_heads;
+    int block, split;
+    kKeyTiles16.find(it, g, unit - it.unit0, &block, &split);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    static_assert(kKeyTiles16.rows == 256, "8 waves of 32 rows");
     const int rho0 = block * 256;
     const int last = min(rho0 + 256, it.rows * g) - 1;
     int t0, t1;
