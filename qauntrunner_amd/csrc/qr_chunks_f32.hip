@@ -1,7 +1,9 @@
 // qr_chunks_f32.hip -- causal attention of chunks of several sequences in fp32 arithmetic on fp32 MFMA
 // tiles: fp32 caches (head size 64, 96, 128, 256) and 16-bit caches with token-major pages (96, 256),
 // whole groups of up to 64 query heads, gfx950.  The tiles are those of one sequence's chunk
-// (qr_chunk_f32.hpp, qr_chunk_f32.hip); here a workgroup finds its chunk first.
+// (qr_chunk_f32.hpp, qr_chunk_f32.hip); here a workgroup finds its chunk first.  Bound by the fp32 MFMAs where
+// the units are long (512 rows of 32 heads after 1536: 161 us, 93 TFLOP/s of the 154 that a large product reaches); three
+// prompts of 61 to 501 rows, 3.8 GFLOP, take 64 us: a tile of a block takes 1.7 us and the longest unit has 14.
 #include "qr_chunk_f32.hpp"
 #include "qr_chunks.hpp"
 
@@ -52,7 +54,7 @@ __global__ void __launch_bounds__(256, (F32Geom<ST, D>::wg_per_cu(PG))) chunks_f
 // Weights of 128 positions of one kv head over a part of its rows: a wave keeps the K rows of 32
 // positions as operands (two M tiles) and takes the rows 16 at a time from LDS, where the workgroup
 // puts them in operand order: chunk 4j + q4 of row l16 at 16 (64 j + lane).  Bound by the fp32
-// MFMAs (2 D flop per score; the layouts of qr_chunk_f32.hpp).
+// MFMAs (2 D flop per score; the layouts of qr_chunk_f32.hpp): 34 us for three prompts' 1.9 GFLOP.
 template <typename ST, int D>
 __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) chunks_f32_weights_kernel(const ChunksK p) {
     using Gm = F32Geom<ST, D>;

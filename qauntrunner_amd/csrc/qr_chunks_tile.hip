@@ -14,9 +14,10 @@
 // Softmax in log2 units with the running maximum held `kHead` above the largest score seen when it
 // last moved: the weights stay at or below 1 (a V near the type's largest value does not overflow)
 // and the accumulators are rescaled only when a score passes it.  Sums are of the fp32 weights.
-// kSplit: queries that are not of the cache's type enter as two parts of it (hi + lo), and so do
-// the weights, which keeps 16 (bf16) or 22 (fp16) bits of both; otherwise the weights are rounded
-// to the type once, as the output is.
+// Queries that are not of the cache's type enter as parts of it, and so do the weights: two parts keep 16 (bf16) or 22
+// (fp16) bits of both.  Few rows, which HBM bounds, take three of bf16, 24 bits: the error of eight verify chunks falls from
+// 4e-6 to 4e-7 for 102 us instead of 87; many rows take two (SPLIT).  Otherwise the weights are rounded to the type once,
+// as the output is.
 //
 // Tiles are copied into LDS by buffer-load DMA as they lie in the page.
 #include "qr_chunks.hpp"
@@ -297,7 +298,9 @@ __device__ __forceinline__ int page_of(const ChunksK& p, int pt_off, int t) {
 // ------------------------------------------------------------------ few rows: HBM-bound
 // RW waves of 32 rows each x PW waves that take one step of 32 positions of every tile.  K and V of a tile are
 // units of a ring in LDS that fills it, most of them in flight while one is used.  With RW = 1 a wave copies its own steps
-// and no wave waits for another before the end, where the PW (m, l, o) of a row merge.
+// and no wave waits for another before the end, where the PW (m, l, o) of a row merge.  16 decode rows of 32 heads over
+// 130 to 16000 fp16 positions: 47 us for 241 MB, 5.1 TB/s; eight chunks of 5 to 9 rows of 64 heads, fp32 queries over 2000 to
+// 32000 bf16 positions: 89 to 99 us for 388 MB, two thirds of it the MFMAs of the three parts, not wholly beside the loads.
 
 template <bool BF16, int D, int PARTS, int RW, int PW, int LDS>
 __device__ __forceinline__ void chunk_stream(const ChunksK& p, const ChunkItem& it, int u, char* lds) {
@@ -496,7 +499,9 @@ __global__ void __launch_bounds__(256, 2) chunks_stream_kernel(const ChunksK p) 
 // ------------------------------------------------------------------ many rows: MFMA-bound
 // Eight waves of 32 rows share every tile of 64 positions.  Waves 0-3 and 4-7 run half a tile apart: while
 // one group's MFMAs run (scores of tile t, weighted V of tile t - 1), the other group computes its
-// softmax on the same SIMDs; a barrier ends each half.
+// softmax on the same SIMDs; a barrier ends each half.  2048 bf16 rows of 32 heads after 6144: 230 to 240 us, 1.0 PFLOP/s of the
+// 1.2 that a large product reaches; the MFMAs and LDS reads alone take 161, the softmax with the copies 117.  Short units
+// pay about 6 us to start and end.
 template <bool BF16, int D, bool SPLIT>
 __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
     constexpr int PARTS = SPLIT ? 2 : 1;
@@ -690,7 +695,9 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
 // Weights of 256 positions of one kv head over a part of its rows: a wave keeps the K rows of 32
 // positions as operands; the workgroup puts 128 rows at a time into LDS as operands (each wave its share of the
 // k-steps), with each row's maximum, 1 / sum, last position seen and score scale.  Bound by the exponentials (16 cycles
-// per 64 of them, 8 for the multiply-adds around each, 16 for the MFMAs of as many scores beside them).
+// per 64 of them, 8 for the multiply-adds around each, 16 for the MFMAs of as many scores beside them) and by what
+// staging the rows takes beside them: six prompts of 101 to 1501 rows, 69 million scores, 46 us (with 64 positions per
+// wave, half the LDS reads, 11 us more).
 template <bool BF16, int D, bool SPLIT>
 __global__ void __launch_bounds__(512, SPLIT && D == 128 ? 1 : 2) chunks_tile_weights_kernel(const ChunksK p) {
     using T = typename Elem<BF16>::T;
