@@ -161,6 +161,9 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
     const int kv = a.geom.kv_heads, gmax = cdiv(a.heads, kv);
     const bool tiles = a.geom.mfma_layout && a.heads % kv == 0;
     const bool f32 = !tiles && chunks_f32_takes(a.dtype, a.geom.head_dim, a.heads, kv);
+    // Three parts of bf16 need more registers than the kernel of many rows has (fp32 rows over a bf16 cache, 2048 after 6144: 645
+    // us here, 414 there with two, whose error is 4e-6 where three have 4e-7).
+    const bool parts3 = chunk_parts(a.dtype, a.act != a.dtype) == 3;
     for (int i = 0; i < a.n; ++i) {
         const long long rows = static_cast<long long>(a.it[i].rows) * gmax;
         if (f32) {
@@ -169,7 +172,7 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
             pl.it[i].blocks = cdiv(a.it[i].rows, kGeom[pl.it[i].kind].rows / gmax);
             continue;
         }
-        pl.it[i].kind = !tiles ? kChunkAny : rows <= 32 ? kChunkStream32 : rows <= 128 ? kChunkStream : kChunkTile;
+        pl.it[i].kind = !tiles ? kChunkAny : rows <= 32 ? kChunkStream32 : rows <= 128 || parts3 ? kChunkStream : kChunkTile;
         pl.it[i].blocks = cdiv(rows, kGeom[pl.it[i].kind].rows);
     }
     // The keys of a kind's blocks are split while its units do not fill the GPU: as many tiles per unit as leave

@@ -15,9 +15,8 @@
 // last moved: the weights stay at or below 1 (a V near the type's largest value does not overflow)
 // and the accumulators are rescaled only when a score passes it.  Sums are of the fp32 weights.
 // Queries that are not of the cache's type enter as parts of it, and so do the weights: two parts keep 16 (bf16) or 22
-// (fp16) bits of both.  Few rows, which HBM bounds, take three of bf16, 24 bits: the error of eight verify chunks falls from
-// 4e-6 to 4e-7 for 102 us instead of 87; many rows take two (SPLIT).  Otherwise the weights are rounded to the type once,
-// as the output is.
+// (fp16) bits of both, three of bf16 24.  bf16 takes three (the error of eight verify chunks 4e-6 with two, 4e-7 with three, 87
+// and 102 us), fp16 two.  Otherwise the weights are rounded to the type once, as the output is.
 //
 // Tiles are copied into LDS by buffer-load DMA as they lie in the page.
 #include "qr_chunks.hpp"
@@ -316,7 +315,8 @@ __device__ __forceinline__ void chunk_stream(const ChunksK& p, const ChunkItem& 
     constexpr int NG = D / 8;                     // f32x4 groups of a row in a lane
     static_assert(NG % PW == 0 && WAVES * 64 * (NG * 16 + 8) <= LDS, "the waves' (acc, m, l) fit");
     static_assert(UL >= 1 && NU >= 4 && (NU - 2) * UL < 64, "vmcnt");
-    const int split = u % it.splits, block = u / it.splits % it.blocks, kvh = u / (it.splits * it.blocks);
+    // (kv heads fastest, so that an XCD keeps few of them in its L2 where a chunk has many blocks; from the last block down)
+    const int kvh = u % p.geom.kv_heads, split = u / p.geom.kv_heads % it.splits, block = it.blocks - 1 - u / p.geom.kv_heads / it.splits;
     const int g = p.heads / p.geom.kv_heads;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rw = wave % RW, pw = wave / RW;
@@ -698,20 +698,21 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
 // per 64 of them, 8 for the multiply-adds around each, 16 for the MFMAs of as many scores beside them) and by what
 // staging the rows takes beside them: six prompts of 101 to 1501 rows, 69 million scores, 46 us (with 64 positions per
 // wave, half the LDS reads, 11 us more).
-template <bool BF16, int D, bool SPLIT>
-__global__ void __launch_bounds__(512, SPLIT && D == 128 ? 1 : 2) chunks_tile_weights_kernel(const ChunksK p) {
+template <bool BF16, int D, int PARTS>
+__global__ void __launch_bounds__(512, PARTS > 1 && D == 128 ? 1 : 2) chunks_tile_weights_kernel(const ChunksK p) {
     using T = typename Elem<BF16>::T;
     using vec8 = typename Elem<BF16>::vec8;
-    constexpr int NK = D / 16, RT = 4, ROWS = 32 * RT;
+    constexpr bool SPLIT = PARTS > 1;
+    constexpr int NK = D / 16, RT = PARTS > 2 ? 2 : 4, ROWS = 32 * RT;
     constexpr int CN = NK * RT / 8;          // operands per wave of a round
-    constexpr int PART = SPLIT ? 2 : 1, QB = NK * RT * 1024;
-    __shared__ __attribute__((aligned(1024))) char lds[2][PART * QB];
+    constexpr int QB = NK * RT * 1024;  // bytes of a part of the rows
+    __shared__ __attribute__((aligned(1024))) char lds[2][PARTS * QB];
     __shared__ float4 info[2][ROWS];
     const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
     const ChunkItem it = p.it[e];
     const int u = blockIdx.x - it.unit0;
     const int kvh = u / it.blocks, g = p.heads / p.geom.kv_heads, rows = it.rows * g;
-    static_assert(ROWS == kWeightTiles16.rows, "rows of a round");
+    static_assert(kWeightTiles16.rows % ROWS == 0, "rounds of whole turns");
     int split, block, splits;
     kWeightTiles16.find(it, g, u - kvh * it.blocks, &block, &split, &splits);
     const int lane = threadIdx.x & 63, half = lane >> 5, n = lane & 31;
@@ -719,8 +720,8 @@ __global__ void __launch_bounds__(512, SPLIT && D == 128 ? 1 : 2) chunks_tile_we
     const int len = it.pos0 + it.rows;
     const int b0 = block * kWeightTiles16.positions, t0 = b0 + 32 * wave;
     const int first = kWeightTiles16.first(it, g, block), rounds = kWeightTiles16.rounds(it, g, block);
-    const int r0 = first + static_cast<int>(static_cast<long long>(rounds) * split / splits) * ROWS;
-    const int r1 = min(rows, first + static_cast<int>(static_cast<long long>(rounds) * (split + 1) / splits) * ROWS);
+    const int r0 = first + static_cast<int>(static_cast<long long>(rounds) * split / splits) * kWeightTiles16.rows;
+    const int r1 = min(rows, first + static_cast<int>(static_cast<long long>(rounds) * (split + 1) / splits) * kWeightTiles16.rows);
     const float sign = p.qscale == 0.f ? 0.f : p.qscale < 0.f ? -1.f : 1.f;
     const float base = p.qscale == 0.f ? 1.f : fabsf(p.qscale);
     auto row_of = [&](int rho) { return static_cast<long long>(it.row0 + rho / g) * p.heads + kvh * g + rho % g; };
@@ -774,20 +775,26 @@ __global__ void __launch_bounds__(512, SPLIT && D == 128 ? 1 : 2) chunks_tile_we
 #pragma unroll
         for (int c = 0; c < CN; ++c) {
             char* o = lds[to] + 1024 * (wave + 8 * c) + 16 * lane;
-            vec8 hi, lo;
+            vec8 hi;
             if (!SPLIT) {
                 hi = raw[SPLIT ? 0 : c];
                 if (p.qscale <= 0.f)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) hi[i] = static_cast<T>(static_cast<float>(hi[i]) * sign);
             } else {
+vec8 part[PARTS];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float v = x[SPLIT ? c : 0][i] * sign;
-                    hi[i] = static_cast<T>(v);
-                    lo[i] = static_cast<T>(v - static_cast<float>(hi[i]));
+                    float v = x[SPLIT ? c : 0][i] * sign;
+#pragma unroll
+                    for (int q = 0; q < PARTS; ++q) {
+                        part[q][i] = static_cast<T>(v);
+                        v -= static_cast<float>(part[q][i]);
+                    }
                 }
-                *reinterpret_cast<vec8*>(o + QB) = lo;
+                hi = part[0];
+#pragma unroll
+                for (int q = 1; q < PARTS; ++q) *reinterpret_cast<vec8*>(o + q * QB) = part[q];
             }
             *reinterpret_cast<vec8*>(o) = hi;
         }
@@ -828,8 +835,8 @@ __global__ void __launch_bounds__(512, SPLIT && D == 128 ? 1 : 2) chunks_tile_we
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk) {
                 const char* q = lds[at] + 1024 * (rt * NK + kk) + 16 * lane;
-                s = mfma32(k[kk], *reinterpret_cast<const vec8*>(q), s);
-                if (SPLIT) s = mfma32(k[kk], *reinterpret_cast<const vec8*>(q + QB), s);
+#pragma unroll
+                for (int x = 0; x < PARTS; ++x) s = mfma32(k[kk], *reinterpret_cast<const vec8*>(q + x * QB), s);
             }
             // rows that do not see every position of the wave's, or stand past the end
             const int last = __float_as_int(f.z) - t0 - 8 * half;
@@ -863,8 +870,10 @@ hipError_t launch_kind(const ChunksK& k, int kind, hipStream_t s) {
     switch (kind) {
         case kChunkStream32: hipLaunchKernelGGL((chunks_stream32_kernel<BF16, D, PARTS>), dim3(k.units), dim3(256), 0, s, k); break;
         case kChunkStream: hipLaunchKernelGGL((chunks_stream_kernel<BF16, D, PARTS>), dim3(k.units), dim3(256), 0, s, k); break;
-        case kChunkTile: hipLaunchKernelGGL((chunks_tile_kernel<BF16, D, SPLIT>), dim3(chunk_grid(k)), dim3(512), 0, s, k); break;
-        default: hipLaunchKernelGGL((chunks_tile_weights_kernel<BF16, D, SPLIT>), dim3(k.units), dim3(512), 0, s, k); break;
+        case kChunkTile:
+            if constexpr (PARTS < 3) hipLaunchKernelGGL((chunks_tile_kernel<BF16, D, SPLIT>), dim3(chunk_grid(k)), dim3(512), 0, s, k);
+            break;
+        default: hipLaunchKernelGGL((chunks_tile_weights_kernel<BF16, D, PARTS>), dim3(k.units), dim3(512), 0, s, k); break;
     }
     return hipGetLastError();
 }
