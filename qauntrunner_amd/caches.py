@@ -129,10 +129,15 @@ def _torch_code(x, what):
 
 
 def _on_device(x, device, what):
-    if not getattr(x, "is_cuda", False):
+    try:
+        at = x.get_device()
+    except AttributeError:
+        at = -1
+    if at == device:
+        return
+    if at < 0:
         raise ValueError(f"{what}: expected a tensor on the GPU")
-    if x.get_device() != device:
-        raise ValueError(f"{what}: the tensor is on device {x.get_device()}, the cache on device {device}")
+    raise ValueError(f"{what}: the tensor is on device {at}, the cache on device {device}")
 
 
 def _whole(x, numel, code, device, what):
@@ -154,11 +159,13 @@ def _strided(x, rows, width, code, device, what):
     _on_device(x, device, what)
     if _torch_code(x, what) != code:
         raise ValueError(f"{what}: dtype {x.dtype} does not match the other rows' dtype")
-    if tuple(x.shape) != (rows, width):
-        raise ValueError(f"{what}: expected [{rows}, {width}], got {list(x.shape)}")
-    if rows and width > 1 and x.stride(1) != 1:
+    shape = x.shape
+    if len(shape) != 2 or shape[0] != rows or shape[1] != width:
+        raise ValueError(f"{what}: expected [{rows}, {width}], got {list(shape)}")
+    between, step = x.stride()
+    if rows and width > 1 and step != 1:
         raise ValueError(f"{what}: the values of a row must stand next to each other")
-    stride = x.stride(0) if rows > 1 else width
+    stride = between if rows > 1 else width
     if stride < width:
         raise ValueError(f"{what}: rows overlap (stride {stride} for {width} values)")
     p = x.data_ptr()

@@ -143,8 +143,14 @@ int qr_kv_append_norm_rope_dev(qr_kv* kv, int n, const int* seq_ids, int layer, 
         a.k_norm = k_norm_dev;
         a.eps = eps;
         a.rot = rotary_dim;
-        for (int i = 0; i < rotary_dim / 2; ++i)
-            a.turn[i] = std::pow(static_cast<double>(theta), -2.0 * i / rotary_dim) / (2.0 * 3.14159265358979323846);
+        if (kv->turn_theta != theta || kv->turn_dim != rotary_dim) {
+            kv->turn.resize(rotary_dim / 2);
+            for (int i = 0; i < rotary_dim / 2; ++i)
+                kv->turn[i] = std::pow(static_cast<double>(theta), -2.0 * i / rotary_dim) / (2.0 * 3.14159265358979323846);
+            kv->turn_theta = theta;
+            kv->turn_dim = rotary_dim;
+        }
+        std::copy(kv->turn.begin(), kv->turn.end(), a.turn);
         long long done = 0;
         for (int i = 0; i < n;) {
             a.n = a.rows = 0;

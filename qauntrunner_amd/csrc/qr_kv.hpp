@@ -20,6 +20,9 @@ struct qr_kv {
     hipEvent_t split_event = nullptr;  // benchmark instrumentation (qr_kv_set_split_event)
     void* scratch = nullptr;           // this device's decode scratch array (no-allocation calls)
     bool device_steps = false;         // the device copy of the page accounting is in use
+    std::vector<double> turn;          // turns per position of the pairs of a rotation of turn_dim values, base turn_theta
+    float turn_theta = 0.f;            // (64 powers take 1.5 us; the last call's stay)
+    int turn_dim = 0;
 };
 
 namespace qr {
