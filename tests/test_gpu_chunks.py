@@ -114,6 +114,45 @@ def test_prompts(gpu, dtype, act, heads, kv_heads, D, weights):
         run(kv, rows, [(0, 400, 800), (1, 0, 515), (2, 129, 1)], heads, kv_heads, D, dtype, act, weights)
 
 
+@pytest.mark.parametrize("dtype,act", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f32")])
+@pytest.mark.parametrize("heads,kv_heads", [(12, 3), (10, 5), (24, 12), (14, 14), (16, 16), (2, 1), (63, 9)])
+def test_kv_heads_over_the_xcds(gpu, dtype, act, heads, kv_heads):
+    """Kernels of many rows deal the kv heads of a launch to eight parts of the GPU: counts that divide and that do not."""
+    kv, rows = filled(heads, kv_heads, 64, dtype, [700, 300, 40])
+    with kv:
+        run(kv, rows, [(1, 1, 299), (0, 290, 410), (2, 0, 40)], heads, kv_heads, 64, dtype, act)
+
+
+@pytest.mark.parametrize("dtype,act", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16")])
+def test_two_graphs_of_one_cache(gpu, dtype, act):
+    """Graphs of a small and a large call share the handle's workspace, which grew between their captures."""
+    lengths = [900, 600, 33]
+    kv, rows = filled(8, 2, 128, dtype, lengths)
+    calls = [([0, 1, 2], [899, 599, 32], [1, 1, 1]), ([0, 2, 1], [300, 0, 0], [600, 33, 600])]
+    with kv:
+        graphs, ins, outs, ws = [], [], [], []
+        for ids, p, n in calls:
+            q = randn(len(graphs), sum(n), 8 * 128, dtype=act)
+            out, w = torch.zeros_like(q), torch.zeros(3, 2, 900, device="cuda")
+            kv.AttentionChunksDev(0, ids, p, n, q, out, 0.1, weights=w)
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                kv.AttentionChunksDev(0, ids, p, n, q, out, 0.1, weights=w)
+            for l, x in zip((graphs, ins, outs, ws), (g, q, out, w)):
+                l.append(x)
+        for turn in range(3):
+            for i in (0, 1, 1, 0):
+                ins[i].copy_(randn(10 + turn, *ins[i].shape, dtype=act))
+                outs[i].zero_()
+                ws[i].zero_()
+                graphs[i].replay()
+            for i, (ids, p, n) in enumerate(calls):
+                out, w = torch.zeros_like(outs[i]), torch.zeros_like(ws[i])
+                kv.AttentionChunksDev(0, ids, p, n, ins[i], out, 0.1, weights=w)
+                assert torch.equal(out, outs[i]) and torch.equal(w, ws[i])
+
+
 @pytest.mark.parametrize("dtype,act", [("f32", "f32"), ("bf16", "bf16")])
 def test_more_chunks_than_one_launch_takes(gpu, dtype, act):
     n = 131
