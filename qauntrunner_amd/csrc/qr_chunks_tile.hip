@@ -237,6 +237,34 @@ struct Rows {
 
     // The row's output or split partial: N groups of 4 dims from group g0 on, of the weighted sums a.
     // Group g holds dims 32 (g / 4) + 8 (g % 4) + 4 half .. + 3.
+    // A sum that is no number though the weights are comes from an infinite V: a part of a weight may be negative, or a weight
+    // round to zero.  It is that infinity, unless the row sees a NaN or both; read again from the page, once per such element.
+    template <int N>
+    __device__ __forceinline__ void settle(const ChunksK& p, const ChunkItem& it, int t0, int t1, int g0, float lsum, f32x4_t (&a)[N]) const {
+        uint64_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) bad |= a[i >> 2][i & 3] == a[i >> 2][i & 3] ? 0 : 1ull << i;
+        if (!on || !(lsum == lsum)) bad = 0;
+        if (!__builtin_amdgcn_ballot_w64(bad != 0)) return;
+        const int kvh = head / (p.heads / p.geom.kv_heads), end = min(t1, lim + 1);
+        while (bad) {
+            const int n = __ffsll(static_cast<unsigned long long>(bad)) - 1;
+            bad &= bad - 1;
+            const int d = 32 * ((g0 + (n >> 2)) >> 2) + 8 * ((g0 + (n >> 2)) & 3) + 4 * half + (n & 3);
+            float least = 0.f, most = 0.f, nan = 0.f;
+            for (int t = t0; t < end; ++t) {
+                const long long phys = p.page_table[it.pt_off + (t >> kPageShift)];
+                const float v = load_elem(p.pool, p.dtype, p.geom.offset(phys, 1, kvh, t & (kPageTokens - 1), d));
+                least = fminf(least, v);
+                most = fmaxf(most, v);
+                if (v != v) nan = v;
+            }
+            const bool minus = least == -INFINITY, plus = most == INFINITY;
+            const float r = nan != nan || minus == plus ? NAN : plus ? INFINITY : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4 * N; ++i) a[i >> 2][i & 3] = i == n ? r : a[i >> 2][i & 3];
+        }
+    }
     template <int N>
     __device__ __forceinline__ void store(const ChunksK& p, const ChunkItem& it, int split, int g0, float lsum, const f32x4_t (&a)[N]) const {
         if (!on) return;
@@ -470,6 +498,7 @@ __device__ __forceinline__ void chunk_stream(const ChunksK& p, const ChunkItem& 
 #pragma unroll
         for (int x = 0; x < PW; ++x) o[q] += xa[((x * RW + rw) * NG + pw * NP + q) * 64 + w.lane] * c[x];
     }
+    w.settle(p, it, t0, t1, pw * NP, L, o);
     w.store(p, it, split, pw * NP, L, o);
     if (pw == 0) w.store_ml(p, it, split, M, L);
 }
@@ -686,6 +715,7 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
 #pragma unroll
     for (int q = 0; q < 4 * R::ND; ++q)
         o[q] = f32x4_t{w.acc[q >> 2][4 * (q & 3)], w.acc[q >> 2][4 * (q & 3) + 1], w.acc[q >> 2][4 * (q & 3) + 2], w.acc[q >> 2][4 * (q & 3) + 3]};
+    w.settle(p, it, t0, t1, 0, w.l, o);
     w.store(p, it, split, 0, w.l, o);
     w.store_ml(p, it, split, w.m, w.l);
 }

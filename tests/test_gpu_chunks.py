@@ -195,6 +195,44 @@ def test_what_a_row_does_not_see_does_not_reach_it(gpu, dtype, act, D):
         assert torch.equal(w, wc)
 
 
+@pytest.mark.parametrize("dtype,act", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("f16", "f32"), ("bf16", "f32")])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [6, 12, 20, 33, 150])
+def test_special_rows_in_a_chunk(gpu, dtype, act, D, n):
+    """A NaN or infinite key or value inside a chunk (of every number of rows that has a kernel) and what lies behind it:
+    rows before it give what they give without, rows that see it show it."""
+    heads, kv_heads, p0 = 8, 2, 210
+    end = p0 + n
+    kv, rows = filled(heads, kv_heads, D, dtype, [end], max_seq=512)
+    tight = tol(dtype, act)
+    with kv:
+        chunks = [(0, p0, n)]
+        clean, wc, _, _ = run(kv, rows, chunks, heads, kv_heads, D, dtype, act)
+        k0, v0 = rows[0]
+        behind = torch.full((512 - end, kv_heads * D), float("nan"), dtype=TORCH[dtype], device="cuda")
+        kv.AppendRangeDev(0, end, behind, behind, dtype, seq_id=0)
+        at = n // 2  # the row whose own position is the special one
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            v = v0[p0 + at:p0 + at + 1].clone()
+            v[0, 1, D - 3] = bad
+            kv.AppendRangeDev(0, p0 + at, k0[p0 + at:p0 + at + 1].reshape(1, -1), v.reshape(1, -1), dtype, seq_id=0)
+            got, w, _, _ = run(kv, rows, chunks, heads, kv_heads, D, dtype, act, check=False)
+            same = torch.ones_like(got, dtype=torch.bool)
+            same[at:, 4:, D - 3] = False
+            assert torch.allclose(got[same].double(), clean[same].double(), rtol=tight, atol=tight)
+            shown = got[at:, 4:, D - 3]
+            assert (shown.isnan() if bad != bad else shown == bad).all()
+            assert torch.equal(w, wc)
+        k = k0[p0 + at:p0 + at + 1].clone()
+        k[0, 0, 2] = float("nan")
+        kv.AppendRangeDev(0, p0 + at, k.reshape(1, -1), v0[p0 + at:p0 + at + 1].reshape(1, -1), dtype, seq_id=0)
+        got, w, _, _ = run(kv, rows, chunks, heads, kv_heads, D, dtype, act, check=False)
+        assert torch.allclose(got[:at].double(), clean[:at].double(), rtol=tight, atol=tight)
+        assert torch.allclose(got[:, 4:].double(), clean[:, 4:].double(), rtol=tight, atol=tight)
+        assert got[at:, :4].isnan().all()
+        assert torch.equal(w[0, 1], wc[0, 1]) and w[0, 0, p0 + at].isnan()
+
+
 @pytest.mark.parametrize("dtype,act", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32")])
 @pytest.mark.parametrize("scale", [0.0, -0.125, 0.5])
 def test_scales(gpu, dtype, act, scale):
