@@ -139,7 +139,6 @@ struct ChunkPlanItem {
 };
 struct ChunksPlan {
     ChunkPlanItem it[kBatch];
-    bool merge;              // some chunk's keys are split
     bool wmerge;             // some chunk's weights are summed in parts
     size_t part_ml, row_ml, row_scale, scores, wpart;  // offsets in the workspace; the partials' sums come first
     size_t workspace_bytes;

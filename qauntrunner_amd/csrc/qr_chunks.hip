@@ -32,13 +32,65 @@ __global__ void __launch_bounds__(64) chunks_merge_any_kernel(const ChunksK p) {
     if (p.row_ml && lane == 0) p.row_ml[rh] = make_float2(m, l);
 }
 
-// The same for the tiles' head sizes: D / 4 threads per (row, head), 4 dims each, the partials of 8
-// splits requested at once (16 rows of 32 heads over 17 splits: 7.6 -> 4 us against one wave per row).
+// Weights from the stored scores of a chunk's rows (up to 32 of a kv head): one thread per position.  The rows' maxima and sums
+// come from the partials, eight threads a row, so that the merge can run beside it.
+__device__ __forceinline__ void add_scores(const ChunksK& p, const ChunkItem& it, int u) {
+    __shared__ float2 row[32];
+    const int t = u % it.blocks * 256 + threadIdx.x, kvh = u / it.blocks;
+    const int g = p.heads / p.geom.kv_heads, stride = chunk_score_len(it);
+    const bool on = t < it.pos0 + it.rows;
+    float* const w = p.weights + (static_cast<long long>(it.seq) * p.geom.kv_heads + kvh) * p.max_seq + t;
+    const float before = on ? *w : 0.f;
+    const int r = threadIdx.x >> 3;
+    float m = -INFINITY, l = 0.f;
+    if (r < it.rows * g) {
+        const long long rh = static_cast<long long>(r / g) * p.heads + kvh * g + r % g;
+        if (it.splits == 1) {
+            const float2 ml = p.row_ml[static_cast<long long>(it.row0) * p.heads + rh];
+            m = ml.x;
+            l = threadIdx.x & 7 ? 0.f : ml.y;
+        } else {
+            const float2* ml = p.part_ml + it.slot0 + rh * it.splits;
+            for (int s = threadIdx.x & 7; s < it.splits; s += 8) m = fmaxf(m, ml[s].x);
+            for (int x = 1; x < 8; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+            for (int s = threadIdx.x & 7; s < it.splits; s += 8) l = fmaf(ml[s].y, ml[s].x == -INFINITY ? 0.f : fast_exp2(ml[s].x - m), l);
+        }
+    }
+    for (int x = 1; x < 8; x <<= 1) l += __shfl_xor(l, x);
+    if ((threadIdx.x & 7) == 0) row[r] = make_float2(m, l);
+    __syncthreads();
+    const float* s = p.scores + it.score0 + static_cast<long long>(kvh) * g * stride + (on ? t : 0);
+    float sum = 0.f;
+    for (int j = 0; j < it.rows; ++j, s += static_cast<long long>(p.heads) * stride) {
+        const bool see = t <= it.pos0 + j;
+#pragma unroll 4
+        for (int h = 0; h < g; ++h) {
+            const float2 ml = row[j * g + h];
+            const float x = fast_exp2(s[static_cast<long long>(h) * stride] - ml.x) / ml.y;
+            if (see) sum += x;
+        }
+    }
+    if (on) *w = before + sum;
+}
+
+// The merge for the tiles' head sizes: D / 4 threads per (row, head), 4 dims each, the partials of 8
+// splits requested at once (16 rows of 32 heads over 17 splits: 7.6 -> 4 us against one wave per row).  Behind a chunk's
+// merge units stand those that add its weights from stored scores: one launch for both (16 decode rows of 130 to
+// 16000 positions with weights 56.7 -> 55.4 us, two of a tiny model 15 -> 12).
+constexpr int merge_rows(int D) { return 256 / (D / 4); }
+__host__ __device__ inline int merge_units(const ChunkItem& it, int heads, int rows) {
+    return it.splits > 1 ? static_cast<int>((static_cast<long long>(it.rows) * heads + rows - 1) / rows) : 0;
+}
 template <int D>
 __global__ void __launch_bounds__(256) chunks_merge_kernel(const ChunksK p) {
-    constexpr int TPR = D / 4, RPB = 256 / TPR, kB = 8;
+    constexpr int TPR = D / 4, RPB = merge_rows(D), kB = 8;
     const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
     const ChunkItem it = p.it[e];
+    const int merges = merge_units(it, p.heads, RPB);
+    if (static_cast<int>(blockIdx.x) - it.unit0 >= merges) {
+        add_scores(p, it, blockIdx.x - it.unit0 - merges);
+        return;
+    }
     const int rr = threadIdx.x / TPR, c = threadIdx.x - rr * TPR;
     const long long r = static_cast<long long>(blockIdx.x - it.unit0) * RPB + rr;
     if (rr >= RPB || r >= static_cast<long long>(it.rows) * p.heads) return;
@@ -96,31 +148,6 @@ __global__ void __launch_bounds__(256) chunks_merge_kernel(const ChunksK p) {
         __builtin_memcpy(static_cast<uint16_t*>(p.out) + rh * D + 4 * c, b, 8);
     }
     if (p.row_ml && c == 0) p.row_ml[rh] = make_float2(m, l);
-}
-
-// Weights from the stored scores of a chunk's rows: one thread per position.  Bound by the scores (16 rows of 32 heads over
-// 57965 positions: 6 us for 9 MB).
-__global__ void __launch_bounds__(256) chunks_scores_kernel(const ChunksK p) {
-    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
-    const ChunkItem it = p.it[e];
-    const int u = blockIdx.x - it.unit0;
-    const int t = u % it.blocks * 256 + threadIdx.x, kvh = u / it.blocks;
-    const int g = p.heads / p.geom.kv_heads, stride = chunk_score_len(it);
-    const bool on = t < it.pos0 + it.rows;
-    float* const w = p.weights + (static_cast<long long>(it.seq) * p.geom.kv_heads + kvh) * p.max_seq + t;
-    const float before = on ? *w : 0.f;
-    const float* s = p.scores + it.score0 + static_cast<long long>(kvh) * g * stride + (on ? t : 0);
-    const float2* ml = p.row_ml + static_cast<long long>(it.row0) * p.heads + kvh * g;
-    float sum = 0.f;
-    for (int j = 0; j < it.rows; ++j, s += static_cast<long long>(p.heads) * stride, ml += p.heads) {
-        const bool see = t <= it.pos0 + j;
-#pragma unroll 4
-        for (int h = 0; h < g; ++h) {
-            const float x = fast_exp2(s[static_cast<long long>(h) * stride] - ml[h].x) / ml[h].y;
-            if (see) sum += x;
-        }
-    }
-    if (on) *w = before + sum;
 }
 
 // Parts of the weights' sums: one thread per position.
@@ -219,10 +246,7 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
                 it.blocks = static_cast<int>(kt.units(a.it[i], gmax, it.per));
                 it.splits = cdiv(tiles_of(i), it.per);
             }
-            if (it.splits > 1) {
-                slots += static_cast<long long>(a.it[i].rows) * a.heads * it.splits;
-                pl.merge = true;
-            }
+            if (it.splits > 1) slots += static_cast<long long>(a.it[i].rows) * a.heads * it.splits;
         }
     }
     long long wslots = 0, scores = 0;
@@ -330,15 +354,19 @@ hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* work
         e = kind == kChunkAny ? launch_chunks_any(k, stream) : kind >= kChunkF32Half ? launch_chunks_f32(k, kind, stream)
           : launch_chunks_tile(k, kind, stream);
     }
-    if (e == hipSuccess && plan.merge) {
-        gather([](const ChunkPlanItem& p) { return p.splits > 1; }, false);
+    auto scored = [&](const ChunkPlanItem& p) { return a.weights && p.wkind == kWeightsScores; };
+    if (e == hipSuccess && gather([&](const ChunkPlanItem& p) { return p.splits > 1 || scored(p); }, false)) {
         const int D = a.geom.head_dim;
         const bool vec = D == 64 || D == 96 || D == 128 || D == 256;
-        const int per = vec ? 256 / (D / 4) : 1;  // rows of a workgroup
+        k.scores = reinterpret_cast<float*>(w + plan.scores);
         k.units = 0;
         for (int i = 0; i < k.n; ++i) {
-            k.it[i].unit0 = k.units;
-            k.units += cdiv(static_cast<long long>(k.it[i].rows) * a.heads, per);
+            ChunkItem& it = k.it[i];
+            it.unit0 = k.units;
+            k.units += merge_units(it, a.heads, vec ? merge_rows(D) : 1);
+            if (!a.weights || it.score0 < 0) continue;
+            it.blocks = cdiv(it.pos0 + it.rows, 256);
+            k.units += it.blocks * kv;
         }
         if (D == 64) hipLaunchKernelGGL(chunks_merge_kernel<64>, dim3(k.units), dim3(256), 0, stream, k);
         else if (D == 96) hipLaunchKernelGGL(chunks_merge_kernel<96>, dim3(k.units), dim3(256), 0, stream, k);
@@ -348,16 +376,10 @@ hipError_t launch_chunks(const ChunksArgs& a, const ChunksPlan& plan, void* work
         e = hipGetLastError();
     }
     if (!a.weights) return e;
-    k.scores = reinterpret_cast<float*>(w + plan.scores);
     for (int kind = 0; kind < kWeightsKinds && e == hipSuccess; ++kind) {
-        if (!gather([&](const ChunkPlanItem& p) { return p.wkind == kind; }, true)) continue;
-        if (kind == kWeightsScores) {
-            hipLaunchKernelGGL(chunks_scores_kernel, dim3(k.units), dim3(256), 0, stream, k);
-            e = hipGetLastError();
-        } else {
-            e = kind == kWeightsAny ? launch_chunks_any_weights(k, stream) : kind == kWeightsF32 ? launch_chunks_f32(k, kChunkKinds, stream)
-              : launch_chunks_tile(k, kChunkKinds, stream);
-        }
+        if (kind == kWeightsScores || !gather([&](const ChunkPlanItem& p) { return p.wkind == kind; }, true)) continue;
+        e = kind == kWeightsAny ? launch_chunks_any_weights(k, stream) : kind == kWeightsF32 ? launch_chunks_f32(k, kChunkKinds, stream)
+          : launch_chunks_tile(k, kChunkKinds, stream);
     }
     if (e == hipSuccess && plan.wmerge) {
         gather([](const ChunkPlanItem& p) { return p.wkind >= kWeightsTile && p.wparts > 1; }, true);
