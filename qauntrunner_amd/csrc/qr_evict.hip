@@ -29,7 +29,8 @@ __device__ __forceinline__ int block_scan(int x, int* wsum) {
     }
     if (lane == 63) wsum[wave] = x;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) x += wsum[w];
+#pragma unroll
+    for (int w = 0; w < kSelThreads / 64; ++w) x += w < wave ? wsum[w] : 0;
     __syncthreads();
     return x;
 }
@@ -488,7 +489,7 @@ struct EvictShape {
     int rows, keep, longest;  // of the entries that give positions up
     int parts;                // workgroups per row, 0: one
 };
-// Rows of more than 32768 positions are shared by workgroups while the counts stay in L2 (8 rows of 65536: 34 us, one
+// Rows of more than 32768 positions are shared by workgroups while the counts stay in L2 (8 rows of 65536: 32 us, one
 // workgroup each 93; 128 rows of up to 17000: 40 us, 27)
 EvictShape evict_shape(const EvictArgs& a) {
     EvictShape s{a.n * a.geom.kv_heads, a.first + a.heavy + a.recent, 0, 0};
