@@ -11,12 +11,15 @@
 // a lane's scores r = 8 s + i are positions 16 s + 8 (lane / 32) + i: its k-slots of PV step s, and
 // V's operand is 8 consecutive positions of a dim, 16 bytes of the page.
 //
-// Softmax in log2 units with the running maximum held `kHead` above the largest score seen when it
-// last moved: the weights stay at or below 1 (a V near the type's largest value does not overflow)
-// and the accumulators are rescaled only when a score passes it.  Sums are of the fp32 weights.
+// Softmax in log2 units: weights 2^(s - m) of at most 2^kTop, m moved (and the accumulators rescaled) only when a score
+// passes m + kTop, and then to leave kHead log2 units to the next move.  bf16 weights stay at or below 1: a V near the type's
+// largest value does not overflow.  fp16 has few exponents below 1 (subnormal from 2^-14, nothing below 2^-25), so its
+// weights go up to 2^15: whole down to 2^-25 of a row's largest or less, and products of up to 2^31 leave the sums room for
+// any number of keys.  Sums are of the fp32 weights.
 // Queries that are not of the cache's type enter as parts of it, and so do the weights: two parts keep 16 (bf16) or 22
-// (fp16) bits of both, three of bf16 24.  bf16 takes three (the error of eight verify chunks 4e-6 with two, 4e-7 with three, 87
-// and 102 us), fp16 two.  Otherwise the weights are rounded to the type once, as the output is.
+// (fp16) bits of both -- of a weight w of the row's largest in fp16 no less than 2^-40 / w -- three of bf16 24.  bf16 takes
+// three (the error of eight verify chunks 4e-6 with two, 4e-7 with three, 87 and 102 us), fp16 two.  Otherwise the weights are
+// rounded to the type once, as the output is.
 //
 // Tiles are copied into LDS by buffer-load DMA as they lie in the page.
 #include "qr_chunks.hpp"
@@ -54,7 +57,7 @@ struct Rows {
     using vec8 = typename Elem<BF16>::vec8;
     static constexpr int NK = D / 16;   // QK k-steps
     static constexpr int ND = D / 32;   // PV dim tiles
-    static constexpr float kHead = SPLIT ? 0.f : 4.f;
+    static constexpr float kTop = BF16 ? 0.f : 15.f, kHead = SPLIT ? 0.f : 4.f;
 
     int lane, half;
     int query, head;     // of row lane % 32
@@ -168,10 +171,15 @@ struct Rows {
         float t = mx[0];
 #pragma unroll
         for (int n = 1; n < 2 * NS; ++n) t = fmaxf(t, mx[n]);
-        t = max_xor32(t) * sscale;
-        const bool grow = t > m;
+        t = max_xor32(t);
+        const bool grow = fmaf(t, sscale, -m) > kTop;
         if (__builtin_amdgcn_ballot_w64(grow)) {
-            const float mn = grow ? t + kHead : m;
+            float mn = fmaf(t, sscale, kHead - kTop);
+            if (fmaf(t, sscale, -mn) > kTop) {  // rounded down, where a step of m is that large
+                const int b = __float_as_int(mn);
+                mn = __int_as_float(b < 0 ? b - 1 : b + 1);
+            }
+            mn = grow ? mn : m;
             const float c = m == -INFINITY ? 0.f : fast_exp2(m - mn);
             if (__builtin_amdgcn_ballot_w64(grow && m != -INFINITY)) {
                 const float cc = grow && m != -INFINITY ? c : 1.f;
