@@ -125,7 +125,7 @@ int qr_kv_append_norm_rope_dev(qr_kv* kv, int n, const int* seq_ids, int layer, 
                 pages += std::max(0, (pos0[i] + rows[i] + kPageTokens - 1) / kPageTokens - kv->store.pages_held(seq_ids[i], layer));
         if (pages > kv->store.capacity()) {
             QR_CHECK_ARG(pages < (1LL << 31), "%lld pages are too many", pages);
-            QR_TRY(kv->store.reserve(static_cast<int>(std::max(pages, std::min(2 * kv->store.capacity(), (1LL << 31) - 1)))));
+            QR_TRY(kv->store.reserve(static_cast<int>(pages)));  // (to twice the pool where that fits)
         }
         for (int i = 0; i < n; ++i)
             if (rows[i]) QR_TRY(kv->store.ensure(seq_ids[i], layer, pos0[i] + rows[i], st));
