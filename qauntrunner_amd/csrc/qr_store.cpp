@@ -34,6 +34,8 @@ DevBuf::~DevBuf() {
 
 int DevBuf::ensure(size_t bytes, bool zero) {
     if (bytes <= size_) return QR_OK;
+    const auto whole = [](size_t n) { return (n + 255) & ~static_cast<size_t>(255); };
+    size_t want = whole(std::max(bytes, size_ * 2));
     if (ptr_ && keep_retired_) {
         retired_.push_back(ptr_);  // a captured graph may still use it: freed with the buffer
         ptr_ = nullptr;
@@ -44,9 +46,12 @@ int DevBuf::ensure(size_t bytes, bool zero) {
         ptr_ = nullptr;
         size_ = 0;
     }
-    size_t want = std::max(bytes, size_ * 2);
-    want = (want + 255) & ~static_cast<size_t>(255);
-    QR_HIP(hipMalloc(&ptr_, want));
+    if (want > whole(bytes) && hipMalloc(&ptr_, want) != hipSuccess) {
+        (void)hipGetLastError();
+        ptr_ = nullptr;
+        want = whole(bytes);  // doubling failed: exactly what is needed
+    }
+    if (!ptr_) QR_HIP(hipMalloc(&ptr_, want));
     size_ = want;
     if (zero) QR_HIP(hipMemset(ptr_, 0, want));
     return QR_OK;

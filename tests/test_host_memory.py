@@ -19,3 +19,42 @@ budget.value = live.value + 18 * page
 assert append(kv, [1], [0], [1]) == 0, L.qr_last_error()
 """)
     assert out.split() == ["pages", "1"]
+
+
+def test_the_workspace_grows_by_doubling(tmp_path):
+    """A decode loop with weights, whose workspace grows with the sequences: few allocations, each a wait for the GPU, and
+    what a captured graph keeps alive stays within twice the largest."""
+    out = run(tmp_path, """
+n = 16
+kv = PagedKvCache(1, 32, 8, 128, 4096, "f16", n)
+seqs = list(range(n))
+assert append(kv, seqs, [0] * n, [4096] * n) == 0
+before, allocations, waits = live.value, mallocs.value, syncs.value
+for captured in (0, 1):
+    capturing.value = captured
+    assert attend(kv, seqs, [0] * n, [1] * n) == 0, L.qr_last_error()
+capturing.value = 0
+for p in range(1, 4096):
+    assert attend(kv, seqs, [p] * n, [1] * n) == 0, L.qr_last_error()
+need = 4 * n * 32 * 4096  # a score per row, head and position, beside which the partials are small
+print(mallocs.value - allocations, syncs.value - waits, (live.value - before) / need)
+""")
+    allocations, waits, held = map(float, out.split())
+    assert allocations <= 20 and waits <= 40 and held <= 6, out
+
+
+def test_the_workspace_takes_what_it_needs_where_it_cannot_double(tmp_path):
+    out = run(tmp_path, """
+kv = PagedKvCache(1, 32, 8, 128, 65536, "f16", 16)
+seqs = list(range(16))
+assert append(kv, seqs, [0] * 16, [65536] * 16) == 0
+before = live.value
+assert attend(kv, seqs, [9999] * 16, [1] * 16) == 0
+small = live.value - before
+budget.value = live.value + small // 4  # room for a quarter more once the old one is given back
+assert attend(kv, seqs, [10999] * 16, [1] * 16) == 0, L.qr_last_error()
+print((live.value - before) / small)
+assert attend(kv, seqs, [39999] * 16, [1] * 16) == _lib.QR_ERR_OUT_OF_MEMORY
+assert attend(kv, seqs, [9999] * 16, [1] * 16) == 0, L.qr_last_error()
+""")
+    assert 1.0 < float(out) < 1.25
