@@ -32,6 +32,7 @@ void clear_error();
     do {                                                                              \
         hipError_t e_ = (call);                                                       \
         if (e_ != hipSuccess) {                                                       \
+            (void)hipGetLastError(); /* else the next launch's check reports it */    \
             ::qr::set_error("%s failed: %s (%s:%d)", #call, hipGetErrorString(e_),    \
                             __FILE__, __LINE__);                                      \
             return e_ == hipErrorOutOfMemory ? QR_ERR_OUT_OF_MEMORY : QR_ERR_HIP;     \

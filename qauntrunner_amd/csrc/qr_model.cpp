@@ -795,6 +795,7 @@ int qr_model_make_resident(qr_model* m) {
     for (int i = 0; i < 2 && st == QR_OK; ++i)
         if (hipHostMalloc(&pinned[i], chunk, hipHostMallocDefault) != hipSuccess ||
             hipEventCreateWithFlags(&done[i], hipEventDisableTiming) != hipSuccess) {
+            (void)hipGetLastError();  // else the next launch's check reports it
             set_error("pinned staging allocation of %zu bytes failed", chunk);
             st = QR_ERR_OUT_OF_MEMORY;
         }

@@ -75,6 +75,7 @@ int qr_weight_create(qr_weight** out, int format, long long rows, int cols, cons
     if (e == hipSuccess) e = hipMalloc(&w->dev, bytes);
     if (e == hipSuccess) e = hipMemcpy(w->dev, host_bytes, bytes, hipMemcpyHostToDevice);
     if (e != hipSuccess) {
+        (void)hipGetLastError();  // else the next launch's check reports it
         set_error("uploading %zu weight bytes failed: %s", bytes, hipGetErrorString(e));
         if (w->dev) (void)hipFree(w->dev);
         if (w->stream) (void)hipStreamDestroy(w->stream);

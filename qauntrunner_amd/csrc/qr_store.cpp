@@ -125,6 +125,7 @@ int PagedStore::grow(long long min_pages) {
         if (e == hipSuccess) return grow_done(fresh, min_pages, pb);
     }
     if (e != hipSuccess) {
+        (void)hipGetLastError();
         set_error("page pool growth to %lld pages (%zu bytes each) failed: %s", cap, pb, hipGetErrorString(e));
         return QR_ERR_OUT_OF_MEMORY;
     }

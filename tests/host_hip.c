@@ -5,6 +5,7 @@
 
 long long hh_live, hh_budget = 1LL << 62, hh_mallocs, hh_syncs, hh_launches;
 int hh_capturing;
+static int last; /* a failed call's error stays until it is asked for */
 
 struct block { void *p; size_t n; struct block *next; };
 static struct block *blocks;
@@ -12,7 +13,7 @@ static long long scratch[1 << 20];
 
 int hipMalloc(void **out, size_t n) {
     *out = NULL;
-    if (hh_live + (long long)n > hh_budget) return 2; /* out of memory */
+    if (hh_live + (long long)n > hh_budget) return last = 2; /* out of memory */
     struct block *b = malloc(sizeof *b);
     b->p = calloc(1, n ? n : 1);
     b->n = n;
@@ -41,7 +42,7 @@ int hipMemcpyAsync(void *to, const void *from, size_t n, int kind, void *stream)
 int hipDeviceSynchronize(void) { ++hh_syncs; return 0; }
 int hipGetDevice(int *d) { *d = 0; return 0; }
 int hipSetDevice(int d) { return d != 0; }
-int hipGetLastError(void) { return 0; }
+int hipGetLastError(void) { int e = last; last = 0; return e; }
 const char *hipGetErrorString(int e) { return e == 2 ? "out of memory" : "error"; }
 int hipGetSymbolAddress(void **out, const void *symbol) { *out = scratch; return 0; }
 int hipStreamCreateWithFlags(void **s, unsigned flags) { *s = &hh_capturing; return 0; }

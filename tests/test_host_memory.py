@@ -58,3 +58,28 @@ assert attend(kv, seqs, [39999] * 16, [1] * 16) == _lib.QR_ERR_OUT_OF_MEMORY
 assert attend(kv, seqs, [9999] * 16, [1] * 16) == 0, L.qr_last_error()
 """)
     assert 1.0 < float(out) < 1.25
+
+
+def test_a_refused_allocation_does_not_fail_the_next_call(tmp_path):
+    """The runtime keeps a failed call's error until it is asked for; the launch checks of a later call must not find it."""
+    run(tmp_path, """
+kv = PagedKvCache(1, 8, 2, 64, 65536, "f32", 8)
+seqs = list(range(8))
+assert append(kv, seqs, [0] * 8, [4096] * 8) == 0
+budget.value = live.value
+assert append(kv, [0], [4096], [65536 - 4096]) == _lib.QR_ERR_OUT_OF_MEMORY  # the pool
+assert append(kv, [0], [0], [1]) == 0, L.qr_last_error()
+assert attend(kv, seqs, [4095] * 8, [1] * 8) == _lib.QR_ERR_OUT_OF_MEMORY  # the workspace
+assert append(kv, [0], [0], [1]) == 0, L.qr_last_error()
+""")
+
+
+def test_a_refused_weight_does_not_fail_the_next_call(tmp_path):
+    run(tmp_path, """
+kv = PagedKvCache(1, 8, 2, 64, 4096, "f32", 1)
+assert append(kv, [0], [0], [16]) == 0
+budget.value = live.value
+w = ctypes.c_void_p()
+assert L.qr_weight_create(ctypes.byref(w), _lib.FORMATS["F32"], 4, 256, rows_memory) == _lib.QR_ERR_OUT_OF_MEMORY
+assert append(kv, [0], [0], [16]) == 0, L.qr_last_error()
+""")
