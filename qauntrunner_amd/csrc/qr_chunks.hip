@@ -179,6 +179,9 @@ struct KindGeom {
 };
 constexpr KindGeom kGeom[kChunkKinds] = {{kChunkAnyRows, kChunkAnyTile, 1024}, {32, 128, 256}, {128, 64, 512}, {256, 64, 256}, {32, 32, 256}, {64, 32, 256}};
 
+// Scores that a launch keeps for its weights: 256 MB, a token of 32 heads over 32768 positions for each of its 64 chunks.
+constexpr long long kMaxScores = 64LL * 32 * 32768;
+
 int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
 }  // namespace
@@ -257,13 +260,19 @@ ChunksPlan plan_chunks(const ChunksArgs& a) {
             ChunkPlanItem& it = pl.it[i];
             it.wkind = it.kind == kChunkAny ? kWeightsAny : it.kind == kChunkStream32 || it.kind == kChunkF32Half ? kWeightsScores
                      : it.kind == kChunkF32 ? kWeightsF32 : kWeightsTile;
-            it.wblocks = cdiv(a.it[i].pos0 + a.it[i].rows, it.wkind == kWeightsAny ? kChunkAnyTile : 256);
             it.score0 = -1;
-            if (it.wkind >= kWeightsTile) rounds += kv * wt.units(a.it[i], gmax, 1);
             if (it.wkind == kWeightsScores) {
-                it.score0 = scores;
-                scores += static_cast<long long>(a.it[i].rows) * a.heads * chunk_score_len(a.it[i]);
+                // up to a bound, the others compute theirs again: the workspace stays with the handle
+                const long long n = static_cast<long long>(a.it[i].rows) * a.heads * chunk_score_len(a.it[i]);
+                if (scores + n <= kMaxScores) {
+                    it.score0 = scores;
+                    scores += n;
+                } else {
+                    it.wkind = tiles ? kWeightsTile : kWeightsF32;
+                }
             }
+            it.wblocks = cdiv(a.it[i].pos0 + a.it[i].rows, it.wkind == kWeightsAny ? kChunkAnyTile : 256);
+            if (it.wkind >= kWeightsTile) rounds += kv * wt.units(a.it[i], gmax, 1);
         }
         // units of an equal share of the rounds
         const long long want = tiles ? 1024 : 512;

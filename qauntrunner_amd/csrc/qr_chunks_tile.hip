@@ -403,7 +403,7 @@ __device__ __forceinline__ void chunk_stream(const ChunksK& p, const ChunkItem& 
     w.init(p, it, kvh, g, rho0 + 32 * rw);
     w.load_q(p, it);
     const int ko = w.k_off(), vo = w.v_off();
-    float* const scores = RW == 1 && p.scores ? p.scores + it.score0 + (static_cast<long long>(w.query) * p.heads + w.head) * chunk_score_len(it) : nullptr;
+    float* const scores = RW == 1 && p.scores && it.score0 >= 0 ? p.scores + it.score0 + (static_cast<long long>(w.query) * p.heads + w.head) * chunk_score_len(it) : nullptr;
 
     for (int i = 0; i < ntiles; ++i) {
         turn();
