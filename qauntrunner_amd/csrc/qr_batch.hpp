@@ -52,6 +52,42 @@ __device__ __forceinline__ void store_out(void* p, int dtype, long long i, float
     else static_cast<uint16_t*>(p)[i] = f32_to_out16(x, dtype);
 }
 
+// Values of V at dim d that are not finite: the first positions in [t0, t1) of each sort, INT_MAX where there is none.  Whole
+// runs of 8 slots are read (16 bytes in the MFMA layout), which lie in held pages where t0 and t1 do.
+struct NotFinite {
+    int plus, minus, nan;
+    // what a sum over positions below `end` is that meets them with weights above zero; `sum` without any
+    __device__ __forceinline__ float settle(int end, float sum) const {
+        const bool p = plus < end, m = minus < end;
+        return nan < end || (p && m) ? NAN : p ? INFINITY : m ? -INFINITY : sum;
+    }
+    __device__ __forceinline__ NotFinite of_lane(int lane) const { return {__shfl(plus, lane), __shfl(minus, lane), __shfl(nan, lane)}; }
+};
+__device__ __forceinline__ NotFinite find_not_finite(const void* pool, const int* pages, const PageGeom& geom, int dtype, int kvh, int d, int t0, int t1) {
+    NotFinite f{0x7FFFFFFF, 0x7FFFFFFF, 0x7FFFFFFF};
+    for (int t = t0 & ~7; t < t1; t += 8) {
+        const long long at = geom.offset(pages[t >> kPageShift], 1, kvh, t & (kPageTokens - 1), d);
+        float v[8];
+        if (geom.mfma_layout) {
+            uint16_t u[8];
+            __builtin_memcpy(u, static_cast<const uint16_t*>(pool) + at, 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = dtype == QR_DTYPE_F16 ? f16_bits_to_f32(u[i]) : bf16_bits_to_f32(u[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = load_elem(pool, dtype, at + i * geom.head_dim);
+        }
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+            if (fabsf(v[i]) < INFINITY || t + i < t0 || t + i >= t1) continue;
+            if (v[i] != v[i]) f.nan = min(f.nan, t + i);
+            else if (v[i] > 0.f) f.plus = min(f.plus, t + i);
+            else f.minus = min(f.minus, t + i);
+        }
+    }
+    return f;
+}
+
 // ------------------------------------------------------------------ append
 struct NormRopeItem {
     int pt_off;  // page-table row of (sequence, layer)
