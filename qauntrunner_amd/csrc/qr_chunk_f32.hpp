@@ -37,6 +37,8 @@ struct ChunkF32K {
     float* scores;           // [nq*heads][score_len] scaled scores, may be null
     int score_len;
     int stride;              // partials of a row, splits or more
+    PageGeom geom;
+    int dtype;               // cache
 };
 
 template <typename ST, int D>
@@ -452,6 +454,37 @@ __device__ __forceinline__ void chunk_f32_tiles(const ChunkF32K& p, int split, i
     }
 
     // lane (q4, l16) holds dims 16 PE g + PE (4q4 + r) + e of row l16 in acc[g][e][r]
+    if constexpr (BATCH) {
+        // A sum that is no number though the weights are: an infinite V of a weight that rounds to zero.  It is that
+        // infinity, unless the row sees a NaN or both; one pass over the unit's values, a dim per lane.
+        bool bad = false;
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int e = 0; e < PE; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) bad |= !(acc[g][e][r] == acc[g][e][r]);
+        bad = bad && row_on && l == l;
+        if (__builtin_amdgcn_ballot_w64(bad)) {
+#pragma unroll 1
+            for (int k = 0; k < (D + 63) / 64; ++k) {
+                const NotFinite f = find_not_finite(p.pool, p.page_table, p.geom, p.dtype, kvh, min(64 * k + lane, D - 1), tile0 * kTP,
+                                                    min((tile0 + ntiles) * kTP, keys));
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    if (16 * PE * g / 64 != k) continue;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int e = 0; e < PE; ++e) {
+                            const NotFinite o = f.of_lane(16 * PE * g % 64 + PE * (4 * q4 + r) + e);
+                            const float x = acc[g][e][r];
+                            acc[g][e][r] = bad && !(x == x) ? o.settle(row_lim + 1, x) : x;
+                        }
+                }
+            }
+        }
+    }
     if (!row_on) return;
     const size_t r0 = static_cast<size_t>(row_q) * p.heads + row_h;
     const size_t slot = r0 * (BATCH ? p.stride : p.splits) + split;

@@ -5,6 +5,10 @@
 namespace qr {
 namespace {
 
+// The weight of a partial or of a sum in a merge.  A weight may round to zero where the formula has none that is: an infinity
+// stays one.
+__device__ __forceinline__ float merge_weight(float x, float w) { return fabsf(x) == INFINITY ? 1.f : w; }
+
 // Merge of the splits, any head size: one wave per (row, head).  A split without keys for the row
 // holds m = -inf, l = 0.
 __global__ void __launch_bounds__(64) chunks_merge_any_kernel(const ChunksK p) {
@@ -24,7 +28,10 @@ __global__ void __launch_bounds__(64) chunks_merge_any_kernel(const ChunksK p) {
         l = fmaf(ml.y, c, l);
 #pragma unroll
         for (int i = 0; i < kGenericMaxDim / 64; ++i)
-            if (lane + 64 * i < D) o[i] = fmaf(p.part_acc[(base + s) * D + lane + 64 * i], c, o[i]);
+            if (lane + 64 * i < D) {
+                const float x = p.part_acc[(base + s) * D + lane + 64 * i];
+                o[i] = fmaf(x, merge_weight(x, c), o[i]);
+            }
     }
 #pragma unroll
     for (int i = 0; i < kGenericMaxDim / 64; ++i)
@@ -122,16 +129,16 @@ __global__ void __launch_bounds__(256) chunks_merge_kernel(const ChunksK p) {
         const float cm = m == -INFINITY ? 0.f : fast_exp2(m - mb);
         l *= cm;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) o[x] *= cm;
+        for (int x = 0; x < 4; ++x) o[x] *= merge_weight(o[x], cm);
 #pragma unroll
         for (int i = 0; i < kB; ++i) {
             if (s0 + i >= parts) continue;
             const float w = ml[i].x == -INFINITY ? 0.f : fast_exp2(ml[i].x - mb);
             l = fmaf(ml[i].y, w, l);
-            o[0] = fmaf(a[i].x, w, o[0]);
-            o[1] = fmaf(a[i].y, w, o[1]);
-            o[2] = fmaf(a[i].z, w, o[2]);
-            o[3] = fmaf(a[i].w, w, o[3]);
+            o[0] = fmaf(a[i].x, merge_weight(a[i].x, w), o[0]);
+            o[1] = fmaf(a[i].y, merge_weight(a[i].y, w), o[1]);
+            o[2] = fmaf(a[i].z, merge_weight(a[i].z, w), o[2]);
+            o[3] = fmaf(a[i].w, merge_weight(a[i].w, w), o[3]);
         }
         m = mb;
     }

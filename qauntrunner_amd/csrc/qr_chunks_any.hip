@@ -122,6 +122,21 @@ __global__ void __launch_bounds__(kThreads) chunks_any_kernel(const ChunksK p) {
         prob[kRows + r] = l;
     }
     __syncthreads();
+    // A sum that is no number though the weights are: an infinite V of a weight that rounds to zero.  It is that infinity,
+    // unless the row sees a NaN or both.
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int d = threadIdx.x + kThreads * c;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) bad |= rho0 + i < rho1 && acc[i][c] != acc[i][c] && prob[kRows + i] == prob[kRows + i];
+        if (d >= D || !bad) continue;
+        const NotFinite f = find_not_finite(p.pool, p.page_table + it.pt_off, p.geom, p.dtype, kvh, d, t0, t1);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+            if (acc[i][c] != acc[i][c] && prob[kRows + i] == prob[kRows + i])
+                acc[i][c] = f.settle(it.pos0 + min(rho0 + i, rho1 - 1) / g + 1, acc[i][c]);
+    }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
         const int rho = rho0 + i;

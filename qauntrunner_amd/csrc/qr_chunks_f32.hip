@@ -48,6 +48,8 @@ __global__ void __launch_bounds__(256, (F32Geom<ST, D>::wg_per_cu(PG))) chunks_f
     k.row_ml = p.row_ml ? p.row_ml + row0 : nullptr;
     k.scores = p.scores && it.score0 >= 0 ? p.scores + it.score0 : nullptr;
     k.score_len = chunk_score_len(it);
+    k.geom = p.geom;
+    k.dtype = p.dtype;
     chunk_f32_tiles<ST, D, PG, true>(k, split, block, kvh, lds);
 }
 
