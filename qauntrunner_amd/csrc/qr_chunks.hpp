@@ -14,7 +14,7 @@ enum ChunkWeights { kWeightsAny, kWeightsScores, kWeightsTile, kWeightsF32, kWei
 
 constexpr int kChunkAnyRows = 8, kChunkAnyTile = 32;
 // Parts of the cache's 16-bit type that the streaming kernel takes a query value and a weight as: queries of another type
-// keep 24 bits in three of bf16, 22 in two of fp16.
+// keep 24 bits in three of bf16, 22 in two of fp16 (of values within 2^-16 of a row's largest; fp16 ends below).
 constexpr int chunk_parts(int cache, bool other) { return !other ? 1 : cache == QR_DTYPE_BF16 ? 3 : 2; }
 struct ChunksK {
     ChunkItem it[kBatch];

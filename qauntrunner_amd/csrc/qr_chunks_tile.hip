@@ -19,7 +19,8 @@
 // Queries that are not of the cache's type enter as parts of it, and so do the weights: two parts keep 16 (bf16) or 22
 // (fp16) bits of both -- of a weight w of the row's largest in fp16 no less than 2^-40 / w -- three of bf16 24.  bf16 takes
 // three (the error of eight verify chunks 4e-6 with two, 4e-7 with three, 87 and 102 us), fp16 two.  Otherwise the weights are
-// rounded to the type once, as the output is.
+// rounded to the type once, as the output is (2048 bf16 rows after 6144: 2.3e-3 from 64 bits where fp32 weights have 1.7e-3; a
+// second part would be half as many MFMAs again).
 //
 // Tiles are copied into LDS by buffer-load DMA as they lie in the page.
 #include "qr_chunks.hpp"
@@ -728,10 +729,10 @@ __global__ void __launch_bounds__(512, 1) chunks_tile_kernel(const ChunksK p) {
 // ------------------------------------------------------------------ weights
 // Weights of 256 positions of one kv head over a part of its rows: a wave keeps the K rows of 32
 // positions as operands; the workgroup puts 128 rows at a time into LDS as operands (each wave its share of the
-// k-steps), with each row's maximum, 1 / sum, last position seen and score scale.  Bound by the exponentials (16 cycles
-// per 64 of them, 8 for the multiply-adds around each, 16 for the MFMAs of as many scores beside them) and by what
-// staging the rows takes beside them: six prompts of 101 to 1501 rows, 69 million scores, 46 us (with 64 positions per
-// wave, half the LDS reads, 11 us more).
+// k-steps), with each row's maximum, 1 / sum, last position seen and score scale.  Six prompts of 101 to 1501 rows, 69
+// million scores: 46 us, of which issue takes 18 (16 cycles per 64 exponentials, 8 for the multiply-adds around them, 16 for
+// the MFMAs); the rest goes with the rows, which every unit takes from memory through registers into LDS (with 64 positions
+// per wave, half the LDS reads, 11 us more).
 template <bool BF16, int D, int PARTS>
 __global__ void __launch_bounds__(512, PARTS > 1 && D == 128 ? 1 : 2) chunks_tile_weights_kernel(const ChunksK p) {
     using T = typename Elem<BF16>::T;
@@ -816,7 +817,7 @@ __global__ void __launch_bounds__(512, PARTS > 1 && D == 128 ? 1 : 2) chunks_til
 #pragma unroll
                     for (int i = 0; i < 8; ++i) hi[i] = static_cast<T>(static_cast<float>(hi[i]) * sign);
             } else {
-vec8 part[PARTS];
+                vec8 part[PARTS];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     float v = x[SPLIT ? c : 0][i] * sign;

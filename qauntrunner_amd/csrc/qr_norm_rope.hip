@@ -116,7 +116,8 @@ template <int T> __device__ __forceinline__ void store_run(void* p, long long at
 
 // V rows of the MFMA page layout, where 8 aligned slots of a dim are 16 bytes: a thread takes 8 dims of such a run, 8 loads
 // of 8 values and 8 stores of 16 bytes, 128 bytes in a row of the page.  Slots outside the chunk are left alone.  5317 rows
-// of 8 heads of 128: 11 us, 3.8 TB/s.
+// of 8 heads of 128: 11 us for 21.8 MB read and written, 1.9 TB/s: one round of 332 workgroups, each its loads and
+// then its stores.
 template <int ACT, int DT>
 __global__ void __launch_bounds__(kThreads) v_runs_kernel(const NormRopeArgs a) {
     const int e = batch_find(a.n, blockIdx.x, [&](int i) { return a.it[i].unit0; });
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(kThreads) v_runs_kernel(const NormRopeArgs a) 
 
 // One workgroup per row and gridDim.y-th part of its heads (K, then q, then V unless it goes by runs).  The loads of all of
 // a thread's items are issued before the angles are computed.  Bound by HBM, for few rows by the launch: four bf16 prompts
-// of 32 / 8 heads (123 MB read and written) 31 us, of which the norms take 2 and the 16-byte pieces of K 6; runs of 8
+// of 32 / 8 heads (q and K: 109 MB read and written) 31 us, 3.5 TB/s, of which the norms take 2 and the 16-byte pieces of K 6; runs of 8
 // values or workgroups of several rows are no faster, 16-bit types that the kernel is not compiled for cost 8.
 template <int ACT, int DT, int IPT>
 __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormRopeArgs a, int lph, int v_heads) {
