@@ -334,10 +334,10 @@ def _powers(x, lo, hi, at):
 def _quantise(x):
     """Codes of 8 bits and exponents of rows x [..., D]: the smallest e with max |x| <= 448 2^e."""
     m, e = torch.frexp(x.abs().amax(-1, keepdim=True))  # the largest is m 2^e, m in [1/2, 1)
-    e = torch.clamp(e - 9 + (m > 448 / 512).int(), -117, 120)
+    e = torch.clamp(e - 9 + (m > 448 / 512).int(), -117, 119)
     # nearest even by an addition that leaves the steps' bits: steps of 2^-3 of a value's power of two, 2^-9 at least
     y = x.double()
-    y = y * _powers(y, -120, 117, -e)
+    y = y * _powers(y, -119, 117, -e)
     step = _powers(y, -9, 5, torch.clamp(torch.frexp(y)[1] - 4, min=-9))
     y = (y + step * (1.5 * 2.0**52)) - step * (1.5 * 2.0**52)
     return y.float().to(torch.float8_e4m3fn).view(torch.uint8), e[..., 0].to(torch.int8)
@@ -358,7 +358,7 @@ def _values(codes, e):
     if codes.dtype != torch.uint8:
         return codes.float()
     y = codes.view(torch.float8_e4m3fn).float()
-    return y * _powers(y, -117, 120, e[..., None])
+    return y * _powers(y, -117, 119, e[..., None])
 
 
 def _norm_rope(x, w, pos, rot):
@@ -454,7 +454,7 @@ def _exact_e4m3(x):
     """The values of 8 bits that rows x [..., D] stand as: of the two steps around x / 2^e the nearer, of two as near the
     even one."""
     x = x.double()
-    units = torch.tensor([2.0**k for k in range(-117, 121)], dtype=torch.float64).to(x.device)
+    units = torch.tensor([2.0**k for k in range(-117, 120)], dtype=torch.float64).to(x.device)
     top = x.abs().max(-1, keepdim=True)[0]
     unit = units[torch.searchsorted(448 * units, top).clamp(max=units.numel() - 1)]  # the first with top <= 448 of it
     y = x.abs() / unit
