@@ -41,7 +41,10 @@ extern "C" {
 enum {
     QR_DTYPE_F32 = 0,
     QR_DTYPE_F16 = 1,
-    QR_DTYPE_BF16 = 2
+    QR_DTYPE_BF16 = 2,
+    /* caches only: one byte per value (4 exponent and 3 mantissa bits, largest 448, no infinities) and one
+     * scale 2^e per (position, kv head) of K and of V; see qr_kv_append_norm_rope_dev */
+    QR_DTYPE_E4M3 = 16
 };
 
 /* weight-row formats: QuantFormat values, Dtypes.cs:6-26 (block specs :38-50).
@@ -81,7 +84,8 @@ const char* qr_status_name(int status);
 
 /* ctor PagedKvCache(layers, heads, kvHeads, headDim, maxSeq), PagedKvCache.cs:29-37.
  * kv_dtype: QR_DTYPE_F32 (the reference's page type, PagedKvCache.cs:17-18),
- * F16 or BF16.  max_batch: number of independent sequences (seq_id 0..max_batch-1),
+ * F16, BF16 or E4M3 (an 8-bit cache: it takes the calls over chunks of several sequences below, without
+ * weights and eviction, and the calls on lengths and pages).  max_batch: number of independent sequences (seq_id 0..max_batch-1),
  * each with its own page table; 1 reproduces the reference.  head_dim: any size from
  * 1 to 512 (the reference takes any).  16-bit caches with head_dim 64 or 128 decode on
  * MFMA tiles; multiples of 8 from 16 to 256 on the streaming kernel; every other size on
@@ -225,7 +229,11 @@ int qr_kv_attention_chunk_step_dev(qr_kv* kv, int seq_id, int layer, int nq, con
  * rope_pos0 null: pos0 (after an eviction a token's slot lies below its position).  The angle is
  * taken in 64 bits (qr_kv_append_rope* keep the reference's fp32 product, which is off by up to
  * 2^-8 of a radian at position 131072).  k and v go to the chunk's slots, q to q_out
- * [rows][heads*head_dim].  q, k, v: rows of `dtype`, q_stride / k_stride / v_stride elements from
+ * [rows][heads*head_dim].  On an 8-bit cache a row of head_dim values x (of k after norm and rotation, of v)
+ * becomes codes c = e4m3(x / 2^e), to nearest even, with e the smallest exponent of -117..119 that keeps the
+ * largest finite |x| at or below 448 2^e; the cache then holds the values c 2^e.  Infinities, and what is past 448 2^119, become 448 2^e of
+ * their sign, NaN stays NaN.  k is normed and rotated in 64 bits before it is rounded, so that a value next to a
+ * border between two codes rounds as the formulas say.  q, k, v: rows of `dtype`, q_stride / k_stride / v_stride elements from
  * one to the next (slices of one fused QKV product).  q and q_out may both be null; q_out may be
  * q where q's rows stand back to back, and must not overlap q, k or v otherwise.  No sequence
  * twice.  rotary_dim even, 0 to head_dim.  SeqLen grows as with qr_kv_append. */
@@ -240,9 +248,33 @@ int qr_kv_append_norm_rope_dev(qr_kv* kv, int n, const int* seq_ids, int layer, 
  *   weights[seq][kv head][t] += sum over the chunk's rows and the kv head's query heads of
  *                               softmax(...)[t],  t = 0 .. pos0 + rows - 1,
  * the same for every run with the same inputs (no atomics); other elements are left alone.  With
- * weights no sequence may stand twice. */
+ * weights no sequence may stand twice.  An 8-bit cache takes no weights. */
 int qr_kv_attention_chunks_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows,
                                const void* q_dev, int dtype, void* attn_dev, float* weights_dev, float scale, void* stream);
+/* What changes the scores of attention (a null pointer, or all members zero: nothing).  Positions are counted over a
+ * chunk's prefix (prefix_len[i] of them) and then its own sequence, whose slot t is position prefix_len[i] + t; a row at
+ * slot s of its sequence stands at position P = prefix_len[i] + s. */
+typedef struct qr_attn_form {
+    float cap;               /* above 0: scores z become cap * tanh(z / cap) */
+    const float* slopes_dev; /* device, [heads]: slopes[h] * |P - t| is taken from a (capped) score; null: nothing */
+    int window;              /* above 0: a row sees t > P - window only */
+    /* host arrays of one entry per chunk; null: zeros */
+    const int* first;        /* rows see t >= first[i] only (the start of a document, padding on the left) */
+    const int* full;         /* rows see the positions t < full[i] behind their own too (a prefix without an order) */
+    const int* prefix_ids;   /* sequence that holds the chunk's prefix */
+    const int* prefix_len;   /* its length in positions; 0: the chunk has none */
+} qr_attn_form;
+/* Attention of the chunks (appended before) in these forms:
+ *   z_t = scale q.k_t, capped, less slope |P - t|;  out = sum softmax(z)_t v_t over the t the row sees:
+ *   first <= t and (t <= P or t < full) and t > P - window.
+ * A row that sees nothing gives zeros.  What stands at positions that a row does not see (NaN too) does not reach it.
+ * Chunks that stand one after another (but for chunks without rows) and name the same prefix and length read it
+ * together, up to 64 of them.  The prefix's sequence holds the same layer's K and V, rotated for positions from 0 on
+ * (append the chunk's own rows with rope_pos0 = prefix_len + pos0).  Any cache type, fp32, fp16 or bf16 queries,
+ * attn of the queries' type.  A sequence may stand in several chunks. */
+int qr_kv_attention_forms_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows,
+                              const void* q_dev, int dtype, void* attn_dev, float scale, const qr_attn_form* form,
+                              void* stream);
 /* Eviction by accumulated weight, for n sequences of which len[i] positions of this layer are
  * held.  Where len exceeds the budget first + heavy + recent, every kv head keeps its first `first`
  * and last `recent` positions and the `heavy` positions between them of the largest weight (ties:
@@ -254,9 +286,13 @@ int qr_kv_attention_chunks_dev(qr_kv* kv, int n, const int* seq_ids, int layer, 
  * done.  Slots behind the kept ones keep what they held.  No sequence twice. */
 int qr_kv_evict_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* len, int first, int heavy, int recent,
                     const float* weights_dev, float* kept_weights_dev, int* kept_dev, void* stream);
-/* The chunks' cache rows as [rows][kv_dim] in the cache's type (qr_kv_read without the host). */
+/* The chunks' cache rows as [rows][kv_dim] in the cache's type, 16 or 32 bits (qr_kv_read without the host). */
 int qr_kv_read_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows, void* k_out_dev,
                    void* v_out_dev, void* stream);
+/* The chunks' cache rows as [rows][kv_dim] values of `dtype` (F32, F16 or BF16), whatever the cache's type: of an 8-bit
+ * cache the values c 2^e, which fp32 and bf16 hold exactly; rounded to nearest even where `dtype` holds fewer bits. */
+int qr_kv_read_as_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows, int dtype,
+                      void* k_out_dev, void* v_out_dev, void* stream);
 /* The HIP device that the cache lives on. */
 int qr_kv_device(const qr_kv* kv, int* out);
 
@@ -284,9 +320,10 @@ int qr_kv_truncate(qr_kv* kv, int seq_id, int len);
 /* SeqLen, PagedKvCache.cs:26. */
 int qr_kv_seq_len(const qr_kv* kv, int seq_id, int* out);
 /* BytesUsed, PagedKvCache.cs:27,56: pages x 256 x kv_dim x elem_bytes x 2 summed over
- * layers and sequences (elem_bytes 4 for f32, matching the reference; 2 for 16-bit). */
+ * layers and sequences (elem_bytes 4 for f32, matching the reference; 2 for 16-bit; 1 for 8-bit and
+ * its scales, one byte per position and kv head). */
 int qr_kv_bytes_used(const qr_kv* kv, long long* out);
-/* BytesPerToken, PagedKvCache.cs:39: kv_dim x elem_bytes x 2 x layers. */
+/* BytesPerToken, PagedKvCache.cs:39: kv_dim x elem_bytes x 2 x layers (8-bit: and the scales). */
 int qr_kv_bytes_per_token(const qr_kv* kv, long long* out);
 /* Copies rows pos0..pos0+n-1 of one layer back to the host as cache-dtype
  * rows [n][kv_dim] (debug copy-out; positions must be resident). */

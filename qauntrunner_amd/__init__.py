@@ -7,6 +7,7 @@ PrefetchPipeline.
 """
 from ._lib import (
     DTYPE_BF16,
+    DTYPE_E4M3,
     DTYPE_F16,
     DTYPE_F32,
     LIB_PATH,
@@ -24,7 +25,7 @@ from .store import DeviceTensor, ModelStore, ModelStoreBuilder, PrefetchPipeline
 from .weights import Weight, matvec_dev, matvec_group_dev, mla_q_absorb_dev, mla_wuv_dev
 
 __all__ = [
-    "DTYPE_BF16", "DTYPE_F16", "DTYPE_F32", "LIB_PATH", "PAGE_TOKENS",
+    "DTYPE_BF16", "DTYPE_E4M3", "DTYPE_F16", "DTYPE_F32", "LIB_PATH", "PAGE_TOKENS",
     "QrError", "QrHipError", "QrInvalidArgument", "QrNotResident", "QrOutOfMemory", "QrOutOfRange",
     "load", "MlaLatentCache", "PagedKvCache", "dtype_code",
     "Weight", "matvec_dev", "matvec_group_dev", "mla_q_absorb_dev", "mla_wuv_dev",

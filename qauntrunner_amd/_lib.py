@@ -19,8 +19,8 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "qr_attn.h")
 
 PAGE_TOKENS = 256
 
-DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
-DTYPES = {"f32": DTYPE_F32, "f16": DTYPE_F16, "bf16": DTYPE_BF16}
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_E4M3 = 0, 1, 2, 16
+DTYPES = {"f32": DTYPE_F32, "f16": DTYPE_F16, "bf16": DTYPE_BF16, "e4m3": DTYPE_E4M3}
 
 # weight-row formats: QuantFormat values (Dtypes.cs:6-26)
 FORMATS = {"F32": 0, "F16": 1, "BF16": 2, "Q4_0": 3, "Q8_0": 4, "Q4_K": 6, "Q6_K": 7}
@@ -69,6 +69,15 @@ _ip = ctypes.POINTER(ctypes.c_int)
 _llp = ctypes.POINTER(ctypes.c_longlong)
 _pp = ctypes.POINTER(ctypes.c_void_p)
 
+
+
+class AttnForm(ctypes.Structure):
+    """qr_attn_form"""
+
+    _fields_ = [("cap", _f), ("slopes_dev", _p), ("window", _i), ("first", _p), ("full", _p), ("prefix_ids", _p),
+                ("prefix_len", _p)]
+
+
 # name -> argtypes (every function returns int unless listed in _RESTYPES)
 SIGNATURES = {
     "qr_abi_version": [],
@@ -97,6 +106,8 @@ SIGNATURES = {
     "qr_kv_attention_chunk_dev": [_p, _i, _i, _i, _i, _p, _i, _p, _f, _p],
     "qr_kv_append_norm_rope_dev": [_p, _i, _p, _i, _p, _p, _p, _p, _ll, _p, _ll, _p, _ll, _i, _p, _p, _p, _f, _f, _i, _p],
     "qr_kv_attention_chunks_dev": [_p, _i, _p, _i, _p, _p, _p, _i, _p, _p, _f, _p],
+    "qr_kv_attention_forms_dev": [_p, _i, _p, _i, _p, _p, _p, _i, _p, _f, _p, _p],
+    "qr_kv_read_as_dev": [_p, _i, _p, _i, _p, _p, _i, _p, _p, _p],
     "qr_kv_evict_dev": [_p, _i, _p, _i, _p, _i, _i, _i, _p, _p, _p, _p],
     "qr_kv_read_dev": [_p, _i, _p, _i, _p, _p, _p, _p, _p],
     "qr_kv_device": [_p, _ip],

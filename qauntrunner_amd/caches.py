@@ -501,6 +501,38 @@ class PagedKvCache:
         check(self._lib.qr_kv_attention_chunks_dev(self._h, len(ids), _address(ids), layer, _address(p), _address(n), qe[0],
                                                    code, oe[0], we[0], scale, _stream_of(stream, dev)))
 
+    def AttentionFormsDev(self, layer, seq_ids, pos0, rows, q, out, scale, cap=0.0, slopes=None, window=0, first=None,
+                          full=None, prefix_ids=None, prefix_len=None, stream=None) -> None:
+        """AttentionChunksDev in other forms (qr_attn_form): scores capped to cap * tanh(z / cap), less slopes[h] (float32
+        [heads]) times the distance; a row at position P sees t > P - window (0: all), t >= first[i], and t <= P or
+        t < full[i] (lists of one entry per chunk, None: zeros); rows that see nothing give zeros.  prefix_ids[i] and
+        prefix_len[i]: sequence and length of the prefix that stands before chunk i's own sequence (length 0: none),
+        read together by chunks that stand one after another and share it; positions are counted from its start."""
+        ids, p, n, total = self._chunks(seq_ids, pos0, rows)
+        dev, qw = self.Device, self.Heads * self.HeadDim
+        code = _torch_code(q, "q")
+        qe = _whole(q, total * qw, code, dev, "q")
+        oe = _whole(out, total * qw, code, dev, "out")
+        if _overlap(oe, qe):
+            raise ValueError("out overlaps q")
+        se = None
+        if slopes is not None:
+            s = _whole(slopes, self.Heads, _lib.DTYPE_F32, dev, "slopes")
+            if _overlap(s, oe):
+                raise ValueError("out overlaps slopes")
+            se = s[0]
+        if (prefix_ids is None) != (prefix_len is None):
+            raise ValueError("prefix_ids and prefix_len come together")
+        lists = []
+        for x, what in ((first, "first"), (full, "full"), (prefix_ids, "prefix_ids"), (prefix_len, "prefix_len")):
+            x = None if x is None else _ints(x, what)
+            if x is not None and len(x) != len(ids):
+                raise ValueError(f"{what} must agree with seq_ids")
+            lists.append(x)
+        form = _lib.AttnForm(cap, se, window, *(_address(x) if x else None for x in lists))
+        check(self._lib.qr_kv_attention_forms_dev(self._h, len(ids), _address(ids), layer, _address(p), _address(n), qe[0],
+                                                  code, oe[0], scale, ctypes.byref(form), _stream_of(stream, dev)))
+
     def EvictDev(self, layer, seq_ids, lengths, first, heavy, recent, weights, kept, kept_weights=None, stream=None) -> None:
         """Eviction by accumulated weight: of each sequence's lengths[i] positions every kv head keeps the first
         `first`, the last `recent` and the `heavy` others of the largest weight, closed up in their order; kept
@@ -532,12 +564,27 @@ class PagedKvCache:
         """The chunks' cache rows as [rows, kv_dim] tensors of the cache's dtype (Read without the host)."""
         ids, p, n, total = self._chunks(seq_ids, pos0, rows)
         dev = self.Device
+        if self.KvDtype == _lib.DTYPE_E4M3:
+            raise ValueError("an 8-bit cache is read as values: ReadAsDev")
         ke = _whole(k_out, total * self.KvDim, self.KvDtype, dev, "k_out")
         ve = _whole(v_out, total * self.KvDim, self.KvDtype, dev, "v_out")
         if _overlap(ke, ve):
             raise ValueError("k_out and v_out overlap")
         check(self._lib.qr_kv_read_dev(self._h, len(ids), _address(ids), layer, _address(p), _address(n), ke[0], ve[0],
                                        _stream_of(stream, dev)))
+
+    def ReadAsDev(self, layer, seq_ids, pos0, rows, k_out, v_out, stream=None) -> None:
+        """The chunks' cache rows as [rows, kv_dim] values of the tensors' dtype (float32, float16 or bfloat16), whatever
+        the cache's: an 8-bit cache's are exact in float32 and bfloat16."""
+        ids, p, n, total = self._chunks(seq_ids, pos0, rows)
+        dev = self.Device
+        code = _torch_code(k_out, "k_out")
+        ke = _whole(k_out, total * self.KvDim, code, dev, "k_out")
+        ve = _whole(v_out, total * self.KvDim, code, dev, "v_out")
+        if _overlap(ke, ve):
+            raise ValueError("k_out and v_out overlap")
+        check(self._lib.qr_kv_read_as_dev(self._h, len(ids), _address(ids), layer, _address(p), _address(n), code, ke[0],
+                                          ve[0], _stream_of(stream, dev)))
 
     # ---- debug copy-out
     def Read(self, layer, pos0, n, seq_id=0):

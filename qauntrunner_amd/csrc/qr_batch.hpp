@@ -116,6 +116,7 @@ struct NormRopeArgs {
     double turn[kMaxRopeHalf];               // revolutions per position of pair i
 };
 hipError_t launch_norm_rope(NormRopeArgs& a, hipStream_t stream);  // sets unit0
+hipError_t launch_quant(NormRopeArgs& a, hipStream_t stream);      // the same on an 8-bit cache
 
 // ------------------------------------------------------------------ rows back
 struct ReadItem {
@@ -130,9 +131,11 @@ struct ReadArgs {
     const int* page_table;
     PageGeom geom;
     int dtype;
+    int act;                 // of k and v where they are values of another type (launch_read_as)
     void *k, *v;             // [rows][kv_heads * head_dim] in the cache's type
 };
-hipError_t launch_read(ReadArgs& a, hipStream_t stream);  // sets unit0
+hipError_t launch_read(ReadArgs& a, hipStream_t stream);     // sets unit0
+hipError_t launch_read_as(ReadArgs& a, hipStream_t stream);  // any cache, values of a.act
 
 // ------------------------------------------------------------------ attention
 struct ChunkItem {

@@ -7,6 +7,7 @@
 #include <vector>
 
 #include "qr_batch.hpp"
+#include "qr_forms.hpp"
 #include "qr_kv.hpp"
 
 using namespace qr;
@@ -67,6 +68,86 @@ int check_aligned(const void* p, size_t to, const char* what) {
 }
 
 const char* offset_bytes(const void* p, long long bytes) { return p ? static_cast<const char*>(p) + bytes : nullptr; }
+
+// Attention of checked chunks (rows in all) in the forms of `f`.
+int attend_forms(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows, const void* q_dev, int dtype,
+                 void* attn_dev, float scale, const qr_attn_form& f, hipStream_t st) {
+    FormsArgs a{};
+    a.pool = kv->store.pool();
+    a.page_table = kv->store.page_table_dev();
+    a.geom = kv->store.geom();
+    a.dtype = kv->dtype;
+    a.act = dtype;
+    a.heads = kv->heads;
+    a.scale = scale;
+    a.cap = f.cap;
+    a.slopes = f.slopes_dev;
+    a.window = f.window;
+    long long done = 0;
+    for (int i = 0; i < n;) {
+        a.n = a.rows = 0;
+        const long long at = done * kv->heads * kv->head_dim * dtype_size(dtype);
+        a.q = offset_bytes(q_dev, at);
+        a.out = const_cast<char*>(offset_bytes(attn_dev, at));
+        for (; i < n && a.n < kBatch; ++i) {
+            if (!rows[i]) continue;
+            FormChunk& c = a.c[a.n++];
+            c = {};
+            c.pt_off = kv->store.pt_offset(seq_ids[i], layer);
+            c.pos0 = pos0[i];
+            c.rows = rows[i];
+            c.row0 = a.rows;
+            c.first = f.first ? f.first[i] : 0;
+            c.full = f.full ? f.full[i] : 0;
+            c.pre_len = f.prefix_len ? f.prefix_len[i] : 0;
+            if (c.pre_len) c.pre_off = kv->store.pt_offset(f.prefix_ids[i], layer);
+            a.rows += rows[i];
+        }
+        done += a.rows;
+        if (!a.n) break;
+        const FormsPlan plan = plan_forms(a);
+        QR_TRY(grow_workspace(kv, plan.workspace_bytes, st));
+        QR_HIP(launch_forms(a, plan, kv->workspace.get(), st));
+    }
+    return QR_OK;
+}
+
+// The chunks' rows in the cache's own type, or as values of another.
+int read_rows(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows, int dtype, void* k_out_dev,
+              void* v_out_dev, hipStream_t st) {
+    QR_TRY(sync_host(kv, st, true));
+    long long total = 0;
+    QR_TRY(check_chunks(kv, n, seq_ids, layer, pos0, rows, &total));
+    for (int i = 0; i < n; ++i)
+        if (rows[i]) QR_TRY(check_resident(kv, seq_ids[i], layer, pos0[i] + rows[i] - 1));
+    if (total == 0) return QR_OK;
+    QR_CHECK_ARG(k_out_dev && v_out_dev, "null output rows");
+    const int es = dtype_size(dtype);
+    QR_TRY(check_aligned(k_out_dev, es, "k_out"));
+    QR_TRY(check_aligned(v_out_dev, es, "v_out"));
+    DeviceGuard dg(kv->device);
+    note_capture(kv, st);
+    ReadArgs a{};
+    a.pool = kv->store.pool();
+    a.page_table = kv->store.page_table_dev();
+    a.geom = kv->store.geom();
+    a.dtype = kv->dtype;
+    a.act = dtype;
+    long long done = 0;
+    for (int i = 0; i < n;) {
+        a.n = a.rows = 0;
+        a.k = const_cast<char*>(offset_bytes(k_out_dev, done * kv->kv_dim * es));
+        a.v = const_cast<char*>(offset_bytes(v_out_dev, done * kv->kv_dim * es));
+        for (; i < n && a.n < kBatch; ++i) {
+            if (!rows[i]) continue;
+            a.it[a.n++] = {kv->store.pt_offset(seq_ids[i], layer), pos0[i], rows[i], a.rows, 0};
+            a.rows += rows[i];
+        }
+        done += a.rows;
+        QR_HIP(dtype == kv->dtype ? launch_read(a, st) : launch_read_as(a, st));
+    }
+    return QR_OK;
+}
 
 }  // namespace
 
@@ -164,7 +245,7 @@ int qr_kv_append_norm_rope_dev(qr_kv* kv, int n, const int* seq_ids, int layer, 
                 a.rows += rows[i];
             }
             done += a.rows;
-            QR_HIP(launch_norm_rope(a, st));
+            QR_HIP(kv->dtype == QR_DTYPE_E4M3 ? launch_quant(a, st) : launch_norm_rope(a, st));
         }
         for (int i = 0; i < n; ++i)
             if (rows[i]) kv->seq_len[seq_ids[i]] = std::max(kv->seq_len[seq_ids[i]], pos0[i] + rows[i]);
@@ -180,6 +261,7 @@ int qr_kv_attention_chunks_dev(qr_kv* kv, int n, const int* seq_ids, int layer, 
         QR_TRY(sync_host(kv, st, true));
         long long total = 0;
         QR_TRY(check_chunks(kv, n, seq_ids, layer, pos0, rows, &total));
+        if (weights_dev) QR_TRY(check_wide(kv));
         if (weights_dev) QR_TRY(check_distinct(kv, n, seq_ids, rows, "its weights would race"));
         QR_CHECK_ARG(dtype_valid(dtype), "unknown q dtype %d", dtype);
         QR_CHECK_ARG(std::isfinite(scale), "scale must be a number");
@@ -193,6 +275,7 @@ int qr_kv_attention_chunks_dev(qr_kv* kv, int n, const int* seq_ids, int layer, 
         QR_TRY(check_aligned(weights_dev, 4, "weights"));
         DeviceGuard dg(kv->device);
         note_capture(kv, st);
+        if (kv->dtype == QR_DTYPE_E4M3) return attend_forms(kv, n, seq_ids, layer, pos0, rows, q_dev, dtype, attn_dev, scale, {}, st);
         ChunksArgs a{};
         a.pool = kv->store.pool();
         a.page_table = kv->store.page_table_dev();
@@ -234,6 +317,7 @@ int qr_kv_evict_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* 
                     const float* weights_dev, float* kept_weights_dev, int* kept_dev, void* stream) {
     return guarded([&]() -> int {
         QR_TRY(check_handle(kv));
+        QR_TRY(check_wide(kv));
         const hipStream_t st = as_stream(stream);
         QR_TRY(sync_host(kv, st, true));
         QR_CHECK_ARG(n >= 0, "negative number of sequences %d", n);
@@ -281,42 +365,67 @@ int qr_kv_evict_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* 
     });
 }
 
-int qr_kv_read_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows, void* k_out_dev,
-                   void* v_out_dev, void* stream) {
+int qr_kv_attention_forms_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows,
+                              const void* q_dev, int dtype, void* attn_dev, float scale, const qr_attn_form* form,
+                              void* stream) {
     return guarded([&]() -> int {
         QR_TRY(check_handle(kv));
         const hipStream_t st = as_stream(stream);
         QR_TRY(sync_host(kv, st, true));
         long long total = 0;
         QR_TRY(check_chunks(kv, n, seq_ids, layer, pos0, rows, &total));
-        for (int i = 0; i < n; ++i)
-            if (rows[i]) QR_TRY(check_resident(kv, seq_ids[i], layer, pos0[i] + rows[i] - 1));
+        QR_CHECK_ARG(dtype_valid(dtype), "unknown q dtype %d", dtype);
+        QR_CHECK_ARG(std::isfinite(scale), "scale must be a number");
+        const qr_attn_form f = form ? *form : qr_attn_form{};
+        QR_CHECK_ARG(std::isfinite(f.cap) && f.cap >= 0.f, "cap must be a number of at least 0");
+        QR_CHECK_ARG(f.window >= 0, "negative window %d", f.window);
+        QR_CHECK_ARG((f.prefix_ids == nullptr) == (f.prefix_len == nullptr), "prefix_ids and prefix_len come together");
+        for (int i = 0; i < n; ++i) {
+            if (!rows[i]) continue;
+            const int len = f.prefix_len ? f.prefix_len[i] : 0;
+            QR_CHECK_ARG(len >= 0, "chunk %d: negative prefix length %d", i, len);
+            if (len) {
+                QR_TRY(check_seq_layer(kv, f.prefix_ids[i], layer));
+                QR_TRY(check_pos(kv, len - 1));
+                QR_TRY(check_resident(kv, f.prefix_ids[i], layer, len - 1));
+            }
+            if (static_cast<long long>(len) + pos0[i] + rows[i] > (1 << 30)) {
+                set_error("chunk %d: positions past 2^30", i);
+                return QR_ERR_OUT_OF_RANGE;
+            }
+            const int first = f.first ? f.first[i] : 0, full = f.full ? f.full[i] : 0;
+            QR_CHECK_ARG(first >= 0 && full >= 0, "chunk %d: negative first %d or full %d", i, first, full);
+            const int last = std::max(pos0[i] + rows[i], full - len) - 1;  // of its own slots
+            QR_TRY(check_pos(kv, last));
+            QR_TRY(check_resident(kv, seq_ids[i], layer, last));
+        }
         if (total == 0) return QR_OK;
-        QR_CHECK_ARG(k_out_dev && v_out_dev, "null output rows");
-        const int es = dtype_size(kv->dtype);
-        QR_TRY(check_aligned(k_out_dev, es, "k_out"));
-        QR_TRY(check_aligned(v_out_dev, es, "v_out"));
+        QR_CHECK_ARG(q_dev && attn_dev, "null q/attn pointer");
+        const int es = dtype_size(dtype);
+        QR_TRY(check_aligned(q_dev, es, "q"));
+        QR_TRY(check_aligned(attn_dev, es, "attn"));
+        QR_TRY(check_aligned(f.slopes_dev, 4, "slopes"));
         DeviceGuard dg(kv->device);
         note_capture(kv, st);
-        ReadArgs a{};
-        a.pool = kv->store.pool();
-        a.page_table = kv->store.page_table_dev();
-        a.geom = kv->store.geom();
-        a.dtype = kv->dtype;
-        long long done = 0;
-        for (int i = 0; i < n;) {
-            a.n = a.rows = 0;
-            a.k = const_cast<char*>(offset_bytes(k_out_dev, done * kv->kv_dim * es));
-            a.v = const_cast<char*>(offset_bytes(v_out_dev, done * kv->kv_dim * es));
-            for (; i < n && a.n < kBatch; ++i) {
-                if (!rows[i]) continue;
-                a.it[a.n++] = {kv->store.pt_offset(seq_ids[i], layer), pos0[i], rows[i], a.rows, 0};
-                a.rows += rows[i];
-            }
-            done += a.rows;
-            QR_HIP(launch_read(a, st));
-        }
-        return QR_OK;
+        return attend_forms(kv, n, seq_ids, layer, pos0, rows, q_dev, dtype, attn_dev, scale, f, st);
+    });
+}
+
+int qr_kv_read_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows, void* k_out_dev,
+                   void* v_out_dev, void* stream) {
+    return guarded([&]() -> int {
+        QR_TRY(check_handle(kv));
+        QR_TRY(check_wide(kv));
+        return read_rows(kv, n, seq_ids, layer, pos0, rows, kv->dtype, k_out_dev, v_out_dev, as_stream(stream));
+    });
+}
+
+int qr_kv_read_as_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows, int dtype,
+                      void* k_out_dev, void* v_out_dev, void* stream) {
+    return guarded([&]() -> int {
+        QR_TRY(check_handle(kv));
+        QR_CHECK_ARG(dtype_valid(dtype), "unknown row dtype %d", dtype);
+        return read_rows(kv, n, seq_ids, layer, pos0, rows, dtype, k_out_dev, v_out_dev, as_stream(stream));
     });
 }
 

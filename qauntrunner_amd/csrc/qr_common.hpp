@@ -45,7 +45,8 @@ void clear_error();
         if (s_ != QR_OK) return s_;  \
     } while (0)
 
-__host__ __device__ inline int dtype_size(int dt) { return dt == QR_DTYPE_F32 ? 4 : 2; }
+__host__ __device__ inline int dtype_size(int dt) { return dt == QR_DTYPE_F32 ? 4 : dt == QR_DTYPE_E4M3 ? 1 : 2; }
+// (types of rows; caches may be of QR_DTYPE_E4M3 too)
 __host__ __device__ inline bool dtype_valid(int dt) {
     return dt == QR_DTYPE_F32 || dt == QR_DTYPE_F16 || dt == QR_DTYPE_BF16;
 }

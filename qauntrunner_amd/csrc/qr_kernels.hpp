@@ -28,18 +28,39 @@ namespace qr {
 // 1 KiB (whole 128-byte lines per wave load, which the loads can mark non-temporal),
 // and 8 consecutive dims of a K row or 8 aligned consecutive tokens of one V dim are one
 // contiguous 16-byte run for the appends.
+//
+// 8-bit caches (scaled): codes are one byte, and behind the planes stand the rows' scales,
+// planes x kv_heads x kPageTokens bytes b of 2^(b - 127).  Head sizes 64 and 128 (mfma_layout)
+// lie as operands of v_mfma_f32_32x32x16: a step of 32 tokens is cut into blocks of 1 KiB of
+// 32 dims, 16 bytes for each of 64 lanes, L = 32 h + m:
+//   K: token 16 h' + 8 s + 4 a + b of the step is m = 16 s + 8 a + 4 h' + b, dims 16 h .. + 15 of
+//      the block (a lane's scores of a step, D[m][row], are then 16 consecutive tokens);
+//   V: dim m of the block, tokens 16 h .. 16 h + 15 of the step.
 struct PageGeom {
     int planes;
     int kv_heads;
     int head_dim;
     int mfma_layout = 0;
+    int scaled = 0;
     __host__ __device__ long long plane_elems() const { return (long long)kv_heads * kPageTokens * head_dim; }
-    __host__ __device__ long long page_elems() const { return plane_elems() * planes; }
+    __host__ __device__ long long page_elems() const {
+        return plane_elems() * planes + (scaled ? (long long)planes * kv_heads * kPageTokens : 0);
+    }
+    // byte offset of a row's scale (scaled)
+    __host__ __device__ long long scale_offset(long long phys, int plane, int kvh, int slot) const {
+        return phys * page_elems() + planes * plane_elems() + ((long long)plane * kv_heads + kvh) * kPageTokens + slot;
+    }
     // element offset of (plane, kv head, slot, dim) inside page `phys`
     __host__ __device__ long long offset(long long phys, int plane, int kvh, int slot, int d) const {
         const long long blk = phys * page_elems() + plane * plane_elems() + (long long)kvh * kPageTokens * head_dim;
         if (!mfma_layout) return blk + (long long)slot * head_dim + d;
         const int r = slot & 31;  // token within its step
+        if (scaled) {
+            const long long to = blk + (long long)(slot >> 5) * 32 * head_dim + 1024 * (d >> 5);
+            if (plane) return to + 16 * (32 * (r >> 4) + (d & 31)) + (r & 15);
+            const int m = 16 * ((r >> 3) & 1) + 8 * ((r >> 2) & 1) + 4 * (r >> 4) + (r & 3);
+            return to + 16 * (32 * ((d >> 4) & 1) + m) + (d & 15);
+        }
         int b, lane;
         if (plane == 0) {
             b = ((r >> 2) & 1) * (head_dim >> 5) + (d >> 5);
@@ -52,7 +73,7 @@ struct PageGeom {
         return blk + (long long)(slot >> 5) * 32 * head_dim + 512 * b + 8 * lane + e;
     }
 };
-// 16-bit GQA caches with head_dim 64 or 128 use the MFMA operand layout (their decode
+// 16- and 8-bit GQA caches with head_dim 64 or 128 use an MFMA operand layout (their decode
 // and chunk kernels run on MFMA tiles).
 inline bool kv_mfma_layout(int dtype, int head_dim) {
     return dtype != QR_DTYPE_F32 && (head_dim == 64 || head_dim == 128);

@@ -35,6 +35,14 @@ inline int check_handle(const qr_kv* kv) {
     return QR_OK;
 }
 
+// The calls that know no 8-bit cache.
+inline int check_wide(const qr_kv* kv) {
+    QR_CHECK_ARG(kv->dtype != QR_DTYPE_E4M3,
+                 "this call takes caches of 16 and 32 bits (an 8-bit cache: append_norm_rope_dev, attention_chunks_dev without "
+                 "weights, attention_forms_dev, read_as_dev)");
+    return QR_OK;
+}
+
 inline int check_seq_layer(const qr_kv* kv, int seq_id, int layer) {
     QR_CHECK_ARG(seq_id >= 0 && seq_id < kv->max_batch, "seq_id %d outside [0, %d)", seq_id, kv->max_batch);
     QR_CHECK_ARG(layer >= 0 && layer < kv->layers, "layer %d outside [0, %d)", layer, kv->layers);

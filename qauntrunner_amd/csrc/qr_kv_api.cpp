@@ -141,7 +141,7 @@ int qr_kv_create(qr_kv** out, int layers, int heads, int kv_heads, int head_dim,
     QR_CHECK_ARG(head_dim >= 1 && head_dim <= kGenericMaxDim, "head_dim %d unsupported (1 to %d)", head_dim,
                  kGenericMaxDim);
     QR_CHECK_ARG(max_seq >= 1, "max_seq must be >= 1 (got %d)", max_seq);
-    QR_CHECK_ARG(dtype_valid(kv_dtype), "unknown kv dtype %d", kv_dtype);
+    QR_CHECK_ARG(dtype_valid(kv_dtype) || kv_dtype == QR_DTYPE_E4M3, "unknown kv dtype %d", kv_dtype);
     QR_CHECK_ARG(max_batch >= 1, "max_batch must be >= 1 (got %d)", max_batch);
     const long long pt_entries = static_cast<long long>(max_batch) * layers * ((max_seq + kPageTokens - 1) / kPageTokens);
     QR_CHECK_ARG(pt_entries < (1LL << 31), "page table of %lld entries is too large", pt_entries);
@@ -168,6 +168,7 @@ int qr_kv_create(qr_kv** out, int layers, int heads, int kv_heads, int head_dim,
     if (st == QR_OK) {
         PageGeom g{2, kv_heads, head_dim};
         g.mfma_layout = kv_mfma_layout(kv_dtype, head_dim) ? 1 : 0;
+        g.scaled = kv_dtype == QR_DTYPE_E4M3 ? 1 : 0;
         st = kv->store.init(g, kv_dtype, layers, max_batch, max_seq);
     }
     if (st == QR_OK) st = decode_scratch_address(kv->device, &kv->scratch);
@@ -208,6 +209,7 @@ int qr_kv_append(qr_kv* kv, int seq_id, int layer, int pos, const float* k, int 
                  int v_len) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(sync_host(kv));
     QR_TRY(check_seq_layer(kv, seq_id, layer));
     QR_TRY(check_pos(kv, pos));
@@ -232,6 +234,7 @@ int qr_kv_append_range(qr_kv* kv, int seq_id, int layer, int pos0, int n, const 
                        int src_dtype) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(sync_host(kv));
     QR_TRY(check_seq_layer(kv, seq_id, layer));
     QR_CHECK_ARG(dtype_valid(src_dtype), "unknown source dtype %d", src_dtype);
@@ -255,6 +258,7 @@ int qr_kv_append_range_dev(qr_kv* kv, int seq_id, int layer, int pos0, int n, co
                            const void* v_dev, int src_dtype, void* stream) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(sync_host(kv, as_stream(stream), true));
     note_capture(kv, as_stream(stream));
     QR_TRY(check_seq_layer(kv, seq_id, layer));
@@ -273,6 +277,7 @@ int qr_kv_append_rope(qr_kv* kv, int seq_id, int layer, int pos, float* q, const
                       float theta) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(sync_host(kv));
     QR_TRY(check_seq_layer(kv, seq_id, layer));
     QR_TRY(check_pos(kv, pos));
@@ -298,6 +303,7 @@ int qr_kv_append_rope_dev(qr_kv* kv, int seq_id, int layer, int pos0, int n, flo
                           const float* v_dev, float theta, void* stream) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(sync_host(kv, as_stream(stream), true));
     note_capture(kv, as_stream(stream));
     QR_TRY(check_seq_layer(kv, seq_id, layer));
@@ -320,6 +326,7 @@ int qr_kv_attention_batch(qr_kv* kv, int n, const int* seq_ids, int layer, const
                           float* attn, float scale) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(sync_host(kv));
     QR_CHECK_ARG(q && attn, "null q/attn pointer");
     std::vector<int> seq_len;
@@ -340,6 +347,7 @@ int qr_kv_attention_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const i
                         float* attn_dev, float scale, void* stream) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(sync_host(kv, as_stream(stream), true));
     note_capture(kv, as_stream(stream));
     QR_CHECK_ARG(q_dev && attn_dev, "null q/attn pointer");
@@ -353,6 +361,7 @@ int qr_kv_attention_dev_noalloc(qr_kv* kv, int n, const int* seq_ids, int layer,
                                 const float* q_dev, float* attn_dev, float scale, void* stream) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(sync_host(kv, as_stream(stream), true));
     note_capture(kv, as_stream(stream));
     QR_CHECK_ARG(q_dev && attn_dev, "null q/attn pointer");
@@ -395,6 +404,7 @@ namespace {
 int chunk_common(qr_kv* kv, int seq_id, int layer, int pos0, int nq, const void* q, int q_dtype,
                  float* attn, bool q_is_dev, bool out_is_dev, float scale, hipStream_t stream) {
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(check_seq_layer(kv, seq_id, layer));
     QR_CHECK_ARG(q && attn, "null q/attn pointer");
     QR_CHECK_ARG(dtype_valid(q_dtype), "unknown q dtype %d", q_dtype);
@@ -464,6 +474,7 @@ int qr_kv_attention_chunk(qr_kv* kv, int seq_id, int layer, int pos0, int nq, co
                           float* attn, float scale) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(sync_host(kv));
     return chunk_common(kv, seq_id, layer, pos0, nq, q, q_dtype, attn, false, false, scale, kv->stream);
 }
@@ -472,6 +483,7 @@ int qr_kv_attention_chunk_dev(qr_kv* kv, int seq_id, int layer, int pos0, int nq
                               int q_dtype, float* attn_dev, float scale, void* stream) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(sync_host(kv, as_stream(stream), true));
     note_capture(kv, as_stream(stream));
     return chunk_common(kv, seq_id, layer, pos0, nq, q_dev, q_dtype, attn_dev, true, true, scale,
@@ -482,6 +494,7 @@ int qr_kv_decode_plan(qr_kv* kv, int n, const int* seq_ids, int layer, const int
                       int* splits) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(sync_host(kv));
     QR_CHECK_ARG(split_tokens && splits, "null output pointer");
     std::vector<int> seq_len;
@@ -561,13 +574,14 @@ int qr_kv_bytes_per_token(const qr_kv* kv, long long* out) {
     clear_error();
     QR_TRY(check_handle(kv));
     QR_CHECK_ARG(out, "null output pointer");
-    *out = static_cast<long long>(kv->kv_dim) * dtype_size(kv->dtype) * 2 * kv->layers;
+    *out = (static_cast<long long>(kv->kv_dim) * dtype_size(kv->dtype) + (kv->store.geom().scaled ? kv->kv_heads : 0)) * 2 * kv->layers;
     return QR_OK;
 }
 
 int qr_kv_read(qr_kv* kv, int seq_id, int layer, int pos0, int n, void* k_out, void* v_out) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(sync_host(kv));
     QR_TRY(check_seq_layer(kv, seq_id, layer));
     QR_CHECK_ARG(n >= 0, "negative row count %d", n);
@@ -697,6 +711,7 @@ int qr_kv_append_rope_step_dev(qr_kv* kv, int seq_id, int layer, const int* pos_
                                const float* k_dev, const float* v_dev, float theta, void* stream) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     return rope_step_dev(kv, seq_id, layer, 1, pos_dev, q_dev, k_dev, v_dev, theta, as_stream(stream));
 }
 
@@ -704,6 +719,7 @@ int qr_kv_append_rope_chunk_step_dev(qr_kv* kv, int seq_id, int layer, int nq, c
                                      const float* k_dev, const float* v_dev, float theta, void* stream) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_CHECK_ARG(nq >= 1 && nq <= kv->max_seq, "nq %d outside [1, %d]", nq, kv->max_seq);
     return rope_step_dev(kv, seq_id, layer, nq, pos0_dev, q_dev, k_dev, v_dev, theta, as_stream(stream));
 }
@@ -712,6 +728,7 @@ int qr_kv_attention_step_dev(qr_kv* kv, int n, const int* seq_ids, int layer, co
                              const float* q_dev, float* attn_dev, float scale, void* stream) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_CHECK_ARG(q_dev && attn_dev && pos_dev, "null q/attn/pos pointer");
     QR_CHECK_ARG(n >= 1 && n <= kMaxDecodeBatch, "batch size %d outside [1, %d] for device positions", n,
                  kMaxDecodeBatch);
@@ -725,6 +742,7 @@ int qr_kv_attention_chunk_step_dev(qr_kv* kv, int seq_id, int layer, int nq, con
                                    int q_dtype, float* attn_dev, float scale, void* stream) {
     clear_error();
     QR_TRY(check_handle(kv));
+    QR_TRY(check_wide(kv));
     QR_TRY(check_seq_layer(kv, seq_id, layer));
     QR_CHECK_ARG(q_dev && attn_dev && pos0_dev, "null q/attn/pos pointer");
     QR_CHECK_ARG(dtype_valid(q_dtype), "unknown q dtype %d", q_dtype);
