@@ -15,7 +15,7 @@ constexpr int kTile = kFormAnyTile;
 
 __device__ __forceinline__ float load_cached(const FormsK& p, long long phys, int plane, int kvh, int slot, int d) {
     const long long at = p.geom.offset(phys, plane, kvh, slot, d);
-    if (!p.geom.scaled) return load_elem(p.pool, p.dtype, at);
+    if (!p.geom.scaled()) return load_elem(p.pool, p.dtype, at);
     const uint8_t* b = reinterpret_cast<const uint8_t*>(p.pool);
     return quant_value<0>(b[at]) * scale_of(b[p.geom.scale_offset(phys, plane, kvh, slot)]);
 }

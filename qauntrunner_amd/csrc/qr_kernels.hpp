@@ -29,8 +29,8 @@ namespace qr {
 // and 8 consecutive dims of a K row or 8 aligned consecutive tokens of one V dim are one
 // contiguous 16-byte run for the appends.
 //
-// 8-bit caches (scaled): codes are one byte, and behind the planes stand the rows' scales,
-// planes x kv_heads x kPageTokens bytes b of 2^(b - 127).  Head sizes 64 and 128 (mfma_layout)
+// 8-bit caches (scaled()): codes are one byte, and behind the planes stand the rows' scales,
+// planes x kv_heads x kPageTokens bytes b of 2^(b - 127).  Head sizes 64 and 128 (bit 0)
 // lie as operands of v_mfma_f32_32x32x16: a step of 32 tokens is cut into blocks of 1 KiB of
 // 32 dims, 16 bytes for each of 64 lanes, L = 32 h + m:
 //   K: token 16 h' + 8 s + 4 a + b of the step is m = 16 s + 8 a + 4 h' + b, dims 16 h .. + 15 of
@@ -40,11 +40,11 @@ struct PageGeom {
     int planes;
     int kv_heads;
     int head_dim;
-    int mfma_layout = 0;
-    int scaled = 0;
+    int mfma_layout = 0;  // bit 0: operand layout; bit 1: 8-bit rows with scales (set on no other cache)
+    __host__ __device__ bool scaled() const { return mfma_layout & 2; }
     __host__ __device__ long long plane_elems() const { return (long long)kv_heads * kPageTokens * head_dim; }
     __host__ __device__ long long page_elems() const {
-        return plane_elems() * planes + (scaled ? (long long)planes * kv_heads * kPageTokens : 0);
+        return plane_elems() * planes + (scaled() ? (long long)planes * kv_heads * kPageTokens : 0);
     }
     // byte offset of a row's scale (scaled)
     __host__ __device__ long long scale_offset(long long phys, int plane, int kvh, int slot) const {
@@ -53,9 +53,9 @@ struct PageGeom {
     // element offset of (plane, kv head, slot, dim) inside page `phys`
     __host__ __device__ long long offset(long long phys, int plane, int kvh, int slot, int d) const {
         const long long blk = phys * page_elems() + plane * plane_elems() + (long long)kvh * kPageTokens * head_dim;
-        if (!mfma_layout) return blk + (long long)slot * head_dim + d;
+        if (!(mfma_layout & 1)) return blk + (long long)slot * head_dim + d;
         const int r = slot & 31;  // token within its step
-        if (scaled) {
+        if (scaled()) {
             const long long to = blk + (long long)(slot >> 5) * 32 * head_dim + 1024 * (d >> 5);
             if (plane) return to + 16 * (32 * (r >> 4) + (d & 31)) + (r & 15);
             const int m = 16 * ((r >> 3) & 1) + 8 * ((r >> 2) & 1) + 4 * (r >> 4) + (r & 3);

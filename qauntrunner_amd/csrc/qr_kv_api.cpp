@@ -168,7 +168,7 @@ int qr_kv_create(qr_kv** out, int layers, int heads, int kv_heads, int head_dim,
     if (st == QR_OK) {
         PageGeom g{2, kv_heads, head_dim};
         g.mfma_layout = kv_mfma_layout(kv_dtype, head_dim) ? 1 : 0;
-        g.scaled = kv_dtype == QR_DTYPE_E4M3 ? 1 : 0;
+        if (kv_dtype == QR_DTYPE_E4M3) g.mfma_layout |= 2;
         st = kv->store.init(g, kv_dtype, layers, max_batch, max_seq);
     }
     if (st == QR_OK) st = decode_scratch_address(kv->device, &kv->scratch);
@@ -574,7 +574,7 @@ int qr_kv_bytes_per_token(const qr_kv* kv, long long* out) {
     clear_error();
     QR_TRY(check_handle(kv));
     QR_CHECK_ARG(out, "null output pointer");
-    *out = (static_cast<long long>(kv->kv_dim) * dtype_size(kv->dtype) + (kv->store.geom().scaled ? kv->kv_heads : 0)) * 2 * kv->layers;
+    *out = (static_cast<long long>(kv->kv_dim) * dtype_size(kv->dtype) + (kv->store.geom().scaled() ? kv->kv_heads : 0)) * 2 * kv->layers;
     return QR_OK;
 }
 

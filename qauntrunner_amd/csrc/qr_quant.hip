@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kThreads) read_as_any_kernel(const ReadArgs a)
     for (int i = threadIdx.x; i < 2 * width; i += kThreads) {
         const int plane = i >= width, c = i - plane * width;
         const long long from = a.geom.offset(phys, plane, c / D, slot, c % D);
-        const float x = a.geom.scaled ? quant_value<0>(bytes[from]) * scale_of(bytes[a.geom.scale_offset(phys, plane, c / D, slot)])
+        const float x = a.geom.scaled() ? quant_value<0>(bytes[from]) * scale_of(bytes[a.geom.scale_offset(phys, plane, c / D, slot)])
                                       : load_elem(a.pool, a.dtype, from);
         store_out(plane ? a.v : a.k, a.act, static_cast<long long>(row) * width + c, x);
     }
