@@ -47,7 +47,22 @@ struct Shape {
     int target;      // units that run at once
     int least;       // tiles of a part, at least
 };
-Shape shape_of(int) { return {kFormAnyRows, kFormAnyTile, 1024, 2}; }
+Shape shape_of(int kind) {
+    switch (kind) {
+        case kFormStream: return {32, 32, 512, 8};
+        case kFormTiles: return {128, 64, 512, 2};
+        default: return {kFormAnyRows, kFormAnyTile, 1024, 2};
+    }
+}
+int kind_of(const FormsArgs& a, int rows) {
+    if (!(a.geom.mfma_layout & 1) || a.heads % a.geom.kv_heads) return kFormAny;
+    return static_cast<long long>(rows) * (a.heads / a.geom.kv_heads) <= 32 ? kFormStream : kFormTiles;
+}
+hipError_t launch(const FormsK& k, int kind, int units, hipStream_t s) {
+    if (kind == kFormAny) return launch_forms_any(k, units, s);
+    if (k.dtype == QR_DTYPE_F16) return launch_forms_f16(k, kind, units, s);
+    return k.dtype == QR_DTYPE_BF16 ? launch_forms_bf16(k, kind, units, s) : launch_forms_e4m3(k, kind, units, s);
+}
 
 // Tiles of the slots that row j of an item sees.
 int tiles_of(const FormsPlan& p, const FormItem& it, int window, int j, int tile) {
@@ -72,7 +87,7 @@ FormsPlan plan_forms(const FormsArgs& a) {
         it.rows = rows;
         it.base = base;
         it.keys = keys;
-        p.kind[p.n] = kFormAny;
+        p.kind[p.n] = kind_of(a, rows);
         ++p.n;
     };
     for (int i = 0; i < a.n; ++i) {
@@ -178,7 +193,7 @@ hipError_t launch_forms(const FormsArgs& a, const FormsPlan& plan, void* workspa
                 units += it.blocks * it.splits * a.geom.kv_heads;
             }
             if (!k.n) continue;
-            const hipError_t e = launch_forms_any(k, units, stream);
+            const hipError_t e = launch(k, kind, units, stream);
             if (e != hipSuccess) return e;
         }
     if (plan.merge) {

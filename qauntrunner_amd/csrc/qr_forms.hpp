@@ -13,7 +13,7 @@
 namespace qr {
 
 // Kernels of a launch.
-enum FormKind { kFormAny, kFormKinds };
+enum FormKind { kFormAny, kFormStream, kFormTiles, kFormKinds };
 constexpr int kFormAnyRows = 8, kFormAnyTile = 32;
 
 // What the host knows of a chunk.
@@ -92,6 +92,10 @@ FormsPlan plan_forms(const FormsArgs& a);
 hipError_t launch_forms(const FormsArgs& a, const FormsPlan& plan, void* workspace, hipStream_t stream);
 
 hipError_t launch_forms_any(const FormsK& k, int units, hipStream_t s);
+// MFMA tiles (kinds kFormStream, kFormTiles): operand page layouts, whole groups.
+hipError_t launch_forms_f16(const FormsK& k, int kind, int units, hipStream_t s);
+hipError_t launch_forms_bf16(const FormsK& k, int kind, int units, hipStream_t s);
+hipError_t launch_forms_e4m3(const FormsK& k, int kind, int units, hipStream_t s);
 
 // Query heads h0 .. h0 + g - 1 read kv head kvh (head h reads h * kv_heads / heads).
 __device__ __forceinline__ void form_heads(const FormsK& p, int kvh, int* h0, int* g) {

@@ -1,0 +1,717 @@
+// qr_forms_mfma.hpp -- attention in its other forms and behind shared prefixes on 32x32x16 MFMA tiles: caches of 16 and 8
+// bits, head sizes 64 and 128 (operand page layouts, qr_kernels.hpp), whole groups of query heads, gfx950.
+//
+// A row is one (query, query head) pair of a kv head; a wave owns 32 rows:
+//   QK  S^T[position][row] = K . q^T    (A = K, B = q)
+//   PV  O^T[dim][row]     += V^T . P^T  (A = V, B = P)
+// v_mfma_f32_32x32x16: A[m = lane % 32][k = 8 (lane / 32) + i], B[k = 8 (lane / 32) + i][n = lane % 32],
+// D[m = 8 (r / 4) + 4 (lane / 32) + r % 4][n = lane % 32].  A row's scores lie in two lanes, l and l ^ 32.  Which position of a
+// step of 32 an A row m stands for is chosen so that a lane's scores r are its k-slots of the PV steps, in order:
+//   16 bits: m = 16 s + 8 a + 4 h + b is position 16 s + 8 h + 4 a + b, score r = 8 s + i position 16 s + 8 (lane / 32) + i;
+//   8 bits:  m = 16 s + 8 a + 4 h + b is position 16 h + 8 s + 4 a + b, score r position 16 (lane / 32) + r, so that a lane's
+//            operands of both PV steps are 16 bytes of the page.
+//
+// 8 bits: codes become bf16 exactly.  K's scale is one number per lane there (a lane holds dims of one position), a factor
+// of the conversion; V's scale differs between a lane's positions and goes into the weights, after their sum.
+//
+// Scores in log2 units: z = s sscale, capped, less the slope; weights 2^(z - m) of at most 2^kTop, m moved (and the
+// accumulators rescaled) only when a score passes m + kTop, and then to leave kHead log2 units to the next move.  bf16
+// weights stay at or below 1; fp16, with few exponents below 1, takes them up to 2^15.  Sums are of the fp32 weights.
+// Queries and weights of a type with more bits than the tile's enter as PARTS of it: bf16 three (24 bits), fp16 two (22).
+#pragma once
+
+#include "qr_forms.hpp"
+#include "qr_mfma.hpp"
+#include "qr_quant.hpp"
+
+namespace qr {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x16_t mfma32(f16x8_t a, f16x8_t b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16_t mfma32(bf16x8_t a, bf16x8_t b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+// (fmaxf's quieting of NaNs, one more v_max each, is not needed: a NaN score reaches its row through its weight.  The
+// compiler does not count the wait states between an MFMA and an asm that reads its result: mfma_done stands between.)
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+__device__ __forceinline__ void mfma_done(f32x16_t (&s)[1]) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s[0])); }
+__device__ __forceinline__ void mfma_done(f32x16_t (&s)[2]) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1])); }
+
+enum FormScores { kScoresPlain, kScoresSlope, kScoresCap };  // (capped scores may have a slope too)
+
+template <int CT> struct FormElem {
+    static constexpr bool BF16 = CT != QR_DTYPE_F16;
+    using T = typename std::conditional<BF16, __bf16, _Float16>::type;
+    typedef T vec8 __attribute__((ext_vector_type(8)));
+};
+
+// 8 codes times `scale`.
+__device__ __forceinline__ bf16x8_t widen8(uint32_t lo, uint32_t hi, float scale) {
+    const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+    const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Page of a slot, by a scalar load (no kernel writes the table while this one runs).
+__device__ __forceinline__ int form_page(const FormsK& p, int pt_off, int t) {
+    return reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p.page_table))[pt_off + (t >> kPageShift)];
+}
+
+// Slots that the rows of a block see: some row [lo, hi], every row [all_lo, all_hi].
+struct FormRange {
+    int lo, hi, all_lo, all_hi;
+    __device__ __forceinline__ bool all(int t, int n) const { return t >= all_lo && t + n - 1 <= all_hi; }
+};
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) x = min(x, __shfl_xor(x, i));
+    return x;
+}
+__device__ __forceinline__ int wave_max(int x) { return ~wave_min(~x); }
+
+// One wave's 32 rows.
+template <int CT, int D, int PARTS, int SCORES>
+struct FormTile {
+    static constexpr bool BF16 = FormElem<CT>::BF16, E8 = CT == QR_DTYPE_E4M3, SPLIT = PARTS > 1;
+    using T = typename FormElem<CT>::T;
+    using vec8 = typename FormElem<CT>::vec8;
+    static constexpr int NK = D / 16;   // QK k-steps
+    static constexpr int ND = D / 32;   // PV dim tiles
+    static constexpr float kTop = BF16 ? 0.f : 15.f, kHead = SPLIT ? 0.f : 4.f;
+
+    int lane, half;
+    int row, head, chunk;  // of row lane % 32
+    bool on;
+    int lo, hi;            // slots that the row sees (none past the item's rows)
+    float away, slope;     // position less the item's base; slope in log2 units
+    vec8 q[PARTS][NK];
+    float sscale;          // log2 units per score
+    float m, l;            // l: this lane's half of the positions
+    f32x16_t acc[ND];
+
+    __device__ __forceinline__ void init(const FormsK& p, const FormItem& it, int kvh, int g, int rho) {
+        lane = threadIdx.x & 63;
+        half = lane >> 5;
+        const int r = rho + (lane & 31);
+        on = r < it.rows * g;
+        const int rr = on ? r : it.rows * g - 1;
+        const int j = rr / g;
+        head = kvh * g + rr - j * g;
+        row = it.row0 + j;
+        const FormSpan s = form_row(p, it, j);
+        chunk = s.chunk;
+        lo = s.lo;
+        hi = on ? s.hi : -1;
+        away = static_cast<float>(s.pos - it.base);
+        slope = SCORES != kScoresPlain && p.slopes ? p.slopes[head] * kLog2e : 0.f;
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+    }
+    __device__ __forceinline__ FormRange range() const {
+        const bool sees = lo <= hi;
+        return {wave_min(sees ? lo : 0x7FFFFFFF), wave_max(sees ? hi : -1), wave_max(on ? lo : -1), wave_min(on ? hi : 0x7FFFFFFF)};
+    }
+
+    // Dims of this lane's part of k-step kk.  The sign of the scale goes into q: the maximum is taken before the scores are
+    // scaled.
+    __device__ __forceinline__ int dim0(int kk) const { return E8 ? 32 * (kk >> 1) + 16 * half + 8 * (kk & 1) : 16 * kk + 8 * half; }
+    __device__ __forceinline__ void load_q(const FormsK& p) {
+        const long long at = (static_cast<long long>(row) * p.heads + head) * D;
+        const float sign = p.qscale == 0.f ? 0.f : p.qscale < 0.f ? -1.f : 1.f;
+        sscale = p.qscale == 0.f ? 1.f : fabsf(p.qscale);
+        float x[NK][8];
+        if (p.act == QR_DTYPE_F32) {
+            const float* f = static_cast<const float*>(p.q) + at;
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) __builtin_memcpy(x[kk], f + dim0(kk), 32);
+        } else {
+            const uint16_t* h = static_cast<const uint16_t*>(p.q) + at;
+            uint16_t u[NK][8];
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) __builtin_memcpy(u[kk], h + dim0(kk), 16);
+            const bool bf = p.act == QR_DTYPE_BF16;
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[kk][i] = bf ? bf16_bits_to_f32(u[kk][i]) : f16_bits_to_f32(u[kk][i]);
+        }
+        float by = sign;
+        if (SPLIT && !BF16) {
+            // fp16 parts: the row's largest value to 2^13 .. 2^14, a power of two that the score scale takes back
+            float a = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(x[kk][i]));
+            a = max_xor32(a);
+            if (a > 1e-30f && a < 3e38f) {
+                const int ex = ilogbf(a) - 13;
+                by = ldexpf(sign, -ex);
+                sscale = ldexpf(sscale, ex);
+            }
+        }
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float v = x[kk][i] * by;
+#pragma unroll
+                for (int c = 0; c < PARTS; ++c) {
+                    q[c][kk][i] = static_cast<T>(v);
+                    v -= static_cast<float>(q[c][kk][i]);
+                }
+            }
+    }
+
+    // Position of score r within its step of 32.
+    __device__ __forceinline__ int at(int r) const { return E8 ? 16 * half + r : 16 * (r >> 3) + 8 * half + (r & 7); }
+
+    // Scores of step t0 in log2 units (plain ones are scaled as they become weights), masked where some row does not see the
+    // whole step: `edge`.
+    __device__ __forceinline__ void form(const FormsK& p, f32x16_t& s, int t0, bool edge) const {
+        if (SCORES == kScoresCap) {
+            // (for 16 bits 1 - 2 / (e^2x + 1): off by a few 2^-24 of the cap, far below the weights' rounding)
+            const float in = (SPLIT ? 1.f : 2.f * kLog2e) * sscale / p.cap;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[r] = SPLIT ? p.cap * tanhf(s[r] * in) : fmaf(-2.f * p.cap, __builtin_amdgcn_rcpf(fast_exp2(s[r] * in) + 1.f), p.cap);
+        }
+        if (SCORES != kScoresPlain) {
+            const float first = static_cast<float>(t0 + (E8 ? 16 : 8) * half) - away;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float d = fabsf(first + static_cast<float>(E8 ? r : 16 * (r >> 3) + (r & 7)));
+                s[r] = SCORES == kScoresCap ? fmaf(-slope, d, s[r]) : fmaf(s[r], sscale, -slope * d);
+            }
+        }
+        if (edge) {
+            const int a = lo - t0 - (E8 ? 16 : 8) * half, b = hi - t0 - (E8 ? 16 : 8) * half;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int x = E8 ? r : 16 * (r >> 3) + (r & 7);
+                if (x < a || x > b) s[r] = -INFINITY;
+            }
+        }
+    }
+
+    // Weights of NS steps' scores, as PV operands (8 bits: times V's scales); rescales what was summed when the maximum moves.
+    template <int NS, class F>
+    __device__ __forceinline__ void softmax(f32x16_t (&s)[NS], vec8 (&w)[PARTS][NS][2], F vscale) {
+        mfma_done(s);
+        float mx[2 * NS];
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            const float a = max3f(s[n][0], s[n][1], s[n][2]), b = max3f(s[n][3], s[n][4], s[n][5]);
+            const float c = max3f(s[n][6], s[n][7], s[n][8]), d = max3f(s[n][9], s[n][10], s[n][11]);
+            mx[2 * n] = max3f(s[n][12], s[n][13], s[n][14]);
+            mx[2 * n] = max3f(mx[2 * n], s[n][15], a);
+            mx[2 * n + 1] = max3f(b, c, d);
+        }
+        float t = mx[0];
+#pragma unroll
+        for (int n = 1; n < 2 * NS; ++n) t = fmaxf(t, mx[n]);
+        t = max_xor32(t);
+        const float by = SCORES == kScoresPlain ? sscale : 1.f;
+        const bool grow = fmaf(t, by, -m) > kTop;
+        if (__builtin_amdgcn_ballot_w64(grow)) {
+            float mn = fmaf(t, by, kHead - kTop);
+            if (fmaf(t, by, -mn) > kTop) {  // rounded down, where a step of m is that large
+                const int b = __float_as_int(mn);
+                mn = __int_as_float(b < 0 ? b - 1 : b + 1);
+            }
+            mn = grow ? mn : m;
+            const float c = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            if (__builtin_amdgcn_ballot_w64(grow && m != -INFINITY)) {
+                const float cc = grow && m != -INFINITY ? c : 1.f;
+                l *= cc;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) acc[d] *= cc;
+            }
+            m = mn;
+        }
+        const float ref = m == -INFINITY ? 0.f : -m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = fast_exp2(SCORES == kScoresPlain ? fmaf(s[n][r], sscale, ref) : s[n][r] + ref);
+                sum[r & 3] += e;
+                float v = E8 ? e * vscale(n, r) : e;
+#pragma unroll
+                for (int c = 0; c < PARTS; ++c) {
+                    w[c][n][r >> 3][r & 7] = static_cast<T>(v);
+                    v -= static_cast<float>(w[c][n][r >> 3][r & 7]);
+                }
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
+
+    // V's element at (slot t, dim d) of the page.
+    __device__ __forceinline__ float v_value(const FormsK& p, int phys, int kvh, int t, int d) const {
+        const long long at = p.geom.offset(phys, 1, kvh, t & (kPageTokens - 1), d);
+        if (E8) return quant_value<0>(static_cast<uint8_t>(p.pool[at]));
+        return static_cast<float>(*reinterpret_cast<const T*>(p.pool + 2 * at));
+    }
+    // A step that not every row sees whole may hold V elements that are not finite at slots some rows do not see, where 0 x inf
+    // would reach them.  Adds them to the rows that see them as they are (no finite weight changes them); the caller clears
+    // them in its operands.
+    __device__ __forceinline__ void add_bad(const FormsK& p, const FormItem& it, int kvh, int t0) {
+        const int phys = form_page(p, it.pt_off, t0);
+#pragma unroll 1
+        for (int k = 0; k < 32; ++k) {
+            const bool sees = t0 + k >= lo && t0 + k <= hi;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float x = v_value(p, phys, kvh, t0 + k, 32 * d + 8 * (r >> 2) + 4 * half + (r & 3));
+                    if (!(fabsf(x) < INFINITY) && sees) acc[d][r] += x;
+                    if ((r & 3) == 3) asm volatile("" ::: "memory");  // no registers for all reads at once
+                }
+        }
+    }
+
+    // The row's output or partial: N groups of 4 dims from group g0 on, of the weighed sums a.  Group g holds dims 32 (g / 4) +
+    // 8 (g % 4) + 4 half .. + 3.
+    __device__ __forceinline__ long long slot(const FormsK& p, const FormItem& it, int split) const {
+        const FormRows& c = p.c[chunk];
+        return c.slot0 + (static_cast<long long>(row - c.row0) * p.heads + head) * c.parts + it.part0 + split;
+    }
+    template <int N>
+    __device__ __forceinline__ void store(const FormsK& p, const FormItem& it, int split, int g0, float lsum, const f32x4_t (&a)[N]) const {
+        if (!on) return;
+        auto dim = [&](int i) { return 32 * ((g0 + i) >> 2) + 8 * ((g0 + i) & 3) + 4 * half; };
+        if (p.c[chunk].parts > 1) {
+            float* o = p.part_acc + slot(p, it, split) * D;
+#pragma unroll
+            for (int i = 0; i < N; ++i) *reinterpret_cast<f32x4_t*>(o + dim(i)) = a[i];
+            return;
+        }
+        const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+        const long long at = (static_cast<long long>(row) * p.heads + head) * D;
+        if (p.act == QR_DTYPE_BF16) store16<__bf16>(static_cast<uint16_t*>(p.out) + at, inv, a, dim);
+        else if (p.act == QR_DTYPE_F16) store16<_Float16>(static_cast<uint16_t*>(p.out) + at, inv, a, dim);
+        else {
+            float* o = static_cast<float*>(p.out) + at;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const f32x4_t x = a[i] * inv;
+                __builtin_memcpy(o + dim(i), &x, 16);
+            }
+        }
+    }
+    // one store per group, element-aligned
+    template <class O, int N, class G>
+    __device__ static __forceinline__ void store16(uint16_t* o, float inv, const f32x4_t (&a)[N], G dim) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const f32x4_t x = a[i] * inv;
+            O b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = static_cast<O>(x[j]);
+            __builtin_memcpy(o + dim(i), b, 8);
+        }
+    }
+    __device__ __forceinline__ void store_ml(const FormsK& p, const FormItem& it, int split, float mm, float lsum) const {
+        if (on && !half && p.c[chunk].parts > 1) p.part_ml[slot(p, it, split)] = make_float2(mm, lsum);
+    }
+};
+
+// ------------------------------------------------------------------ few rows: HBM-bound
+// Up to 32 rows; four waves take every fourth step of 32 slots, their operands straight from the page into registers, one step
+// ahead, and merge at the end.  No wave waits for another before that.
+template <int CT, int D> struct FormStep {  // one step's operands
+    using E = FormElem<CT>;
+    static constexpr bool E8 = CT == QR_DTYPE_E4M3;
+    static constexpr int N = E8 ? D / 32 : D / 16;  // 16-byte loads of K and of V
+    uint4 k[N], v[N];
+    uint4 vs;            // 8 bits: scale bytes of V at the lane's 16 positions
+    uint32_t ks;         // and of K at its own
+};
+
+template <int CT, int D, int PARTS, int SCORES>
+__global__ void __launch_bounds__(256, 2) forms_stream_kernel(const FormsK p) {
+    using F = FormTile<CT, D, PARTS, SCORES>;
+    using vec8 = typename F::vec8;
+    constexpr bool E8 = F::E8;
+    constexpr int NG = D / 8;  // f32x4 groups of a row in a lane
+    constexpr int ES = E8 ? 1 : 2;
+    __shared__ f32x4_t xa[4 * NG * 64];
+    __shared__ float2 xm[4 * 64];
+    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
+    const FormItem it = p.it[e];
+    const int u = blockIdx.x - it.unit0, kv = p.geom.kv_heads, g = p.heads / kv;
+    const int kvh = u % kv, split = u / kv % it.splits, block = it.blocks - 1 - u / kv / it.splits;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    F w;
+    w.init(p, it, kvh, g, 32 * block);
+    const FormRange range = w.range();
+    const int step0 = range.lo >> 5, steps = range.lo > range.hi ? 0 : (range.hi >> 5) - step0 + 1;
+    const int s0 = step0 + static_cast<int>(static_cast<long long>(steps) * split / it.splits);
+    const int s1 = step0 + static_cast<int>(static_cast<long long>(steps) * (split + 1) / it.splits);
+
+    const long long page_bytes = p.geom.page_elems() * ES, plane_bytes = p.geom.plane_elems() * ES;
+    const long long head_bytes = static_cast<long long>(kvh) * kPageTokens * D * ES;
+    const int m_ = w.lane & 31, sx = m_ >> 4, ax = (m_ >> 3) & 1, hx = (m_ >> 2) & 1, bx = m_ & 3;
+    // this lane's part of the operands of a step
+    const int ko = E8 ? 16 * w.lane : 1024 * ax * (D / 32) + 16 * (16 * w.half + 4 * (2 * sx + hx) + bx);
+    const int vo = E8 ? 16 * w.lane : 1024 * (m_ >> 4) + 16 * (16 * w.half + (w.lane & 15));
+    auto load = [&](FormStep<CT, D>& o, int st, int phys) __attribute__((always_inline)) {
+        const char* page = p.pool + static_cast<long long>(phys) * page_bytes;
+        const char* k = page + head_bytes + static_cast<long long>(st & 7) * 32 * D * ES;
+        const char* v = k + plane_bytes;
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        auto get = [](const char* a) __attribute__((always_inline)) {
+            const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a));
+            return make_uint4(x[0], x[1], x[2], x[3]);
+        };
+#pragma unroll
+        for (int i = 0; i < FormStep<CT, D>::N; ++i) o.k[i] = get(k + ko + (E8 ? 1024 : 512) * i);
+        if (E8) {
+            const char* sc = page + 2 * plane_bytes + kvh * kPageTokens + 32 * (st & 7);
+            o.ks = static_cast<uint8_t>(sc[16 * hx + 8 * sx + 4 * ax + bx]);
+            o.vs = *reinterpret_cast<const uint4*>(sc + kv * kPageTokens + 16 * w.half);
+        }
+#pragma unroll
+        for (int i = 0; i < FormStep<CT, D>::N; ++i) o.v[i] = get(v + vo + (E8 ? 1024 * i : 2048 * (i % F::ND) + 512 * (i / F::ND)));
+    };
+    auto page = [&](int st) __attribute__((always_inline)) { return st < s1 ? form_page(p, it.pt_off, 32 * st) : 0; };
+    auto as8 = [](uint4 x) __attribute__((always_inline)) {
+        vec8 r;
+        __builtin_memcpy(&r, &x, 16);
+        return r;
+    };
+    auto compute = [&](FormStep<CT, D>& o, int st) __attribute__((always_inline)) {
+        f32x16_t s[1];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+        const float ks = E8 ? scale_of(o.ks) : 1.f;
+#pragma unroll
+        for (int kk = 0; kk < F::NK; ++kk) {
+            vec8 a;
+            if constexpr (E8) {
+                const uint4 x = o.k[kk >> 1];
+                a = kk & 1 ? widen8(x.z, x.w, ks) : widen8(x.x, x.y, ks);
+            } else {
+                a = as8(o.k[kk]);
+            }
+#pragma unroll
+            for (int c = 0; c < PARTS; ++c) s[0] = mfma32(a, w.q[c][kk], s[0]);
+        }
+        const bool edge = !range.all(32 * st, 32);
+        w.form(p, s[0], 32 * st, edge);
+        if (edge) {
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < FormStep<CT, D>::N; ++i) {
+                uint32_t x[4] = {o.v[i].x, o.v[i].y, o.v[i].z, o.v[i].w};
+                constexpr uint32_t exps = E8 ? 0x7F7F7F7Fu : F::BF16 ? 0x7F807F80u : 0x7C007C00u;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t y = ~x[j] & exps;  // an element of zeros: not a number or infinite
+                    bad |= E8 ? ((y - 0x01010101u) & ~y & 0x80808080u) != 0 : (y & 0xFFFFu) == 0 || (y >> 16) == 0;
+                }
+            }
+            if (__builtin_amdgcn_ballot_w64(bad)) {
+                w.add_bad(p, it, kvh, 32 * st);
+#pragma unroll
+                for (int i = 0; i < FormStep<CT, D>::N; ++i) {
+                    uint32_t x[4] = {o.v[i].x, o.v[i].y, o.v[i].z, o.v[i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int b = 0; b < 32; b += 8 * ES) {
+                            constexpr uint32_t exps = E8 ? 0x7Fu : F::BF16 ? 0x7F80u : 0x7C00u;
+                            if ((x[j] >> b & exps) == exps) x[j] &= ~((E8 ? 0xFFu : 0xFFFFu) << b);
+                        }
+                    o.v[i] = make_uint4(x[0], x[1], x[2], x[3]);
+                }
+            }
+        }
+        vec8 wt[PARTS][1][2];
+        const uint32_t vs[4] = {o.vs.x, o.vs.y, o.vs.z, o.vs.w};
+        w.template softmax<1>(s, wt, [&](int, int r) __attribute__((always_inline)) { return scale_of(vs[r >> 2] >> (8 * (r & 3)) & 0xFF); });
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int d = 0; d < F::ND; ++d) {
+                vec8 a;
+                if constexpr (E8) a = x ? widen8(o.v[d].z, o.v[d].w, 1.f) : widen8(o.v[d].x, o.v[d].y, 1.f);
+                else a = as8(o.v[x * F::ND + d]);
+#pragma unroll
+                for (int c = 0; c < PARTS; ++c) w.acc[d] = mfma32(a, wt[c][0][x], w.acc[d]);
+            }
+    };
+    FormStep<CT, D> a, b;
+    int st = s0 + wave;
+    int phys = page(st + 4);
+    if (st < s1) load(a, st, page(st));
+    w.load_q(p);
+    for (; st < s1; st += 8) {
+        if (st + 4 < s1) load(b, st + 4, phys);
+        phys = page(st + 8);
+        compute(a, st);
+        if (st + 4 >= s1) break;
+        if (st + 8 < s1) load(a, st + 8, phys);
+        phys = page(st + 12);
+        compute(b, st + 4);
+    }
+    w.l = sum_xor32(w.l);
+
+    // the waves merge: each adds up a quarter of the dim groups
+#pragma unroll
+    for (int d = 0; d < F::ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            xa[(wave * NG + 4 * d + i) * 64 + w.lane] = f32x4_t{w.acc[d][4 * i], w.acc[d][4 * i + 1], w.acc[d][4 * i + 2], w.acc[d][4 * i + 3]};
+    xm[wave * 64 + w.lane] = make_float2(w.m, w.l);
+    __syncthreads();
+    float M = -INFINITY, L = 0.f, c[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) M = fmaxf(M, xm[x * 64 + w.lane].x);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        const float2 ml = xm[x * 64 + w.lane];
+        c[x] = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - M);
+        L = fmaf(ml.y, c[x], L);
+    }
+    constexpr int NP = NG / 4;
+    f32x4_t o[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[i] += xa[(x * NG + wave * NP + i) * 64 + w.lane] * c[x];
+    }
+    w.store(p, it, split, wave * NP, L, o);
+    if (wave == 0) w.store_ml(p, it, split, M, L);
+}
+
+// ------------------------------------------------------------------ many rows: bound by MFMAs and the softmax
+// Four waves of 32 rows share every tile of 64 slots in LDS, the next one requested while one is used; two workgroups on a CU,
+// so that one's softmax runs beside the other's MFMAs.  16 bits: tiles are copied by buffer-load DMA as they lie in the page.
+// 8 bits: a thread takes 16 bytes of K and V through registers and writes them as bf16 operands, once for the four waves.
+constexpr int kFormTileRows = 128, kFormTile = 64;
+
+template <int CT, int D, int PARTS, int SCORES>
+__global__ void __launch_bounds__(256, 2) forms_tile_kernel(const FormsK p) {
+    using F = FormTile<CT, D, PARTS, SCORES>;
+    using vec8 = typename F::vec8;
+    using T = typename F::T;
+    constexpr bool E8 = F::E8;
+    constexpr int ES = E8 ? 1 : 2;
+    constexpr int SB = 64 * D;          // bytes of a step's operands of K (or V) in LDS
+    constexpr int KB = 2 * SB;          // of a tile
+    constexpr int PER = KB / 1024 / 4;  // DMA loads per wave for a tile of K (or V)
+    constexpr int NP = 64 * D / 16 / 256;  // 8 bits: 16-byte pieces of K (or V) per thread
+    __shared__ __attribute__((aligned(1024))) char lds[4 * KB];  // two K tiles, two V tiles
+    __shared__ float vscale[2][64];
+    __shared__ int spans[4][4];
+    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
+    const FormItem it = p.it[e];
+    const int u = blockIdx.x - it.unit0, kv = p.geom.kv_heads, g = p.heads / kv;
+    const int kvh = u % kv, split = u / kv % it.splits, block = it.blocks - 1 - u / kv / it.splits;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    F w;
+    w.init(p, it, kvh, g, kFormTileRows * block + 32 * wave);
+    FormRange range = w.range();
+    if (w.lane == 0) {
+        spans[wave][0] = range.lo;
+        spans[wave][1] = range.hi;
+        spans[wave][2] = range.all_lo;
+        spans[wave][3] = range.all_hi;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        range.lo = min(range.lo, spans[i][0]);
+        range.hi = max(range.hi, spans[i][1]);
+        range.all_lo = max(range.all_lo, spans[i][2]);
+        range.all_hi = min(range.all_hi, spans[i][3]);
+    }
+    range.lo = __builtin_amdgcn_readfirstlane(range.lo);
+    range.hi = __builtin_amdgcn_readfirstlane(range.hi);
+    range.all_lo = __builtin_amdgcn_readfirstlane(range.all_lo);
+    range.all_hi = __builtin_amdgcn_readfirstlane(range.all_hi);
+    const int tile0 = range.lo / kFormTile, tiles = range.lo > range.hi ? 0 : range.hi / kFormTile - tile0 + 1;
+    const int i0 = tile0 + static_cast<int>(static_cast<long long>(tiles) * split / it.splits);
+    const int i1 = tile0 + static_cast<int>(static_cast<long long>(tiles) * (split + 1) / it.splits);
+
+    const long long page_bytes = p.geom.page_elems() * ES, plane_bytes = p.geom.plane_elems() * ES;
+    const long long head_bytes = static_cast<long long>(kvh) * kPageTokens * D * ES;
+    auto page = [&](int i) { return i < i1 ? form_page(p, it.pt_off, kFormTile * i) : 0; };
+    auto k_at = [&](int i) { return lds + (i & 1) * KB; };
+    auto v_at = [&](int i) { return lds + (2 + (i & 1)) * KB; };
+    // 16 bits: request tile i
+    auto dma = [&](int i, int phys) __attribute__((always_inline)) {
+        const char* base = p.pool + static_cast<long long>(phys) * page_bytes + head_bytes + static_cast<long long>(kFormTile * i & (kPageTokens - 1)) * D * 2;
+        const bool in = i < i1;  // past the last tile: no records, no memory is read
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, in ? KB : 0, kBufferFlags);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + plane_bytes), 0, in ? KB : 0, kBufferFlags);
+#pragma unroll
+        for (int c = 0; c < PER; ++c) buffer_load_lds16(rk, k_at(i) + 1024 * (wave + 4 * c), 16 * w.lane, 1024 * (wave + 4 * c));
+#pragma unroll
+        for (int c = 0; c < PER; ++c) buffer_load_lds16(rv, v_at(i) + 1024 * (wave + 4 * c), 16 * w.lane, 1024 * (wave + 4 * c));
+    };
+    // 8 bits: pieces of tile i into registers, and from there into LDS
+    uint4 pk[E8 ? NP : 1], pv[E8 ? NP : 1];
+    uint32_t ps[E8 ? NP : 1], pvs = 0;
+    auto fetch = [&](int i, int phys) __attribute__((always_inline)) {
+        if (i >= i1) return;
+        const char* pg = p.pool + static_cast<long long>(phys) * page_bytes;
+        const char* base = pg + head_bytes + static_cast<long long>(kFormTile * i & (kPageTokens - 1)) * D;
+        const char* sc = pg + 2 * plane_bytes + kvh * kPageTokens + (kFormTile * i & (kPageTokens - 1));
+#pragma unroll
+        for (int c = 0; c < NP; ++c) {
+            const int x = threadIdx.x + 256 * c, m = x & 31;  // piece x: step x / (2 D), lane x % 64
+            pk[c] = *reinterpret_cast<const uint4*>(base + 16 * x);
+            pv[c] = *reinterpret_cast<const uint4*>(base + plane_bytes + 16 * x);
+            ps[c] = static_cast<uint8_t>(sc[32 * (x / (2 * D)) + 16 * (m >> 2 & 1) + 8 * (m >> 4) + 4 * (m >> 3 & 1) + (m & 3)]);
+        }
+        if (threadIdx.x < 64) pvs = static_cast<uint8_t>(sc[kv * kPageTokens + threadIdx.x]);
+    };
+    auto put = [&](int i) __attribute__((always_inline)) {
+        if (i >= i1) return;
+        if constexpr (E8) {
+#pragma unroll
+            for (int c = 0; c < NP; ++c) {
+                const int x = threadIdx.x + 256 * c, st = x / (2 * D), j = x / 64 % (D / 32), l = x & 63;
+                const float ks = scale_of(ps[c]);
+                bf16x8_t* k = reinterpret_cast<bf16x8_t*>(k_at(i) + SB * st + 2048 * j + 16 * l);
+                k[0] = widen8(pk[c].x, pk[c].y, ks);
+                k[64] = widen8(pk[c].z, pk[c].w, ks);
+                bf16x8_t* v = reinterpret_cast<bf16x8_t*>(v_at(i) + SB * st + 1024 * j + 16 * l);
+                v[0] = widen8(pv[c].x, pv[c].y, 1.f);
+                v[64 * F::ND] = widen8(pv[c].z, pv[c].w, 1.f);
+            }
+            if (threadIdx.x < 64) vscale[i & 1][threadIdx.x] = scale_of(pvs);
+        }
+    };
+    // this lane's part of the operands: K of step st, k-step kk; V of step st, PV step x, dim tile d
+    const int m_ = w.lane & 31, sx = m_ >> 4, ax = (m_ >> 3) & 1, hx = (m_ >> 2) & 1, bx = m_ & 3;
+    const int ko = E8 ? 16 * w.lane : 1024 * ax * (D / 32) + 16 * (16 * w.half + 4 * (2 * sx + hx) + bx);
+    const int vo = E8 ? 16 * w.lane : 1024 * (m_ >> 4) + 16 * (16 * w.half + (w.lane & 15));
+    auto k_op = [&](const char* k, int st, int kk) __attribute__((always_inline)) {
+        return *reinterpret_cast<const vec8*>(k + SB * st + ko + (E8 ? 1024 : 512) * kk);
+    };
+    auto v_op = [&](const char* v, int st, int x, int d) __attribute__((always_inline)) {
+        return *reinterpret_cast<const vec8*>(v + SB * st + vo + (E8 ? 1024 * (x * F::ND + d) : 2048 * d + 512 * x));
+    };
+    int phys = page(i0 + 1);
+    if (E8) fetch(i0, page(i0));
+    else if (i0 < i1) dma(i0, page(i0));
+    w.load_q(p);
+    if (E8) {
+        put(i0);
+        fetch(i0 + 1, phys);
+        phys = page(i0 + 2);
+    }
+    for (int i = i0; i < i1; ++i) {
+        if (E8) {
+            __syncthreads();  // tile i is written, tile i - 1 was read
+        } else {
+            wait_dma();
+            lds_barrier_dma_in_flight();
+            if (i + 1 < i1) dma(i + 1, phys);
+            phys = page(i + 2);
+        }
+        const char* const k = k_at(i);
+        char* const v = v_at(i);
+        f32x16_t s[2];
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[st][r] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < F::NK; ++kk) {
+                const vec8 a = k_op(k, st, kk);
+#pragma unroll
+                for (int c = 0; c < PARTS; ++c) s[st] = mfma32(a, w.q[c][kk], s[st]);
+            }
+        }
+        const bool edge = !range.all(kFormTile * i, kFormTile);
+#pragma unroll
+        for (int st = 0; st < 2; ++st) w.form(p, s[st], kFormTile * i + 32 * st, edge);
+        if (edge) {
+            // V elements that are not finite: a product of all of them with zeros shows them (the same in every wave)
+            vec8 zero;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) zero[j] = static_cast<T>(0.f);
+            f32x16_t z;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) z[j] = 0.f;
+#pragma unroll
+            for (int c = 0; c < KB / 1024; ++c) z = mfma32(*reinterpret_cast<const vec8*>(v + 1024 * c + 16 * w.lane), zero, z);
+            float t = 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) t += z[j];
+            if (__builtin_amdgcn_ballot_w64(!(t == 0.f))) {
+                w.add_bad(p, it, kvh, kFormTile * i);
+                w.add_bad(p, it, kvh, kFormTile * i + 32);
+                lds_barrier_dma_in_flight();
+                for (int c = threadIdx.x; c < KB / 2; c += 256) {
+                    T* x = reinterpret_cast<T*>(v) + c;
+                    if (!(fabsf(static_cast<float>(*x)) < INFINITY)) *x = static_cast<T>(0.f);
+                }
+                lds_barrier_dma_in_flight();
+            }
+        }
+        vec8 wt[PARTS][2][2];
+        w.template softmax<2>(s, wt, [&](int n, int r) __attribute__((always_inline)) { return vscale[i & 1][32 * n + 16 * w.half + r]; });
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int d = 0; d < F::ND; ++d) {
+                    const vec8 a = v_op(v, st, x, d);
+#pragma unroll
+                    for (int c = 0; c < PARTS; ++c) w.acc[d] = mfma32(a, wt[c][st][x], w.acc[d]);
+                }
+        if (E8) {
+            put(i + 1);
+            fetch(i + 2, phys);
+            phys = page(i + 3);
+        }
+    }
+    w.l = sum_xor32(w.l);
+    f32x4_t o[4 * F::ND];
+#pragma unroll
+    for (int i = 0; i < 4 * F::ND; ++i)
+        o[i] = f32x4_t{w.acc[i >> 2][4 * (i & 3)], w.acc[i >> 2][4 * (i & 3) + 1], w.acc[i >> 2][4 * (i & 3) + 2], w.acc[i >> 2][4 * (i & 3) + 3]};
+    w.store(p, it, split, 0, w.l, o);
+    w.store_ml(p, it, split, w.m, w.l);
+}
+
+template <int CT, int D, int PARTS, int SCORES> hipError_t form_launch(const FormsK& k, int kind, int units, hipStream_t s) {
+    if (kind == kFormStream) hipLaunchKernelGGL((forms_stream_kernel<CT, D, PARTS, SCORES>), dim3(units), dim3(256), 0, s, k);
+    else hipLaunchKernelGGL((forms_tile_kernel<CT, D, PARTS, SCORES>), dim3(units), dim3(256), 0, s, k);
+    return hipGetLastError();
+}
+template <int CT, int D, int PARTS> hipError_t form_launch_scores(const FormsK& k, int kind, int units, hipStream_t s) {
+    if (k.cap > 0.f) return form_launch<CT, D, PARTS, kScoresCap>(k, kind, units, s);
+    if (k.slopes) return form_launch<CT, D, PARTS, kScoresSlope>(k, kind, units, s);
+    return form_launch<CT, D, PARTS, kScoresPlain>(k, kind, units, s);
+}
+// Queries that the tile's type holds enter as one part, others as two of fp16 or three of bf16.
+template <int CT> hipError_t form_launch_type(const FormsK& k, int kind, int units, hipStream_t s) {
+    constexpr int OWN = CT == QR_DTYPE_F16 ? QR_DTYPE_F16 : QR_DTYPE_BF16, PARTS = CT == QR_DTYPE_F16 ? 2 : 3;
+    if (k.geom.head_dim == 128) return k.act == OWN ? form_launch_scores<CT, 128, 1>(k, kind, units, s) : form_launch_scores<CT, 128, PARTS>(k, kind, units, s);
+    return k.act == OWN ? form_launch_scores<CT, 64, 1>(k, kind, units, s) : form_launch_scores<CT, 64, PARTS>(k, kind, units, s);
+}
+
+}  // namespace qr
