@@ -260,17 +260,18 @@ struct FormTile {
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
 
-    // V's element at (slot t, dim d) of the page.
-    __device__ __forceinline__ float v_value(const FormsK& p, int phys, int kvh, int t, int d) const {
-        const long long at = p.geom.offset(phys, 1, kvh, t & (kPageTokens - 1), d);
-        if (E8) return quant_value<0>(static_cast<uint8_t>(p.pool[at]));
-        return static_cast<float>(*reinterpret_cast<const T*>(p.pool + 2 * at));
+    // V's element of slot t and dim d of a step of the page (8 bits: without its scale).
+    __device__ __forceinline__ static float v_value(const char* step, int t, int d) {
+        if (E8) return quant_value<0>(static_cast<uint8_t>(step[1024 * (d >> 5) + 16 * (32 * (t >> 4) + (d & 31)) + (t & 15)]));
+        return static_cast<float>(*reinterpret_cast<const T*>(step + 1024 * (d >> 4) + 16 * (16 * (t >> 3) + (d & 15)) + 2 * (t & 7)));
     }
     // A step that not every row sees whole may hold V elements that are not finite at slots some rows do not see, where 0 x inf
     // would reach them.  Adds them to the rows that see them as they are (no finite weight changes them); the caller clears
     // them in its operands.
     __device__ __forceinline__ void add_bad(const FormsK& p, const FormItem& it, int kvh, int t0) {
-        const int phys = form_page(p, it.pt_off, t0);
+        constexpr int ES = E8 ? 1 : 2;
+        const char* const step = p.pool + (static_cast<long long>(form_page(p, it.pt_off, t0)) * p.geom.page_elems() + p.geom.plane_elems() +
+                                           static_cast<long long>(kvh) * kPageTokens * D + (t0 & (kPageTokens - 1)) * D) * ES;
 #pragma unroll 1
         for (int k = 0; k < 32; ++k) {
             const bool sees = t0 + k >= lo && t0 + k <= hi;
@@ -278,9 +279,9 @@ struct FormTile {
             for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const float x = v_value(p, phys, kvh, t0 + k, 32 * d + 8 * (r >> 2) + 4 * half + (r & 3));
+                    const float x = v_value(step, k, 32 * d + 8 * (r >> 2) + 4 * half + (r & 3));
                     if (!(fabsf(x) < INFINITY) && sees) acc[d][r] += x;
-                    if ((r & 3) == 3) asm volatile("" ::: "memory");  // no registers for all reads at once
+                    if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // no registers for all reads at once
                 }
         }
     }
@@ -332,8 +333,9 @@ struct FormTile {
 };
 
 // ------------------------------------------------------------------ few rows: HBM-bound
-// Up to 32 rows; four waves take every fourth step of 32 slots, their operands straight from the page into registers, one step
-// ahead, and merge at the end.  No wave waits for another before that.
+// Up to 32 rows; four waves take every fourth step of 32 slots, their operands straight from the page into registers (K of the
+// next step while this one's softmax runs, V while the next one's scores are computed), and merge at the end.  No wave waits
+// for another before that.
 template <int CT, int D> struct FormStep {  // one step's operands
     using E = FormElem<CT>;
     static constexpr bool E8 = CT == QR_DTYPE_E4M3;
@@ -370,24 +372,25 @@ __global__ void __launch_bounds__(256, 2) forms_stream_kernel(const FormsK p) {
     // this lane's part of the operands of a step
     const int ko = E8 ? 16 * w.lane : 1024 * ax * (D / 32) + 16 * (16 * w.half + 4 * (2 * sx + hx) + bx);
     const int vo = E8 ? 16 * w.lane : 1024 * (m_ >> 4) + 16 * (16 * w.half + (w.lane & 15));
-    auto load = [&](FormStep<CT, D>& o, int st, int phys) __attribute__((always_inline)) {
+    FormStep<CT, D> o;
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    auto get = [](const char* a) __attribute__((always_inline)) {
+        const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a));
+        return make_uint4(x[0], x[1], x[2], x[3]);
+    };
+    auto load_k = [&](int st, int phys) __attribute__((always_inline)) {
         const char* page = p.pool + static_cast<long long>(phys) * page_bytes;
         const char* k = page + head_bytes + static_cast<long long>(st & 7) * 32 * D * ES;
-        const char* v = k + plane_bytes;
-        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-        auto get = [](const char* a) __attribute__((always_inline)) {
-            const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a));
-            return make_uint4(x[0], x[1], x[2], x[3]);
-        };
 #pragma unroll
         for (int i = 0; i < FormStep<CT, D>::N; ++i) o.k[i] = get(k + ko + (E8 ? 1024 : 512) * i);
-        if (E8) {
-            const char* sc = page + 2 * plane_bytes + kvh * kPageTokens + 32 * (st & 7);
-            o.ks = static_cast<uint8_t>(sc[16 * hx + 8 * sx + 4 * ax + bx]);
-            o.vs = *reinterpret_cast<const uint4*>(sc + kv * kPageTokens + 16 * w.half);
-        }
+        if (E8) o.ks = static_cast<uint8_t>(page[2 * plane_bytes + kvh * kPageTokens + 32 * (st & 7) + 16 * hx + 8 * sx + 4 * ax + bx]);
+    };
+    auto load_v = [&](int st, int phys) __attribute__((always_inline)) {
+        const char* page = p.pool + static_cast<long long>(phys) * page_bytes;
+        const char* v = page + plane_bytes + head_bytes + static_cast<long long>(st & 7) * 32 * D * ES;
 #pragma unroll
         for (int i = 0; i < FormStep<CT, D>::N; ++i) o.v[i] = get(v + vo + (E8 ? 1024 * i : 2048 * (i % F::ND) + 512 * (i / F::ND)));
+        if (E8) o.vs = *reinterpret_cast<const uint4*>(page + 2 * plane_bytes + (kv + kvh) * kPageTokens + 32 * (st & 7) + 16 * w.half);
     };
     auto page = [&](int st) __attribute__((always_inline)) { return st < s1 ? form_page(p, it.pt_off, 32 * st) : 0; };
     auto as8 = [](uint4 x) __attribute__((always_inline)) {
@@ -395,7 +398,15 @@ __global__ void __launch_bounds__(256, 2) forms_stream_kernel(const FormsK p) {
         __builtin_memcpy(&r, &x, 16);
         return r;
     };
-    auto compute = [&](FormStep<CT, D>& o, int st) __attribute__((always_inline)) {
+    int st = s0 + wave;
+    int phys = page(st);
+    if (st < s1) {
+        load_k(st, phys);
+        load_v(st, phys);
+    }
+    w.load_q(p);
+    for (; st < s1; st += 4) {
+        phys = page(st + 4);
         f32x16_t s[1];
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
@@ -412,6 +423,8 @@ __global__ void __launch_bounds__(256, 2) forms_stream_kernel(const FormsK p) {
 #pragma unroll
             for (int c = 0; c < PARTS; ++c) s[0] = mfma32(a, w.q[c][kk], s[0]);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if (st + 4 < s1) load_k(st + 4, phys);
         const bool edge = !range.all(32 * st, 32);
         w.form(p, s[0], 32 * st, edge);
         if (edge) {
@@ -455,20 +468,8 @@ __global__ void __launch_bounds__(256, 2) forms_stream_kernel(const FormsK p) {
 #pragma unroll
                 for (int c = 0; c < PARTS; ++c) w.acc[d] = mfma32(a, wt[c][0][x], w.acc[d]);
             }
-    };
-    FormStep<CT, D> a, b;
-    int st = s0 + wave;
-    int phys = page(st + 4);
-    if (st < s1) load(a, st, page(st));
-    w.load_q(p);
-    for (; st < s1; st += 8) {
-        if (st + 4 < s1) load(b, st + 4, phys);
-        phys = page(st + 8);
-        compute(a, st);
-        if (st + 4 >= s1) break;
-        if (st + 8 < s1) load(a, st + 8, phys);
-        phys = page(st + 12);
-        compute(b, st + 4);
+        __builtin_amdgcn_sched_barrier(0);
+        if (st + 4 < s1) load_v(st + 4, phys);
     }
     w.l = sum_xor32(w.l);
 
@@ -490,14 +491,14 @@ __global__ void __launch_bounds__(256, 2) forms_stream_kernel(const FormsK p) {
         L = fmaf(ml.y, c[x], L);
     }
     constexpr int NP = NG / 4;
-    f32x4_t o[NP];
+    f32x4_t out[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        out[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) o[i] += xa[(x * NG + wave * NP + i) * 64 + w.lane] * c[x];
+        for (int x = 0; x < 4; ++x) out[i] += xa[(x * NG + wave * NP + i) * 64 + w.lane] * c[x];
     }
-    w.store(p, it, split, wave * NP, L, o);
+    w.store(p, it, split, wave * NP, L, out);
     if (wave == 0) w.store_ml(p, it, split, M, L);
 }
 
