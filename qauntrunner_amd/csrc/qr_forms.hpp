@@ -13,7 +13,7 @@
 namespace qr {
 
 // Kernels of a launch.
-enum FormKind { kFormAny, kFormStream, kFormTiles, kFormKinds };
+enum FormKind { kFormAny, kFormStream, kFormTiles, kFormF32Half, kFormF32, kFormKinds };
 constexpr int kFormAnyRows = 8, kFormAnyTile = 32;
 
 // What the host knows of a chunk.
@@ -58,9 +58,11 @@ struct FormItem {
     int keys;                // slots
     int unit0, blocks, splits;
     int part0;               // part of a row that split 0 is
+    int kind;
 };
+constexpr int kFormItems = 2 * kBatch;  // of a launch: a prefix and the own keys for each chunk
 struct FormsK {
-    FormItem it[kBatch];
+    FormItem it[kFormItems];
     FormRows c[kBatch];
     int n;                   // items of this launch
     int chunks;
@@ -80,8 +82,7 @@ struct FormsK {
 
 // How a call's work is cut.
 struct FormsPlan {
-    FormItem it[2 * kBatch];
-    int kind[2 * kBatch];
+    FormItem it[kFormItems];
     int n;
     FormRows c[kBatch];
     size_t part_ml;          // offset in the workspace; the partials' sums come first
@@ -93,9 +94,19 @@ hipError_t launch_forms(const FormsArgs& a, const FormsPlan& plan, void* workspa
 
 hipError_t launch_forms_any(const FormsK& k, int units, hipStream_t s);
 // MFMA tiles (kinds kFormStream, kFormTiles): operand page layouts, whole groups.
-hipError_t launch_forms_f16(const FormsK& k, int kind, int units, hipStream_t s);
-hipError_t launch_forms_bf16(const FormsK& k, int kind, int units, hipStream_t s);
-hipError_t launch_forms_e4m3(const FormsK& k, int kind, int units, hipStream_t s);
+// fp32 tiles (kinds kFormF32Half, kFormF32): fp32 caches of head size 64 or 128, whole groups.
+hipError_t launch_forms_f32(const FormsK& k, int units, hipStream_t s);
+hipError_t launch_forms_f16(const FormsK& k, int units, hipStream_t s);
+hipError_t launch_forms_bf16(const FormsK& k, int units, hipStream_t s);
+hipError_t launch_forms_e4m3(const FormsK& k, int units, hipStream_t s);
+
+// Item of a unit.
+__device__ __forceinline__ int form_find(const FormsK& p, int unit) {
+    static_assert(kFormItems == 128, "two ballots");
+    const int lane = threadIdx.x & 63;
+    const bool a = lane < p.n && p.it[lane].unit0 <= unit, b = lane + 64 < p.n && p.it[lane + 64].unit0 <= unit;
+    return __builtin_amdgcn_readfirstlane(static_cast<int>(__popcll(__builtin_amdgcn_ballot_w64(a)) + __popcll(__builtin_amdgcn_ballot_w64(b))) - 1);
+}
 
 // Query heads h0 .. h0 + g - 1 read kv head kvh (head h reads h * kv_heads / heads).
 __device__ __forceinline__ void form_heads(const FormsK& p, int kvh, int* h0, int* g) {
@@ -132,5 +143,24 @@ __device__ __forceinline__ float form_score(float z, float cap, float slope, flo
     return slope != 0.f ? fmaf(-slope, fabsf(away), z) : z;
 }
 constexpr float kLog2e = 1.4426950408889634f;
+
+enum FormScores { kScoresPlain, kScoresSlope, kScoresCap };  // (capped scores may have a slope too)
+
+// Page of a slot, by a scalar load (no kernel writes the table while this one runs).
+__device__ __forceinline__ int form_page(const FormsK& p, int pt_off, int t) {
+    return reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p.page_table))[pt_off + (t >> kPageShift)];
+}
+
+// Slots that the rows of a block see: some row [lo, hi], every row [all_lo, all_hi].
+struct FormRange {
+    int lo, hi, all_lo, all_hi;
+    __device__ __forceinline__ bool all(int t, int n) const { return t >= all_lo && t + n - 1 <= all_hi; }
+};
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) x = min(x, __shfl_xor(x, i));
+    return x;
+}
+__device__ __forceinline__ int wave_max(int x) { return ~wave_min(~x); }
 
 }  // namespace qr

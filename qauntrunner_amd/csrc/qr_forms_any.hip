@@ -50,8 +50,7 @@ __global__ void __launch_bounds__(kThreads) forms_any_kernel(const FormsK p) {
     float* const tile = q + kRows * D;           // [32][D + 1]
     float* const prob = tile + kTile * (D + 1);  // [8][32]
     float* const corr = prob + kRows * kTile;    // [8]
-    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
-    const FormItem it = p.it[e];
+    const FormItem it = p.it[form_find(p, blockIdx.x)];
     const int u = blockIdx.x - it.unit0;
     const int split = u % it.splits, block = u / it.splits % it.blocks, kvh = u / (it.splits * it.blocks);
     int h0, g;

@@ -3,6 +3,6 @@
 
 namespace qr {
 
-hipError_t launch_forms_bf16(const FormsK& k, int kind, int units, hipStream_t s) { return form_launch_type<QR_DTYPE_BF16>(k, kind, units, s); }
+hipError_t launch_forms_bf16(const FormsK& k, int units, hipStream_t s) { return form_launch_type<QR_DTYPE_BF16>(k, units, s); }
 
 }  // namespace qr

@@ -46,8 +46,6 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
 __device__ __forceinline__ void mfma_done(f32x16_t (&s)[1]) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s[0])); }
 __device__ __forceinline__ void mfma_done(f32x16_t (&s)[2]) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1])); }
 
-enum FormScores { kScoresPlain, kScoresSlope, kScoresCap };  // (capped scores may have a slope too)
-
 template <int CT> struct FormElem {
     static constexpr bool BF16 = CT != QR_DTYPE_F16;
     using T = typename std::conditional<BF16, __bf16, _Float16>::type;
@@ -60,23 +58,6 @@ __device__ __forceinline__ bf16x8_t widen8(uint32_t lo, uint32_t hi, float scale
     const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
     return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-
-// Page of a slot, by a scalar load (no kernel writes the table while this one runs).
-__device__ __forceinline__ int form_page(const FormsK& p, int pt_off, int t) {
-    return reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p.page_table))[pt_off + (t >> kPageShift)];
-}
-
-// Slots that the rows of a block see: some row [lo, hi], every row [all_lo, all_hi].
-struct FormRange {
-    int lo, hi, all_lo, all_hi;
-    __device__ __forceinline__ bool all(int t, int n) const { return t >= all_lo && t + n - 1 <= all_hi; }
-};
-__device__ __forceinline__ int wave_min(int x) {
-#pragma unroll
-    for (int i = 1; i < 64; i <<= 1) x = min(x, __shfl_xor(x, i));
-    return x;
-}
-__device__ __forceinline__ int wave_max(int x) { return ~wave_min(~x); }
 
 // One wave's 32 rows.
 template <int CT, int D, int PARTS, int SCORES>
@@ -346,17 +327,15 @@ template <int CT, int D> struct FormStep {  // one step's operands
 };
 
 template <int CT, int D, int PARTS, int SCORES>
-__global__ void __launch_bounds__(256, 2) forms_stream_kernel(const FormsK p) {
+__device__ __forceinline__ void forms_stream(const FormsK& p, const FormItem& it, int u, char* lds, char* rest) {
     using F = FormTile<CT, D, PARTS, SCORES>;
     using vec8 = typename F::vec8;
     constexpr bool E8 = F::E8;
     constexpr int NG = D / 8;  // f32x4 groups of a row in a lane
     constexpr int ES = E8 ? 1 : 2;
-    __shared__ f32x4_t xa[4 * NG * 64];
-    __shared__ float2 xm[4 * 64];
-    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
-    const FormItem it = p.it[e];
-    const int u = blockIdx.x - it.unit0, kv = p.geom.kv_heads, g = p.heads / kv;
+    f32x4_t* const xa = reinterpret_cast<f32x4_t*>(lds);  // [4][NG][64]
+    float2* const xm = reinterpret_cast<float2*>(rest);   // [4][64]
+    const int kv = p.geom.kv_heads, g = p.heads / kv;
     const int kvh = u % kv, split = u / kv % it.splits, block = it.blocks - 1 - u / kv / it.splits;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     F w;
@@ -509,7 +488,7 @@ __global__ void __launch_bounds__(256, 2) forms_stream_kernel(const FormsK p) {
 constexpr int kFormTileRows = 128, kFormTile = 64;
 
 template <int CT, int D, int PARTS, int SCORES>
-__global__ void __launch_bounds__(256, 2) forms_tile_kernel(const FormsK p) {
+__device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, int u, char* lds, char* rest) {
     using F = FormTile<CT, D, PARTS, SCORES>;
     using vec8 = typename F::vec8;
     using T = typename F::T;
@@ -519,12 +498,10 @@ __global__ void __launch_bounds__(256, 2) forms_tile_kernel(const FormsK p) {
     constexpr int KB = 2 * SB;          // of a tile
     constexpr int PER = KB / 1024 / 4;  // DMA loads per wave for a tile of K (or V)
     constexpr int NP = 64 * D / 16 / 256;  // 8 bits: 16-byte pieces of K (or V) per thread
-    __shared__ __attribute__((aligned(1024))) char lds[4 * KB];  // two K tiles, two V tiles
-    __shared__ float vscale[2][64];
-    __shared__ int spans[4][4];
-    const int e = batch_find(p.n, blockIdx.x, [&](int i) { return p.it[i].unit0; });
-    const FormItem it = p.it[e];
-    const int u = blockIdx.x - it.unit0, kv = p.geom.kv_heads, g = p.heads / kv;
+    // lds: two K tiles, two V tiles
+    float(*const vscale)[64] = reinterpret_cast<float(*)[64]>(rest);            // [2][64]
+    int(*const spans)[4] = reinterpret_cast<int(*)[4]>(rest + 2 * 64 * 4);      // [4][4]
+    const int kv = p.geom.kv_heads, g = p.heads / kv;
     const int kvh = u % kv, split = u / kv % it.splits, block = it.blocks - 1 - u / kv / it.splits;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     F w;
@@ -698,21 +675,28 @@ __global__ void __launch_bounds__(256, 2) forms_tile_kernel(const FormsK p) {
     w.store_ml(p, it, split, w.m, w.l);
 }
 
-template <int CT, int D, int PARTS, int SCORES> hipError_t form_launch(const FormsK& k, int kind, int units, hipStream_t s) {
-    if (kind == kFormStream) hipLaunchKernelGGL((forms_stream_kernel<CT, D, PARTS, SCORES>), dim3(units), dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((forms_tile_kernel<CT, D, PARTS, SCORES>), dim3(units), dim3(256), 0, s, k);
+// Items of both sorts in one launch: what one leaves of HBM or the MFMAs the other takes (64 rows behind 8192 shared positions
+// and their own keys).
+template <int CT, int D, int PARTS, int SCORES>
+__global__ void __launch_bounds__(256, 2) forms_mfma_kernel(const FormsK p) {
+    __shared__ __attribute__((aligned(1024))) char lds[512 * D];
+    __shared__ __attribute__((aligned(16))) char rest[2048];
+    const FormItem it = p.it[form_find(p, blockIdx.x)];
+    const int u = blockIdx.x - it.unit0;
+    if (it.kind == kFormStream) forms_stream<CT, D, PARTS, SCORES>(p, it, u, lds, rest);
+    else forms_tile<CT, D, PARTS, SCORES>(p, it, u, lds, rest);
+}
+template <int CT, int D, int PARTS> hipError_t form_launch_scores(const FormsK& k, int units, hipStream_t s) {
+    if (k.cap > 0.f) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresCap>), dim3(units), dim3(256), 0, s, k);
+    else if (k.slopes) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresSlope>), dim3(units), dim3(256), 0, s, k);
+    else hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresPlain>), dim3(units), dim3(256), 0, s, k);
     return hipGetLastError();
 }
-template <int CT, int D, int PARTS> hipError_t form_launch_scores(const FormsK& k, int kind, int units, hipStream_t s) {
-    if (k.cap > 0.f) return form_launch<CT, D, PARTS, kScoresCap>(k, kind, units, s);
-    if (k.slopes) return form_launch<CT, D, PARTS, kScoresSlope>(k, kind, units, s);
-    return form_launch<CT, D, PARTS, kScoresPlain>(k, kind, units, s);
-}
 // Queries that the tile's type holds enter as one part, others as two of fp16 or three of bf16.
-template <int CT> hipError_t form_launch_type(const FormsK& k, int kind, int units, hipStream_t s) {
+template <int CT> hipError_t form_launch_type(const FormsK& k, int units, hipStream_t s) {
     constexpr int OWN = CT == QR_DTYPE_F16 ? QR_DTYPE_F16 : QR_DTYPE_BF16, PARTS = CT == QR_DTYPE_F16 ? 2 : 3;
-    if (k.geom.head_dim == 128) return k.act == OWN ? form_launch_scores<CT, 128, 1>(k, kind, units, s) : form_launch_scores<CT, 128, PARTS>(k, kind, units, s);
-    return k.act == OWN ? form_launch_scores<CT, 64, 1>(k, kind, units, s) : form_launch_scores<CT, 64, PARTS>(k, kind, units, s);
+    if (k.geom.head_dim == 128) return k.act == OWN ? form_launch_scores<CT, 128, 1>(k, units, s) : form_launch_scores<CT, 128, PARTS>(k, units, s);
+    return k.act == OWN ? form_launch_scores<CT, 64, 1>(k, units, s) : form_launch_scores<CT, 64, PARTS>(k, units, s);
 }
 
 }  // namespace qr
