@@ -23,6 +23,7 @@ __global__ void __launch_bounds__(kThreads) forms_merge_kernel(const FormsK p, i
     const int D = p.geom.head_dim, lane = threadIdx.x & 63;
     const long long slot = c.slot0 + (static_cast<long long>(row - c.row0) * p.heads + h) * c.parts;
     const long long to = (static_cast<long long>(row) * p.heads + h) * D;
+    if (p.part_ml[slot].y == kFormDone) return;  // one part wrote the output
     float M = -INFINITY;
     for (int x = lane; x < c.parts; x += 64) M = fmaxf(M, p.part_ml[slot + x].x);
 #pragma unroll
@@ -89,18 +90,31 @@ __global__ void __launch_bounds__(kThreads) forms_merge_kernel(const FormsK p, i
         if (lane + 64 * i < D) store_out(p.out, p.act, to + lane + 64 * i, L == 0.f ? 0.f : o[i] / L);
 }
 
+// Queries that the MFMA tiles take in one part.
+bool whole_queries(const FormsArgs& a) { return a.act == (a.dtype == QR_DTYPE_F16 ? QR_DTYPE_F16 : QR_DTYPE_BF16); }
+
+// What a unit of a kernel costs, in microseconds: a tile where as many units run as fit at once (`slots`), where half as many do,
+// and the unit's start and end.  Measured (D = 128, one part): 64 slots of 128 rows 2.4 and 1.4; a streamed step of 32 slots by
+// its bytes, 5 TB/s over all slots; fp32 steps of 16 slots as streamed ones for 16 rows, by their MFMAs for 32.
 struct Shape {
-    int rows, tile;  // (query, head) rows of a block, slots of a tile
-    int target;      // units that run at once
-    int least;       // tiles of a part, at least
+    int slots, least;   // tiles that a part has at least
+    float full, half, start;
 };
-Shape shape_of(int kind) {
+Shape shape_of(const FormsArgs& a, int kind) {
+    const float wide = a.geom.head_dim / 128.f;
     switch (kind) {
-        case kFormStream: return {32, 32, 512, 8};
-        case kFormTiles: return {128, 64, 512, 8};
-        case kFormF32Half: return {16, 16, 512, 8};
-        case kFormF32: return {32, 16, 512, 8};
-        default: return {kFormAnyRows, kFormAnyTile, 1024, 2};
+        case kFormStream: {
+            const float t = wide * (a.geom.scaled() ? 0.9f : 1.7f);
+            return {256, 16, 0.5f * t, 0.4f * t, 5.f};
+        }
+        case kFormTilesHalf:
+        case kFormTiles: {
+            const float t = wide * 2.f * (kind == kFormTilesHalf ? 0.5f : 1.f) * (!whole_queries(a) ? 2.2f : 1.f) * (a.cap > 0.f ? 1.35f : 1.f);
+            return {256, 4, t, t, 6.f};
+        }
+        case kFormF32Half: return {512, 8, wide * 1.7f, wide * 1.f, 5.f};
+        case kFormF32: return {512, 8, wide * 1.f, wide * 0.55f, 5.f};
+        default: return {1024, 2, 4.f, 2.f, 5.f};
     }
 }
 int kind_of(const FormsArgs& a, int rows) {
@@ -108,7 +122,7 @@ int kind_of(const FormsArgs& a, int rows) {
     if ((D != 64 && D != 128) || a.heads % a.geom.kv_heads) return kFormAny;
     const long long n = static_cast<long long>(rows) * (a.heads / a.geom.kv_heads);
     if (a.dtype == QR_DTYPE_F32) return n <= 16 ? kFormF32Half : kFormF32;
-    return n <= 32 ? kFormStream : kFormTiles;
+    return n <= 32 ? kFormStream : n <= 128 || !whole_queries(a) ? kFormTilesHalf : kFormTiles;
 }
 hipError_t launch(const FormsK& k, int units, hipStream_t s) {
     if (k.it[0].kind == kFormAny) return launch_forms_any(k, units, s);
@@ -117,12 +131,66 @@ hipError_t launch(const FormsK& k, int units, hipStream_t s) {
     return k.dtype == QR_DTYPE_BF16 ? launch_forms_bf16(k, units, s) : launch_forms_e4m3(k, units, s);
 }
 
-// Tiles of the slots that row j of an item sees.
-int tiles_of(const FormsPlan& p, const FormItem& it, int window, int j, int tile) {
-    int c = it.c0;
-    while (c + 1 < it.c0 + it.nc && p.c[c + 1].row0 <= it.row0 + j) ++c;
-    const FormSpan s = form_span(p.c[c], it.row0 + j, window, it.base, it.keys);
-    return s.lo > s.hi ? 0 : s.hi / tile - s.lo / tile + 1;
+// Blocks of an item, of which some stand for the others: their tiles.
+struct Sample {
+    int item, tiles;
+    float units;  // of this length, all kv heads
+};
+struct Cut {
+    int per;
+    float us;
+};
+// The cut with which the kernel's units and the partials' way through memory take least: all blocks whole, the fewest tiles of a part
+// with which the units run at once, or some between and beyond.
+int best_per(const FormsArgs& a, const FormsPlan& p, const Shape& s, int kind, const Sample* smp, int n) {
+    const int kv = a.geom.kv_heads, rows = form_rows(kind);
+    const float partial = (a.geom.head_dim * 4 + 8) * 0.5e-6f;  // written and read at 4 TB/s
+    int most = 1;
+    for (int i = 0; i < n; ++i) most = std::max(most, smp[i].tiles);
+    auto units = [&](int per) {
+        float u = 0.f;
+        for (int i = 0; i < n; ++i) u += smp[i].units * static_cast<float>((smp[i].tiles + per - 1) / per);
+        return u;
+    };
+    auto cost = [&](int per) {
+        float u = 0.f, work = 0.f, parts = 0.f;
+        for (int i = 0; i < n; ++i) {
+            const FormItem& it = p.it[smp[i].item];
+            const int c = (smp[i].tiles + per - 1) / per;
+            u += smp[i].units * c;
+            work += smp[i].units * smp[i].tiles;
+            const long long all = static_cast<long long>(it.rows) * (a.heads / kv);
+            if (c > 1 || p.c[it.c0].parts) parts += smp[i].units * c * static_cast<float>(std::min<long long>(rows, all));
+        }
+        const float at_once = std::min(1.f, std::max(0.f, 2.f * u / s.slots - 1.f));
+        const float run = u <= s.slots ? std::min(per, most) * (s.half + (s.full - s.half) * at_once) : work * s.full / s.slots + 0.5f * std::min(per, most) * s.half;
+        return run + s.start * std::max(1.f, u / s.slots) + parts * partial + (parts > 0.f ? 4.f : 0.f);
+    };
+    int fit = std::min(most, s.least), hi = most;
+    while (fit < hi) {
+        const int mid = fit + (hi - fit) / 2;
+        if (units(mid) <= s.slots) hi = mid;
+        else fit = mid + 1;
+    }
+    Cut best = {most, cost(most)};
+    auto consider = [&](int per) {
+        if (per < std::min(most, s.least) || per >= most) return;
+        const float us = cost(per);
+        if (us < best.us) best = {per, us};
+    };
+    consider(fit);
+    for (const int k : {2, 3, 4, 6, 8, 12, 16}) consider((most + k - 1) / k);
+    // (the partials of a launch stay below 256 MB: 64 bf16 sequences of 8 rows behind 65536 positions)
+    for (;; best.per += (best.per + 3) / 4) {
+        double bytes = 0;
+        for (int i = 0; i < p.n; ++i) {
+            int len = 0;
+            for (int x = 0; x < n; ++x)
+                if (smp[x].item == i) len = std::max(len, smp[x].tiles);
+            if (len > best.per) bytes += (a.geom.head_dim * 4.0 + 8) * p.it[i].rows * a.heads * ((len + best.per - 1) / best.per);
+        }
+        if (bytes <= (256 << 20)) return best.per;
+    }
 }
 
 }  // namespace
@@ -163,43 +231,45 @@ FormsPlan plan_forms(const FormsArgs& a) {
         const FormChunk& c = a.c[i];
         add(c.pt_off, i, 1, c.rows, c.pre_len, std::max(c.pos0 + c.rows, c.full - c.pre_len));
     }
-    // tiles of a part: the fewest with which the units still run at once, or the partials stay below 256 MB
-    struct Cost {
-        long long blocks;
-        int avg, most;
-    } cost[kFormItems];
-    for (int i = 0; i < p.n; ++i) {
-        FormItem& it = p.it[i];
-        const Shape s = shape_of(p.it[i].kind);
-        it.blocks = static_cast<int>((static_cast<long long>(it.rows) * g + s.rows - 1) / s.rows);
-        const int x = tiles_of(p, it, a.window, 0, s.tile), y = tiles_of(p, it, a.window, it.rows - 1, s.tile);
-        int most = std::max(x, y);
-        for (int c = 1; c < it.nc; ++c) most = std::max(most, tiles_of(p, it, a.window, p.c[it.c0 + c].row0 - it.row0, s.tile));
-        cost[i] = {static_cast<long long>(it.blocks) * kv, std::max(1, (x + y + 1) / 2), std::max(1, most)};
-    }
-    const long long partial = static_cast<long long>(a.geom.head_dim) * 4 + 8;
+    for (int i = 0; i < p.n; ++i)  // lists of each row, for now
+        for (int c = 0; c < p.it[i].nc; ++c) ++p.c[p.it[i].c0 + c].parts;
+    for (int i = 0; i < a.n; ++i) --p.c[i].parts;
+    constexpr int kSamples = 8;
+    Sample smp[kFormItems * kSamples];
     for (int kind = 0; kind < kFormKinds; ++kind) {
-        const Shape s = shape_of(kind);
-        int lo = s.least, hi = s.least;
-        for (int i = 0; i < p.n; ++i)
-            if (p.it[i].kind == kind) hi = std::max(hi, cost[i].most);
-        auto fits = [&](int per) {
-            long long units = 0, bytes = 0;
-            for (int i = 0; i < p.n; ++i)
-                if (p.it[i].kind == kind) {
-                    units += cost[i].blocks * ((cost[i].avg + per - 1) / per);
-                    bytes += partial * p.it[i].rows * a.heads * ((cost[i].avg + per - 1) / per);
+        int n = 0;
+        for (int i = 0; i < p.n; ++i) {
+            FormItem& it = p.it[i];
+            if (it.kind != kind) continue;
+            it.blocks = static_cast<int>((static_cast<long long>(it.rows) * g + form_rows(kind) - 1) / form_rows(kind));
+            it.per = 1;
+            it.splits = 0x7FFFFFFF;
+            if (it.nc > 1) {  // (rows of many chunks: whatever one of them sees of the prefix)
+                int tiles = 1;
+                for (int c = 0; c < it.nc; ++c) {
+                    const FormRows& r = p.c[it.c0 + c];
+                    const FormSpan x = form_span(r, r.row0, a.window, it.base, it.keys);
+                    if (x.lo <= x.hi) tiles = std::max(tiles, x.hi / form_tile(kind) - x.lo / form_tile(kind) + 1);
                 }
-            return units <= s.target && bytes <= (256LL << 20);
-        };
-        while (lo < hi) {
-            const int mid = lo + (hi - lo) / 2;
-            if (fits(mid)) hi = mid;
-            else lo = mid + 1;
+                smp[n++] = {i, tiles, static_cast<float>(it.blocks) * kv};
+                continue;
+            }
+            const int m = std::min(it.blocks, kSamples);
+            for (int x = 0; x < m; ++x) {
+                const int b = m == 1 ? 0 : static_cast<int>(static_cast<long long>(it.blocks - 1) * x / (m - 1));
+                smp[n++] = {i, form_parts(it, p.c[it.c0], a.window, g, form_rows(kind), form_tile(kind), b), static_cast<float>(it.blocks) * kv / m};
+            }
         }
-        for (int i = 0; i < p.n; ++i)
-            if (p.it[i].kind == kind) p.it[i].splits = (cost[i].avg + lo - 1) / lo;
+        if (!n) continue;
+        const int per = best_per(a, p, shape_of(a, kind), kind, smp, n);
+        for (int x = 0; x < n; ++x) {
+            FormItem& it = p.it[smp[x].item];
+            if (x == 0 || smp[x - 1].item != smp[x].item) it.splits = 1;
+            it.splits = std::max(it.splits, (smp[x].tiles + per - 1) / per);
+            it.per = it.nc == 1 ? per : 0;
+        }
     }
+    for (int i = 0; i < a.n; ++i) p.c[i].parts = 0;
     for (int i = 0; i < p.n; ++i) {
         FormItem& it = p.it[i];
         it.part0 = p.c[it.c0].parts;  // the chunks of an item have had the same lists before it
@@ -235,13 +305,19 @@ hipError_t launch_forms(const FormsArgs& a, const FormsPlan& plan, void* workspa
     k.window = a.window;
     k.part_acc = static_cast<float*>(workspace);
     k.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + plan.part_ml);
+    const int g = (a.heads + a.geom.kv_heads - 1) / a.geom.kv_heads;
     int units = 0;
     for (int pass = 0; pass < 2; ++pass)  // the items of many rows first: theirs are the longest units
         for (int i = 0; i < plan.n; ++i) {
-            if ((plan.it[i].kind == kFormTiles || plan.it[i].kind == kFormF32) != (pass == 0)) continue;
+            if ((plan.it[i].kind != kFormStream && plan.it[i].kind != kFormF32Half) != (pass == 0)) continue;
             FormItem& it = k.it[k.n++] = plan.it[i];
             it.unit0 = units;
-            units += it.blocks * it.splits * a.geom.kv_heads;
+            int n = it.blocks * it.splits;
+            if (it.per && it.splits > 1) {
+                n = 0;
+                for (int b = 0; b < it.blocks; ++b) n += form_parts(it, k.c[it.c0], a.window, g, form_rows(it.kind), form_tile(it.kind), b);
+            }
+            units += n * a.geom.kv_heads;
         }
     const hipError_t e = launch(k, units, stream);
     if (e != hipSuccess) return e;

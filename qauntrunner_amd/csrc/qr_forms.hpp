@@ -13,7 +13,7 @@
 namespace qr {
 
 // Kernels of a launch.
-enum FormKind { kFormAny, kFormStream, kFormTiles, kFormF32Half, kFormF32, kFormKinds };
+enum FormKind { kFormAny, kFormStream, kFormTilesHalf, kFormTiles, kFormF32Half, kFormF32, kFormKinds };
 constexpr int kFormAnyRows = 8, kFormAnyTile = 32;
 
 // What the host knows of a chunk.
@@ -56,8 +56,10 @@ struct FormItem {
     int row0, rows;
     int base;                // position of slot 0
     int keys;                // slots
-    int unit0, blocks, splits;
-    int part0;               // part of a row that split 0 is
+    int unit0, blocks;
+    int splits;              // parts of the block that has the most
+    int per;                 // tiles of a part, up to; 0: every block has `splits` parts
+    int part0;               // part of a row that a block's first one is
     int kind;
 };
 constexpr int kFormItems = 2 * kBatch;  // of a launch: a prefix and the own keys for each chunk
@@ -100,6 +102,69 @@ hipError_t launch_forms_f16(const FormsK& k, int units, hipStream_t s);
 hipError_t launch_forms_bf16(const FormsK& k, int units, hipStream_t s);
 hipError_t launch_forms_e4m3(const FormsK& k, int units, hipStream_t s);
 
+// (query, head) rows of a block and slots of a tile of each kernel.
+__host__ __device__ constexpr int form_rows(int kind) {
+    return kind == kFormAny ? kFormAnyRows : kind == kFormTiles ? 256 : kind == kFormTilesHalf ? 128 : kind == kFormF32Half ? 16 : 32;
+}
+__host__ __device__ constexpr int form_tile(int kind) {
+    return kind == kFormTiles || kind == kFormTilesHalf ? 64 : kind == kFormF32Half || kind == kFormF32 ? 16 : 32;
+}
+
+// Row `row` of a chunk: its position, and the slots lo .. hi of `keys` slots from position `base` on that it sees (lo > hi: none).
+struct FormSpan {
+    int chunk;
+    int pos;
+    int lo, hi;
+};
+__host__ __device__ inline FormSpan form_span(const FormRows& r, int row, int window, int base, int keys) {
+    const int pos = r.p0 + row - r.row0;
+    const int from = window && pos - window + 1 > r.first ? pos - window + 1 : r.first;
+    const int to = pos > r.full - 1 ? pos : r.full - 1;
+    const int lo = from > base ? from - base : 0, hi = to - base < keys - 1 ? to - base : keys - 1;
+    return {0, pos, lo, hi};
+}
+// Parts of a block's keys (of an item of one chunk, g query heads per kv head): what the last and first of its rows see, a rule that
+// the host's count of units and the kernels share.
+__host__ __device__ inline int form_parts(const FormItem& it, const FormRows& r, int window, int g, int rows, int tile, int block) {
+    if (!it.per) return it.splits;
+    const int end = (block + 1) * rows < it.rows * g ? (block + 1) * rows : it.rows * g;
+    const FormSpan a = form_span(r, it.row0 + block * rows / g, window, it.base, it.keys);
+    const FormSpan b = form_span(r, it.row0 + (end - 1) / g, window, it.base, it.keys);
+    const int lo = a.lo < b.lo ? a.lo : b.lo, hi = a.hi > b.hi ? a.hi : b.hi;
+    const int n = hi < lo ? 1 : (hi / tile - lo / tile + it.per) / it.per;
+    return n < it.splits ? n : it.splits;
+}
+
+// A unit of an item: kv heads fastest (an XCD keeps few of them in its L2), from the last block, which sees the most keys, down.
+struct FormUnit {
+    int kvh, block, part, parts;
+};
+__device__ __forceinline__ FormUnit form_unit(const FormsK& p, const FormItem& it, int g, int rows, int tile, int unit) {
+    const int kv = p.geom.kv_heads, kvh = unit % kv;
+    int u = unit / kv;
+    if (!it.per || it.splits == 1) {
+        const int b = u / it.splits;
+        return {kvh, it.blocks - 1 - b, u - b * it.splits, it.splits};
+    }
+    const FormRows r = p.c[it.c0];
+    const int lane = threadIdx.x & 63;
+    for (int b0 = it.blocks - 1;; b0 -= 64) {  // 64 blocks at a time, a running sum of their parts over the lanes
+        const int n = b0 - lane >= 0 ? form_parts(it, r, p.window, g, rows, tile, b0 - lane) : 0;
+        int sum = n;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            const int o = __shfl_up(sum, x);
+            sum += lane >= x ? o : 0;
+        }
+        const int all = __builtin_amdgcn_readfirstlane(__shfl(sum, 63));
+        if (u < all || b0 < 64) {
+            const int l = __builtin_amdgcn_readfirstlane(static_cast<int>(__popcll(__builtin_amdgcn_ballot_w64(sum <= u))));
+            return {kvh, b0 - l, __builtin_amdgcn_readfirstlane(u - __shfl(sum - n, l)), __builtin_amdgcn_readfirstlane(__shfl(n, l))};
+        }
+        u -= all;
+    }
+}
+
 // Item of a unit.
 __device__ __forceinline__ int form_find(const FormsK& p, int unit) {
     static_assert(kFormItems == 128, "two ballots");
@@ -115,19 +180,7 @@ __device__ __forceinline__ void form_heads(const FormsK& p, int kvh, int* h0, in
     *g = ((kvh + 1) * p.heads + kv - 1) / kv - *h0;
 }
 
-// Row j of an item: its position, and the slots lo .. hi of the item's keys that it sees (lo > hi: none).
-struct FormSpan {
-    int chunk;
-    int pos;
-    int lo, hi;
-};
-__host__ __device__ inline FormSpan form_span(const FormRows& r, int row, int window, int base, int keys) {
-    const int pos = r.p0 + row - r.row0;
-    const int from = window ? (pos - window + 1 > r.first ? pos - window + 1 : r.first) : r.first;
-    const int to = pos > r.full - 1 ? pos : r.full - 1;
-    const int lo = from > base ? from - base : 0, hi = to - base < keys - 1 ? to - base : keys - 1;
-    return {0, pos, lo, hi};
-}
+// Row j of an item.
 __device__ __forceinline__ FormSpan form_row(const FormsK& p, const FormItem& it, int j) {
     const int row = it.row0 + j;
     int c = it.c0;
@@ -135,6 +188,18 @@ __device__ __forceinline__ FormSpan form_row(const FormsK& p, const FormItem& it
     FormSpan s = form_span(p.c[c], row, p.window, it.base, it.keys);
     s.chunk = c;
     return s;
+}
+
+// A block of one part whose rows have no other list needs no partials: it writes the output, and marks the rows' first partial.
+__device__ __forceinline__ bool form_whole(const FormRows& c, const FormItem& it, int parts) { return parts == 1 && c.parts == it.splits; }
+constexpr float kFormDone = -1.f;  // a sum that no part has
+
+// (m, l) of a row's part; the last of a block's parts fills those that its rows have and it has not.
+__device__ __forceinline__ void form_store_ml(const FormsK& p, const FormRows& c, const FormItem& it, long long slot, const FormUnit& u, float m, float l) {
+    if (c.parts == 1) return;
+    p.part_ml[slot] = form_whole(c, it, u.parts) ? make_float2(0.f, kFormDone) : make_float2(m, l);
+    if (u.part == u.parts - 1)
+        for (int x = u.parts; x < it.splits; ++x) p.part_ml[slot + x - u.part] = make_float2(-INFINITY, 0.f);
 }
 
 // A score in log2 units capped and less its slope: cap tanh(z / cap) = cap (1 - 2 / (e^(2 z / cap) + 1)).

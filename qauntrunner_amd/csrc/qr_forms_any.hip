@@ -52,10 +52,11 @@ __global__ void __launch_bounds__(kThreads) forms_any_kernel(const FormsK p) {
     float* const corr = prob + kRows * kTile;    // [8]
     const FormItem it = p.it[form_find(p, blockIdx.x)];
     const int u = blockIdx.x - it.unit0;
-    const int split = u % it.splits, block = u / it.splits % it.blocks, kvh = u / (it.splits * it.blocks);
+    const FormUnit un = form_unit(p, it, (p.heads + p.geom.kv_heads - 1) / p.geom.kv_heads, kRows, kTile, u);
+    const int split = un.part, kvh = un.kvh;
     int h0, g;
     form_heads(p, kvh, &h0, &g);
-    const int rho0 = block * kRows;
+    const int rho0 = un.block * kRows;
     if (rho0 >= it.rows * g) return;
     const int rho1 = min(rho0 + kRows, it.rows * g);
     if (threadIdx.x < kRows) {
@@ -79,8 +80,8 @@ __global__ void __launch_bounds__(kThreads) forms_any_kernel(const FormsK p) {
             last = max(last, hi[i]);
         }
     const int tile0 = first / kTile, tiles = last < first ? 0 : last / kTile - tile0 + 1;
-    const int t0 = (tile0 + static_cast<int>(static_cast<long long>(tiles) * split / it.splits)) * kTile;
-    const int t1 = (tile0 + static_cast<int>(static_cast<long long>(tiles) * (split + 1) / it.splits)) * kTile;
+    const int t0 = (tile0 + static_cast<int>(static_cast<long long>(tiles) * split / un.parts)) * kTile;
+    const int t1 = (tile0 + static_cast<int>(static_cast<long long>(tiles) * (split + 1) / un.parts)) * kTile;
 
     const int r = threadIdx.x >> 5, tl = threadIdx.x & 31;  // this thread's score
     const float slope = p.slopes ? p.slopes[h0 + min(rho0 + r, rho1 - 1) % g] * kLog2e : 0.f;
@@ -144,10 +145,10 @@ __global__ void __launch_bounds__(kThreads) forms_any_kernel(const FormsK p) {
         for (int c2 = 0; c2 < NC; ++c2) {
             const int d = threadIdx.x + kThreads * c2;
             if (d >= D) continue;
-            if (c.parts == 1) store_out(p.out, p.act, (static_cast<long long>(row) * p.heads + h0 + rho % g) * D + d, li == 0.f ? 0.f : acc[i][c2] / li);
+            if (form_whole(c, it, un.parts)) store_out(p.out, p.act, (static_cast<long long>(row) * p.heads + h0 + rho % g) * D + d, li == 0.f ? 0.f : acc[i][c2] / li);
             else p.part_acc[slot * D + d] = acc[i][c2];
         }
-        if (threadIdx.x == 0 && c.parts > 1) p.part_ml[slot] = make_float2(mi, li);
+        if (threadIdx.x == 0) form_store_ml(p, c, it, slot, un, mi, li);
     }
 }
 

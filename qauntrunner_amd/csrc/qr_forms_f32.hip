@@ -25,7 +25,9 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
     constexpr int NK = D / 16, NJ = D / 64, NG = D / 16;  // NG: f32x4 groups of a row tile in a lane
     // xa: [4][RT][NG][64], xm: [4][RT][64]
     const int kv = p.geom.kv_heads, g = p.heads / kv;
-    const int kvh = u % kv, split = u / kv % it.splits, block = it.blocks - 1 - u / kv / it.splits;
+    const FormUnit un = form_unit(p, it, g, 16 * RT, form_tile(kFormF32), u);
+    static_assert(form_tile(kFormF32) == 16 && form_rows(kFormF32) == 32 && form_rows(kFormF32Half) == 16, "steps and row tiles");
+    const int kvh = un.kvh, split = un.part, block = un.block;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, Q = lane >> 4;
     int row[RT], head[RT], lo[RT], hi[RT], chunk[RT];
     bool on[RT];
@@ -57,8 +59,8 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
     range = {__builtin_amdgcn_readfirstlane(wave_min(range.lo)), __builtin_amdgcn_readfirstlane(wave_max(range.hi)),
              __builtin_amdgcn_readfirstlane(wave_max(range.all_lo)), __builtin_amdgcn_readfirstlane(wave_min(range.all_hi))};
     const int step0 = range.lo >> 4, steps = range.lo > range.hi ? 0 : (range.hi >> 4) - step0 + 1;
-    const int s0 = step0 + static_cast<int>(static_cast<long long>(steps) * split / it.splits);
-    const int s1 = step0 + static_cast<int>(static_cast<long long>(steps) * (split + 1) / it.splits);
+    const int s0 = __builtin_amdgcn_readfirstlane(step0 + static_cast<int>(static_cast<long long>(steps) * split / un.parts));
+    const int s1 = __builtin_amdgcn_readfirstlane(step0 + static_cast<int>(static_cast<long long>(steps) * (split + 1) / un.parts));
 
     const long long page_elems = p.geom.page_elems(), plane = p.geom.plane_elems();
     const float* const pool = reinterpret_cast<const float*>(p.pool) + static_cast<long long>(kvh) * kPageTokens * D;
@@ -213,8 +215,8 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
         }
         if (!on[t]) continue;
         const FormRows& ch = p.c[chunk[t]];
-        const int parts = ch.parts;
-        const long long slot = ch.slot0 + (static_cast<long long>(row[t] - ch.row0) * p.heads + head[t]) * parts + it.part0 + split;
+        const bool whole = form_whole(ch, it, un.parts);
+        const long long slot = ch.slot0 + (static_cast<long long>(row[t] - ch.row0) * p.heads + head[t]) * ch.parts + it.part0 + split;
         const float inv = L == 0.f ? 0.f : 1.f / L;
         const long long at = (static_cast<long long>(row[t]) * p.heads + head[t]) * D;
 #pragma unroll
@@ -223,7 +225,7 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
             f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int y = 0; y < 4; ++y) o += xa[((y * RT + t) * NG + i) * 64 + lane] * c[y];
-            if (parts > 1) {
+            if (!whole) {
                 *reinterpret_cast<f32x4_t*>(p.part_acc + slot * D + d) = o;
             } else {
                 o *= inv;
@@ -237,7 +239,7 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
                 }
             }
         }
-        if (parts > 1 && wave == 0 && Q == 0) p.part_ml[slot] = make_float2(M, L);
+        if (wave == 0 && Q == 0) form_store_ml(p, ch, it, slot, un, M, L);
     }
 }
 

@@ -59,6 +59,27 @@ __device__ __forceinline__ bf16x8_t widen8(uint32_t lo, uint32_t hi, float scale
     return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// Copies into LDS by buffer loads, 16 or 4 bytes per lane to `to` + 16 (4) lane; past the source's bytes zeros.  As asm: behind a
+// load that the compiler knows to write LDS it waits for memory before the next read of LDS, whichever bytes that reads, and
+// the tiles ahead would be awaited in every turn (three quarters of the time of a tile).  Nothing is written to registers;
+// wait_vmcnt and a barrier stand between a copy and the reads of its bytes.  (s_nop: a scalar that a vector instruction wrote is
+// read by a buffer load five wait states later at the earliest.  Nothing else here uses m0.)
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x4_t dma_source(const char* base, int bytes) {
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    return u32x4_t{static_cast<uint32_t>(b), static_cast<uint32_t>(b >> 32) & 0xFFFFu, static_cast<uint32_t>(bytes), kBufferFlags};
+}
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+    return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p)));
+}
+__device__ __forceinline__ void dma16(u32x4_t source, const char* to, uint32_t at, uint32_t from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 : : "s"(lds_address(to)), "v"(at), "s"(source), "s"(from) : "memory");
+}
+__device__ __forceinline__ void dma4(u32x4_t source, const char* to, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(lds_address(to)), "v"(at), "s"(source) : "memory");
+}
+
 // One wave's 32 rows.
 template <int CT, int D, int PARTS, int SCORES>
 struct FormTile {
@@ -188,9 +209,9 @@ struct FormTile {
         }
     }
 
-    // Weights of NS steps' scores, as PV operands (8 bits: times V's scales); rescales what was summed when the maximum moves.
-    template <int NS, class F>
-    __device__ __forceinline__ void softmax(f32x16_t (&s)[NS], vec8 (&w)[PARTS][NS][2], F vscale) {
+    // The row's maximum with NS steps' scores; what was summed so far has to be weighed by the result.
+    template <int NS>
+    __device__ __forceinline__ float raise(f32x16_t (&s)[NS]) {
         mfma_done(s);
         float mx[2 * NS];
 #pragma unroll
@@ -206,23 +227,26 @@ struct FormTile {
         for (int n = 1; n < 2 * NS; ++n) t = fmaxf(t, mx[n]);
         t = max_xor32(t);
         const float by = SCORES == kScoresPlain ? sscale : 1.f;
-        const bool grow = fmaf(t, by, -m) > kTop;
-        if (__builtin_amdgcn_ballot_w64(grow)) {
-            float mn = fmaf(t, by, kHead - kTop);
-            if (fmaf(t, by, -mn) > kTop) {  // rounded down, where a step of m is that large
-                const int b = __float_as_int(mn);
-                mn = __int_as_float(b < 0 ? b - 1 : b + 1);
-            }
-            mn = grow ? mn : m;
-            const float c = m == -INFINITY ? 0.f : fast_exp2(m - mn);
-            if (__builtin_amdgcn_ballot_w64(grow && m != -INFINITY)) {
-                const float cc = grow && m != -INFINITY ? c : 1.f;
-                l *= cc;
-#pragma unroll
-                for (int d = 0; d < ND; ++d) acc[d] *= cc;
-            }
-            m = mn;
+        if (!(fmaf(t, by, -m) > kTop)) return 1.f;
+        float mn = fmaf(t, by, kHead - kTop);
+        if (fmaf(t, by, -mn) > kTop) {  // rounded down, where a step of m is that large
+            const int b = __float_as_int(mn);
+            mn = __int_as_float(b < 0 ? b - 1 : b + 1);
         }
+        const float c = m == -INFINITY ? 1.f : fast_exp2(m - mn);  // (nothing was summed yet)
+        m = mn;
+        return c;
+    }
+    __device__ __forceinline__ void rescale(float c) {
+        if (__builtin_amdgcn_ballot_w64(c != 1.f)) {
+            l *= c;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) acc[d] *= c;
+        }
+    }
+    // Weights of NS steps' scores, as PV operands (8 bits: times V's scales); their sum.
+    template <int NS, class F>
+    __device__ __forceinline__ float weigh(const f32x16_t (&s)[NS], vec8 (&w)[PARTS][NS][2], F vscale) const {
         const float ref = m == -INFINITY ? 0.f : -m;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -238,7 +262,12 @@ struct FormTile {
                     v -= static_cast<float>(w[c][n][r >> 3][r & 7]);
                 }
             }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
+    template <int NS, class F>
+    __device__ __forceinline__ void softmax(f32x16_t (&s)[NS], vec8 (&w)[PARTS][NS][2], F vscale) {
+        rescale(raise(s));
+        l += weigh(s, w, vscale);
     }
 
     // V's element of slot t and dim d of a step of the page (8 bits: without its scale).
@@ -274,11 +303,11 @@ struct FormTile {
         return c.slot0 + (static_cast<long long>(row - c.row0) * p.heads + head) * c.parts + it.part0 + split;
     }
     template <int N>
-    __device__ __forceinline__ void store(const FormsK& p, const FormItem& it, int split, int g0, float lsum, const f32x4_t (&a)[N]) const {
+    __device__ __forceinline__ void store(const FormsK& p, const FormItem& it, const FormUnit& u, int g0, float lsum, const f32x4_t (&a)[N]) const {
         if (!on) return;
         auto dim = [&](int i) { return 32 * ((g0 + i) >> 2) + 8 * ((g0 + i) & 3) + 4 * half; };
-        if (p.c[chunk].parts > 1) {
-            float* o = p.part_acc + slot(p, it, split) * D;
+        if (!form_whole(p.c[chunk], it, u.parts)) {
+            float* o = p.part_acc + slot(p, it, u.part) * D;
 #pragma unroll
             for (int i = 0; i < N; ++i) *reinterpret_cast<f32x4_t*>(o + dim(i)) = a[i];
             return;
@@ -308,13 +337,55 @@ struct FormTile {
             __builtin_memcpy(o + dim(i), b, 8);
         }
     }
-    __device__ __forceinline__ void store_ml(const FormsK& p, const FormItem& it, int split, float mm, float lsum) const {
-        if (on && !half && p.c[chunk].parts > 1) p.part_ml[slot(p, it, split)] = make_float2(mm, lsum);
+    __device__ __forceinline__ void store_ml(const FormsK& p, const FormItem& it, const FormUnit& u, float mm, float lsum) const {
+        if (on && !half) form_store_ml(p, p.c[chunk], it, slot(p, it, u.part), u, mm, lsum);
     }
 };
 
+// The PW waves of a row group merge: each adds up its share of the dim groups.  (Afterwards lds and rest may be used again only behind
+// a barrier.)
+template <class F, int RW, int PW>
+__device__ __forceinline__ void merge_waves(const FormsK& p, const FormItem& it, const FormUnit& un, F& w, int rw, int pw, char* lds, char* rest) {
+    constexpr int NG = 4 * F::ND, NP = NG / PW;  // f32x4 groups of a row in a lane; of them a wave's
+    f32x4_t out[NP];
+    float M = w.m, L = w.l;
+    if constexpr (PW == 1) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) out[i] = f32x4_t{w.acc[i >> 2][4 * (i & 3)], w.acc[i >> 2][4 * (i & 3) + 1], w.acc[i >> 2][4 * (i & 3) + 2], w.acc[i >> 2][4 * (i & 3) + 3]};
+    } else {
+        f32x4_t* const xa = reinterpret_cast<f32x4_t*>(lds);  // [row group][wave][NG][64]
+        float2* const xm = reinterpret_cast<float2*>(rest);   // [row group][wave][64]
+        wait_dma();
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+            xa[((rw * PW + pw) * NG + i) * 64 + w.lane] = f32x4_t{w.acc[i >> 2][4 * (i & 3)], w.acc[i >> 2][4 * (i & 3) + 1], w.acc[i >> 2][4 * (i & 3) + 2], w.acc[i >> 2][4 * (i & 3) + 3]};
+        xm[(rw * PW + pw) * 64 + w.lane] = make_float2(w.m, w.l);
+        __syncthreads();
+        float c[PW];
+        M = -INFINITY;
+        L = 0.f;
+#pragma unroll
+        for (int x = 0; x < PW; ++x) M = fmaxf(M, xm[(rw * PW + x) * 64 + w.lane].x);
+#pragma unroll
+        for (int x = 0; x < PW; ++x) {
+            const float2 ml = xm[(rw * PW + x) * 64 + w.lane];
+            c[x] = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - M);
+            L = fmaf(ml.y, c[x], L);
+        }
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            out[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < PW; ++x) out[i] += xa[((rw * PW + x) * NG + pw * NP + i) * 64 + w.lane] * c[x];
+        }
+    }
+    w.store(p, it, un, pw * NP, L, out);
+    if (pw == 0) w.store_ml(p, it, un, M, L);
+}
+
 // ------------------------------------------------------------------ few rows: HBM-bound
-// Up to 32 rows; four waves take every fourth step of 32 slots, their operands straight from the page into registers (K of the
+// Up to 32 rows; eight waves take every eighth step of 32 slots, their operands straight from the page into registers (K of the
 // next step while this one's softmax runs, V while the next one's scores are computed), and merge at the end.  No wave waits
 // for another before that.
 template <int CT, int D> struct FormStep {  // one step's operands
@@ -331,19 +402,19 @@ __device__ __forceinline__ void forms_stream(const FormsK& p, const FormItem& it
     using F = FormTile<CT, D, PARTS, SCORES>;
     using vec8 = typename F::vec8;
     constexpr bool E8 = F::E8;
-    constexpr int NG = D / 8;  // f32x4 groups of a row in a lane
+    constexpr int ROWS = form_rows(kFormStream), TILE = form_tile(kFormStream);
+    static_assert(ROWS == 32 && TILE == 32, "a wave's rows and steps");
     constexpr int ES = E8 ? 1 : 2;
-    f32x4_t* const xa = reinterpret_cast<f32x4_t*>(lds);  // [4][NG][64]
-    float2* const xm = reinterpret_cast<float2*>(rest);   // [4][64]
     const int kv = p.geom.kv_heads, g = p.heads / kv;
-    const int kvh = u % kv, split = u / kv % it.splits, block = it.blocks - 1 - u / kv / it.splits;
+    const FormUnit un = form_unit(p, it, g, ROWS, TILE, u);
+    const int kvh = un.kvh, split = un.part, block = un.block;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     F w;
     w.init(p, it, kvh, g, 32 * block);
     const FormRange range = w.range();
     const int step0 = range.lo >> 5, steps = range.lo > range.hi ? 0 : (range.hi >> 5) - step0 + 1;
-    const int s0 = step0 + static_cast<int>(static_cast<long long>(steps) * split / it.splits);
-    const int s1 = step0 + static_cast<int>(static_cast<long long>(steps) * (split + 1) / it.splits);
+    const int s0 = __builtin_amdgcn_readfirstlane(step0 + static_cast<int>(static_cast<long long>(steps) * split / un.parts));
+    const int s1 = __builtin_amdgcn_readfirstlane(step0 + static_cast<int>(static_cast<long long>(steps) * (split + 1) / un.parts));
 
     const long long page_bytes = p.geom.page_elems() * ES, plane_bytes = p.geom.plane_elems() * ES;
     const long long head_bytes = static_cast<long long>(kvh) * kPageTokens * D * ES;
@@ -384,8 +455,8 @@ __device__ __forceinline__ void forms_stream(const FormsK& p, const FormItem& it
         load_v(st, phys);
     }
     w.load_q(p);
-    for (; st < s1; st += 4) {
-        phys = page(st + 4);
+    for (; st < s1; st += 8) {
+        phys = page(st + 8);
         f32x16_t s[1];
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
@@ -403,7 +474,7 @@ __device__ __forceinline__ void forms_stream(const FormsK& p, const FormItem& it
             for (int c = 0; c < PARTS; ++c) s[0] = mfma32(a, w.q[c][kk], s[0]);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (st + 4 < s1) load_k(st + 4, phys);
+        if (st + 8 < s1) load_k(st + 8, phys);
         const bool edge = !range.all(32 * st, 32);
         w.form(p, s[0], 32 * st, edge);
         if (edge) {
@@ -448,64 +519,52 @@ __device__ __forceinline__ void forms_stream(const FormsK& p, const FormItem& it
                 for (int c = 0; c < PARTS; ++c) w.acc[d] = mfma32(a, wt[c][0][x], w.acc[d]);
             }
         __builtin_amdgcn_sched_barrier(0);
-        if (st + 4 < s1) load_v(st + 4, phys);
+        if (st + 8 < s1) load_v(st + 8, phys);
     }
     w.l = sum_xor32(w.l);
 
-    // the waves merge: each adds up a quarter of the dim groups
-#pragma unroll
-    for (int d = 0; d < F::ND; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            xa[(wave * NG + 4 * d + i) * 64 + w.lane] = f32x4_t{w.acc[d][4 * i], w.acc[d][4 * i + 1], w.acc[d][4 * i + 2], w.acc[d][4 * i + 3]};
-    xm[wave * 64 + w.lane] = make_float2(w.m, w.l);
-    __syncthreads();
-    float M = -INFINITY, L = 0.f, c[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) M = fmaxf(M, xm[x * 64 + w.lane].x);
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-        const float2 ml = xm[x * 64 + w.lane];
-        c[x] = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - M);
-        L = fmaf(ml.y, c[x], L);
-    }
-    constexpr int NP = NG / 4;
-    f32x4_t out[NP];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-        out[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int x = 0; x < 4; ++x) out[i] += xa[(x * NG + wave * NP + i) * 64 + w.lane] * c[x];
-    }
-    w.store(p, it, split, wave * NP, L, out);
-    if (wave == 0) w.store_ml(p, it, split, M, L);
+    merge_waves<F, 1, 8>(p, it, un, w, 0, wave, lds, rest);
 }
 
 // ------------------------------------------------------------------ many rows: bound by MFMAs and the softmax
-// Four waves of 32 rows share every tile of 64 slots in LDS, the next one requested while one is used; two workgroups on a CU,
-// so that one's softmax runs beside the other's MFMAs.  16 bits: tiles are copied by buffer-load DMA as they lie in the page.
-// 8 bits: a thread takes 16 bytes of K and V through registers and writes them as bf16 operands, once for the four waves.
-constexpr int kFormTileRows = 128, kFormTile = 64;
+// Eight waves, RW of them of 32 rows each; with RW = 8 a wave takes whole tiles of 64 slots, with RW = 4 two waves share a row group, a
+// step of 32 of every tile each.  A tile's K and V lie in rings in LDS that fill it, the tiles ahead requested while one is
+// used: one tile ahead leaves a workgroup waiting for memory (128 rows over 8000 positions: 1.8 us a tile where the MFMAs take 0.4).
+// 16 bits: tiles are copied by buffer-load DMA as they lie in the page.  8 bits: the codes are copied so, and become bf16 operands
+// in a second ring two tiles ahead of the scores, once for all waves.
+template <int CT, int D> struct FormRings {
+    static constexpr bool E8 = CT == QR_DTYPE_E4M3;
+    static constexpr int KB = 128 * D;            // bytes of a tile's operands of K (or V)
+    static constexpr int NST = E8 ? 2 : 4;        // tiles of operands of each
+    static constexpr int RAW = 3;                 // 8 bits: tiles of codes of each
+    static constexpr int RAW0 = 2 * NST * KB;     // first byte of the codes' ring
+    static constexpr int BYTES = E8 ? RAW0 + 2 * RAW * KB / 2 : RAW0;
+    static constexpr int WAVES = 1024 * D;        // eight waves' sums, at the end
+    static constexpr int LDS = BYTES > WAVES ? BYTES : WAVES;
+    static constexpr int REST = 4096 + 4 * 64 * 4 + 128;  // (maximum, sum) of the waves, or scales; scales of V; spans
+};
 
-template <int CT, int D, int PARTS, int SCORES>
+template <int CT, int D, int PARTS, int SCORES, int RW>
 __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, int u, char* lds, char* rest) {
     using F = FormTile<CT, D, PARTS, SCORES>;
+    using L = FormRings<CT, D>;
     using vec8 = typename F::vec8;
     using T = typename F::T;
     constexpr bool E8 = F::E8;
-    constexpr int ES = E8 ? 1 : 2;
-    constexpr int SB = 64 * D;          // bytes of a step's operands of K (or V) in LDS
-    constexpr int KB = 2 * SB;          // of a tile
-    constexpr int PER = KB / 1024 / 4;  // DMA loads per wave for a tile of K (or V)
-    constexpr int NP = 64 * D / 16 / 256;  // 8 bits: 16-byte pieces of K (or V) per thread
-    // lds: two K tiles, two V tiles
-    float(*const vscale)[64] = reinterpret_cast<float(*)[64]>(rest);            // [2][64]
-    int(*const spans)[4] = reinterpret_cast<int(*)[4]>(rest + 2 * 64 * 4);      // [4][4]
+    constexpr int ES = E8 ? 1 : 2, NS = RW == 8 ? 2 : 1;
+    constexpr int ROWS = 32 * RW, TILE = form_tile(kFormTiles);
+    static_assert(TILE == 64 && form_tile(kFormTilesHalf) == 64 && form_rows(kFormTiles) == 256 && form_rows(kFormTilesHalf) == 128, "two steps, eight or four waves");
+    constexpr int SB = 64 * D, KB = L::KB;         // bytes of a step's and of a tile's operands
+    constexpr int PER = KB * ES / 2 / 1024 / 8;    // DMA loads per wave for a tile of K (or V); 0: half the waves make one
+    constexpr int NPER = PER ? PER : 1;
+    float(*const vscale)[64] = reinterpret_cast<float(*)[64]>(rest + 4096);               // [4][64]
+    int(*const spans)[4] = reinterpret_cast<int(*)[4]>(rest + 4096 + 4 * 64 * 4);         // [8][4]
     const int kv = p.geom.kv_heads, g = p.heads / kv;
-    const int kvh = u % kv, split = u / kv % it.splits, block = it.blocks - 1 - u / kv / it.splits;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const FormUnit un = form_unit(p, it, g, ROWS, TILE, u);
+    const int kvh = un.kvh, split = un.part, block = un.block;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % RW, st0 = wave / RW;  // its row group and first step
     F w;
-    w.init(p, it, kvh, g, kFormTileRows * block + 32 * wave);
+    w.init(p, it, kvh, g, ROWS * block + 32 * rw);
     FormRange range = w.range();
     if (w.lane == 0) {
         spans[wave][0] = range.lo;
@@ -515,7 +574,7 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RW; ++i) {
         range.lo = min(range.lo, spans[i][0]);
         range.hi = max(range.hi, spans[i][1]);
         range.all_lo = max(range.all_lo, spans[i][2]);
@@ -525,58 +584,62 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
     range.hi = __builtin_amdgcn_readfirstlane(range.hi);
     range.all_lo = __builtin_amdgcn_readfirstlane(range.all_lo);
     range.all_hi = __builtin_amdgcn_readfirstlane(range.all_hi);
-    const int tile0 = range.lo / kFormTile, tiles = range.lo > range.hi ? 0 : range.hi / kFormTile - tile0 + 1;
-    const int i0 = tile0 + static_cast<int>(static_cast<long long>(tiles) * split / it.splits);
-    const int i1 = tile0 + static_cast<int>(static_cast<long long>(tiles) * (split + 1) / it.splits);
+    const int tile0 = range.lo / TILE, tiles = range.lo > range.hi ? 0 : range.hi / TILE - tile0 + 1;
+    // (the same in every lane: buffer resources and page lookups are scalar)
+    const int i0 = __builtin_amdgcn_readfirstlane(tile0 + static_cast<int>(static_cast<long long>(tiles) * split / un.parts));
+    const int i1 = __builtin_amdgcn_readfirstlane(tile0 + static_cast<int>(static_cast<long long>(tiles) * (split + 1) / un.parts));
 
     const long long page_bytes = p.geom.page_elems() * ES, plane_bytes = p.geom.plane_elems() * ES;
     const long long head_bytes = static_cast<long long>(kvh) * kPageTokens * D * ES;
-    auto page = [&](int i) { return i < i1 ? form_page(p, it.pt_off, kFormTile * i) : 0; };
-    auto k_at = [&](int i) { return lds + (i & 1) * KB; };
-    auto v_at = [&](int i) { return lds + (2 + (i & 1)) * KB; };
-    // 16 bits: request tile i
-    auto dma = [&](int i, int phys) __attribute__((always_inline)) {
-        const char* base = p.pool + static_cast<long long>(phys) * page_bytes + head_bytes + static_cast<long long>(kFormTile * i & (kPageTokens - 1)) * D * 2;
-        const bool in = i < i1;  // past the last tile: no records, no memory is read
-        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, in ? KB : 0, kBufferFlags);
-        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + plane_bytes), 0, in ? KB : 0, kBufferFlags);
-#pragma unroll
-        for (int c = 0; c < PER; ++c) buffer_load_lds16(rk, k_at(i) + 1024 * (wave + 4 * c), 16 * w.lane, 1024 * (wave + 4 * c));
-#pragma unroll
-        for (int c = 0; c < PER; ++c) buffer_load_lds16(rv, v_at(i) + 1024 * (wave + 4 * c), 16 * w.lane, 1024 * (wave + 4 * c));
+    auto page = [&](int i) { return i < i1 ? form_page(p, it.pt_off, TILE * i) : 0; };
+    // (tile numbers are not negative)
+    auto k_at = [&](int i) { return lds + (static_cast<unsigned>(i) % L::NST) * KB; };
+    auto v_at = [&](int i) { return lds + (L::NST + static_cast<unsigned>(i) % L::NST) * KB; };
+    auto raw_at = [&](int i, bool v) { return lds + L::RAW0 + ((v ? L::RAW : 0) + static_cast<unsigned>(i) % L::RAW) * (KB / 2); };
+    // request K or V of tile i (8 bits: its codes, and with K the 64 scales of K and of V, the same by every wave), a load at a time
+    auto source = [&](int i, int phys, bool v) __attribute__((always_inline)) {
+        const char* base = p.pool + static_cast<long long>(phys) * page_bytes + head_bytes + (v ? plane_bytes : 0) + static_cast<long long>(TILE * i & (kPageTokens - 1)) * D * ES;
+        return dma_source(base, i < i1 ? KB * ES / 2 : 0);  // past the last tile: no records, no memory is read
     };
-    // 8 bits: pieces of tile i into registers, and from there into LDS
-    uint4 pk[E8 ? NP : 1], pv[E8 ? NP : 1];
-    uint32_t ps[E8 ? NP : 1], pvs = 0;
-    auto fetch = [&](int i, int phys) __attribute__((always_inline)) {
-        if (i >= i1) return;
-        const char* pg = p.pool + static_cast<long long>(phys) * page_bytes;
-        const char* base = pg + head_bytes + static_cast<long long>(kFormTile * i & (kPageTokens - 1)) * D;
-        const char* sc = pg + 2 * plane_bytes + kvh * kPageTokens + (kFormTile * i & (kPageTokens - 1));
-#pragma unroll
-        for (int c = 0; c < NP; ++c) {
-            const int x = threadIdx.x + 256 * c, m = x & 31;  // piece x: step x / (2 D), lane x % 64
-            pk[c] = *reinterpret_cast<const uint4*>(base + 16 * x);
-            pv[c] = *reinterpret_cast<const uint4*>(base + plane_bytes + 16 * x);
-            ps[c] = static_cast<uint8_t>(sc[32 * (x / (2 * D)) + 16 * (m >> 2 & 1) + 8 * (m >> 4) + 4 * (m >> 3 & 1) + (m & 3)]);
-        }
-        if (threadIdx.x < 64) pvs = static_cast<uint8_t>(sc[kv * kPageTokens + threadIdx.x]);
+    auto load = [&](u32x4_t r, int i, bool v, int c) __attribute__((always_inline)) {
+        const int x = (PER ? wave : wave & 3) + 8 * c;  // (half a tile's loads each, twice)
+        dma16(r, (E8 ? raw_at(i, v) : v ? v_at(i) : k_at(i)) + 1024 * x, 16 * w.lane, 1024 * x);
     };
-    auto put = [&](int i) __attribute__((always_inline)) {
-        if (i >= i1) return;
+    auto load_scales = [&](int i, int phys) __attribute__((always_inline)) {
+        const char* sc = p.pool + static_cast<long long>(phys) * page_bytes + 2 * plane_bytes + kvh * kPageTokens + (TILE * i & (kPageTokens - 1));
+        // lanes from 32 on: past the records
+        dma4(dma_source(sc, i < i1 ? kv * kPageTokens + 64 : 0), rest + 256 * (i & 7), w.lane < 16 ? 4 * w.lane : kv * kPageTokens + 4 * (w.lane - 16));
+    };
+    auto request = [&](int i, int phys, bool v) __attribute__((always_inline)) {
+        const u32x4_t r = source(i, phys, v);
+#pragma unroll
+        for (int c = 0; c < NPER; ++c) load(r, i, v, c);
+        if (E8 && !v) load_scales(i, phys);
+    };
+    constexpr int LOADS = E8 ? 2 * NPER + 1 : 2 * NPER;  // per wave of K and V of a tile
+    // 8 bits: codes of K or V of tile i, which have landed, into operands; the scales of V with K.  First what is read, then what is
+    // written.
+    struct Codes {
+        uint4 y;
+        uint32_t scale, vscale;
+    };
+    constexpr int PIECES = 4 * D;  // of 16 bytes: step x / (2 D), lane x % 64; D = 64: half the waves take K, half V
+    const int piece = threadIdx.x & (PIECES - 1);
+    auto codes = [&](int i, bool v) __attribute__((always_inline)) -> Codes {
+        const int m = piece & 31;
+        const uint8_t* sc = reinterpret_cast<const uint8_t*>(rest) + 256 * (i & 7);
+        return {*reinterpret_cast<const uint4*>(raw_at(i, v) + 16 * piece),
+                v ? 0u : sc[32 * (piece / (2 * D)) + 16 * (m >> 2 & 1) + 8 * (m >> 4) + 4 * (m >> 3 & 1) + (m & 3)], v ? 0u : sc[64 + (piece & 63)]};
+    };
+    auto widen = [&](const Codes& c, int i, bool v) __attribute__((always_inline)) {
         if constexpr (E8) {
-#pragma unroll
-            for (int c = 0; c < NP; ++c) {
-                const int x = threadIdx.x + 256 * c, st = x / (2 * D), j = x / 64 % (D / 32), l = x & 63;
-                const float ks = scale_of(ps[c]);
-                bf16x8_t* k = reinterpret_cast<bf16x8_t*>(k_at(i) + SB * st + 2048 * j + 16 * l);
-                k[0] = widen8(pk[c].x, pk[c].y, ks);
-                k[64] = widen8(pk[c].z, pk[c].w, ks);
-                bf16x8_t* v = reinterpret_cast<bf16x8_t*>(v_at(i) + SB * st + 1024 * j + 16 * l);
-                v[0] = widen8(pv[c].x, pv[c].y, 1.f);
-                v[64 * F::ND] = widen8(pv[c].z, pv[c].w, 1.f);
-            }
-            if (threadIdx.x < 64) vscale[i & 1][threadIdx.x] = scale_of(pvs);
+            if (PIECES < 512 && (threadIdx.x >= PIECES) != v) return;
+            const int st = piece / (2 * D), j = piece / 64 % (D / 32), l = piece & 63;
+            const float by = v ? 1.f : scale_of(c.scale);
+            bf16x8_t* to = reinterpret_cast<bf16x8_t*>(v ? v_at(i) + SB * st + 1024 * j + 16 * l : k_at(i) + SB * st + 2048 * j + 16 * l);
+            to[0] = widen8(c.y.x, c.y.y, by);
+            to[v ? 64 * F::ND : 64] = widen8(c.y.z, c.y.w, by);
+            if (!v && piece < 64) vscale[i & 3][piece] = scale_of(c.vscale);
         }
     };
     // this lane's part of the operands: K of step st, k-step kk; V of step st, PV step x, dim tile d
@@ -584,34 +647,15 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
     const int ko = E8 ? 16 * w.lane : 1024 * ax * (D / 32) + 16 * (16 * w.half + 4 * (2 * sx + hx) + bx);
     const int vo = E8 ? 16 * w.lane : 1024 * (m_ >> 4) + 16 * (16 * w.half + (w.lane & 15));
     auto k_op = [&](const char* k, int st, int kk) __attribute__((always_inline)) {
-        return *reinterpret_cast<const vec8*>(k + SB * st + ko + (E8 ? 1024 : 512) * kk);
+        return *reinterpret_cast<const vec8*>(k + SB * (st0 + st) + ko + (E8 ? 1024 : 512) * kk);
     };
     auto v_op = [&](const char* v, int st, int x, int d) __attribute__((always_inline)) {
-        return *reinterpret_cast<const vec8*>(v + SB * st + vo + (E8 ? 1024 * (x * F::ND + d) : 2048 * d + 512 * x));
+        return *reinterpret_cast<const vec8*>(v + SB * (st0 + st) + vo + (E8 ? 1024 * (x * F::ND + d) : 2048 * d + 512 * x));
     };
-    int phys = page(i0 + 1);
-    if (E8) fetch(i0, page(i0));
-    else if (i0 < i1) dma(i0, page(i0));
-    w.load_q(p);
-    if (E8) {
-        put(i0);
-        fetch(i0 + 1, phys);
-        phys = page(i0 + 2);
-    }
-    for (int i = i0; i < i1; ++i) {
-        if (E8) {
-            __syncthreads();  // tile i is written, tile i - 1 was read
-        } else {
-            wait_dma();
-            lds_barrier_dma_in_flight();
-            if (i + 1 < i1) dma(i + 1, phys);
-            phys = page(i + 2);
-        }
+    auto qk = [&](f32x16_t (&s)[NS], int i) __attribute__((always_inline)) {
         const char* const k = k_at(i);
-        char* const v = v_at(i);
-        f32x16_t s[2];
 #pragma unroll
-        for (int st = 0; st < 2; ++st) {
+        for (int st = 0; st < NS; ++st) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[st][r] = 0.f;
 #pragma unroll
@@ -621,37 +665,11 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
                 for (int c = 0; c < PARTS; ++c) s[st] = mfma32(a, w.q[c][kk], s[st]);
             }
         }
-        const bool edge = !range.all(kFormTile * i, kFormTile);
+    };
+    auto pv = [&](const vec8 (&wt)[PARTS][NS][2], int i) __attribute__((always_inline)) {
+        const char* const v = v_at(i);
 #pragma unroll
-        for (int st = 0; st < 2; ++st) w.form(p, s[st], kFormTile * i + 32 * st, edge);
-        if (edge) {
-            // V elements that are not finite: a product of all of them with zeros shows them (the same in every wave)
-            vec8 zero;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) zero[j] = static_cast<T>(0.f);
-            f32x16_t z;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) z[j] = 0.f;
-#pragma unroll
-            for (int c = 0; c < KB / 1024; ++c) z = mfma32(*reinterpret_cast<const vec8*>(v + 1024 * c + 16 * w.lane), zero, z);
-            float t = 0.f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) t += z[j];
-            if (__builtin_amdgcn_ballot_w64(!(t == 0.f))) {
-                w.add_bad(p, it, kvh, kFormTile * i);
-                w.add_bad(p, it, kvh, kFormTile * i + 32);
-                lds_barrier_dma_in_flight();
-                for (int c = threadIdx.x; c < KB / 2; c += 256) {
-                    T* x = reinterpret_cast<T*>(v) + c;
-                    if (!(fabsf(static_cast<float>(*x)) < INFINITY)) *x = static_cast<T>(0.f);
-                }
-                lds_barrier_dma_in_flight();
-            }
-        }
-        vec8 wt[PARTS][2][2];
-        w.template softmax<2>(s, wt, [&](int n, int r) __attribute__((always_inline)) { return vscale[i & 1][32 * n + 16 * w.half + r]; });
-#pragma unroll
-        for (int st = 0; st < 2; ++st)
+        for (int st = 0; st < NS; ++st)
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -660,36 +678,273 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
 #pragma unroll
                     for (int c = 0; c < PARTS; ++c) w.acc[d] = mfma32(a, wt[c][st][x], w.acc[d]);
                 }
-        if (E8) {
-            put(i + 1);
-            fetch(i + 2, phys);
-            phys = page(i + 3);
+    };
+    auto edge = [&](int i) __attribute__((always_inline)) { return !range.all(TILE * i, TILE); };
+    // V elements that are not finite, of a tile that not every row sees whole: a product of all of them with zeros shows them (the
+    // same in every wave).
+    auto check_v = [&](int i) __attribute__((always_inline)) {
+        char* const v = v_at(i);
+        vec8 zero;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) zero[j] = static_cast<T>(0.f);
+        f32x16_t z;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) z[j] = 0.f;
+#pragma unroll
+        for (int c = 0; c < KB / 1024; ++c) z = mfma32(*reinterpret_cast<const vec8*>(v + 1024 * c + 16 * w.lane), zero, z);
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) t += z[j];
+        if (__builtin_amdgcn_ballot_w64(!(t == 0.f))) {
+#pragma unroll 1
+            for (int st = 0; st < NS; ++st) w.add_bad(p, it, kvh, TILE * i + 32 * (st0 + st));
+            lds_barrier_dma_in_flight();
+            for (int c = threadIdx.x; c < KB / 2; c += 512) {
+                T* x = reinterpret_cast<T*>(v) + c;
+                if (!(fabsf(static_cast<float>(*x)) < INFINITY)) *x = static_cast<T>(0.f);
+            }
+            lds_barrier_dma_in_flight();
+        }
+    };
+    auto v_scale = [&](int i) {
+        return [&, i](int n, int r) __attribute__((always_inline)) { return vscale[i & 3][32 * (st0 + n) + 16 * w.half + r]; };
+    };
+    auto form = [&](f32x16_t (&s)[NS], int i) __attribute__((always_inline)) {
+        const bool e = edge(i);
+#pragma unroll
+        for (int st = 0; st < NS; ++st) w.form(p, s[st], TILE * i + 32 * (st0 + st), e);
+    };
+    w.load_q(p);
+    if (i0 < i1) {
+        if constexpr (PARTS == 1) {
+            // Tile i's softmax runs between the MFMAs of the scores of tile i + 1 and of V of tile i - 1: none of the three needs
+            // another.  At the turn in front of it K of tile i + 1 and V of tile i - 1 are there for every wave, and what the last turn
+            // read is free: 16 bits K of tile i and V of tile i - 2, 8 bits also the codes of K of tile i + 1 and of V of tile i - 1.
+            constexpr int KA = E8 ? 4 : L::NST, VA = E8 ? 2 : L::NST - 2;  // a turn requests K of tile i + KA, V of tile i + VA
+            f32x16_t s[2][NS];
+            uint32_t wt[NS][2][4];  // a tile's weights, as operands
+            int phys[5];            // of tiles i .. i + 4
+#pragma unroll
+            for (int x = 0; x < 5; ++x) phys[x] = page(i0 + x);
+#pragma unroll
+            for (int x = 0; x < KA; ++x) {
+                if (E8 && x == 3) {  // the ring of codes holds three tiles: two become operands first
+                    wait_vmcnt<LOADS>();
+                    lds_barrier_dma_in_flight();
+                    widen(codes(i0, false), i0, false);
+                    widen(codes(i0 + 1, false), i0 + 1, false);
+                    lds_barrier_dma_in_flight();
+                }
+                request(i0 + x, phys[x], false);
+                if (x >= KA - VA) request(i0 + x - (KA - VA), phys[x - (KA - VA)], true);
+            }
+            if (!E8) {
+                wait_vmcnt<(KA - 1 + VA) * NPER>();
+                lds_barrier_dma_in_flight();
+            }
+            qk(s[0], i0);
+            auto weights8 = [](const uint32_t (&x)[4]) __attribute__((always_inline)) {
+                vec8 r;
+                __builtin_memcpy(&r, x, 16);
+                return r;
+            };
+            // V of tile i - 1, then the scores of tile i + 1, an operand read kAhead MFMAs in front of its use, and beside them tile i's
+            // weights, two at a time (left to itself, the compiler computes all weights, then has each MFMA wait for its operand).  The
+            // weights follow the MFMAs that take the last tile's by ND, into their registers.  A load takes its wave some hundred cycles to
+            // issue when eight waves issue at once (four in front of the MFMAs: 1470 cycles of 5260 a tile), so the requests stand
+            // between them too, and with 8 bits what becomes operands.
+            constexpr int kAhead = E8 ? 3 : 4;
+            auto between = [&](int i, const f32x16_t (&s)[NS], f32x16_t (&next)[NS], uint32_t (&wt)[NS][2][4], auto first, auto extra, auto convert) __attribute__((always_inline)) {
+                constexpr bool PV = !decltype(first)::value;
+                constexpr int NQ = NS * F::NK, OPS = PV ? 2 * NQ : NQ, PAIRS = 8 * NS;
+                static_assert(NS * 2 * F::ND == NQ && F::NK % 4 == 0, "as many of each");
+                const char *const k = k_at(i + 1), *const v = v_at(PV ? i - 1 : i);
+                vec8 ring[kAhead];
+                auto read = [&](int x) __attribute__((always_inline)) -> vec8 {
+                    if (PV && x < NQ) return v_op(v, x / (2 * F::ND), x / F::ND % 2, x % F::ND);
+                    const int j = PV ? x - NQ : x;
+                    return k_op(k, j % NS, j / NS);
+                };
+#pragma unroll
+                for (int x = 0; x < kAhead; ++x) ring[x] = read(x);
+                const float ref = w.m == -INFINITY ? 0.f : -w.m;
+                float sum[2] = {0.f, 0.f}, e[2];
+                float2 vs[2];
+                auto scales = [&](int y) __attribute__((always_inline)) {
+                    return *reinterpret_cast<const float2*>(&vscale[i & 3][32 * (st0 + (y >> 3)) + 16 * w.half + 2 * (y & 7)]);
+                };
+                if (E8) vs[0] = scales(0);
+                auto begin = [&](int y) __attribute__((always_inline)) {
+                    const int n = y >> 3, r = 2 * (y & 7);
+                    if (E8 && y + 1 < PAIRS) vs[(y & 1) ^ 1] = scales(y + 1);
+                    e[0] = s[n][r];
+                    e[1] = s[n][r + 1];
+                    asm volatile("" : "+v"(e[0]), "+v"(e[1]));  // not before the MFMA in front
+                    e[0] = fast_exp2(SCORES == kScoresPlain ? fmaf(e[0], w.sscale, ref) : e[0] + ref);
+                    e[1] = fast_exp2(SCORES == kScoresPlain ? fmaf(e[1], w.sscale, ref) : e[1] + ref);
+                };
+                auto end = [&](int y) __attribute__((always_inline)) {
+                    const int n = y >> 3, r = 2 * (y & 7);
+                    sum[0] += e[0];
+                    sum[1] += e[1];
+                    if (E8) {
+                        e[0] *= vs[y & 1].x;
+                        e[1] *= vs[y & 1].y;
+                    }
+                    typedef float f32x2 __attribute__((ext_vector_type(2)));
+                    typedef T T2 __attribute__((ext_vector_type(2)));
+                    const T2 pair = __builtin_convertvector((f32x2{e[0], e[1]}), T2);
+                    uint32_t b;
+                    __builtin_memcpy(&b, &pair, 4);
+                    asm volatile("" : "+v"(b), "+v"(sum[0]), "+v"(sum[1]));  // nor after the next
+                    wt[n][r >> 3][(r & 7) >> 1] = b;
+                };
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 0; x < OPS + (PV ? F::ND : 0); ++x) {
+                    if (x < OPS) {
+                        if (PV && x < NQ) {
+                            w.acc[x % F::ND] = mfma32(ring[x % kAhead], weights8(wt[x / (2 * F::ND)][x / F::ND % 2]), w.acc[x % F::ND]);
+                        } else {
+                            const int j = PV ? x - NQ : x, st = j % NS, kk = j / NS;
+                            if (kk == 0)
+#pragma unroll
+                                for (int r = 0; r < 16; ++r) next[st][r] = 0.f;
+                            next[st] = mfma32(ring[x % kAhead], w.q[0][kk], next[st]);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int k = 0; k < LOADS; ++k)
+                            if (k * OPS / LOADS == x) extra(k);
+                        if (E8) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (k * OPS / 4 == x) convert(k);
+                        }
+                    }
+                    if constexpr (PV) {
+                        constexpr int SP = OPS / PAIRS;  // MFMAs to a pair
+                        const int t = x - F::ND;
+                        if (t >= 0 && t % SP == 0) begin(t / SP);
+                        if (SP > 1 && t >= 0 && t % SP == 0) asm volatile("" : "+v"(e[0]), "+v"(e[1]));
+                        if (t >= 0 && t % SP == SP - 1) end(t / SP);
+                    } else {
+#pragma unroll
+                        for (int y = x * PAIRS / OPS; y < (x + 1) * PAIRS / OPS; ++y) {
+                            begin(y);
+                            end(y);
+                        }
+                    }
+                    if (x + kAhead < OPS) ring[x % kAhead] = read(x + kAhead);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                return sum[0] + sum[1];
+            };
+            auto tile = [&](int i, f32x16_t (&s)[NS], f32x16_t (&next)[NS], auto first) __attribute__((always_inline)) {
+                wait_vmcnt<E8 ? LOADS : (L::NST - 2) * LOADS>();
+                lds_barrier_dma_in_flight();
+                const int pk = phys[KA], pv_ = phys[VA];
+                const u32x4_t rk = source(i + KA, pk, false), rv = source(i + VA, pv_, true);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) phys[x] = phys[x + 1];
+                phys[4] = page(i + 5);
+                Codes ck, cv;
+                auto extra = [&](int k) __attribute__((always_inline)) {
+                    if (k < NPER) load(rk, i + KA, false, k);
+                    else if (k < 2 * NPER) load(rv, i + VA, true, k - NPER);
+                    else load_scales(i + KA, pk);
+                };
+                auto convert = [&](int k) __attribute__((always_inline)) {
+                    if (k == 0) ck = codes(i + 2, false);
+                    if (k == 1) widen(ck, i + 2, false);
+                    if (k == 2) cv = codes(i, true);
+                    if (k == 3) widen(cv, i, true);
+                };
+                if (!first.value && edge(i - 1)) check_v(i - 1);
+                form(s, i);
+                const float c = w.raise(s);
+                const float sum = between(i, s, next, wt, first, extra, convert);
+                w.rescale(c);
+                w.l += sum;
+            };
+            tile(i0, s[0], s[1], std::true_type{});
+            int i = i0 + 1;
+            for (; i + 1 < i1; i += 2) {
+                tile(i, s[1], s[0], std::false_type{});
+                tile(i + 1, s[0], s[1], std::false_type{});
+            }
+            if (i < i1) tile(i, s[1], s[0], std::false_type{});
+            wait_dma();
+            lds_barrier_dma_in_flight();
+            if (edge(i1 - 1)) check_v(i1 - 1);
+            vec8 last[PARTS][NS][2];
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                last[0][n][0] = weights8(wt[n][0]);
+                last[0][n][1] = weights8(wt[n][1]);
+            }
+            pv(last, i1 - 1);
+        } else {
+            // Parts take the registers: one tile after another.  At the turn in front of tile i its K and V are there for every wave (8 bits:
+            // the codes of the next tile's, which become operands behind it), and what the last turn read is free.
+            constexpr int AHEAD = E8 ? 3 : L::NST - 1;  // a turn requests K and V of tile i + AHEAD
+            int phys[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) phys[x] = page(i0 + x);
+#pragma unroll
+            for (int x = 0; x < AHEAD; ++x) {
+                request(i0 + x, phys[x], false);
+                request(i0 + x, phys[x], true);
+            }
+            if (E8) {
+                wait_vmcnt<2 * LOADS>();
+                lds_barrier_dma_in_flight();
+                widen(codes(i0, false), i0, false);
+                widen(codes(i0, true), i0, true);
+            }
+            for (int i = i0; i < i1; ++i) {
+                wait_vmcnt<E8 ? LOADS : (AHEAD - 1) * LOADS>();
+                lds_barrier_dma_in_flight();
+                request(i + AHEAD, phys[AHEAD], false);
+                request(i + AHEAD, phys[AHEAD], true);
+#pragma unroll
+                for (int x = 0; x < 3; ++x) phys[x] = phys[x + 1];
+                phys[3] = page(i + 4);
+                if (E8) {
+                    widen(codes(i + 1, false), i + 1, false);
+                    widen(codes(i + 1, true), i + 1, true);
+                }
+                f32x16_t s[NS];
+                qk(s, i);
+                form(s, i);
+                if (edge(i)) check_v(i);
+                vec8 wt[PARTS][NS][2];
+                w.softmax(s, wt, v_scale(i));
+                pv(wt, i);
+            }
         }
     }
     w.l = sum_xor32(w.l);
-    f32x4_t o[4 * F::ND];
-#pragma unroll
-    for (int i = 0; i < 4 * F::ND; ++i)
-        o[i] = f32x4_t{w.acc[i >> 2][4 * (i & 3)], w.acc[i >> 2][4 * (i & 3) + 1], w.acc[i >> 2][4 * (i & 3) + 2], w.acc[i >> 2][4 * (i & 3) + 3]};
-    w.store(p, it, split, 0, w.l, o);
-    w.store_ml(p, it, split, w.m, w.l);
+    merge_waves<F, RW, 8 / RW>(p, it, un, w, rw, wave / RW, lds, rest);
 }
 
 // Items of both sorts in one launch: what one leaves of HBM or the MFMAs the other takes (64 rows behind 8192 shared positions
 // and their own keys).
 template <int CT, int D, int PARTS, int SCORES>
-__global__ void __launch_bounds__(256, 2) forms_mfma_kernel(const FormsK p) {
-    __shared__ __attribute__((aligned(1024))) char lds[512 * D];
-    __shared__ __attribute__((aligned(16))) char rest[2048];
+__global__ void __launch_bounds__(512, 1) forms_mfma_kernel(const FormsK p) {
+    using L = FormRings<CT, D>;
+    __shared__ __attribute__((aligned(1024))) char lds[L::LDS];
+    __shared__ __attribute__((aligned(16))) char rest[L::REST];
     const FormItem it = p.it[form_find(p, blockIdx.x)];
     const int u = blockIdx.x - it.unit0;
     if (it.kind == kFormStream) forms_stream<CT, D, PARTS, SCORES>(p, it, u, lds, rest);
-    else forms_tile<CT, D, PARTS, SCORES>(p, it, u, lds, rest);
+    else if (PARTS > 1 || it.kind == kFormTilesHalf) forms_tile<CT, D, PARTS, SCORES, 4>(p, it, u, lds, rest);
+    else if constexpr (PARTS == 1) forms_tile<CT, D, PARTS, SCORES, 8>(p, it, u, lds, rest);
 }
 template <int CT, int D, int PARTS> hipError_t form_launch_scores(const FormsK& k, int units, hipStream_t s) {
-    if (k.cap > 0.f) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresCap>), dim3(units), dim3(256), 0, s, k);
-    else if (k.slopes) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresSlope>), dim3(units), dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresPlain>), dim3(units), dim3(256), 0, s, k);
+    if (k.cap > 0.f) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresCap>), dim3(units), dim3(512), 0, s, k);
+    else if (k.slopes) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresSlope>), dim3(units), dim3(512), 0, s, k);
+    else hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresPlain>), dim3(units), dim3(512), 0, s, k);
     return hipGetLastError();
 }
 // Queries that the tile's type holds enter as one part, others as two of fp16 or three of bf16.
