@@ -93,28 +93,25 @@ __global__ void __launch_bounds__(kThreads) forms_merge_kernel(const FormsK p, i
 // Queries that the MFMA tiles take in one part.
 bool whole_queries(const FormsArgs& a) { return a.act == (a.dtype == QR_DTYPE_F16 ? QR_DTYPE_F16 : QR_DTYPE_BF16); }
 
-// What a unit of a kernel costs, in microseconds: a tile where as many units run as fit at once (`slots`), where half as many do,
-// and the unit's start and end.  Measured (D = 128, one part): 64 slots of 128 rows 2.4 and 1.4; a streamed step of 32 slots by
-// its bytes, 5 TB/s over all slots; fp32 steps of 16 slots as streamed ones for 16 rows, by their MFMAs for 32.
+// What a unit of a kernel takes, in microseconds: a tile of it, its start and end, and its share of what runs at once on a CU.
+// Measured (D = 128): a tile of 64 slots 2.2 for 128 rows, 1.3 for 64, 1.4 times as long with capped scores and 2.2 times in parts; a
+// streamed step of 32 slots by its bytes, 5 TB/s over all CUs; fp32 steps of 16 slots as streamed ones for 16 rows, by their
+// MFMAs for 32.
 struct Shape {
-    int slots, least;   // tiles that a part has at least
-    float full, half, start;
+    float tile, start, share;
+    int least;  // tiles that a part has at least
 };
+constexpr float kCus = 256.f;
 Shape shape_of(const FormsArgs& a, int kind) {
     const float wide = a.geom.head_dim / 128.f;
+    const float tile = wide * (whole_queries(a) ? 1.f : 2.2f) * (a.cap > 0.f ? 1.4f : a.slopes ? 1.2f : 1.f);
     switch (kind) {
-        case kFormStream: {
-            const float t = wide * (a.geom.scaled() ? 0.9f : 1.7f);
-            return {256, 16, 0.5f * t, 0.4f * t, 5.f};
-        }
-        case kFormTilesHalf:
-        case kFormTiles: {
-            const float t = wide * 2.f * (kind == kFormTilesHalf ? 0.5f : 1.f) * (!whole_queries(a) ? 2.2f : 1.f) * (a.cap > 0.f ? 1.35f : 1.f);
-            return {256, 4, t, t, 6.f};
-        }
-        case kFormF32Half: return {512, 8, wide * 1.7f, wide * 1.f, 5.f};
-        case kFormF32: return {512, 8, wide * 1.f, wide * 0.55f, 5.f};
-        default: return {1024, 2, 4.f, 2.f, 5.f};
+        case kFormStream: return {wide * (a.geom.scaled() ? 0.9f : 1.7f), 5.f, 0.5f, 8};
+        case kFormTilesHalf: return {1.3f * tile, 6.f, 0.5f, 4};
+        case kFormTiles: return {2.2f * tile, 6.f, 0.5f, 4};
+        case kFormF32Half: return {wide * 1.7f, 5.f, 0.5f, 8};
+        case kFormF32: return {wide * 1.f, 5.f, 0.5f, 8};
+        default: return {4.f, 5.f, 0.25f, 2};
     }
 }
 int kind_of(const FormsArgs& a, int rows) {
@@ -122,7 +119,7 @@ int kind_of(const FormsArgs& a, int rows) {
     if ((D != 64 && D != 128) || a.heads % a.geom.kv_heads) return kFormAny;
     const long long n = static_cast<long long>(rows) * (a.heads / a.geom.kv_heads);
     if (a.dtype == QR_DTYPE_F32) return n <= 16 ? kFormF32Half : kFormF32;
-    return n <= 32 ? kFormStream : n <= 128 || !whole_queries(a) ? kFormTilesHalf : kFormTiles;
+    return n <= 32 ? kFormStream : n <= 64 ? kFormTilesHalf : kFormTiles;
 }
 hipError_t launch(const FormsK& k, int units, hipStream_t s) {
     if (k.it[0].kind == kFormAny) return launch_forms_any(k, units, s);
@@ -131,65 +128,65 @@ hipError_t launch(const FormsK& k, int units, hipStream_t s) {
     return k.dtype == QR_DTYPE_BF16 ? launch_forms_bf16(k, units, s) : launch_forms_e4m3(k, units, s);
 }
 
+int per_of(const Shape& s, float part) { return std::max(s.least, static_cast<int>(std::min(1e9f, part / s.tile + 0.999f))); }
+
 // Blocks of an item, of which some stand for the others: their tiles.
 struct Sample {
     int item, tiles;
     float units;  // of this length, all kv heads
 };
-struct Cut {
-    int per;
-    float us;
-};
-// The cut with which the kernel's units and the partials' way through memory take least: all blocks whole, the fewest tiles of a part
-// with which the units run at once, or some between and beyond.
-int best_per(const FormsArgs& a, const FormsPlan& p, const Shape& s, int kind, const Sample* smp, int n) {
-    const int kv = a.geom.kv_heads, rows = form_rows(kind);
+// The time of a part with which the units and the partials' way through memory take least: whole blocks, an even share of what
+// the CUs run at once, or some between and beyond.
+float best_part(const FormsArgs& a, const FormsPlan& p, const Sample* smp, int n) {
+    const int kv = a.geom.kv_heads;
     const float partial = (a.geom.head_dim * 4 + 8) * 0.5e-6f;  // written and read at 4 TB/s
-    int most = 1;
-    for (int i = 0; i < n; ++i) most = std::max(most, smp[i].tiles);
-    auto units = [&](int per) {
-        float u = 0.f;
-        for (int i = 0; i < n; ++i) u += smp[i].units * static_cast<float>((smp[i].tiles + per - 1) / per);
-        return u;
-    };
-    auto cost = [&](int per) {
-        float u = 0.f, work = 0.f, parts = 0.f;
+    Shape shape[kFormKinds];
+    for (int k = 0; k < kFormKinds; ++k) shape[k] = shape_of(a, k);
+    float whole = 0.f, work = 0.f;
+    for (int i = 0; i < n; ++i) {
+        const Shape& s = shape[p.it[smp[i].item].kind];
+        whole = std::max(whole, smp[i].tiles * s.tile);
+        work += smp[i].units * smp[i].tiles * s.tile * s.share;
+    }
+    auto cost = [&](float part) {
+        float busy = 0.f, used = 0.f, longest = 0.f, parts = 0.f;
         for (int i = 0; i < n; ++i) {
             const FormItem& it = p.it[smp[i].item];
-            const int c = (smp[i].tiles + per - 1) / per;
-            u += smp[i].units * c;
-            work += smp[i].units * smp[i].tiles;
-            const long long all = static_cast<long long>(it.rows) * (a.heads / kv);
-            if (c > 1 || p.c[it.c0].parts) parts += smp[i].units * c * static_cast<float>(std::min<long long>(rows, all));
+            const Shape& s = shape[it.kind];
+            const int per = per_of(s, part), c = (smp[i].tiles + per - 1) / per;
+            const float t = s.start + s.tile * static_cast<float>((smp[i].tiles + c - 1) / c);
+            busy += smp[i].units * c * t * s.share;
+            used += smp[i].units * c * s.share;
+            longest = std::max(longest, t);
+            const long long rows = static_cast<long long>(it.rows) * (a.heads / kv);
+            if (c > 1 || p.c[it.c0].parts) parts += smp[i].units * c * static_cast<float>(std::min<long long>(form_rows(it.kind), rows));
         }
-        const float at_once = std::min(1.f, std::max(0.f, 2.f * u / s.slots - 1.f));
-        const float run = u <= s.slots ? std::min(per, most) * (s.half + (s.full - s.half) * at_once) : work * s.full / s.slots + 0.5f * std::min(per, most) * s.half;
-        return run + s.start * std::max(1.f, u / s.slots) + parts * partial + (parts > 0.f ? 4.f : 0.f);
+        const float run = used <= kCus ? longest : std::max(longest, busy / kCus + 0.5f * longest);
+        return run + parts * partial + (parts > 0.f ? 4.f : 0.f);
     };
-    int fit = std::min(most, s.least), hi = most;
-    while (fit < hi) {
-        const int mid = fit + (hi - fit) / 2;
-        if (units(mid) <= s.slots) hi = mid;
-        else fit = mid + 1;
-    }
-    Cut best = {most, cost(most)};
-    auto consider = [&](int per) {
-        if (per < std::min(most, s.least) || per >= most) return;
-        const float us = cost(per);
-        if (us < best.us) best = {per, us};
+    float best = whole, least = cost(whole);
+    auto consider = [&](float part) {
+        const float us = cost(part);
+        if (us < least) {
+            least = us;
+            best = part;
+        }
     };
-    consider(fit);
-    for (const int k : {2, 3, 4, 6, 8, 12, 16}) consider((most + k - 1) / k);
+    const float even = work / kCus;
+    for (const float f : {0.5f, 0.7f, 0.85f, 1.f, 1.04f, 1.08f, 1.15f, 1.25f, 1.4f, 1.7f, 2.f, 3.f})
+        if (even * f < whole) consider(even * f);
     // (the partials of a launch stay below 256 MB: 64 bf16 sequences of 8 rows behind 65536 positions)
-    for (;; best.per += (best.per + 3) / 4) {
+    for (;; best *= 1.25f) {
         double bytes = 0;
-        for (int i = 0; i < p.n; ++i) {
-            int len = 0;
-            for (int x = 0; x < n; ++x)
-                if (smp[x].item == i) len = std::max(len, smp[x].tiles);
-            if (len > best.per) bytes += (a.geom.head_dim * 4.0 + 8) * p.it[i].rows * a.heads * ((len + best.per - 1) / best.per);
+        for (int i = 0; i < n;) {
+            const FormItem& it = p.it[smp[i].item];
+            const int per = per_of(shape[it.kind], best);
+            int most = 1, j = i;
+            for (; j < n && smp[j].item == smp[i].item; ++j) most = std::max(most, (smp[j].tiles + per - 1) / per);
+            if (most > 1) bytes += (a.geom.head_dim * 4.0 + 8) * it.rows * a.heads * most;
+            i = j;
         }
-        if (bytes <= (256 << 20)) return best.per;
+        if (bytes <= (256 << 20)) return best;
     }
 }
 
@@ -236,38 +233,36 @@ FormsPlan plan_forms(const FormsArgs& a) {
     for (int i = 0; i < a.n; ++i) --p.c[i].parts;
     constexpr int kSamples = 8;
     Sample smp[kFormItems * kSamples];
-    for (int kind = 0; kind < kFormKinds; ++kind) {
-        int n = 0;
-        for (int i = 0; i < p.n; ++i) {
-            FormItem& it = p.it[i];
-            if (it.kind != kind) continue;
-            it.blocks = static_cast<int>((static_cast<long long>(it.rows) * g + form_rows(kind) - 1) / form_rows(kind));
-            it.per = 1;
-            it.splits = 0x7FFFFFFF;
-            if (it.nc > 1) {  // (rows of many chunks: whatever one of them sees of the prefix)
-                int tiles = 1;
-                for (int c = 0; c < it.nc; ++c) {
-                    const FormRows& r = p.c[it.c0 + c];
-                    const FormSpan x = form_span(r, r.row0, a.window, it.base, it.keys);
-                    if (x.lo <= x.hi) tiles = std::max(tiles, x.hi / form_tile(kind) - x.lo / form_tile(kind) + 1);
-                }
-                smp[n++] = {i, tiles, static_cast<float>(it.blocks) * kv};
-                continue;
+    int n = 0;
+    for (int i = 0; i < p.n; ++i) {
+        FormItem& it = p.it[i];
+        const int rows = form_rows(it.kind), tile = form_tile(it.kind);
+        it.blocks = static_cast<int>((static_cast<long long>(it.rows) * g + rows - 1) / rows);
+        it.per = 1;
+        it.splits = 0x7FFFFFFF;
+        if (it.nc > 1) {  // (rows of many chunks: whatever one of them sees of the prefix)
+            int tiles = 1;
+            for (int c = 0; c < it.nc; ++c) {
+                const FormRows& r = p.c[it.c0 + c];
+                const FormSpan x = form_span(r, r.row0, a.window, it.base, it.keys);
+                if (x.lo <= x.hi) tiles = std::max(tiles, x.hi / tile - x.lo / tile + 1);
             }
-            const int m = std::min(it.blocks, kSamples);
-            for (int x = 0; x < m; ++x) {
-                const int b = m == 1 ? 0 : static_cast<int>(static_cast<long long>(it.blocks - 1) * x / (m - 1));
-                smp[n++] = {i, form_parts(it, p.c[it.c0], a.window, g, form_rows(kind), form_tile(kind), b), static_cast<float>(it.blocks) * kv / m};
-            }
+            smp[n++] = {i, tiles, static_cast<float>(it.blocks) * kv};
+            continue;
         }
-        if (!n) continue;
-        const int per = best_per(a, p, shape_of(a, kind), kind, smp, n);
-        for (int x = 0; x < n; ++x) {
-            FormItem& it = p.it[smp[x].item];
-            if (x == 0 || smp[x - 1].item != smp[x].item) it.splits = 1;
-            it.splits = std::max(it.splits, (smp[x].tiles + per - 1) / per);
-            it.per = it.nc == 1 ? per : 0;
+        const int m = std::min(it.blocks, kSamples);
+        for (int x = 0; x < m; ++x) {
+            const int b = m == 1 ? 0 : static_cast<int>(static_cast<long long>(it.blocks - 1) * x / (m - 1));
+            smp[n++] = {i, form_parts(it, p.c[it.c0], a.window, g, rows, tile, b), static_cast<float>(it.blocks) * kv / m};
         }
+    }
+    const float part = best_part(a, p, smp, n);
+    for (int x = 0; x < n; ++x) {
+        FormItem& it = p.it[smp[x].item];
+        const int per = per_of(shape_of(a, it.kind), part);
+        if (x == 0 || smp[x - 1].item != smp[x].item) it.splits = 1;
+        it.splits = std::max(it.splits, (smp[x].tiles + per - 1) / per);
+        it.per = it.nc == 1 ? per : 0;
     }
     for (int i = 0; i < a.n; ++i) p.c[i].parts = 0;
     for (int i = 0; i < p.n; ++i) {

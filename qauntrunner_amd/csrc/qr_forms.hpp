@@ -104,7 +104,7 @@ hipError_t launch_forms_e4m3(const FormsK& k, int units, hipStream_t s);
 
 // (query, head) rows of a block and slots of a tile of each kernel.
 __host__ __device__ constexpr int form_rows(int kind) {
-    return kind == kFormAny ? kFormAnyRows : kind == kFormTiles ? 256 : kind == kFormTilesHalf ? 128 : kind == kFormF32Half ? 16 : 32;
+    return kind == kFormAny ? kFormAnyRows : kind == kFormTiles ? 128 : kind == kFormTilesHalf ? 64 : kind == kFormF32Half ? 16 : 32;
 }
 __host__ __device__ constexpr int form_tile(int kind) {
     return kind == kFormTiles || kind == kFormTilesHalf ? 64 : kind == kFormF32Half || kind == kFormF32 ? 16 : 32;
@@ -183,6 +183,11 @@ __device__ __forceinline__ void form_heads(const FormsK& p, int kvh, int* h0, in
 // Row j of an item.
 __device__ __forceinline__ FormSpan form_row(const FormsK& p, const FormItem& it, int j) {
     const int row = it.row0 + j;
+    if (it.nc == 1) {  // (scalar loads)
+        FormSpan s = form_span(p.c[it.c0], row, p.window, it.base, it.keys);
+        s.chunk = it.c0;
+        return s;
+    }
     int c = it.c0;
     for (int i = 1; i < it.nc; ++i) c += p.c[it.c0 + i].row0 <= row;
     FormSpan s = form_span(p.c[c], row, p.window, it.base, it.keys);

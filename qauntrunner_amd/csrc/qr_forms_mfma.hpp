@@ -59,7 +59,7 @@ __device__ __forceinline__ bf16x8_t widen8(uint32_t lo, uint32_t hi, float scale
     return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Copies into LDS by buffer loads, 16 or 4 bytes per lane to `to` + 16 (4) lane; past the source's bytes zeros.  As asm: behind a
+// Copies into LDS by buffer loads, 16 bytes per lane to `to` + 16 lane; past the source's bytes zeros.  As asm: behind a
 // load that the compiler knows to write LDS it waits for memory before the next read of LDS, whichever bytes that reads, and
 // the tiles ahead would be awaited in every turn (three quarters of the time of a tile).  Nothing is written to registers;
 // wait_vmcnt and a barrier stand between a copy and the reads of its bytes.  (s_nop: a scalar that a vector instruction wrote is
@@ -76,10 +76,6 @@ __device__ __forceinline__ void dma16(u32x4_t source, const char* to, uint32_t a
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  : : "s"(lds_address(to)), "v"(at), "s"(source), "s"(from) : "memory");
 }
-__device__ __forceinline__ void dma4(u32x4_t source, const char* to, uint32_t at) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(lds_address(to)), "v"(at), "s"(source) : "memory");
-}
-
 // One wave's 32 rows.
 template <int CT, int D, int PARTS, int SCORES>
 struct FormTile {
@@ -385,7 +381,7 @@ __device__ __forceinline__ void merge_waves(const FormsK& p, const FormItem& it,
 }
 
 // ------------------------------------------------------------------ few rows: HBM-bound
-// Up to 32 rows; eight waves take every eighth step of 32 slots, their operands straight from the page into registers (K of the
+// Up to 32 rows; four waves take every fourth step of 32 slots, their operands straight from the page into registers (K of the
 // next step while this one's softmax runs, V while the next one's scores are computed), and merge at the end.  No wave waits
 // for another before that.
 template <int CT, int D> struct FormStep {  // one step's operands
@@ -455,8 +451,8 @@ __device__ __forceinline__ void forms_stream(const FormsK& p, const FormItem& it
         load_v(st, phys);
     }
     w.load_q(p);
-    for (; st < s1; st += 8) {
-        phys = page(st + 8);
+    for (; st < s1; st += 4) {
+        phys = page(st + 4);
         f32x16_t s[1];
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
@@ -474,7 +470,7 @@ __device__ __forceinline__ void forms_stream(const FormsK& p, const FormItem& it
             for (int c = 0; c < PARTS; ++c) s[0] = mfma32(a, w.q[c][kk], s[0]);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (st + 8 < s1) load_k(st + 8, phys);
+        if (st + 4 < s1) load_k(st + 4, phys);
         const bool edge = !range.all(32 * st, 32);
         w.form(p, s[0], 32 * st, edge);
         if (edge) {
@@ -519,50 +515,46 @@ __device__ __forceinline__ void forms_stream(const FormsK& p, const FormItem& it
                 for (int c = 0; c < PARTS; ++c) w.acc[d] = mfma32(a, wt[c][0][x], w.acc[d]);
             }
         __builtin_amdgcn_sched_barrier(0);
-        if (st + 8 < s1) load_v(st + 8, phys);
+        if (st + 4 < s1) load_v(st + 4, phys);
     }
     w.l = sum_xor32(w.l);
 
-    merge_waves<F, 1, 8>(p, it, un, w, 0, wave, lds, rest);
+    merge_waves<F, 1, 4>(p, it, un, w, 0, wave, lds, rest);
 }
 
 // ------------------------------------------------------------------ many rows: bound by MFMAs and the softmax
-// Eight waves, RW of them of 32 rows each; with RW = 8 a wave takes whole tiles of 64 slots, with RW = 4 two waves share a row group, a
-// step of 32 of every tile each.  A tile's K and V lie in rings in LDS that fill it, the tiles ahead requested while one is
-// used: one tile ahead leaves a workgroup waiting for memory (128 rows over 8000 positions: 1.8 us a tile where the MFMAs take 0.4).
-// 16 bits: tiles are copied by buffer-load DMA as they lie in the page.  8 bits: the codes are copied so, and become bf16 operands
-// in a second ring two tiles ahead of the scores, once for all waves.
-template <int CT, int D> struct FormRings {
-    static constexpr bool E8 = CT == QR_DTYPE_E4M3;
-    static constexpr int KB = 128 * D;            // bytes of a tile's operands of K (or V)
-    static constexpr int NST = E8 ? 2 : 4;        // tiles of operands of each
-    static constexpr int RAW = 3;                 // 8 bits: tiles of codes of each
-    static constexpr int RAW0 = 2 * NST * KB;     // first byte of the codes' ring
-    static constexpr int BYTES = E8 ? RAW0 + 2 * RAW * KB / 2 : RAW0;
-    static constexpr int WAVES = 1024 * D;        // eight waves' sums, at the end
-    static constexpr int LDS = BYTES > WAVES ? BYTES : WAVES;
-    static constexpr int REST = 4096 + 4 * 64 * 4 + 128;  // (maximum, sum) of the waves, or scales; scales of V; spans
+// Four waves, RW of them of 32 rows each; with RW = 4 a wave takes whole tiles of 64 slots, with RW = 2 two waves share a row group, a
+// step of 32 of every tile each.  K and V of a tile are shared through LDS, two tiles of each, and two workgroups on a CU fill
+// each other's barriers, starts and ends (one of eight waves and 256 rows: six prompts of 101 to 1501 rows with capped scores 118 us).
+// 16 bits: tiles are copied by buffer-load DMA as they lie in the page.  8 bits: a thread takes 16 bytes of K and V through
+// registers and writes them as bf16 operands, once for all waves.
+template <int D> struct FormRings {
+    static constexpr int KB = 128 * D;                       // bytes of a tile's operands of K (or V)
+    static constexpr int NST = 2;                            // tiles of each
+    static constexpr int LDS = 2 * NST * KB;                 // (four waves' sums, at the end, are as many)
+    static constexpr int REST = 4 * 64 * 8 + 4 * 64 * 4 + 64;  // (maximum, sum) of the waves; scales of V; spans
 };
 
 template <int CT, int D, int PARTS, int SCORES, int RW>
 __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, int u, char* lds, char* rest) {
     using F = FormTile<CT, D, PARTS, SCORES>;
-    using L = FormRings<CT, D>;
+    using L = FormRings<D>;
     using vec8 = typename F::vec8;
     using T = typename F::T;
     constexpr bool E8 = F::E8;
-    constexpr int ES = E8 ? 1 : 2, NS = RW == 8 ? 2 : 1;
+    constexpr int ES = E8 ? 1 : 2, STEPS = RW / 2, NS = PARTS == 1 ? STEPS : 1;  // steps of a tile that are a wave's; of them at a time
     constexpr int ROWS = 32 * RW, TILE = form_tile(kFormTiles);
-    static_assert(TILE == 64 && form_tile(kFormTilesHalf) == 64 && form_rows(kFormTiles) == 256 && form_rows(kFormTilesHalf) == 128, "two steps, eight or four waves");
+    static_assert(TILE == 64 && form_tile(kFormTilesHalf) == 64 && form_rows(kFormTiles) == 128 && form_rows(kFormTilesHalf) == 64, "two steps, four or two waves of rows");
     constexpr int SB = 64 * D, KB = L::KB;         // bytes of a step's and of a tile's operands
-    constexpr int PER = KB * ES / 2 / 1024 / 8;    // DMA loads per wave for a tile of K (or V); 0: half the waves make one
-    constexpr int NPER = PER ? PER : 1;
-    float(*const vscale)[64] = reinterpret_cast<float(*)[64]>(rest + 4096);               // [4][64]
-    int(*const spans)[4] = reinterpret_cast<int(*)[4]>(rest + 4096 + 4 * 64 * 4);         // [8][4]
+    constexpr int PER = KB / 1024 / 4;             // DMA loads per wave for a tile of K (or V)
+    constexpr int NP = 64 * D / 16 / 256;          // 8 bits: 16-byte pieces of K (or V) per thread
+    float(*const vscale)[64] = reinterpret_cast<float(*)[64]>(rest + 4 * 64 * 8);             // [4][64]
+    int(*const spans)[4] = reinterpret_cast<int(*)[4]>(rest + 4 * 64 * 8 + 4 * 64 * 4);       // [4][4]
     const int kv = p.geom.kv_heads, g = p.heads / kv;
     const FormUnit un = form_unit(p, it, g, ROWS, TILE, u);
     const int kvh = un.kvh, split = un.part, block = un.block;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % RW, st0 = wave / RW;  // its row group and first step
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % RW;
+    int st0 = wave / RW;  // its first step
     F w;
     w.init(p, it, kvh, g, ROWS * block + 32 * rw);
     FormRange range = w.range();
@@ -595,52 +587,59 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
     // (tile numbers are not negative)
     auto k_at = [&](int i) { return lds + (static_cast<unsigned>(i) % L::NST) * KB; };
     auto v_at = [&](int i) { return lds + (L::NST + static_cast<unsigned>(i) % L::NST) * KB; };
-    auto raw_at = [&](int i, bool v) { return lds + L::RAW0 + ((v ? L::RAW : 0) + static_cast<unsigned>(i) % L::RAW) * (KB / 2); };
-    // request K or V of tile i (8 bits: its codes, and with K the 64 scales of K and of V, the same by every wave), a load at a time
+    // 16 bits: request K or V of tile i, a load at a time
     auto source = [&](int i, int phys, bool v) __attribute__((always_inline)) {
         const char* base = p.pool + static_cast<long long>(phys) * page_bytes + head_bytes + (v ? plane_bytes : 0) + static_cast<long long>(TILE * i & (kPageTokens - 1)) * D * ES;
-        return dma_source(base, i < i1 ? KB * ES / 2 : 0);  // past the last tile: no records, no memory is read
+        return dma_source(base, i < i1 ? KB : 0);  // past the last tile: no records, no memory is read
     };
     auto load = [&](u32x4_t r, int i, bool v, int c) __attribute__((always_inline)) {
-        const int x = (PER ? wave : wave & 3) + 8 * c;  // (half a tile's loads each, twice)
-        dma16(r, (E8 ? raw_at(i, v) : v ? v_at(i) : k_at(i)) + 1024 * x, 16 * w.lane, 1024 * x);
-    };
-    auto load_scales = [&](int i, int phys) __attribute__((always_inline)) {
-        const char* sc = p.pool + static_cast<long long>(phys) * page_bytes + 2 * plane_bytes + kvh * kPageTokens + (TILE * i & (kPageTokens - 1));
-        // lanes from 32 on: past the records
-        dma4(dma_source(sc, i < i1 ? kv * kPageTokens + 64 : 0), rest + 256 * (i & 7), w.lane < 16 ? 4 * w.lane : kv * kPageTokens + 4 * (w.lane - 16));
+        dma16(r, (v ? v_at(i) : k_at(i)) + 1024 * (wave + 4 * c), 16 * w.lane, 1024 * (wave + 4 * c));
     };
     auto request = [&](int i, int phys, bool v) __attribute__((always_inline)) {
         const u32x4_t r = source(i, phys, v);
 #pragma unroll
-        for (int c = 0; c < NPER; ++c) load(r, i, v, c);
-        if (E8 && !v) load_scales(i, phys);
+        for (int c = 0; c < PER; ++c) load(r, i, v, c);
     };
-    constexpr int LOADS = E8 ? 2 * NPER + 1 : 2 * NPER;  // per wave of K and V of a tile
-    // 8 bits: codes of K or V of tile i, which have landed, into operands; the scales of V with K.  First what is read, then what is
-    // written.
-    struct Codes {
-        uint4 y;
-        uint32_t scale, vscale;
-    };
-    constexpr int PIECES = 4 * D;  // of 16 bytes: step x / (2 D), lane x % 64; D = 64: half the waves take K, half V
-    const int piece = threadIdx.x & (PIECES - 1);
-    auto codes = [&](int i, bool v) __attribute__((always_inline)) -> Codes {
-        const int m = piece & 31;
-        const uint8_t* sc = reinterpret_cast<const uint8_t*>(rest) + 256 * (i & 7);
-        return {*reinterpret_cast<const uint4*>(raw_at(i, v) + 16 * piece),
-                v ? 0u : sc[32 * (piece / (2 * D)) + 16 * (m >> 2 & 1) + 8 * (m >> 4) + 4 * (m >> 3 & 1) + (m & 3)], v ? 0u : sc[64 + (piece & 63)]};
-    };
-    auto widen = [&](const Codes& c, int i, bool v) __attribute__((always_inline)) {
-        if constexpr (E8) {
-            if (PIECES < 512 && (threadIdx.x >= PIECES) != v) return;
-            const int st = piece / (2 * D), j = piece / 64 % (D / 32), l = piece & 63;
-            const float by = v ? 1.f : scale_of(c.scale);
-            bf16x8_t* to = reinterpret_cast<bf16x8_t*>(v ? v_at(i) + SB * st + 1024 * j + 16 * l : k_at(i) + SB * st + 2048 * j + 16 * l);
-            to[0] = widen8(c.y.x, c.y.y, by);
-            to[v ? 64 * F::ND : 64] = widen8(c.y.z, c.y.w, by);
-            if (!v && piece < 64) vscale[i & 3][piece] = scale_of(c.vscale);
+    constexpr int LOADS = E8 ? 0 : 2 * PER;  // per wave of K and V of a tile
+    // 8 bits: pieces of K or V of tile i into registers (the scales of V with K), and from there as operands into LDS
+    uint4 pk[E8 ? NP : 1], pv_[E8 ? NP : 1];
+    uint32_t ps[E8 ? NP : 1], pvs = 0;
+    auto fetch = [&](int i, int phys, bool v) __attribute__((always_inline)) {
+        if (i >= i1) return;
+        const char* pg = p.pool + static_cast<long long>(phys) * page_bytes;
+        const char* base = pg + head_bytes + static_cast<long long>(TILE * i & (kPageTokens - 1)) * D;
+        if (v) {
+#pragma unroll
+            for (int c = 0; c < NP; ++c) pv_[c] = *reinterpret_cast<const uint4*>(base + plane_bytes + 16 * (threadIdx.x + 256 * c));
+            return;
         }
+        const char* sc = pg + 2 * plane_bytes + kvh * kPageTokens + (TILE * i & (kPageTokens - 1));
+#pragma unroll
+        for (int c = 0; c < NP; ++c) {
+            const int x = threadIdx.x + 256 * c, m = x & 31;  // piece x: step x / (2 D), lane x % 64
+            pk[c] = *reinterpret_cast<const uint4*>(base + 16 * x);
+            ps[c] = static_cast<uint8_t>(sc[32 * (x / (2 * D)) + 16 * (m >> 2 & 1) + 8 * (m >> 4) + 4 * (m >> 3 & 1) + (m & 3)]);
+        }
+        if (threadIdx.x < 64) pvs = static_cast<uint8_t>(sc[kv * kPageTokens + threadIdx.x]);
+    };
+    auto put = [&](int i, bool v) __attribute__((always_inline)) {
+        if constexpr (E8) {
+#pragma unroll
+            for (int c = 0; c < NP; ++c) {
+                const int x = threadIdx.x + 256 * c, st = x / (2 * D), j = x / 64 % (D / 32), l = x & 63;
+                const float by = v ? 1.f : scale_of(ps[c]);
+                const uint4 y = v ? pv_[c] : pk[c];
+                bf16x8_t* to = reinterpret_cast<bf16x8_t*>(v ? v_at(i) + SB * st + 1024 * j + 16 * l : k_at(i) + SB * st + 2048 * j + 16 * l);
+                to[0] = widen8(y.x, y.y, by);
+                to[v ? 64 * F::ND : 64] = widen8(y.z, y.w, by);
+            }
+            if (!v && threadIdx.x < 64) vscale[i & 3][threadIdx.x] = scale_of(pvs);
+        }
+    };
+    // what was requested (or put) in the last turn is there for every wave, what it read is free
+    auto turn = [&]() __attribute__((always_inline)) {
+        if (!E8) wait_dma();
+        lds_barrier_dma_in_flight();
     };
     // this lane's part of the operands: K of step st, k-step kk; V of step st, PV step x, dim tile d
     const int m_ = w.lane & 31, sx = m_ >> 4, ax = (m_ >> 3) & 1, hx = (m_ >> 2) & 1, bx = m_ & 3;
@@ -697,9 +696,9 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
         for (int j = 0; j < 16; ++j) t += z[j];
         if (__builtin_amdgcn_ballot_w64(!(t == 0.f))) {
 #pragma unroll 1
-            for (int st = 0; st < NS; ++st) w.add_bad(p, it, kvh, TILE * i + 32 * (st0 + st));
+            for (int st = 0; st < STEPS; ++st) w.add_bad(p, it, kvh, TILE * i + 32 * (wave / RW + st));
             lds_barrier_dma_in_flight();
-            for (int c = threadIdx.x; c < KB / 2; c += 512) {
+            for (int c = threadIdx.x; c < KB / 2; c += 256) {
                 T* x = reinterpret_cast<T*>(v) + c;
                 if (!(fabsf(static_cast<float>(*x)) < INFINITY)) *x = static_cast<T>(0.f);
             }
@@ -714,34 +713,31 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
 #pragma unroll
         for (int st = 0; st < NS; ++st) w.form(p, s[st], TILE * i + 32 * (st0 + st), e);
     };
-    w.load_q(p);
     if (i0 < i1) {
         if constexpr (PARTS == 1) {
             // Tile i's softmax runs between the MFMAs of the scores of tile i + 1 and of V of tile i - 1: none of the three needs
-            // another.  At the turn in front of it K of tile i + 1 and V of tile i - 1 are there for every wave, and what the last turn
-            // read is free: 16 bits K of tile i and V of tile i - 2, 8 bits also the codes of K of tile i + 1 and of V of tile i - 1.
-            constexpr int KA = E8 ? 4 : L::NST, VA = E8 ? 2 : L::NST - 2;  // a turn requests K of tile i + KA, V of tile i + VA
+            // another.  At the turn in front of it K of tile i + 1 and V of tile i - 1 are there; K of tile i + 2 and V of tile i come over
+            // what the last turn read.
             f32x16_t s[2][NS];
             uint32_t wt[NS][2][4];  // a tile's weights, as operands
-            int phys[5];            // of tiles i .. i + 4
+            int phys[3];            // of tiles i .. i + 2
 #pragma unroll
-            for (int x = 0; x < 5; ++x) phys[x] = page(i0 + x);
-#pragma unroll
-            for (int x = 0; x < KA; ++x) {
-                if (E8 && x == 3) {  // the ring of codes holds three tiles: two become operands first
-                    wait_vmcnt<LOADS>();
-                    lds_barrier_dma_in_flight();
-                    widen(codes(i0, false), i0, false);
-                    widen(codes(i0 + 1, false), i0 + 1, false);
-                    lds_barrier_dma_in_flight();
-                }
-                request(i0 + x, phys[x], false);
-                if (x >= KA - VA) request(i0 + x - (KA - VA), phys[x - (KA - VA)], true);
+            for (int x = 0; x < 3; ++x) phys[x] = page(i0 + x);
+            if (E8) {
+                fetch(i0, phys[0], false);
+                w.load_q(p);
+                put(i0, false);
+                fetch(i0 + 1, phys[1], false);
+                put(i0 + 1, false);
+                fetch(i0 + 2, phys[2], false);
+                fetch(i0, phys[0], true);
+            } else {
+                request(i0, phys[0], false);
+                request(i0 + 1, phys[1], false);
+                w.load_q(p);
+                wait_vmcnt<PER>();
             }
-            if (!E8) {
-                wait_vmcnt<(KA - 1 + VA) * NPER>();
-                lds_barrier_dma_in_flight();
-            }
+            lds_barrier_dma_in_flight();
             qk(s[0], i0);
             auto weights8 = [](const uint32_t (&x)[4]) __attribute__((always_inline)) {
                 vec8 r;
@@ -753,8 +749,8 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
             // weights follow the MFMAs that take the last tile's by ND, into their registers.  A load takes its wave some hundred cycles to
             // issue when eight waves issue at once (four in front of the MFMAs: 1470 cycles of 5260 a tile), so the requests stand
             // between them too, and with 8 bits what becomes operands.
-            constexpr int kAhead = E8 ? 3 : 4;
-            auto between = [&](int i, const f32x16_t (&s)[NS], f32x16_t (&next)[NS], uint32_t (&wt)[NS][2][4], auto first, auto extra, auto convert) __attribute__((always_inline)) {
+            constexpr int kAhead = 4, EXTRAS = E8 ? 4 : LOADS;
+            auto between = [&](int i, const f32x16_t (&s)[NS], f32x16_t (&next)[NS], uint32_t (&wt)[NS][2][4], auto first, auto extra) __attribute__((always_inline)) {
                 constexpr bool PV = !decltype(first)::value;
                 constexpr int NQ = NS * F::NK, OPS = PV ? 2 * NQ : NQ, PAIRS = 8 * NS;
                 static_assert(NS * 2 * F::ND == NQ && F::NK % 4 == 0, "as many of each");
@@ -813,14 +809,10 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
                             next[st] = mfma32(ring[x % kAhead], w.q[0][kk], next[st]);
                         }
                         __builtin_amdgcn_sched_barrier(0);
+                        constexpr int EACH = (EXTRAS + OPS - 1) / OPS;
 #pragma unroll
-                        for (int k = 0; k < LOADS; ++k)
-                            if (k * OPS / LOADS == x) extra(k);
-                        if (E8) {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (k * OPS / 4 == x) convert(k);
-                        }
+                        for (int k = EACH * x; k < EACH * (x + 1); ++k)
+                            if (k < EXTRAS) extra(k);
                     }
                     if constexpr (PV) {
                         constexpr int SP = OPS / PAIRS;  // MFMAs to a pair
@@ -841,29 +833,27 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
                 return sum[0] + sum[1];
             };
             auto tile = [&](int i, f32x16_t (&s)[NS], f32x16_t (&next)[NS], auto first) __attribute__((always_inline)) {
-                wait_vmcnt<E8 ? LOADS : (L::NST - 2) * LOADS>();
-                lds_barrier_dma_in_flight();
-                const int pk = phys[KA], pv_ = phys[VA];
-                const u32x4_t rk = source(i + KA, pk, false), rv = source(i + VA, pv_, true);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) phys[x] = phys[x + 1];
-                phys[4] = page(i + 5);
-                Codes ck, cv;
+                turn();
+                const int p0 = phys[0], p1 = phys[1], p2 = phys[2], p3 = page(i + 3);
+                const u32x4_t rk = source(i + 2, p2, false), rv = source(i, p0, true);
+                phys[0] = p1;
+                phys[1] = p2;
+                phys[2] = p3;
                 auto extra = [&](int k) __attribute__((always_inline)) {
-                    if (k < NPER) load(rk, i + KA, false, k);
-                    else if (k < 2 * NPER) load(rv, i + VA, true, k - NPER);
-                    else load_scales(i + KA, pk);
-                };
-                auto convert = [&](int k) __attribute__((always_inline)) {
-                    if (k == 0) ck = codes(i + 2, false);
-                    if (k == 1) widen(ck, i + 2, false);
-                    if (k == 2) cv = codes(i, true);
-                    if (k == 3) widen(cv, i, true);
+                    if (!E8) {
+                        if (k < PER) load(rk, i + 2, false, k);
+                        else load(rv, i, true, k - PER);
+                        return;
+                    }
+                    if (k == 0) put(i + 2, false);
+                    if (k == 1) fetch(i + 3, p3, false);
+                    if (k == 2) put(i, true);
+                    if (k == 3) fetch(i + 1, p1, true);
                 };
                 if (!first.value && edge(i - 1)) check_v(i - 1);
                 form(s, i);
                 const float c = w.raise(s);
-                const float sum = between(i, s, next, wt, first, extra, convert);
+                const float sum = between(i, s, next, wt, first, extra);
                 w.rescale(c);
                 w.l += sum;
             };
@@ -874,8 +864,7 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
                 tile(i + 1, s[0], s[1], std::false_type{});
             }
             if (i < i1) tile(i, s[1], s[0], std::false_type{});
-            wait_dma();
-            lds_barrier_dma_in_flight();
+            turn();
             if (edge(i1 - 1)) check_v(i1 - 1);
             vec8 last[PARTS][NS][2];
 #pragma unroll
@@ -885,66 +874,70 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
             }
             pv(last, i1 - 1);
         } else {
-            // Parts take the registers: one tile after another.  At the turn in front of tile i its K and V are there for every wave (8 bits:
-            // the codes of the next tile's, which become operands behind it), and what the last turn read is free.
-            constexpr int AHEAD = E8 ? 3 : L::NST - 1;  // a turn requests K and V of tile i + AHEAD
-            int phys[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) phys[x] = page(i0 + x);
-#pragma unroll
-            for (int x = 0; x < AHEAD; ++x) {
-                request(i0 + x, phys[x], false);
-                request(i0 + x, phys[x], true);
-            }
+            // Parts take the registers: one step after another.
+            int phys = page(i0 + 1);
+            const int p0 = page(i0);
             if (E8) {
-                wait_vmcnt<2 * LOADS>();
-                lds_barrier_dma_in_flight();
-                widen(codes(i0, false), i0, false);
-                widen(codes(i0, true), i0, true);
+                fetch(i0, p0, false);
+                fetch(i0, p0, true);
+                w.load_q(p);
+                put(i0, false);
+                put(i0, true);
+                fetch(i0 + 1, phys, false);
+                fetch(i0 + 1, phys, true);
+                phys = page(i0 + 2);
+            } else {
+                request(i0, p0, false);
+                request(i0, p0, true);
+                w.load_q(p);
             }
             for (int i = i0; i < i1; ++i) {
-                wait_vmcnt<E8 ? LOADS : (AHEAD - 1) * LOADS>();
-                lds_barrier_dma_in_flight();
-                request(i + AHEAD, phys[AHEAD], false);
-                request(i + AHEAD, phys[AHEAD], true);
-#pragma unroll
-                for (int x = 0; x < 3; ++x) phys[x] = phys[x + 1];
-                phys[3] = page(i + 4);
+                turn();
                 if (E8) {
-                    widen(codes(i + 1, false), i + 1, false);
-                    widen(codes(i + 1, true), i + 1, true);
+                    put(i + 1, false);
+                    put(i + 1, true);
+                    fetch(i + 2, phys, false);
+                    fetch(i + 2, phys, true);
+                    phys = page(i + 3);
+                } else {
+                    request(i + 1, phys, false);
+                    request(i + 1, phys, true);
+                    phys = page(i + 2);
                 }
-                f32x16_t s[NS];
-                qk(s, i);
-                form(s, i);
                 if (edge(i)) check_v(i);
-                vec8 wt[PARTS][NS][2];
-                w.softmax(s, wt, v_scale(i));
-                pv(wt, i);
+#pragma unroll 1
+                for (st0 = wave / RW; st0 < wave / RW + STEPS; ++st0) {
+                    f32x16_t s[NS];
+                    qk(s, i);
+                    form(s, i);
+                    vec8 wt[PARTS][NS][2];
+                    w.softmax(s, wt, v_scale(i));
+                    pv(wt, i);
+                }
             }
         }
     }
     w.l = sum_xor32(w.l);
-    merge_waves<F, RW, 8 / RW>(p, it, un, w, rw, wave / RW, lds, rest);
+    merge_waves<F, RW, 4 / RW>(p, it, un, w, rw, wave / RW, lds, rest);
 }
 
 // Items of both sorts in one launch: what one leaves of HBM or the MFMAs the other takes (64 rows behind 8192 shared positions
 // and their own keys).
 template <int CT, int D, int PARTS, int SCORES>
-__global__ void __launch_bounds__(512, 1) forms_mfma_kernel(const FormsK p) {
-    using L = FormRings<CT, D>;
+__global__ void __launch_bounds__(256, 2) forms_mfma_kernel(const FormsK p) {
+    using L = FormRings<D>;
     __shared__ __attribute__((aligned(1024))) char lds[L::LDS];
     __shared__ __attribute__((aligned(16))) char rest[L::REST];
     const FormItem it = p.it[form_find(p, blockIdx.x)];
     const int u = blockIdx.x - it.unit0;
     if (it.kind == kFormStream) forms_stream<CT, D, PARTS, SCORES>(p, it, u, lds, rest);
-    else if (PARTS > 1 || it.kind == kFormTilesHalf) forms_tile<CT, D, PARTS, SCORES, 4>(p, it, u, lds, rest);
-    else if constexpr (PARTS == 1) forms_tile<CT, D, PARTS, SCORES, 8>(p, it, u, lds, rest);
+    else if (it.kind == kFormTilesHalf) forms_tile<CT, D, PARTS, SCORES, 2>(p, it, u, lds, rest);
+    else forms_tile<CT, D, PARTS, SCORES, 4>(p, it, u, lds, rest);
 }
 template <int CT, int D, int PARTS> hipError_t form_launch_scores(const FormsK& k, int units, hipStream_t s) {
-    if (k.cap > 0.f) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresCap>), dim3(units), dim3(512), 0, s, k);
-    else if (k.slopes) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresSlope>), dim3(units), dim3(512), 0, s, k);
-    else hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresPlain>), dim3(units), dim3(512), 0, s, k);
+    if (k.cap > 0.f) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresCap>), dim3(units), dim3(256), 0, s, k);
+    else if (k.slopes) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresSlope>), dim3(units), dim3(256), 0, s, k);
+    else hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresPlain>), dim3(units), dim3(256), 0, s, k);
     return hipGetLastError();
 }
 // Queries that the tile's type holds enter as one part, others as two of fp16 or three of bf16.
