@@ -15,11 +15,11 @@ constexpr int kThreads = 256;
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads) forms_merge_kernel(const FormsK p, int rows) {
     const long long at = static_cast<long long>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
-    const int row = __builtin_amdgcn_readfirstlane(static_cast<int>(at / p.heads)), h = __builtin_amdgcn_readfirstlane(static_cast<int>(at % p.heads));
-    if (row >= rows) return;
-    const int e = batch_find(p.chunks, row, [&](int i) { return p.c[i].row0; });
+    const int of = __builtin_amdgcn_readfirstlane(static_cast<int>(at / p.heads)), h = __builtin_amdgcn_readfirstlane(static_cast<int>(at % p.heads));
+    if (of >= rows) return;
+    const int e = batch_find(p.chunks, of, [&](int i) { return p.c[i].full; });  // (here a chunk's first row of the merge)
     const FormRows c = p.c[e];
-    if (c.parts == 1) return;
+    const int row = c.row0 + of - c.full;
     const int D = p.geom.head_dim, lane = threadIdx.x & 63;
     const long long slot = c.slot0 + (static_cast<long long>(row - c.row0) * p.heads + h) * c.parts;
     const long long to = (static_cast<long long>(row) * p.heads + h) * D;
@@ -161,7 +161,7 @@ float best_part(const FormsArgs& a, const FormsPlan& p, const Sample* smp, int n
             const long long rows = static_cast<long long>(it.rows) * (a.heads / kv);
             if (c > 1 || p.c[it.c0].parts) parts += smp[i].units * c * static_cast<float>(std::min<long long>(form_rows(it.kind), rows));
         }
-        const float run = used <= kCus ? longest : std::max(longest, busy / kCus + 0.5f * longest);
+        const float run = used <= kCus ? longest : std::max(longest, busy / kCus + 0.25f * longest);
         return run + parts * partial + (parts > 0.f ? 4.f : 0.f);
     };
     float best = whole, least = cost(whole);
@@ -173,7 +173,7 @@ float best_part(const FormsArgs& a, const FormsPlan& p, const Sample* smp, int n
         }
     };
     const float even = work / kCus;
-    for (const float f : {0.5f, 0.7f, 0.85f, 1.f, 1.04f, 1.08f, 1.15f, 1.25f, 1.4f, 1.7f, 2.f, 3.f})
+    for (const float f : {0.35f, 0.5f, 0.7f, 0.85f, 1.f, 1.04f, 1.08f, 1.15f, 1.25f, 1.4f, 1.7f, 2.f, 3.f})
         if (even * f < whole) consider(even * f);
     // (the partials of a launch stay below 256 MB: 64 bf16 sequences of 8 rows behind 65536 positions)
     for (;; best *= 1.25f) {
@@ -263,6 +263,7 @@ FormsPlan plan_forms(const FormsArgs& a) {
         if (x == 0 || smp[x - 1].item != smp[x].item) it.splits = 1;
         it.splits = std::max(it.splits, (smp[x].tiles + per - 1) / per);
         it.per = it.nc == 1 ? per : 0;
+        p.us[smp[x].item] = std::max(p.us[smp[x].item], shape_of(a, it.kind).tile * static_cast<float>(std::min(per, smp[x].tiles)));
     }
     for (int i = 0; i < a.n; ++i) p.c[i].parts = 0;
     for (int i = 0; i < p.n; ++i) {
@@ -301,26 +302,41 @@ hipError_t launch_forms(const FormsArgs& a, const FormsPlan& plan, void* workspa
     k.part_acc = static_cast<float*>(workspace);
     k.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + plan.part_ml);
     const int g = (a.heads + a.geom.kv_heads - 1) / a.geom.kv_heads;
+    // the longest units first
+    int order[kFormItems];
+    float us[kFormItems];
+    for (int i = 0; i < plan.n; ++i) {
+        order[i] = i;
+        us[i] = plan.us[i];
+    }
+    std::sort(order, order + plan.n, [&](int x, int y) { return us[x] != us[y] ? us[x] > us[y] : x < y; });
     int units = 0;
-    for (int pass = 0; pass < 2; ++pass)  // the items of many rows first: theirs are the longest units
-        for (int i = 0; i < plan.n; ++i) {
-            if ((plan.it[i].kind != kFormStream && plan.it[i].kind != kFormF32Half) != (pass == 0)) continue;
-            FormItem& it = k.it[k.n++] = plan.it[i];
-            it.unit0 = units;
-            int n = it.blocks * it.splits;
-            if (it.per && it.splits > 1) {
-                n = 0;
-                for (int b = 0; b < it.blocks; ++b) n += form_parts(it, k.c[it.c0], a.window, g, form_rows(it.kind), form_tile(it.kind), b);
-            }
-            units += n * a.geom.kv_heads;
+    for (int i = 0; i < plan.n; ++i) {
+        FormItem& it = k.it[k.n++] = plan.it[order[i]];
+        it.unit0 = units;
+        int n = it.blocks * it.splits;
+        if (it.per && it.splits > 1) {
+            n = 0;
+            for (int b = 0; b < it.blocks; ++b) n += form_parts(it, k.c[it.c0], a.window, g, form_rows(it.kind), form_tile(it.kind), b);
         }
+        units += n * a.geom.kv_heads;
+    }
     const hipError_t e = launch(k, units, stream);
     if (e != hipSuccess) return e;
     if (plan.merge) {
-        const long long waves = static_cast<long long>(a.rows) * a.heads;
+        // the chunks whose rows have several parts
+        k.chunks = 0;
+        int rows = 0;
+        for (int i = 0; i < a.n; ++i) {
+            if (plan.c[i].parts == 1) continue;
+            FormRows& c = k.c[k.chunks++] = plan.c[i];
+            c.full = rows;  // (its first row of the merge)
+            rows += c.rows;
+        }
+        const long long waves = static_cast<long long>(rows) * a.heads;
         const dim3 grid(static_cast<unsigned>((waves + 3) / 4));
-        if (a.geom.head_dim == 64 || a.geom.head_dim == 128) hipLaunchKernelGGL(forms_merge_kernel<true>, grid, dim3(kThreads), 0, stream, k, a.rows);
-        else hipLaunchKernelGGL(forms_merge_kernel<false>, grid, dim3(kThreads), 0, stream, k, a.rows);
+        if (a.geom.head_dim == 64 || a.geom.head_dim == 128) hipLaunchKernelGGL(forms_merge_kernel<true>, grid, dim3(kThreads), 0, stream, k, rows);
+        else hipLaunchKernelGGL(forms_merge_kernel<false>, grid, dim3(kThreads), 0, stream, k, rows);
         return hipGetLastError();
     }
     return hipSuccess;

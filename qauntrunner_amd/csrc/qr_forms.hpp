@@ -85,6 +85,7 @@ struct FormsK {
 // How a call's work is cut.
 struct FormsPlan {
     FormItem it[kFormItems];
+    float us[kFormItems];    // of an item's longest unit, by the plan
     int n;
     FormRows c[kBatch];
     size_t part_ml;          // offset in the workspace; the partials' sums come first

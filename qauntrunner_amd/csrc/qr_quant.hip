@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(const NormRopeArgs 
     }
     __syncthreads();
     const int D = a.geom.head_dim, kvh = a.geom.kv_heads;
-    const int pos = a.it[e].pos0 + j, slot = pos & (kPageTokens - 1);
+    const int pos = a.it[e].pos0 + j, scalet = pos & (kPageTokens - 1);
     const long long phys = a.page_table[a.it[e].pt_off + (pos >> kPageShift)];
     uint8_t* const pool = static_cast<uint8_t*>(a.pool);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -104,9 +104,9 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(const NormRopeArgs 
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const float x = quant_round(ldexp(y[c], -ex));
-            if (lane + 64 * c < D) pool[a.geom.offset(phys, is_v, hh, slot, lane + 64 * c)] = quant4(x, 0.f, 0.f, 0.f) & 0xFF;
+            if (lane + 64 * c < D) pool[a.geom.offset(phys, is_v, hh, scalet, lane + 64 * c)] = quant4(x, 0.f, 0.f, 0.f) & 0xFF;
         }
-        if (lane == 0) pool[a.geom.scale_offset(phys, is_v, hh, slot)] = ex + 127;
+        if (lane == 0) pool[a.geom.scale_offset(phys, is_v, hh, scalet)] = ex + 127;
     }
 }
 
@@ -114,14 +114,14 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(const NormRopeArgs 
 __global__ void __launch_bounds__(kThreads) read_as_any_kernel(const ReadArgs a) {
     const int row = blockIdx.x;
     const int e = batch_find(a.n, row, [&](int i) { return a.it[i].row0; });
-    const int pos = a.it[e].pos0 + row - a.it[e].row0, slot = pos & (kPageTokens - 1);
+    const int pos = a.it[e].pos0 + row - a.it[e].row0, scalet = pos & (kPageTokens - 1);
     const long long phys = a.page_table[a.it[e].pt_off + (pos >> kPageShift)];
     const int D = a.geom.head_dim, width = a.geom.kv_heads * D;
     const uint8_t* const bytes = static_cast<const uint8_t*>(a.pool);
     for (int i = threadIdx.x; i < 2 * width; i += kThreads) {
         const int plane = i >= width, c = i - plane * width;
-        const long long from = a.geom.offset(phys, plane, c / D, slot, c % D);
-        const float x = a.geom.scaled() ? quant_value<0>(bytes[from]) * scale_of(bytes[a.geom.scale_offset(phys, plane, c / D, slot)])
+        const long long from = a.geom.offset(phys, plane, c / D, scalet, c % D);
+        const float x = a.geom.scaled() ? quant_value<0>(bytes[from]) * scale_of(bytes[a.geom.scale_offset(phys, plane, c / D, scalet)])
                                       : load_elem(a.pool, a.dtype, from);
         store_out(plane ? a.v : a.k, a.act, static_cast<long long>(row) * width + c, x);
     }
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) quant_kernel(const NormRopeArgs a, i
     const int kv = a.geom.kv_heads;
     const int row = blockIdx.x;
     const int e = batch_find(a.n, row, [&](int i) { return a.it[i].row0; });
-    const int j = row - a.it[e].row0, pos = a.it[e].pos0 + j, slot = pos & (kPageTokens - 1);
+    const int j = row - a.it[e].row0, pos = a.it[e].pos0 + j, scalet = pos & (kPageTokens - 1);
     const int qh = a.q ? a.heads : 0, heads = kv + qh + v_heads;
     const int li = threadIdx.x & (LPH - 1);
     const bool pair = 8 * li < a.rot;
@@ -269,14 +269,14 @@ __global__ void __launch_bounds__(kThreads) quant_kernel(const NormRopeArgs a, i
         for (int i = 0; i < 8; ++i) y[i] = quant_round(x[i] * unit);
         const uint32_t c[2] = {quant4(y[0], y[1], y[2], y[3]), quant4(y[4], y[5], y[6], y[7])};
         if (is_k) {
-            *reinterpret_cast<uint32_t*>(pool + a.geom.offset(phys, 0, hh, slot, at_a)) = c[0];
-            *reinterpret_cast<uint32_t*>(pool + a.geom.offset(phys, 0, hh, slot, at_b)) = c[1];
+            *reinterpret_cast<uint32_t*>(pool + a.geom.offset(phys, 0, hh, scalet, at_a)) = c[0];
+            *reinterpret_cast<uint32_t*>(pool + a.geom.offset(phys, 0, hh, scalet, at_b)) = c[1];
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                pool[a.geom.offset(phys, 1, hh, slot, (i < 4 ? at_a : at_b - 4) + i)] = static_cast<uint8_t>(c[i >> 2] >> (8 * (i & 3)));
+                pool[a.geom.offset(phys, 1, hh, scalet, (i < 4 ? at_a : at_b - 4) + i)] = static_cast<uint8_t>(c[i >> 2] >> (8 * (i & 3)));
         }
-        if (li == 0) pool[a.geom.scale_offset(phys, !is_k, hh, slot)] = ex + 127;
+        if (li == 0) pool[a.geom.scale_offset(phys, !is_k, hh, scalet)] = ex + 127;
     }
 }
 
@@ -290,7 +290,7 @@ __device__ __forceinline__ void transpose4(const uint32_t (&x)[4], uint32_t (&y)
     y[3] = __builtin_amdgcn_perm(d, b, 0x07060302);
 }
 
-// V by runs of 16 slots, which are 16 bytes of a dim in the page: a workgroup takes a run of 256 / (D / 8) heads' rows, 8 values
+// V by runs of 16 scalets, which are 16 bytes of a dim in the page: a workgroup takes a run of 256 / (D / 8) heads' rows, 8 values
 // per thread, and hands the codes through LDS to threads of 4 dims each.  Slots outside the chunk are left alone.
 template <int ACT, int D>
 __global__ void __launch_bounds__(kThreads) quant_v_kernel(const NormRopeArgs a) {
@@ -355,33 +355,36 @@ __global__ void __launch_bounds__(kThreads) quant_v_kernel(const NormRopeArgs a)
     }
 }
 
-// 4 codes of a scale as 4 values of dtype T at o (element-aligned).
-template <int T> __device__ __forceinline__ void widen4(uint32_t c, float scale, void* o) {
+// 8 codes of a scale as 8 values of dtype T at o (element-aligned).
+template <int T> __device__ __forceinline__ void widen8(uint32_t lo, uint32_t hi, float scale, void* o) {
     if constexpr (T == QR_DTYPE_BF16) {
         typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-        const bf16x2 y[2] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, true)};
-        __builtin_memcpy(o, y, 8);
+        const bf16x2 y[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true),
+                             __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true)};
+        __builtin_memcpy(o, y, 16);
     } else {
-        const float x[4] = {quant_value<0>(c) * scale, quant_value<1>(c) * scale, quant_value<2>(c) * scale, quant_value<3>(c) * scale};
+        const float x[8] = {quant_value<0>(lo) * scale, quant_value<1>(lo) * scale, quant_value<2>(lo) * scale, quant_value<3>(lo) * scale,
+                            quant_value<0>(hi) * scale, quant_value<1>(hi) * scale, quant_value<2>(hi) * scale, quant_value<3>(hi) * scale};
         if constexpr (T == QR_DTYPE_F32) {
-            __builtin_memcpy(o, x, 16);
+            __builtin_memcpy(o, x, 32);
         } else {
-            uint16_t b[4];
+            uint16_t b[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) b[i] = f32_to_out16(x[i], T);
-            __builtin_memcpy(o, b, 8);
+            for (int i = 0; i < 8; ++i) b[i] = f32_to_out16(x[i], T);
+            __builtin_memcpy(o, b, 16);
         }
     }
 }
 
-// Rows of the 8-bit operand layout back as values: a workgroup takes 128 slots of a kv head, K by 16 dims of a slot per thread, V
-// by 4 dims of 16 slots (64 bytes of the page), whose codes are transposed in registers.
+// Rows of the 8-bit operand layout back as values: a workgroup takes 128 scalets of a kv head, K by 16 dims of a scalet per thread (the
+// D / 16 threads of a scalet beside each other: whole lines of the page, whole rows of the output), V by 8 dims of 8 scalets, whose
+// codes are transposed in registers.
 constexpr int kReadRun = 128;
 template <int T, int D>
 __global__ void __launch_bounds__(kThreads) read_as_kernel(const ReadArgs a) {
     typedef typename std::conditional<T == QR_DTYPE_F32, float, uint16_t>::type E;
-    constexpr int KP = kReadRun * D / 16 / kThreads;  // pieces of K per thread
-    constexpr int VT = kReadRun / 16 * D / 4;         // threads that take V
+    constexpr int P = D / 16, KP = kReadRun * P / kThreads;  // pieces of a scalet; of K per thread
+    static_assert(kReadRun / 8 * (D / 8) <= kThreads, "threads that take V");
     const int e = batch_find(a.n, blockIdx.x, [&](int i) { return a.it[i].unit0; });
     const ReadItem it = a.it[e];
     const int kv = a.geom.kv_heads, u = blockIdx.x - it.unit0, kvh = u % kv;
@@ -395,56 +398,56 @@ __global__ void __launch_bounds__(kThreads) read_as_kernel(const ReadArgs a) {
     auto row = [&](void* to, int t) __attribute__((always_inline)) {
         return static_cast<E*>(to) + (static_cast<long long>(it.row0 + p0 + t - it.pos0) * kv + kvh) * D;
     };
-    uint4 kc[KP], vc[4], vs;
+    uint4 kc[KP];
     uint32_t ks[KP];
     int kt[KP];
+    const int piece = threadIdx.x % P;  // dims 16 piece ..
 #pragma unroll
     for (int c = 0; c < KP; ++c) {
-        const int x = threadIdx.x + kThreads * c, m = x & 31;  // piece x: step x / (2 D), lane x % 64
-        kt[c] = 32 * (x / (2 * D)) + 16 * (m >> 2 & 1) + 8 * (m >> 4) + 4 * (m >> 3 & 1) + (m & 3);
+        const int x = threadIdx.x / P + kThreads / P * c, m = x & 31;  // step x / 32, row m of it
+        kt[c] = 32 * (x >> 5) + 16 * (m >> 2 & 1) + 8 * (m >> 4) + 4 * (m >> 3 & 1) + (m & 3);
         if (p0 + kt[c] >= it.pos0 && p0 + kt[c] < end) {
-            kc[c] = *reinterpret_cast<const uint4*>(k + 16 * x);
+            kc[c] = *reinterpret_cast<const uint4*>(k + (x >> 5) * 32 * D + 1024 * (piece >> 1) + 16 * (32 * (piece & 1) + m));
             ks[c] = scales[kt[c]];
         }
     }
-    const int run = threadIdx.x / (D / 4), n = threadIdx.x % (D / 4);  // slots 16 run .., dims 4 n ..
-    const bool takes = static_cast<int>(threadIdx.x) < VT && p0 + 16 * run < end && p0 + 16 * run + 16 > it.pos0;
+    const int run = threadIdx.x / (D / 8), n = threadIdx.x % (D / 8);  // scalets 8 run .., dims 8 n ..
+    const bool takes = run < kReadRun / 8 && p0 + 8 * run < end && p0 + 8 * run + 8 > it.pos0;
+    uint2 vc[8], vs;
     if (takes) {
-        const uint8_t* b = v + (run >> 1) * 32 * D + 1024 * (n >> 3) + 16 * (32 * (run & 1) + 4 * (n & 7));
+        const uint8_t* b = v + (run >> 2) * 32 * D + 1024 * (n >> 2) + 16 * (32 * (run >> 1 & 1) + 8 * (n & 3)) + 8 * (run & 1);
 #pragma unroll
-        for (int d = 0; d < 4; ++d) vc[d] = *reinterpret_cast<const uint4*>(b + 16 * d);
-        vs = *reinterpret_cast<const uint4*>(scales + kv * kPageTokens + 16 * run);
+        for (int d = 0; d < 8; ++d) vc[d] = *reinterpret_cast<const uint2*>(b + 16 * d);
+        vs = *reinterpret_cast<const uint2*>(scales + kv * kPageTokens + 8 * run);
     }
 #pragma unroll
     for (int c = 0; c < KP; ++c) {
         if (p0 + kt[c] < it.pos0 || p0 + kt[c] >= end) continue;
-        const int x = threadIdx.x + kThreads * c;
-        E* o = row(a.k, kt[c]) + 32 * (x / 64 % (D / 32)) + 16 * (x >> 5 & 1);
+        E* o = row(a.k, kt[c]) + 16 * piece;
         const float scale = scale_of(ks[c]);
-        const uint32_t w[4] = {kc[c].x, kc[c].y, kc[c].z, kc[c].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) widen4<T>(w[i], scale, o + 4 * i);
+        widen8<T>(kc[c].x, kc[c].y, scale, o);
+        widen8<T>(kc[c].z, kc[c].w, scale, o + 8);
     }
     if (!takes) return;
-    const uint32_t w[4][4] = {{vc[0].x, vc[0].y, vc[0].z, vc[0].w}, {vc[1].x, vc[1].y, vc[1].z, vc[1].w}, {vc[2].x, vc[2].y, vc[2].z, vc[2].w},
-                              {vc[3].x, vc[3].y, vc[3].z, vc[3].w}};
-    const uint32_t sc[4] = {vs.x, vs.y, vs.z, vs.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t x[4] = {w[0][i], w[1][i], w[2][i], w[3][i]};
-        uint32_t y[4];
-        transpose4(x, y);
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t lo[4] = {i ? vc[0].y : vc[0].x, i ? vc[1].y : vc[1].x, i ? vc[2].y : vc[2].x, i ? vc[3].y : vc[3].x};
+        const uint32_t hi[4] = {i ? vc[4].y : vc[4].x, i ? vc[5].y : vc[5].x, i ? vc[6].y : vc[6].x, i ? vc[7].y : vc[7].x};
+        uint32_t y[4], z[4];
+        transpose4(lo, y);
+        transpose4(hi, z);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const int p = p0 + 16 * run + 4 * i + t;
-            if (p >= it.pos0 && p < end) widen4<T>(y[t], scale_of(sc[i] >> (8 * t) & 0xFF), row(a.v, 16 * run + 4 * i + t) + 4 * n);
+            const int p = p0 + 8 * run + 4 * i + t;
+            const float scale = scale_of((i ? vs.y : vs.x) >> (8 * t) & 0xFF);
+            if (p >= it.pos0 && p < end) widen8<T>(y[t], z[t], scale, row(a.v, 8 * run + 4 * i + t) + 8 * n);
         }
     }
 }
 
 template <int ACT, int D> void launch_rows(NormRopeArgs& a, hipStream_t s) {
     constexpr int LPH = D / 8, GROUPS = kThreads / LPH / 16;
-    // V goes by runs of 16 slots unless the chunks have few rows: single bytes otherwise, but one launch
+    // V goes by runs of 16 scalets unless the chunks have few rows: single bytes otherwise, but one launch
     const bool runs = a.rows >= 4 * a.n;
     if (runs) {
         int groups = 0;
@@ -456,8 +459,8 @@ template <int ACT, int D> void launch_rows(NormRopeArgs& a, hipStream_t s) {
         hipLaunchKernelGGL((quant_v_kernel<ACT, D>), dim3(groups), dim3(kThreads), 0, s, a);
     }
     const int v_heads = runs ? 0 : a.geom.kv_heads, heads = a.geom.kv_heads + (a.q ? a.heads : 0) + v_heads;
-    const int slots = (heads * LPH + kThreads - 1) / kThreads, ipt = std::min(slots, 4);
-    const dim3 grid(a.rows, (slots + ipt - 1) / ipt);
+    const int scalets = (heads * LPH + kThreads - 1) / kThreads, ipt = std::min(scalets, 4);
+    const dim3 grid(a.rows, (scalets + ipt - 1) / ipt);
     if (ipt == 1) hipLaunchKernelGGL((quant_kernel<ACT, D, 1>), grid, dim3(kThreads), 0, s, a, v_heads);
     else if (ipt == 2) hipLaunchKernelGGL((quant_kernel<ACT, D, 2>), grid, dim3(kThreads), 0, s, a, v_heads);
     else if (ipt == 3) hipLaunchKernelGGL((quant_kernel<ACT, D, 3>), grid, dim3(kThreads), 0, s, a, v_heads);
