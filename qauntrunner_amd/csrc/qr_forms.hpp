@@ -215,7 +215,7 @@ __device__ __forceinline__ float form_score(float z, float cap, float slope, flo
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
-enum FormScores { kScoresPlain, kScoresSlope, kScoresCap };  // (capped scores may have a slope too)
+enum FormScores { kScoresPlain, kScoresSlope, kScoresCap, kScoresBoth };
 
 // Page of a slot, by a scalar load (no kernel writes the table while this one runs).
 __device__ __forceinline__ int form_page(const FormsK& p, int pt_off, int t) {

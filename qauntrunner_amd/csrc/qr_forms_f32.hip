@@ -46,7 +46,7 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
         lo[t] = s.lo;
         hi[t] = on[t] ? s.hi : -1;
         away[t] = static_cast<float>(s.pos - it.base);
-        slope[t] = SCORES != kScoresPlain && p.slopes ? p.slopes[head[t]] * kLog2e : 0.f;
+        slope[t] = SCORES == kScoresSlope || SCORES == kScoresBoth ? p.slopes[head[t]] * kLog2e : 0.f;
         if (lo[t] <= hi[t]) {
             range.lo = min(range.lo, lo[t]);
             range.hi = max(range.hi, hi[t]);
@@ -87,10 +87,21 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const long long at = (static_cast<long long>(row[t]) * p.heads + head[t]) * D + 4 * Q;
+        if (p.act == QR_DTYPE_F32) {
 #pragma unroll
-        for (int j = 0; j < NK; ++j)
+            for (int j = 0; j < NK; ++j) __builtin_memcpy(&q[t][j], static_cast<const float*>(p.q) + at + 16 * j, 16);
+        } else {
+            uint16_t x[NK][4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) q[t][j][c] = load_elem(p.q, p.act, at + 16 * j + c) * p.qscale;
+            for (int j = 0; j < NK; ++j) __builtin_memcpy(x[j], static_cast<const uint16_t*>(p.q) + at + 16 * j, 8);
+            const bool bf = p.act == QR_DTYPE_BF16;
+#pragma unroll
+            for (int j = 0; j < NK; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) q[t][j][c] = bf ? bf16_bits_to_f32(x[j][c]) : f16_bits_to_f32(x[j][c]);
+        }
+#pragma unroll
+        for (int j = 0; j < NK; ++j) q[t][j] *= p.qscale;
     }
     float m[RT], l[RT];
     f32x4_t acc[RT][NJ][4];
@@ -125,8 +136,8 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
             const int t1 = t0 + 4 * Q;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                if (SCORES == kScoresCap) z[r] = p.cap * tanhf(z[r] / p.cap);
-                if (SCORES != kScoresPlain) z[r] = fmaf(-slope[t], fabsf(static_cast<float>(t1 + r) - away[t]), z[r]);
+                if (SCORES == kScoresCap || SCORES == kScoresBoth) z[r] = p.cap * tanhf(z[r] / p.cap);
+                if (SCORES == kScoresSlope || SCORES == kScoresBoth) z[r] = fmaf(-slope[t], fabsf(static_cast<float>(t1 + r) - away[t]), z[r]);
                 if (edge && (t1 + r < lo[t] || t1 + r > hi[t])) z[r] = -INFINITY;
             }
             const float top = max_xor32(max_xor16(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]))));
@@ -253,7 +264,8 @@ __global__ void __launch_bounds__(kThreads, 2) forms_f32_kernel(const FormsK p) 
     else forms_f32<D, 2, SCORES>(p, it, u, xa, xm);
 }
 template <int D> hipError_t launch_scores(const FormsK& k, int units, hipStream_t s) {
-    if (k.cap > 0.f) hipLaunchKernelGGL((forms_f32_kernel<D, kScoresCap>), dim3(units), dim3(kThreads), 0, s, k);
+    if (k.cap > 0.f && k.slopes) hipLaunchKernelGGL((forms_f32_kernel<D, kScoresBoth>), dim3(units), dim3(kThreads), 0, s, k);
+    else if (k.cap > 0.f) hipLaunchKernelGGL((forms_f32_kernel<D, kScoresCap>), dim3(units), dim3(kThreads), 0, s, k);
     else if (k.slopes) hipLaunchKernelGGL((forms_f32_kernel<D, kScoresSlope>), dim3(units), dim3(kThreads), 0, s, k);
     else hipLaunchKernelGGL((forms_f32_kernel<D, kScoresPlain>), dim3(units), dim3(kThreads), 0, s, k);
     return hipGetLastError();

@@ -43,6 +43,11 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
     return r;
 }
 
+__device__ __forceinline__ float max3abs(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, |%1|, |%2|, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 __device__ __forceinline__ void mfma_done(f32x16_t (&s)[1]) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s[0])); }
 __device__ __forceinline__ void mfma_done(f32x16_t (&s)[2]) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1])); }
 
@@ -94,6 +99,10 @@ struct FormTile {
     vec8 q[PARTS][NK];
     float sscale;          // log2 units per score
     float m, l;            // l: this lane's half of the positions
+    float cap[5], by[5];   // the capped score of a small s: s (cap[0] + cap[1] s^2 + ... + cap[4] s^8); what the tile takes
+    float small;           // |s| up to which it is
+    float hidden;          // what stands for a score that the row does not see
+    bool wide;             // the tile's scores are capped already
     f32x16_t acc[ND];
 
     __device__ __forceinline__ void init(const FormsK& p, const FormItem& it, int kvh, int g, int rho) {
@@ -110,9 +119,10 @@ struct FormTile {
         lo = s.lo;
         hi = on ? s.hi : -1;
         away = static_cast<float>(s.pos - it.base);
-        slope = SCORES != kScoresPlain && p.slopes ? p.slopes[head] * kLog2e : 0.f;
+        slope = SCORES == kScoresSlope || SCORES == kScoresBoth ? p.slopes[head] * kLog2e : 0.f;
         m = -INFINITY;
         l = 0.f;
+        hidden = -INFINITY;
 #pragma unroll
         for (int t = 0; t < ND; ++t)
 #pragma unroll
@@ -172,27 +182,74 @@ struct FormTile {
                     v -= static_cast<float>(q[c][kk][i]);
                 }
             }
+        init_cap(p);
     }
 
     // Position of score r within its step of 32.
     __device__ __forceinline__ int at(int r) const { return E8 ? 16 * half + r : 16 * (r >> 3) + 8 * half + (r & 7); }
 
-    // Scores of step t0 in log2 units (plain ones are scaled as they become weights), masked where some row does not see the
-    // whole step: `edge`.
+    // Capped scores without slopes ascend with the products, so that the maximum is taken of these, and a product becomes its
+    // capped score where it becomes a weight (PER_WEIGHT): 1 - 2 / (e^2x + 1) would be two more operations of a quarter of the rate
+    // for each, but scores are mostly far below the cap, and tanh x / x on |x| <= 1/2 is a polynomial of x^2 (least squares at
+    // Chebyshev's points, off by 6e-9; its last coefficient is positive, which leaves a masked product's -infinity).  Tiles with
+    // larger ones are capped in front, and the coefficients become those of s.
+    static constexpr bool PER_WEIGHT = SCORES == kScoresCap && !SPLIT;
+    __device__ __forceinline__ void init_cap(const FormsK& p) {
+        if (!PER_WEIGHT) return;
+        const float in = sscale / p.cap, i2 = in * in;
+        cap[0] = p.cap * in * 0.99999999f;
+        cap[1] = p.cap * in * i2 * -0.33333072f;
+        cap[2] = p.cap * in * i2 * i2 * 0.1332483f;
+        cap[3] = p.cap * in * i2 * i2 * i2 * -0.05298926f;
+        cap[4] = p.cap * in * i2 * i2 * i2 * i2 * 0.01714132f;
+        small = 0.5f / in;
+    }
+    __device__ __forceinline__ float capped(float s, float add) const {
+        const float x = s * s;
+        return fmaf(s, fmaf(fmaf(fmaf(fmaf(by[4], x, by[3]), x, by[2]), x, by[1]), x, by[0]), add);
+    }
+    // NS steps' products, from step t0 on, as `form` leaves them.
+    template <int NS>
+    __device__ __forceinline__ void prepare(const FormsK& p, f32x16_t (&s)[NS], int t0, bool edge) {
+        if (PER_WEIGHT) {
+            mfma_done(s);
+            float most = 0.f;
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) most = max3abs(s[n][r], s[n][r + 1], most);
+            wide = __builtin_amdgcn_ballot_w64(!(most <= small)) != 0;
+            hidden = wide ? -1e18f : -INFINITY;  // (0 x infinity would be no number)
+#pragma unroll
+            for (int i = 0; i < 5; ++i) by[i] = wide ? (i == 0 ? 1.f : 0.f) : cap[i];
+            if (wide) {
+                const float in = 2.f * kLog2e * sscale / p.cap;
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[n][r] = fmaf(-2.f * p.cap, __builtin_amdgcn_rcpf(fast_exp2(s[n][r] * in) + 1.f), p.cap);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NS; ++n) form(p, s[n], t0 + 32 * n, edge);
+    }
+
+    // Scores of step t0 in log2 units (plain ones are scaled as they become weights, those PER_WEIGHT capped too), masked where
+    // some row does not see the whole step: `edge`.
     __device__ __forceinline__ void form(const FormsK& p, f32x16_t& s, int t0, bool edge) const {
-        if (SCORES == kScoresCap) {
+        if ((SCORES == kScoresCap && !PER_WEIGHT) || SCORES == kScoresBoth) {
             // (for 16 bits 1 - 2 / (e^2x + 1): off by a few 2^-24 of the cap, far below the weights' rounding)
             const float in = (SPLIT ? 1.f : 2.f * kLog2e) * sscale / p.cap;
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 s[r] = SPLIT ? p.cap * tanhf(s[r] * in) : fmaf(-2.f * p.cap, __builtin_amdgcn_rcpf(fast_exp2(s[r] * in) + 1.f), p.cap);
         }
-        if (SCORES != kScoresPlain) {
+        if (SCORES == kScoresSlope || SCORES == kScoresBoth) {
             const float first = static_cast<float>(t0 + (E8 ? 16 : 8) * half) - away;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float d = fabsf(first + static_cast<float>(E8 ? r : 16 * (r >> 3) + (r & 7)));
-                s[r] = SCORES == kScoresCap ? fmaf(-slope, d, s[r]) : fmaf(s[r], sscale, -slope * d);
+                s[r] = SCORES == kScoresBoth ? fmaf(-slope, d, s[r]) : fmaf(s[r], sscale, -slope * d);
             }
         }
         if (edge) {
@@ -200,7 +257,7 @@ struct FormTile {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int x = E8 ? r : 16 * (r >> 3) + (r & 7);
-                if (x < a || x > b) s[r] = -INFINITY;
+                if (x < a || x > b) s[r] = hidden;
             }
         }
     }
@@ -222,6 +279,7 @@ struct FormTile {
 #pragma unroll
         for (int n = 1; n < 2 * NS; ++n) t = fmaxf(t, mx[n]);
         t = max_xor32(t);
+        if (PER_WEIGHT) t = wide ? (t > -1e17f ? t : -INFINITY) : capped(t, 0.f);
         const float by = SCORES == kScoresPlain ? sscale : 1.f;
         if (!(fmaf(t, by, -m) > kTop)) return 1.f;
         float mn = fmaf(t, by, kHead - kTop);
@@ -240,6 +298,10 @@ struct FormTile {
             for (int d = 0; d < ND; ++d) acc[d] *= c;
         }
     }
+    // What a weight is a power of 2 of.
+    __device__ __forceinline__ float logit(float s, float ref) const {
+        return SCORES == kScoresPlain ? fmaf(s, sscale, ref) : PER_WEIGHT ? capped(s, ref) : s + ref;
+    }
     // Weights of NS steps' scores, as PV operands (8 bits: times V's scales); their sum.
     template <int NS, class F>
     __device__ __forceinline__ float weigh(const f32x16_t (&s)[NS], vec8 (&w)[PARTS][NS][2], F vscale) const {
@@ -249,7 +311,7 @@ struct FormTile {
         for (int n = 0; n < NS; ++n)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float e = fast_exp2(SCORES == kScoresPlain ? fmaf(s[n][r], sscale, ref) : s[n][r] + ref);
+                const float e = fast_exp2(logit(s[n][r], ref));
                 sum[r & 3] += e;
                 float v = E8 ? e * vscale(n, r) : e;
 #pragma unroll
@@ -472,7 +534,7 @@ __device__ __forceinline__ void forms_stream(const FormsK& p, const FormItem& it
         __builtin_amdgcn_sched_barrier(0);
         if (st + 4 < s1) load_k(st + 4, phys);
         const bool edge = !range.all(32 * st, 32);
-        w.form(p, s[0], 32 * st, edge);
+        w.prepare(p, s, 32 * st, edge);
         if (edge) {
             bool bad = false;
 #pragma unroll
@@ -708,11 +770,7 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
     auto v_scale = [&](int i) {
         return [&, i](int n, int r) __attribute__((always_inline)) { return vscale[i & 3][32 * (st0 + n) + 16 * w.half + r]; };
     };
-    auto form = [&](f32x16_t (&s)[NS], int i) __attribute__((always_inline)) {
-        const bool e = edge(i);
-#pragma unroll
-        for (int st = 0; st < NS; ++st) w.form(p, s[st], TILE * i + 32 * (st0 + st), e);
-    };
+    auto form = [&](f32x16_t (&s)[NS], int i) __attribute__((always_inline)) { w.prepare(p, s, TILE * i + 32 * st0, edge(i)); };
     if (i0 < i1) {
         if constexpr (PARTS == 1) {
             // Tile i's softmax runs between the MFMAs of the scores of tile i + 1 and of V of tile i - 1: none of the three needs
@@ -776,8 +834,8 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
                     e[0] = s[n][r];
                     e[1] = s[n][r + 1];
                     asm volatile("" : "+v"(e[0]), "+v"(e[1]));  // not before the MFMA in front
-                    e[0] = fast_exp2(SCORES == kScoresPlain ? fmaf(e[0], w.sscale, ref) : e[0] + ref);
-                    e[1] = fast_exp2(SCORES == kScoresPlain ? fmaf(e[1], w.sscale, ref) : e[1] + ref);
+                    e[0] = fast_exp2(w.logit(e[0], ref));
+                    e[1] = fast_exp2(w.logit(e[1], ref));
                 };
                 auto end = [&](int y) __attribute__((always_inline)) {
                     const int n = y >> 3, r = 2 * (y & 7);
@@ -935,7 +993,8 @@ __global__ void __launch_bounds__(256, 2) forms_mfma_kernel(const FormsK p) {
     else forms_tile<CT, D, PARTS, SCORES, 4>(p, it, u, lds, rest);
 }
 template <int CT, int D, int PARTS> hipError_t form_launch_scores(const FormsK& k, int units, hipStream_t s) {
-    if (k.cap > 0.f) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresCap>), dim3(units), dim3(256), 0, s, k);
+    if (k.cap > 0.f && k.slopes) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresBoth>), dim3(units), dim3(256), 0, s, k);
+    else if (k.cap > 0.f) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresCap>), dim3(units), dim3(256), 0, s, k);
     else if (k.slopes) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresSlope>), dim3(units), dim3(256), 0, s, k);
     else hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresPlain>), dim3(units), dim3(256), 0, s, k);
     return hipGetLastError();
