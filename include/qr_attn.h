@@ -231,12 +231,12 @@ int qr_kv_attention_chunk_step_dev(qr_kv* kv, int seq_id, int layer, int nq, con
  * 2^-8 of a radian at position 131072).  k and v go to the chunk's slots, q to q_out
  * [rows][heads*head_dim].  On an 8-bit cache a row of head_dim values x (of k after norm and rotation, of v)
  * becomes codes c = e4m3(x / 2^e), to nearest even, with e the smallest exponent of -117..119 that keeps the
- * largest finite |x| at or below 448 2^e; the cache then holds the values c 2^e.  Infinities, and what is past 448 2^119, become 448 2^e of
- * their sign, NaN stays NaN.  k is normed and rotated in 64 bits before it is rounded, so that a value next to a
- * border between two codes rounds as the formulas say.  q, k, v: rows of `dtype`, q_stride / k_stride / v_stride elements from
- * one to the next (slices of one fused QKV product).  q and q_out may both be null; q_out may be
- * q where q's rows stand back to back, and must not overlap q, k or v otherwise.  No sequence
- * twice.  rotary_dim even, 0 to head_dim.  SeqLen grows as with qr_kv_append. */
+ * largest finite |x| at or below 448 2^e; the cache then holds the values c 2^e.  Infinities, and what is past
+ * 448 2^119, become 448 2^e of their sign, NaN stays NaN.  k is normed and rotated in 64 bits before it is
+ * rounded, so that a value next to a border between two codes rounds as the formulas say.
+ * q, k, v: rows of `dtype`, q_stride / k_stride / v_stride elements from one to the next (slices of one fused
+ * QKV product).  q and q_out may both be null; q_out may be q where q's rows stand back to back, and must not
+ * overlap q, k or v otherwise.  No sequence twice.  rotary_dim even, 0 to head_dim.  SeqLen grows as with qr_kv_append. */
 int qr_kv_append_norm_rope_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows,
                                const int* rope_pos0, const void* q_dev, long long q_stride, const void* k_dev,
                                long long k_stride, const void* v_dev, long long v_stride, int dtype, void* q_out_dev,
@@ -255,7 +255,7 @@ int qr_kv_attention_chunks_dev(qr_kv* kv, int n, const int* seq_ids, int layer, 
  * chunk's prefix (prefix_len[i] of them) and then its own sequence, whose slot t is position prefix_len[i] + t; a row at
  * slot s of its sequence stands at position P = prefix_len[i] + s. */
 typedef struct qr_attn_form {
-    float cap;               /* above 0: scores z become cap * tanh(z / cap) */
+    float cap;               /* 0.001 to 1000000: scores z become cap * tanh(z / cap); 0: they stay */
     const float* slopes_dev; /* device, [heads]: slopes[h] * |P - t| is taken from a (capped) score; null: nothing */
     int window;              /* above 0: a row sees t > P - window only */
     /* host arrays of one entry per chunk; null: zeros */

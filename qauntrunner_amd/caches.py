@@ -503,7 +503,7 @@ class PagedKvCache:
 
     def AttentionFormsDev(self, layer, seq_ids, pos0, rows, q, out, scale, cap=0.0, slopes=None, window=0, first=None,
                           full=None, prefix_ids=None, prefix_len=None, stream=None) -> None:
-        """AttentionChunksDev in other forms (qr_attn_form): scores capped to cap * tanh(z / cap), less slopes[h] (float32
+        """AttentionChunksDev in other forms (qr_attn_form): scores capped to cap * tanh(z / cap) (0: not), less slopes[h] (float32
         [heads]) times the distance; a row at position P sees t > P - window (0: all), t >= first[i], and t <= P or
         t < full[i] (lists of one entry per chunk, None: zeros); rows that see nothing give zeros.  prefix_ids[i] and
         prefix_len[i]: sequence and length of the prefix that stands before chunk i's own sequence (length 0: none),

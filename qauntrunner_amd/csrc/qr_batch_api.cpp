@@ -377,7 +377,7 @@ int qr_kv_attention_forms_dev(qr_kv* kv, int n, const int* seq_ids, int layer, c
         QR_CHECK_ARG(dtype_valid(dtype), "unknown q dtype %d", dtype);
         QR_CHECK_ARG(std::isfinite(scale), "scale must be a number");
         const qr_attn_form f = form ? *form : qr_attn_form{};
-        QR_CHECK_ARG(std::isfinite(f.cap) && f.cap >= 0.f, "cap must be a number of at least 0");
+        QR_CHECK_ARG(f.cap == 0.f || (f.cap >= 1e-3f && f.cap <= 1e6f), "cap must be 0 or a number from 0.001 to 1000000");
         QR_CHECK_ARG(f.window >= 0, "negative window %d", f.window);
         QR_CHECK_ARG((f.prefix_ids == nullptr) == (f.prefix_len == nullptr), "prefix_ids and prefix_len come together");
         for (int i = 0; i < n; ++i) {

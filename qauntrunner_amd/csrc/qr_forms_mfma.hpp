@@ -20,6 +20,8 @@
 // Queries and weights of a type with more bits than the tile's enter as PARTS of it: bf16 three (24 bits), fp16 two (22).
 #pragma once
 
+#include <cmath>
+
 #include "qr_forms.hpp"
 #include "qr_mfma.hpp"
 #include "qr_quant.hpp"
@@ -101,7 +103,6 @@ struct FormTile {
     float m, l;            // l: this lane's half of the positions
     float cap[5], by[5];   // the capped score of a small s: s (cap[0] + cap[1] s^2 + ... + cap[4] s^8); what the tile takes
     float small;           // |s| up to which it is
-    float hidden;          // what stands for a score that the row does not see
     bool wide;             // the tile's scores are capped already
     f32x16_t acc[ND];
 
@@ -119,10 +120,9 @@ struct FormTile {
         lo = s.lo;
         hi = on ? s.hi : -1;
         away = static_cast<float>(s.pos - it.base);
-        slope = SCORES == kScoresSlope || SCORES == kScoresBoth ? p.slopes[head] * kLog2e : 0.f;
+        slope = (SCORES == kScoresSlope || SCORES == kScoresBoth) && p.slopes ? p.slopes[head] * kLog2e : 0.f;
         m = -INFINITY;
         l = 0.f;
-        hidden = -INFINITY;
 #pragma unroll
         for (int t = 0; t < ND; ++t)
 #pragma unroll
@@ -191,17 +191,20 @@ struct FormTile {
     // Capped scores without slopes ascend with the products, so that the maximum is taken of these, and a product becomes its
     // capped score where it becomes a weight (PER_WEIGHT): 1 - 2 / (e^2x + 1) would be two more operations of a quarter of the rate
     // for each, but scores are mostly far below the cap, and tanh x / x on |x| <= 1/2 is a polynomial of x^2 (least squares at
-    // Chebyshev's points, off by 6e-9; its last coefficient is positive, which leaves a masked product's -infinity).  Tiles with
-    // larger ones are capped in front, and the coefficients become those of s.
+    // Chebyshev's points, off by 6e-9; its last coefficient is positive).  Tiles with larger ones are capped in front, and the
+    // coefficients become those of s.  Where they would leave fp32's range the launch takes kScoresBoth (per_weight).
+    static constexpr float kTanh[5] = {0.99999999f, -0.33333072f, 0.1332483f, -0.05298926f, 0.01714132f};
     static constexpr bool PER_WEIGHT = SCORES == kScoresCap && !SPLIT;
+    // What stands for a score that the row does not see; a polynomial of it is a large negative number or -infinity.
+    static constexpr float kHidden = PER_WEIGHT ? -1e18f : -INFINITY;
     __device__ __forceinline__ void init_cap(const FormsK& p) {
         if (!PER_WEIGHT) return;
         const float in = sscale / p.cap, i2 = in * in;
-        cap[0] = p.cap * in * 0.99999999f;
-        cap[1] = p.cap * in * i2 * -0.33333072f;
-        cap[2] = p.cap * in * i2 * i2 * 0.1332483f;
-        cap[3] = p.cap * in * i2 * i2 * i2 * -0.05298926f;
-        cap[4] = p.cap * in * i2 * i2 * i2 * i2 * 0.01714132f;
+        cap[0] = p.cap * in * kTanh[0];
+        cap[1] = p.cap * in * i2 * kTanh[1];
+        cap[2] = p.cap * in * i2 * i2 * kTanh[2];
+        cap[3] = p.cap * in * i2 * i2 * i2 * kTanh[3];
+        cap[4] = p.cap * in * i2 * i2 * i2 * i2 * kTanh[4];
         small = 0.5f / in;
     }
     __device__ __forceinline__ float capped(float s, float add) const {
@@ -219,7 +222,6 @@ struct FormTile {
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) most = max3abs(s[n][r], s[n][r + 1], most);
             wide = __builtin_amdgcn_ballot_w64(!(most <= small)) != 0;
-            hidden = wide ? -1e18f : -INFINITY;  // (0 x infinity would be no number)
 #pragma unroll
             for (int i = 0; i < 5; ++i) by[i] = wide ? (i == 0 ? 1.f : 0.f) : cap[i];
             if (wide) {
@@ -238,11 +240,19 @@ struct FormTile {
     // some row does not see the whole step: `edge`.
     __device__ __forceinline__ void form(const FormsK& p, f32x16_t& s, int t0, bool edge) const {
         if ((SCORES == kScoresCap && !PER_WEIGHT) || SCORES == kScoresBoth) {
-            // (for 16 bits 1 - 2 / (e^2x + 1): off by a few 2^-24 of the cap, far below the weights' rounding)
-            const float in = (SPLIT ? 1.f : 2.f * kLog2e) * sscale / p.cap;
+            const float in = sscale / p.cap;
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                s[r] = SPLIT ? p.cap * tanhf(s[r] * in) : fmaf(-2.f * p.cap, __builtin_amdgcn_rcpf(fast_exp2(s[r] * in) + 1.f), p.cap);
+            for (int r = 0; r < 16; ++r) {
+                const float t = s[r] * in, x = t * t;
+                if (SPLIT) {
+                    s[r] = p.cap * tanhf(t);
+                } else {
+                    // (the quotient loses a small tanh's bits: 2^-24 of the cap)
+                    const float a = t * fmaf(fmaf(fmaf(fmaf(kTanh[4], x, kTanh[3]), x, kTanh[2]), x, kTanh[1]), x, kTanh[0]);
+                    const float b = fmaf(-2.f, __builtin_amdgcn_rcpf(fast_exp2(t * (2.f * kLog2e)) + 1.f), 1.f);
+                    s[r] = p.cap * (fabsf(t) <= 0.5f ? a : b);
+                }
+            }
         }
         if (SCORES == kScoresSlope || SCORES == kScoresBoth) {
             const float first = static_cast<float>(t0 + (E8 ? 16 : 8) * half) - away;
@@ -257,7 +267,7 @@ struct FormTile {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int x = E8 ? r : 16 * (r >> 3) + (r & 7);
-                if (x < a || x > b) s[r] = hidden;
+                if (x < a || x > b) s[r] = kHidden;
             }
         }
     }
@@ -279,7 +289,7 @@ struct FormTile {
 #pragma unroll
         for (int n = 1; n < 2 * NS; ++n) t = fmaxf(t, mx[n]);
         t = max_xor32(t);
-        if (PER_WEIGHT) t = wide ? (t > -1e17f ? t : -INFINITY) : capped(t, 0.f);
+        if (PER_WEIGHT) t = t > 0.1f * kHidden ? capped(t, 0.f) : -INFINITY;
         const float by = SCORES == kScoresPlain ? sscale : 1.f;
         if (!(fmaf(t, by, -m) > kTop)) return 1.f;
         float mn = fmaf(t, by, kHead - kTop);
@@ -973,6 +983,7 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
                     pv(wt, i);
                 }
             }
+            wait_dma();  // (of the tile behind the last: nothing is read, but zeros are written)
         }
     }
     w.l = sum_xor32(w.l);
@@ -993,7 +1004,9 @@ __global__ void __launch_bounds__(256, 2) forms_mfma_kernel(const FormsK p) {
     else forms_tile<CT, D, PARTS, SCORES, 4>(p, it, u, lds, rest);
 }
 template <int CT, int D, int PARTS> hipError_t form_launch_scores(const FormsK& k, int units, hipStream_t s) {
-    if (k.cap > 0.f && k.slopes) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresBoth>), dim3(units), dim3(256), 0, s, k);
+    const double in = std::fabs(k.qscale) / static_cast<double>(k.cap), last = k.cap * std::pow(in, 9.0) * 0.017;  // the last coefficient
+    const bool per_weight = in < 1e3 && last > 1e-36 && last < 1e30;
+    if (k.cap > 0.f && (k.slopes || !per_weight)) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresBoth>), dim3(units), dim3(256), 0, s, k);
     else if (k.cap > 0.f) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresCap>), dim3(units), dim3(256), 0, s, k);
     else if (k.slopes) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresSlope>), dim3(units), dim3(256), 0, s, k);
     else hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresPlain>), dim3(units), dim3(256), 0, s, k);

@@ -60,7 +60,7 @@ def test_refusals_at_the_c_entry(tmp_path):
     run(tmp_path, HEAD + """
 assert append(kv, [0, 1], [0, 0], [300, 40]) == 0, L.qr_last_error()
 before = launches.value
-assert forms(scale=nan) == BAD and forms(act=16) == BAD and forms(act=7) == BAD and forms(cap=-1.0) == BAD and forms(cap=inf) == BAD
+assert forms(scale=nan) == BAD and forms(act=16) == BAD and forms(act=7) == BAD and forms(cap=-1.0) == BAD and forms(cap=inf) == BAD and forms(cap=1e-4) == BAD and forms(cap=2e6) == BAD
 assert forms(window=-1) == BAD and forms(first=[-1]) == BAD and forms(full=[-1]) == BAD and forms(layer=2) == BAD and forms(seqs=[3]) == BAD
 assert forms(rows=[-1]) == BAD and forms(q=None) == BAD and forms(out=None) == BAD and forms(q=ROWS + 2) == BAD and forms(slopes=ROWS + 2) == BAD
 assert forms(prefix_ids=[3], prefix_len=[1]) == BAD and forms(prefix_ids=[1], prefix_len=[-1]) == BAD

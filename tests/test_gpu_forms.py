@@ -17,7 +17,7 @@ import torch
 
 import qauntrunner_amd as qr
 from tests.chunkutil import TORCH, randn, row_errors
-from tests.formutil import filled_as, forms64
+from tests.formutil import e4m3_values, filled_as, forms64
 
 pytestmark = pytest.mark.gpu
 
@@ -277,6 +277,71 @@ def test_two_graphs_of_one_cache(gpu, dtype, act, heads, kv_heads, D):
                 run(kv, rows, [(0, 2000, 3)], dtype, act)
 
 
+@pytest.mark.parametrize("dtype,act", TYPES)
+@pytest.mark.parametrize("cap", [0.001, 1.0, 30.0, 1e6])
+@pytest.mark.parametrize("n", [1, 40, 150])
+def test_caps_of_every_size(gpu, dtype, act, cap, n):
+    """Scores far below the cap, about it and far beyond, with a mask in the first tile.  (A cap of 0.001 leaves nearly even
+    weights, one of a million none but the scores' own.)"""
+    kv, rows = filled_as(8, 2, 64, dtype, [400])
+    with kv:
+        run(kv, rows, [(0, 230, n)], dtype, act, cap=cap, first=[7])
+
+
+@pytest.mark.parametrize("dtype,act,D", [("f32", "f32", 64), ("f32", "bf16", 128), ("f16", "f16", 128), ("bf16", "bf16", 64), ("e4m3", "bf16", 128),
+                                         ("e4m3", "f16", 64), ("bf16", "f32", 24)])
+def test_rows_off_vector_alignment_and_another_stream(gpu, dtype, act, D):
+    """q and out one element behind a vector boundary, on a stream that is not the current one; the values around out stay."""
+    heads, n = 8, 50
+    kv, rows = filled_as(heads, 2, D, dtype, [300, 90])
+    width = n * heads * D
+    q = torch.zeros(width + 8, dtype=TORCH[act], device="cuda")[1:width + 1].view(n, heads * D)
+    q.copy_(randn(3, n, heads * D, dtype=act))
+    whole = torch.full((width + 8,), 7.0, dtype=TORCH[act], device="cuda")
+    out = whole[1:width + 1].view(n, heads * D)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with kv:
+        kv.AttentionFormsDev(0, [0, 1, 0], [200, 60, 299], [19, 30, 1], q, out, D**-0.5, window=120, prefix_ids=[1] * 3, prefix_len=[33] * 3, stream=s)
+        s.synchronize()
+        want, size = expected(rows, [(0, 200, 19), (1, 60, 30), (0, 299, 1)], q.view(n, heads, D), D**-0.5, heads, 2, D, prefix=[(1, 33)] * 3, window=120)
+        assert row_errors(out.view(n, heads, D), want, size) <= tol(dtype, act, 0)
+        assert (whole[:1] == 7).all() and (whole[width + 1:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype,act", [("bf16", "bf16"), ("e4m3", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("n", [1, 5, 20, 70])
+def test_positions_far_behind_a_long_prefix(gpu, dtype, act, n):
+    """Slopes and windows over positions past 2^16, of which the prefix holds most: distances are whole numbers of 32 bits."""
+    kv, rows = filled_as(8, 2, 64, dtype, [100, 70000])
+    with kv:
+        run(kv, rows, [(0, 100 - n, n)] * 2, dtype, act, prefix=[(1, 70000)] * 2, slopes=True)
+        run(kv, rows, [(0, 100 - n, n)] * 2, dtype, act, prefix=[(1, 70000)] * 2, window=300, first=[0, 69990])
+        run(kv, rows, [(1, 69999 - n, n), (0, 0, n)], dtype, act, prefix=[(1, 500), (1, 69999)], cap=30.0)
+
+
+@pytest.mark.parametrize("dtype,act", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("e4m3", "bf16"), ("e4m3", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("n", [1, 12, 40])
+@pytest.mark.parametrize("mass", [0.9, 0.999])
+def test_small_weights_beside_a_large_one(gpu, dtype, act, n, mass):
+    """One key takes nearly all of a row's weight and holds no value: the output is what the many small weights leave (2^-15 to
+    2^-23 of the largest).  Each weight is rounded relative to itself, so the tolerances are those of the other rows."""
+    from tests.test_gpu_chunks_sink import sink_queries, sink_rows
+
+    length, heads, kv_heads, D = 2048, 32, 8, 64
+    k, v = sink_rows(D, "bf16" if dtype == "e4m3" else dtype, length, math.log(length * mass / (1 - mass)) + 0.5)
+    with qr.PagedKvCache(1, heads, kv_heads, D, length, dtype) as kv:
+        kv.AppendNormRopeDev(0, [0], [0], [length], None, k.view(length, -1), v.view(length, -1), None, None, None, 1e-6, 1e4, rotary_dim=0)
+        if dtype == "e4m3":
+            k, v = e4m3_values(k), e4m3_values(v)
+        q = sink_queries(5, n, D, act)
+        out = torch.empty(n, heads * D, dtype=TORCH[act], device="cuda")
+        kv.AttentionFormsDev(0, [0], [length - n], [n], q, out, D**-0.5)
+        want, size = forms64(q.view(n, heads, D), k, v, length - n, D**-0.5, heads, kv_heads)
+        e = row_errors(out.view(n, heads, D), want, size)
+        assert e <= tol(dtype, act, 0), f"{e:.3g}"
+
+
 def test_a_serving_step(gpu):
     """The calls as they are used: a prompt's prefix enters an 8-bit cache once, sequences behind it append and attend, each
     position rotated by where it stands behind the prefix; the same as sequences that hold the prefix themselves."""
@@ -323,7 +388,7 @@ def test_refusals(gpu):
         call()
         call(rows=[0], q=q[:0], out=out[:0])
         kv.AttentionFormsDev(0, [], [], [], q[:0], out[:0], 1.0, first=[])
-        for bad in (dict(cap=-1.0), dict(cap=math.nan), dict(cap=math.inf), dict(window=-1), dict(first=[-1]), dict(full=[-5]), dict(scale=math.nan),
+        for bad in (dict(cap=-1.0), dict(cap=math.nan), dict(cap=math.inf), dict(cap=1e-4), dict(cap=2e6), dict(window=-1), dict(first=[-1]), dict(full=[-5]), dict(scale=math.nan),
                     dict(prefix_ids=[2], prefix_len=[5]), dict(prefix_ids=[1], prefix_len=[-1]), dict(ids=[2])):
             with pytest.raises(qr.QrInvalidArgument):
                 call(**bad)

@@ -55,7 +55,7 @@ def test_append_and_read_back(gpu, name, D, act):
             assert kv.seq_len(i) >= m
 
 
-@pytest.mark.parametrize("rot,norms,rope", [(0, True, None), (64, False, None), (32, True, [1000, 5, 77])])
+@pytest.mark.parametrize("rot,norms,rope", [(0, True, None), (20, True, None), (8, True, [2**20, 100000, 2**30]), (64, False, None), (32, True, [1000, 5, 77])])
 def test_partial_rotation(gpu, rot, norms, rope):
     kv_heads, D, n = 3, 64, [5, 1, 40]
     total = sum(n)
