@@ -28,8 +28,8 @@ __global__ void __launch_bounds__(kThreads) forms_merge_kernel(const FormsK p, i
     for (int x = lane; x < c.parts; x += 64) M = fmaxf(M, p.part_ml[slot + x].x);
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
-    // weight of a part: nothing of one that saw nothing
-    auto weight = [&](float2 ml) __attribute__((always_inline)) { return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - M); };
+    auto saw_nothing = [](float2 ml) __attribute__((always_inline)) { return ml.x == -INFINITY && ml.y == 0.f; };  // (its sums may not have been written)
+    auto weight = [&](float2 ml) __attribute__((always_inline)) { return ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - M); };  // (1: a sum that is no number)
     float L = 0.f;
     if (VEC) {
         const int gl = D / 4, per = 64 / gl, sub = lane / gl, d = 4 * (lane % gl);  // gl: 16 or 32
@@ -45,13 +45,13 @@ __global__ void __launch_bounds__(kThreads) forms_merge_kernel(const FormsK p, i
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float w = x0 + per * i < c.parts ? weight(ml[i]) : 0.f;
-                if (w == 0.f) continue;  // (its sums may not have been written)
+                if (x0 + per * i >= c.parts || saw_nothing(ml[i])) continue;
+                const float w = weight(ml[i]);
                 L = fmaf(ml[i].y, w, L);
-                o[0] = fmaf(a[i].x, w, o[0]);
-                o[1] = fmaf(a[i].y, w, o[1]);
-                o[2] = fmaf(a[i].z, w, o[2]);
-                o[3] = fmaf(a[i].w, w, o[3]);
+                o[0] += form_weighed(a[i].x, w);
+                o[1] += form_weighed(a[i].y, w);
+                o[2] += form_weighed(a[i].z, w);
+                o[3] += form_weighed(a[i].w, w);
             }
         }
         for (int x = gl; x < 64; x <<= 1) {
@@ -78,12 +78,12 @@ __global__ void __launch_bounds__(kThreads) forms_merge_kernel(const FormsK p, i
     for (int i = 0; i < NC; ++i) o[i] = 0.f;
     for (int x = 0; x < c.parts; ++x) {
         const float2 ml = p.part_ml[slot + x];
+        if (saw_nothing(ml)) continue;
         const float w = weight(ml);
-        if (w == 0.f) continue;
         L = fmaf(ml.y, w, L);
 #pragma unroll
         for (int i = 0; i < NC; ++i)
-            if (lane + 64 * i < D) o[i] = fmaf(p.part_acc[(slot + x) * D + lane + 64 * i], w, o[i]);
+            if (lane + 64 * i < D) o[i] += form_weighed(p.part_acc[(slot + x) * D + lane + 64 * i], w);
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i)

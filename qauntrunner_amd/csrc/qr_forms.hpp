@@ -208,6 +208,17 @@ __device__ __forceinline__ void form_store_ml(const FormsK& p, const FormRows& c
         for (int x = u.parts; x < it.splits; ++x) p.part_ml[slot + x - u.part] = make_float2(-INFINITY, 0.f);
 }
 
+// What a part's sums add to the whole: an infinite one shows however little the part weighs.
+template <class V> __device__ __forceinline__ V form_weighed(V o, float w) {
+    V x = o * w;
+    if constexpr (std::is_same<V, float>::value) return x == x ? x : o;
+    else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = x[i] == x[i] ? x[i] : o[i];
+        return x;
+    }
+}
+
 // A score in log2 units capped and less its slope: cap tanh(z / cap) = cap (1 - 2 / (e^(2 z / cap) + 1)).
 __device__ __forceinline__ float form_score(float z, float cap, float slope, float away) {
     if (cap > 0.f) z = cap * tanhf(z / cap);

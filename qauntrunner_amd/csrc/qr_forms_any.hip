@@ -134,6 +134,27 @@ __global__ void __launch_bounds__(kThreads) forms_any_kernel(const FormsK p) {
         prob[kRows + r] = l;
     }
     __syncthreads();
+    // A sum that is no number while that of its weights is: an infinite V whose weight is zero in 32 bits, but none in the
+    // formula.  The row shows the sum of these elements, found in one pass over the dim.
+#pragma unroll
+    for (int c2 = 0; c2 < NC; ++c2) {
+        const int d = threadIdx.x + kThreads * c2;
+        bool lost = false;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) lost |= acc[i][c2] != acc[i][c2] && prob[kRows + i] == prob[kRows + i];
+        if (d >= D || !lost || p.geom.scaled()) continue;
+        float shown[kRows] = {};
+        for (int t = t0; t < min(t1, last + 1); ++t) {
+            const float x = load_cached(p, p.page_table[it.pt_off + (t >> kPageShift)], 1, kvh, t & (kPageTokens - 1), d);
+            if (fabsf(x) < INFINITY) continue;
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+                if (t >= lo[i] && t <= hi[i]) shown[i] += x;
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+            if (acc[i][c2] != acc[i][c2]) acc[i][c2] = shown[i];
+    }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
         const int rho = rho0 + i;
@@ -142,6 +163,7 @@ __global__ void __launch_bounds__(kThreads) forms_any_kernel(const FormsK p) {
         const int row = it.row0 + rho / g;
         const float mi = prob[i], li = prob[kRows + i];
         const long long slot = c.slot0 + (static_cast<long long>(row - c.row0) * p.heads + h0 + rho % g) * c.parts + it.part0 + split;
+#pragma unroll
         for (int c2 = 0; c2 < NC; ++c2) {
             const int d = threadIdx.x + kThreads * c2;
             if (d >= D) continue;

@@ -31,7 +31,8 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, Q = lane >> 4;
     int row[RT], head[RT], lo[RT], hi[RT], chunk[RT];
     bool on[RT];
-    float away[RT], slope[RT];
+    int away[RT];
+    float slope[RT];
     f32x4_t q[RT][NK];
     FormRange range{0x7FFFFFFF, -1, -1, 0x7FFFFFFF};
 #pragma unroll
@@ -45,7 +46,7 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
         chunk[t] = s.chunk;
         lo[t] = s.lo;
         hi[t] = on[t] ? s.hi : -1;
-        away[t] = static_cast<float>(s.pos - it.base);
+        away[t] = s.pos - it.base;
         slope[t] = SCORES == kScoresSlope || SCORES == kScoresBoth ? p.slopes[head[t]] * kLog2e : 0.f;
         if (lo[t] <= hi[t]) {
             range.lo = min(range.lo, lo[t]);
@@ -114,6 +115,33 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[t][j][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
+    // V elements of the loaded step that are not finite; they as they are to the rows that see them.
+    auto bad_v = [&]() __attribute__((always_inline)) {
+        bool bad = false;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) bad |= !(fabsf(v[r][j][c]) < INFINITY);
+        return __builtin_amdgcn_ballot_w64(bad) != 0;
+    };
+    auto add_bad = [&](int st, int phys) __attribute__((always_inline)) {
+        const float* b = pool + phys * page_elems + plane + static_cast<long long>(16 * (st & 15)) * D;
+#pragma unroll 1
+        for (int x = 0; x < 16; ++x)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4_t y = *reinterpret_cast<const f32x4_t*>(b + x * D + 64 * j + 16 * Q + 4 * i);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int t = 0; t < RT; ++t)
+                            if (!(fabsf(y[c]) < INFINITY) && 16 * st + x >= lo[t] && 16 * st + x <= hi[t]) acc[t][j][c][i] += y[c];
+                }
+    };
     for (; st < s1; st += 4) {
         const int now = phys, t0 = 16 * st;
         phys = page(st + 4);
@@ -137,7 +165,7 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 if (SCORES == kScoresCap || SCORES == kScoresBoth) z[r] = p.cap * tanhf(z[r] / p.cap);
-                if (SCORES == kScoresSlope || SCORES == kScoresBoth) z[r] = fmaf(-slope[t], fabsf(static_cast<float>(t1 + r) - away[t]), z[r]);
+                if (SCORES == kScoresSlope || SCORES == kScoresBoth) z[r] = fmaf(-slope[t], fabsf(static_cast<float>(t1 + r - away[t])), z[r]);
                 if (edge && (t1 + r < lo[t] || t1 + r > hi[t])) z[r] = -INFINITY;
             }
             const float top = max_xor32(max_xor16(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]))));
@@ -159,28 +187,8 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
         if (edge) {
             // Elements of V that are not finite would reach rows that do not see them as 0 x inf: they are added to the rows that see
             // them as they are (no finite weight changes them), and cleared.
-            bool bad = false;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) bad |= !(fabsf(v[r][j][c]) < INFINITY);
-            if (__builtin_amdgcn_ballot_w64(bad)) {
-                const float* b = pool + now * page_elems + plane + static_cast<long long>(16 * (st & 15)) * D;
-#pragma unroll 1
-                for (int x = 0; x < 16; ++x)
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const f32x4_t y = *reinterpret_cast<const f32x4_t*>(b + x * D + 64 * j + 16 * Q + 4 * i);
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                                for (int t = 0; t < RT; ++t)
-                                    if (!(fabsf(y[c]) < INFINITY) && t0 + x >= lo[t] && t0 + x <= hi[t]) acc[t][j][c][i] += y[c];
-                        }
+            if (bad_v()) {
+                add_bad(st, now);
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -201,10 +209,40 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
         if (st + 4 < s1) load_v(st + 4, phys);
     }
 
-    // the waves merge: wave w adds up row groups w, w + 4, ... of (tile, j, i), 4 dims each
+    // A sum that is no number while that of its weights is: an infinite V whose weight is zero in 32 bits, but none in the
+    // formula.  The row shows the sum of these elements.
+    bool lost = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         l[t] = sum_xor32(sum_xor16(l[t]));
+        f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum += acc[t][j][c];
+        const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        lost |= all != all && l[t] == l[t];
+    }
+    if (__builtin_amdgcn_ballot_w64(lost)) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[t][j][c][i] = acc[t][j][c][i] != acc[t][j][c][i] ? 0.f : acc[t][j][c][i];
+#pragma unroll 1
+        for (st = s0 + wave; st < s1; st += 4) {
+            phys = page(st);
+            load_v(st, phys);
+            if (bad_v()) add_bad(st, phys);
+        }
+    }
+
+    // the waves merge: wave w adds up row groups w, w + 4, ... of (tile, j, i), 4 dims each
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -235,7 +273,7 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
             const int i = wave * (NG / 4) + x, d = 64 * (i >> 2) + 16 * Q + 4 * (i & 3);
             f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int y = 0; y < 4; ++y) o += xa[((y * RT + t) * NG + i) * 64 + lane] * c[y];
+            for (int y = 0; y < 4; ++y) o += form_weighed(xa[((y * RT + t) * NG + i) * 64 + lane], c[y]);
             if (!whole) {
                 *reinterpret_cast<f32x4_t*>(p.part_acc + slot * D + d) = o;
             } else {

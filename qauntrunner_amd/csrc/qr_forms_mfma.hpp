@@ -97,7 +97,8 @@ struct FormTile {
     int row, head, chunk;  // of row lane % 32
     bool on;
     int lo, hi;            // slots that the row sees (none past the item's rows)
-    float away, slope;     // position less the item's base; slope in log2 units
+    int away;              // position less the item's base
+    float slope;           // in log2 units
     vec8 q[PARTS][NK];
     float sscale;          // log2 units per score
     float m, l;            // l: this lane's half of the positions
@@ -119,7 +120,7 @@ struct FormTile {
         chunk = s.chunk;
         lo = s.lo;
         hi = on ? s.hi : -1;
-        away = static_cast<float>(s.pos - it.base);
+        away = s.pos - it.base;
         slope = (SCORES == kScoresSlope || SCORES == kScoresBoth) && p.slopes ? p.slopes[head] * kLog2e : 0.f;
         m = -INFINITY;
         l = 0.f;
@@ -255,7 +256,7 @@ struct FormTile {
             }
         }
         if (SCORES == kScoresSlope || SCORES == kScoresBoth) {
-            const float first = static_cast<float>(t0 + (E8 ? 16 : 8) * half) - away;
+            const float first = static_cast<float>(t0 + (E8 ? 16 : 8) * half - away);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float d = fabsf(first + static_cast<float>(E8 ? r : 16 * (r >> 3) + (r & 7)));
@@ -364,6 +365,36 @@ struct FormTile {
         }
     }
 
+    // A sum that is no number while that of its weights is: an infinite V of little weight (0 x inf), or one between the parts of a
+    // weight (inf - inf).  No weight of the formula is zero, so the row shows the sum of these elements.  Steps step0, step0 +
+    // stride, ... below step1 were the wave's.  (8 bits hold no infinity.)
+    __device__ __forceinline__ void settle(const FormsK& p, const FormItem& it, int kvh, int step0, int step1, int stride) {
+        if (E8) return;
+        float sum = 0.f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum += acc[d][r];
+        if (!__builtin_amdgcn_ballot_w64(sum != sum && l == l)) return;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] = acc[d][r] != acc[d][r] ? 0.f : acc[d][r];
+#pragma unroll 1
+        for (int st = step0; st < step1; st += stride) {
+            const char* const step = p.pool + (static_cast<long long>(form_page(p, it.pt_off, 32 * st)) * p.geom.page_elems() + p.geom.plane_elems() +
+                                               static_cast<long long>(kvh) * kPageTokens * D + (32 * st & (kPageTokens - 1)) * D) * 2;
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const vec8 x = *reinterpret_cast<const vec8*>(step + 16 * (lane + 64 * i));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) bad |= !(fabsf(static_cast<float>(x[j])) < INFINITY);
+            }
+            if (__builtin_amdgcn_ballot_w64(bad)) add_bad(p, it, kvh, 32 * st);
+        }
+    }
+
     // The row's output or partial: N groups of 4 dims from group g0 on, of the weighed sums a.  Group g holds dims 32 (g / 4) +
     // 8 (g % 4) + 4 half .. + 3.
     __device__ __forceinline__ long long slot(const FormsK& p, const FormItem& it, int split) const {
@@ -445,7 +476,7 @@ __device__ __forceinline__ void merge_waves(const FormsK& p, const FormItem& it,
         for (int i = 0; i < NP; ++i) {
             out[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int x = 0; x < PW; ++x) out[i] += xa[((rw * PW + x) * NG + pw * NP + i) * 64 + w.lane] * c[x];
+            for (int x = 0; x < PW; ++x) out[i] += form_weighed(xa[((rw * PW + x) * NG + pw * NP + i) * 64 + w.lane], c[x]);
         }
     }
     w.store(p, it, un, pw * NP, L, out);
@@ -590,7 +621,7 @@ __device__ __forceinline__ void forms_stream(const FormsK& p, const FormItem& it
         if (st + 4 < s1) load_v(st + 4, phys);
     }
     w.l = sum_xor32(w.l);
-
+    w.settle(p, it, kvh, s0 + wave, s1, 4);
     merge_waves<F, 1, 4>(p, it, un, w, 0, wave, lds, rest);
 }
 
@@ -987,6 +1018,7 @@ __device__ __forceinline__ void forms_tile(const FormsK& p, const FormItem& it, 
         }
     }
     w.l = sum_xor32(w.l);
+    w.settle(p, it, kvh, 2 * i0 + wave / RW, 2 * i1, RW == 4 ? 1 : 2);
     merge_waves<F, RW, 4 / RW>(p, it, un, w, rw, wave / RW, lds, rest);
 }
 

@@ -403,3 +403,65 @@ def test_refusals(gpu):
                     dict(slopes=out.view(-1)[:8])):
             with pytest.raises(ValueError):
                 call(**bad)
+
+
+@pytest.mark.parametrize("dtype,act,D", [("bf16", "bf16", 128), ("f16", "f16", 64), ("f16", "f32", 128), ("bf16", "f32", 64), ("f32", "f32", 64),
+                                         ("f32", "f32", 128), ("f32", "bf16", 96), ("bf16", "bf16", 20)])
+@pytest.mark.parametrize("n", [1, 12, 25, 70])
+@pytest.mark.parametrize("seqs", [1, 24])  # the keys split over many workgroups, and not
+@pytest.mark.parametrize("at", [3, 2100])  # before and behind the keys of large weight
+@pytest.mark.parametrize("form", ["plain", "cap", "prefix"])
+def test_infinite_values_of_little_weight(gpu, form, dtype, act, D, n, seqs, at):
+    """A weight of e^-190 is zero in 32 bits, but none in the formula: a row that sees an infinite V shows that infinity
+    whatever its weight (a cap of 1e5 leaves the scores as they are to 1e-6 of them), and NaN where it sees both or a NaN."""
+    heads, kv_heads, length = 8, 2, 2500
+    if D == 20 and seqs > 1:
+        seqs = 8
+    k, v = (randn(s, length, kv_heads, D, dtype="f32") for s in (1, 2))
+    k[:, :, 0] = 0
+    k[max(at - 200, 0):at + 200, :, 0] = -(190 * math.sqrt(D) / 8)  # against queries of 8 there; whole parts of split keys
+    inf = math.inf
+    v[at, 0, 1], v[at, 0, 3], v[at, 1, D - 1], v[at, 1, 2] = inf, -inf, inf, math.nan
+    v[at + 40, :, 3] = inf
+    k, v = k.to(TORCH[dtype]), v.to(TORCH[dtype])
+    q = randn(3, seqs * n, heads, D, dtype="f32")
+    q[:, :, 0] = 8
+    q = q.to(TORCH[act])
+    out = torch.empty_like(q)
+    front = 2200 if form == "prefix" else 0
+    own = length - front
+    with qr.PagedKvCache(1, heads, kv_heads, D, length, dtype, seqs + 1) as kv:
+        if front:
+            kv.AppendRangeDev(0, 0, k[:front].reshape(front, -1), v[:front].reshape(front, -1), dtype, seq_id=seqs)
+        for s in range(seqs):
+            kv.AppendRangeDev(0, 0, k[front:].reshape(own, -1), v[front:].reshape(own, -1), dtype, seq_id=s)
+        more = dict(prefix_ids=[seqs] * seqs, prefix_len=[front] * seqs) if front else dict(cap=1e5) if form == "cap" else {}
+        kv.AttentionFormsDev(0, list(range(seqs)), [own - n] * seqs, [n] * seqs, q, out, D**-0.5, **more)
+    for s in (0, seqs - 1):
+        got = out[s * n:(s + 1) * n].double()
+        assert (got[:, :4, 1] == inf).all() and got[:, :4, 3].isnan().all()
+        assert (got[:, 4:, D - 1] == inf).all() and got[:, 4:, 2].isnan().all() and (got[:, 4:, 3] == inf).all()
+        want, size = forms64(q[s * n:(s + 1) * n], k, torch.where(v.isfinite(), v, 0), length - n, D**-0.5, heads, kv_heads, cap=more.get("cap", 0.0))
+        for x in (got, want):
+            for h, d in ((slice(0, 4), 1), (slice(0, 4), 3), (slice(4, 8), D - 1), (slice(4, 8), 2), (slice(4, 8), 3)):
+                x[:, h, d] = 0
+        e = row_errors(got, want, size)
+        assert e <= tol(dtype, act, more.get("cap", 0.0)), f"out: {e:.3g}"
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_slopes_over_far_positions(gpu, dtype):
+    """Distances of rows past position 2^24, where fp32 has no odd numbers, are exact: the slope's differences between
+    neighbouring keys are the formula's."""
+    heads, kv_heads, D, base, n = 2, 1, 64, 2**24 + 129, 40
+    with qr.PagedKvCache(1, heads, kv_heads, D, 2**24 + 512, dtype, 1) as kv:
+        k, v = (randn(s, n, kv_heads, D, dtype=dtype) for s in (1, 2))
+        kv.AppendNormRopeDev(0, [0], [base], [n], None, k.view(n, -1), v.view(n, -1), None, None, None, 1e-6, 1e4, rotary_dim=0)
+        for m in (1, n):
+            q = randn(3, m, heads, D, dtype=dtype)
+            out = torch.empty_like(q)
+            slopes = torch.tensor([2.0, 0.5], device="cuda")
+            kv.AttentionFormsDev(0, [0], [base + n - m], [m], q, out, D**-0.5, slopes=slopes, first=[base])
+            want, size = forms64(q, k, v, n - m, D**-0.5, heads, kv_heads, slopes=slopes)
+            e = row_errors(out, want, size)
+            assert e <= tol(dtype, dtype, 0), f"{e:.3g}"
