@@ -11,7 +11,8 @@ constexpr int kThreads = 256;
 
 // out of a row's parts: a wave per (row, head), the parts' sums weighed by 2^(m - M).  A row that saw nothing is zeros.  A
 // partial's sums are D / 4 lanes' float4, so that a wave reads several of them at once, and each lane four ahead (VEC; other
-// head sizes: a lane every 64th value of one).
+// head sizes: a lane every 64th value of one).  Bound by latency: 4 to 5 us for 16 to 1500 rows, 8 for 115 rows of 64 heads in some
+// ten parts.
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads) forms_merge_kernel(const FormsK p, int rows) {
     const long long at = static_cast<long long>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
@@ -32,7 +33,7 @@ __global__ void __launch_bounds__(kThreads) forms_merge_kernel(const FormsK p, i
     auto weight = [&](float2 ml) __attribute__((always_inline)) { return ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - M); };  // (1: a sum that is no number)
     float L = 0.f;
     if (VEC) {
-        const int gl = D / 4, per = 64 / gl, sub = lane / gl, d = 4 * (lane % gl);  // gl: 16 or 32
+        const int gl = D / 4, per = 64 / gl, sub = lane / gl, d = 4 * (lane % gl);  // gl: 16, 32 or 64
         float o[4] = {0.f, 0.f, 0.f, 0.f};
         for (int x0 = sub; x0 < c.parts; x0 += 4 * per) {
             float4 a[4];
@@ -95,8 +96,9 @@ bool whole_queries(const FormsArgs& a) { return a.act == (a.dtype == QR_DTYPE_F1
 
 // What a unit of a kernel takes, in microseconds: a tile of it, its start and end, and its share of what runs at once on a CU.
 // Measured (D = 128): a tile of 64 slots 2.2 for 128 rows, 1.3 for 64, 1.4 times as long with capped scores and 2.2 times in parts; a
-// streamed step of 32 slots by its bytes, 5 TB/s over all CUs; fp32 steps of 16 slots as streamed ones for 16 rows, by their
-// MFMAs for 32.
+// streamed step of 32 slots by its bytes, 5 TB/s over all CUs; fp32 MFMAs' steps of 16 slots by their bytes for 16 rows, by their
+// MFMAs for 32.  (With 0.4 to 1.5 times the part that this gives, the cases it was tried on took 0 to 30% longer, but for 8-bit verify
+// chunks of 64 rows behind 16001 positions, 10% shorter at 0.6.)
 struct Shape {
     float tile, start, share;
     int least;  // tiles that a part has at least
@@ -105,25 +107,27 @@ constexpr float kCus = 256.f;
 Shape shape_of(const FormsArgs& a, int kind) {
     const float wide = a.geom.head_dim / 128.f;
     const float tile = wide * (whole_queries(a) ? 1.f : 2.2f) * (a.cap > 0.f ? 1.4f : a.slopes ? 1.2f : 1.f);
+    // one workgroup on a CU at head size 256, which has it to itself
+    auto alone = [&](Shape s) { return a.geom.head_dim == 256 ? Shape{0.5f * s.tile, s.start, 1.f, s.least} : s; };
     switch (kind) {
         case kFormStream: return {wide * (a.geom.scaled() ? 0.9f : 1.7f), 5.f, 0.5f, 8};
         case kFormTilesHalf: return {1.3f * tile, 6.f, 0.5f, 4};
         case kFormTiles: return {2.2f * tile, 6.f, 0.5f, 4};
-        case kFormF32Half: return {wide * 1.7f, 5.f, 0.5f, 8};
-        case kFormF32: return {wide * 1.f, 5.f, 0.5f, 8};
+        case kFormF32Half: return alone({wide * (a.dtype == QR_DTYPE_F32 ? 1.7f : 1.f), 5.f, 0.5f, 8});
+        case kFormF32: return alone({wide * 1.f, 5.f, 0.5f, 8});
         default: return {4.f, 5.f, 0.25f, 2};
     }
 }
 int kind_of(const FormsArgs& a, int rows) {
     const int D = a.geom.head_dim;
-    if ((D != 64 && D != 128) || a.heads % a.geom.kv_heads) return kFormAny;
+    if ((D != 64 && D != 96 && D != 128 && D != 256) || a.heads % a.geom.kv_heads) return kFormAny;
     const long long n = static_cast<long long>(rows) * (a.heads / a.geom.kv_heads);
-    if (a.dtype == QR_DTYPE_F32) return n <= 16 ? kFormF32Half : kFormF32;
+    if (a.dtype == QR_DTYPE_F32 || !(a.geom.mfma_layout & 1)) return n <= 16 ? kFormF32Half : kFormF32;
     return n <= 32 ? kFormStream : n <= 64 ? kFormTilesHalf : kFormTiles;
 }
 hipError_t launch(const FormsK& k, int units, hipStream_t s) {
     if (k.it[0].kind == kFormAny) return launch_forms_any(k, units, s);
-    if (k.dtype == QR_DTYPE_F32) return launch_forms_f32(k, units, s);
+    if (k.it[0].kind == kFormF32Half || k.it[0].kind == kFormF32) return launch_forms_f32(k, units, s);
     if (k.dtype == QR_DTYPE_F16) return launch_forms_f16(k, units, s);
     return k.dtype == QR_DTYPE_BF16 ? launch_forms_bf16(k, units, s) : launch_forms_e4m3(k, units, s);
 }
@@ -335,7 +339,7 @@ hipError_t launch_forms(const FormsArgs& a, const FormsPlan& plan, void* workspa
         }
         const long long waves = static_cast<long long>(rows) * a.heads;
         const dim3 grid(static_cast<unsigned>((waves + 3) / 4));
-        if (a.geom.head_dim == 64 || a.geom.head_dim == 128) hipLaunchKernelGGL(forms_merge_kernel<true>, grid, dim3(kThreads), 0, stream, k, rows);
+        if (a.geom.head_dim == 64 || a.geom.head_dim == 128 || a.geom.head_dim == 256) hipLaunchKernelGGL(forms_merge_kernel<true>, grid, dim3(kThreads), 0, stream, k, rows);
         else hipLaunchKernelGGL(forms_merge_kernel<false>, grid, dim3(kThreads), 0, stream, k, rows);
         return hipGetLastError();
     }

@@ -97,7 +97,7 @@ hipError_t launch_forms(const FormsArgs& a, const FormsPlan& plan, void* workspa
 
 hipError_t launch_forms_any(const FormsK& k, int units, hipStream_t s);
 // MFMA tiles (kinds kFormStream, kFormTiles): operand page layouts, whole groups.
-// fp32 tiles (kinds kFormF32Half, kFormF32): fp32 caches of head size 64 or 128, whole groups.
+// fp32 tiles (kinds kFormF32Half, kFormF32): head sizes 64, 96, 128 and 256 of rows in order in the page, whole groups.
 hipError_t launch_forms_f32(const FormsK& k, int units, hipStream_t s);
 hipError_t launch_forms_f16(const FormsK& k, int units, hipStream_t s);
 hipError_t launch_forms_bf16(const FormsK& k, int units, hipStream_t s);

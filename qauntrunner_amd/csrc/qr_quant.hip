@@ -57,7 +57,8 @@ __device__ __forceinline__ void norm_rotate(T (&y)[NC], int lane, int D, const f
     __builtin_amdgcn_wave_barrier();
 }
 
-// Any head size: one workgroup per row, one wave per head, a lane every 64th value.
+// Any head size: one workgroup per row, one wave per head, a lane every 64th value.  (The simple form, for caches without an operand
+// layout and rotations that split a run of 4: 512 rows of 32 + 8 + 8 heads of 96 take 21 us.)
 __global__ void __launch_bounds__(kThreads) quant_any_kernel(const NormRopeArgs a) {
     __shared__ double csd[kMaxRopeHalf], snd[kMaxRopeHalf];
     __shared__ float cs[kMaxRopeHalf], sn[kMaxRopeHalf];
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(const NormRopeArgs 
     }
     __syncthreads();
     const int D = a.geom.head_dim, kvh = a.geom.kv_heads;
-    const int pos = a.it[e].pos0 + j, scalet = pos & (kPageTokens - 1);
+    const int pos = a.it[e].pos0 + j, slot = pos & (kPageTokens - 1);
     const long long phys = a.page_table[a.it[e].pt_off + (pos >> kPageShift)];
     uint8_t* const pool = static_cast<uint8_t*>(a.pool);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -104,24 +105,25 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(const NormRopeArgs 
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const float x = quant_round(ldexp(y[c], -ex));
-            if (lane + 64 * c < D) pool[a.geom.offset(phys, is_v, hh, scalet, lane + 64 * c)] = quant4(x, 0.f, 0.f, 0.f) & 0xFF;
+            if (lane + 64 * c < D) pool[a.geom.offset(phys, is_v, hh, slot, lane + 64 * c)] = quant4(x, 0.f, 0.f, 0.f) & 0xFF;
         }
-        if (lane == 0) pool[a.geom.scale_offset(phys, is_v, hh, scalet)] = ex + 127;
+        if (lane == 0) pool[a.geom.scale_offset(phys, is_v, hh, slot)] = ex + 127;
     }
 }
 
-// Rows back as values of a.act, any cache: a workgroup per row.
+// Rows back as values of a.act, any cache: a workgroup per row.  (8-bit rows of 8 heads of 96 as bf16: 302 MB in 182 us, bound by
+// single bytes; the operand layout's kernel below does without.)
 __global__ void __launch_bounds__(kThreads) read_as_any_kernel(const ReadArgs a) {
     const int row = blockIdx.x;
     const int e = batch_find(a.n, row, [&](int i) { return a.it[i].row0; });
-    const int pos = a.it[e].pos0 + row - a.it[e].row0, scalet = pos & (kPageTokens - 1);
+    const int pos = a.it[e].pos0 + row - a.it[e].row0, slot = pos & (kPageTokens - 1);
     const long long phys = a.page_table[a.it[e].pt_off + (pos >> kPageShift)];
     const int D = a.geom.head_dim, width = a.geom.kv_heads * D;
     const uint8_t* const bytes = static_cast<const uint8_t*>(a.pool);
     for (int i = threadIdx.x; i < 2 * width; i += kThreads) {
         const int plane = i >= width, c = i - plane * width;
-        const long long from = a.geom.offset(phys, plane, c / D, scalet, c % D);
-        const float x = a.geom.scaled() ? quant_value<0>(bytes[from]) * scale_of(bytes[a.geom.scale_offset(phys, plane, c / D, scalet)])
+        const long long from = a.geom.offset(phys, plane, c / D, slot, c % D);
+        const float x = a.geom.scaled() ? quant_value<0>(bytes[from]) * scale_of(bytes[a.geom.scale_offset(phys, plane, c / D, slot)])
                                       : load_elem(a.pool, a.dtype, from);
         store_out(plane ? a.v : a.k, a.act, static_cast<long long>(row) * width + c, x);
     }
@@ -187,7 +189,10 @@ template <class T, int LPH> __device__ __forceinline__ void norm_rotate8(T (&x)[
 }
 __device__ __forceinline__ float quant_unit(int ex) { return pow2f(-ex); }
 
-// One workgroup per row and gridDim.y-th part of its heads (K, then q, then V unless it goes by runs).
+// One workgroup per row and gridDim.y-th part of its heads (K, then q, then V unless it goes by runs), all loads of its items first.
+// Bound by HBM, less what 64 bits cost: 5317 bf16 rows of 32 + 8 heads take 31 to 33 us for 104 MB, 3.2 TB/s where a copy reaches
+// 4.8 (angles and rotation of K in 64 bits are 6 of them; sine and cosine by a table product in 64 bits were no faster).  Words of
+// K at two places of the row cost a line of the page each, which the row's other heads fill.
 template <int ACT, int D, int IPT>
 __global__ void __launch_bounds__(kThreads) quant_kernel(const NormRopeArgs a, int v_heads) {
     constexpr int LPH = D / 8;
@@ -195,7 +200,7 @@ __global__ void __launch_bounds__(kThreads) quant_kernel(const NormRopeArgs a, i
     const int kv = a.geom.kv_heads;
     const int row = blockIdx.x;
     const int e = batch_find(a.n, row, [&](int i) { return a.it[i].row0; });
-    const int j = row - a.it[e].row0, pos = a.it[e].pos0 + j, scalet = pos & (kPageTokens - 1);
+    const int j = row - a.it[e].row0, pos = a.it[e].pos0 + j, slot = pos & (kPageTokens - 1);
     const int qh = a.q ? a.heads : 0, heads = kv + qh + v_heads;
     const int li = threadIdx.x & (LPH - 1);
     const bool pair = 8 * li < a.rot;
@@ -269,14 +274,14 @@ __global__ void __launch_bounds__(kThreads) quant_kernel(const NormRopeArgs a, i
         for (int i = 0; i < 8; ++i) y[i] = quant_round(x[i] * unit);
         const uint32_t c[2] = {quant4(y[0], y[1], y[2], y[3]), quant4(y[4], y[5], y[6], y[7])};
         if (is_k) {
-            *reinterpret_cast<uint32_t*>(pool + a.geom.offset(phys, 0, hh, scalet, at_a)) = c[0];
-            *reinterpret_cast<uint32_t*>(pool + a.geom.offset(phys, 0, hh, scalet, at_b)) = c[1];
+            *reinterpret_cast<uint32_t*>(pool + a.geom.offset(phys, 0, hh, slot, at_a)) = c[0];
+            *reinterpret_cast<uint32_t*>(pool + a.geom.offset(phys, 0, hh, slot, at_b)) = c[1];
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                pool[a.geom.offset(phys, 1, hh, scalet, (i < 4 ? at_a : at_b - 4) + i)] = static_cast<uint8_t>(c[i >> 2] >> (8 * (i & 3)));
+                pool[a.geom.offset(phys, 1, hh, slot, (i < 4 ? at_a : at_b - 4) + i)] = static_cast<uint8_t>(c[i >> 2] >> (8 * (i & 3)));
         }
-        if (li == 0) pool[a.geom.scale_offset(phys, !is_k, hh, scalet)] = ex + 127;
+        if (li == 0) pool[a.geom.scale_offset(phys, !is_k, hh, slot)] = ex + 127;
     }
 }
 
@@ -290,8 +295,10 @@ __device__ __forceinline__ void transpose4(const uint32_t (&x)[4], uint32_t (&y)
     y[3] = __builtin_amdgcn_perm(d, b, 0x07060302);
 }
 
-// V by runs of 16 scalets, which are 16 bytes of a dim in the page: a workgroup takes a run of 256 / (D / 8) heads' rows, 8 values
-// per thread, and hands the codes through LDS to threads of 4 dims each.  Slots outside the chunk are left alone.
+// V by runs of 16 slots, which are 16 bytes of a dim in the page: a workgroup takes a run of 256 / (D / 8) heads' rows, 8 values
+// per thread, and hands the codes through LDS to threads of 4 dims each.  Slots outside the chunk are left alone.  As part of
+// quant_kernel it wrote single bytes: a line of the page for each (16 sequences of one row: 7 us, where a second launch would be 4 more;
+// 5317 rows: these 16 MB take 9 us).
 template <int ACT, int D>
 __global__ void __launch_bounds__(kThreads) quant_v_kernel(const NormRopeArgs a) {
     constexpr int LPH = D / 8, GROUPS = kThreads / LPH / 16;  // (run, head) pairs of a workgroup
@@ -376,14 +383,15 @@ template <int T> __device__ __forceinline__ void widen8(uint32_t lo, uint32_t hi
     }
 }
 
-// Rows of the 8-bit operand layout back as values: a workgroup takes 128 scalets of a kv head, K by 16 dims of a scalet per thread (the
-// D / 16 threads of a scalet beside each other: whole lines of the page, whole rows of the output), V by 8 dims of 8 scalets, whose
-// codes are transposed in registers.
+// Rows of the 8-bit operand layout back as values: a workgroup takes 128 slots of a kv head, K by 16 dims of a slot per thread (the
+// D / 16 threads of a slot beside each other: whole lines of the page, whole rows of the output), V by 8 dims of 8 slots, whose
+// codes are transposed in registers.  Bound by HBM, two thirds of it writes: 808 MB in 165 to 178 us, 4.5 to 4.9
+// TB/s (a copy: 4.8); with 8-byte stores 221.
 constexpr int kReadRun = 128;
 template <int T, int D>
 __global__ void __launch_bounds__(kThreads) read_as_kernel(const ReadArgs a) {
     typedef typename std::conditional<T == QR_DTYPE_F32, float, uint16_t>::type E;
-    constexpr int P = D / 16, KP = kReadRun * P / kThreads;  // pieces of a scalet; of K per thread
+    constexpr int P = D / 16, KP = kReadRun * P / kThreads;  // pieces of a slot; of K per thread
     static_assert(kReadRun / 8 * (D / 8) <= kThreads, "threads that take V");
     const int e = batch_find(a.n, blockIdx.x, [&](int i) { return a.it[i].unit0; });
     const ReadItem it = a.it[e];
@@ -411,7 +419,7 @@ __global__ void __launch_bounds__(kThreads) read_as_kernel(const ReadArgs a) {
             ks[c] = scales[kt[c]];
         }
     }
-    const int run = threadIdx.x / (D / 8), n = threadIdx.x % (D / 8);  // scalets 8 run .., dims 8 n ..
+    const int run = threadIdx.x / (D / 8), n = threadIdx.x % (D / 8);  // slots 8 run .., dims 8 n ..
     const bool takes = run < kReadRun / 8 && p0 + 8 * run < end && p0 + 8 * run + 8 > it.pos0;
     uint2 vc[8], vs;
     if (takes) {
@@ -447,7 +455,7 @@ __global__ void __launch_bounds__(kThreads) read_as_kernel(const ReadArgs a) {
 
 template <int ACT, int D> void launch_rows(NormRopeArgs& a, hipStream_t s) {
     constexpr int LPH = D / 8, GROUPS = kThreads / LPH / 16;
-    // V goes by runs of 16 scalets unless the chunks have few rows: single bytes otherwise, but one launch
+    // V goes by runs of 16 slots unless the chunks have few rows: single bytes otherwise, but one launch
     const bool runs = a.rows >= 4 * a.n;
     if (runs) {
         int groups = 0;
@@ -459,8 +467,8 @@ template <int ACT, int D> void launch_rows(NormRopeArgs& a, hipStream_t s) {
         hipLaunchKernelGGL((quant_v_kernel<ACT, D>), dim3(groups), dim3(kThreads), 0, s, a);
     }
     const int v_heads = runs ? 0 : a.geom.kv_heads, heads = a.geom.kv_heads + (a.q ? a.heads : 0) + v_heads;
-    const int scalets = (heads * LPH + kThreads - 1) / kThreads, ipt = std::min(scalets, 4);
-    const dim3 grid(a.rows, (scalets + ipt - 1) / ipt);
+    const int turns = (heads * LPH + kThreads - 1) / kThreads, ipt = std::min(turns, 4);
+    const dim3 grid(a.rows, (turns + ipt - 1) / ipt);
     if (ipt == 1) hipLaunchKernelGGL((quant_kernel<ACT, D, 1>), grid, dim3(kThreads), 0, s, a, v_heads);
     else if (ipt == 2) hipLaunchKernelGGL((quant_kernel<ACT, D, 2>), grid, dim3(kThreads), 0, s, a, v_heads);
     else if (ipt == 3) hipLaunchKernelGGL((quant_kernel<ACT, D, 3>), grid, dim3(kThreads), 0, s, a, v_heads);

@@ -465,3 +465,32 @@ def test_slopes_over_far_positions(gpu, dtype):
             want, size = forms64(q, k, v, n - m, D**-0.5, heads, kv_heads, slopes=slopes)
             e = row_errors(out, want, size)
             assert e <= tol(dtype, dtype, 0), f"{e:.3g}"
+
+
+@pytest.mark.parametrize("heads,kv_heads,D", [(8, 2, 96), (28, 4, 96), (8, 2, 256), (16, 1, 256), (3, 3, 256), (5, 2, 256), (40, 2, 96)])
+@pytest.mark.parametrize("dtype,act", TYPES)
+def test_wide_and_odd_heads(gpu, dtype, act, heads, kv_heads, D):
+    """Head sizes whose rows lie in order in the page: every form, single tokens, blocks of several row tiles, a prefix."""
+    kv, rows = filled_as(heads, kv_heads, D, dtype, LENGTHS)
+    with kv:
+        for name in CHUNKS:
+            for form in FORMS:
+                run(kv, rows, CHUNKS[name], dtype, act, **FORMS[form])
+        run(kv, rows, [(0, 7, 1), (1, 300, 1), (2, 255, 2)], dtype, act, prefix=[(4, 777)] * 3, window=600, cap=20.0)
+        run(kv, rows, [(4, 900, 101), (3, 100, 3)], dtype, act, prefix=[(1, 257), (0, 0)], first=[300, 101], full=[1200, 0], slopes=True)
+
+
+@pytest.mark.parametrize("D", [96, 256])
+@pytest.mark.parametrize("dtype,act", TYPES)
+@pytest.mark.parametrize("odd", [math.nan, math.inf])
+def test_what_no_row_sees_does_not_matter_in_wide_heads(gpu, odd, dtype, act, D):
+    def edit(i, k, v):
+        for t in (0, 100, 255, 256, 291, 292):
+            k[t], v[t] = odd, -odd
+
+    kv, rows = filled_as(8, 2, D, dtype, [600], edit=edit)
+    clean = [(k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0)) for k, v in rows]
+    with kv:
+        for n in (1, 9, 70):
+            run(kv, clean, [(0, 400, n)], dtype, act, first=[293])
+            run(kv, clean, [(0, 400, n)], dtype, act, window=108 if n == 1 else 50)
