@@ -95,10 +95,11 @@ __global__ void __launch_bounds__(kThreads) forms_merge_kernel(const FormsK p, i
 bool whole_queries(const FormsArgs& a) { return a.act == (a.dtype == QR_DTYPE_F16 ? QR_DTYPE_F16 : QR_DTYPE_BF16); }
 
 // What a unit of a kernel takes, in microseconds: a tile of it, its start and end, and its share of what runs at once on a CU.
-// Measured (D = 128): a tile of 64 slots 2.2 for 128 rows, 1.3 for 64, 1.4 times as long with capped scores and 2.2 times in parts; a
+// Measured (D = 128): a tile of 64 slots 2.2 for 128 rows, 1.3 for 64 (8 bits, whose codes
+// become operands whatever the rows: 3.0 and 2.6), 1.4 times as long with capped scores and 2.2 times in parts; a
 // streamed step of 32 slots by its bytes, 5 TB/s over all CUs; fp32 MFMAs' steps of 16 slots by their bytes for 16 rows, by their
-// MFMAs for 32.  (With 0.4 to 1.5 times the part that this gives, the cases it was tried on took 0 to 30% longer, but for 8-bit verify
-// chunks of 64 rows behind 16001 positions, 10% shorter at 0.6.)
+// MFMAs for 32.  (With 0.4 to 1.5 times the part that this gives, the cases it was tried on took 0 to 30% longer.  16 verify chunks of 64
+// heads behind two prefixes of 16001 positions, 8 bits: 129 us with the tiles of 16 bits, 114 with these.)
 struct Shape {
     float tile, start, share;
     int least;  // tiles that a part has at least
@@ -111,8 +112,8 @@ Shape shape_of(const FormsArgs& a, int kind) {
     auto alone = [&](Shape s) { return a.geom.head_dim == 256 ? Shape{0.5f * s.tile, s.start, 1.f, s.least} : s; };
     switch (kind) {
         case kFormStream: return {wide * (a.geom.scaled() ? 0.9f : 1.7f), 5.f, 0.5f, 8};
-        case kFormTilesHalf: return {1.3f * tile, 6.f, 0.5f, 4};
-        case kFormTiles: return {2.2f * tile, 6.f, 0.5f, 4};
+        case kFormTilesHalf: return {(a.geom.scaled() ? 2.5f : 1.3f) * tile, 6.f, 0.5f, 4};
+        case kFormTiles: return {(a.geom.scaled() ? 3.f : 2.2f) * tile, 6.f, 0.5f, 4};
         case kFormF32Half: return alone({wide * (a.dtype == QR_DTYPE_F32 ? 1.7f : 1.f), 5.f, 0.5f, 8});
         case kFormF32: return alone({wide * 1.f, 5.f, 0.5f, 8});
         default: return {4.f, 5.f, 0.25f, 2};
