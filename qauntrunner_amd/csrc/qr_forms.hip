@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace qr {
 namespace {
@@ -34,32 +35,39 @@ __global__ void __launch_bounds__(kThreads) forms_merge_kernel(const FormsK p, i
     float L = 0.f;
     if (VEC) {
         const int gl = D / 4, per = 64 / gl, sub = lane / gl, d = 4 * (lane % gl);  // gl: 16, 32 or 64
-        float o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int x0 = sub; x0 < c.parts; x0 += 4 * per) {
-            float4 a[4];
-            float2 ml[4];
+        float o[4];
+        auto join = [&](auto shown) __attribute__((always_inline)) {
+            L = o[0] = o[1] = o[2] = o[3] = 0.f;
+            for (int x0 = sub; x0 < c.parts; x0 += 4 * per) {
+                float4 a[4];
+                float2 ml[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int x = min(x0 + per * i, c.parts - 1);
-                ml[i] = p.part_ml[slot + x];
-                a[i] = *reinterpret_cast<const float4*>(p.part_acc + (slot + x) * D + d);
+                for (int i = 0; i < 4; ++i) {
+                    const int x = min(x0 + per * i, c.parts - 1);
+                    ml[i] = p.part_ml[slot + x];
+                    a[i] = *reinterpret_cast<const float4*>(p.part_acc + (slot + x) * D + d);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (x0 + per * i >= c.parts || saw_nothing(ml[i])) continue;
+                    const float w = weight(ml[i]);
+                    L = fmaf(ml[i].y, w, L);
+                    auto add = [&](float& to, float of) __attribute__((always_inline)) { to = decltype(shown)::value ? to + form_weighed(of, w) : fmaf(of, w, to); };
+                    add(o[0], a[i].x);
+                    add(o[1], a[i].y);
+                    add(o[2], a[i].z);
+                    add(o[3], a[i].w);
+                }
             }
+            for (int x = gl; x < 64; x <<= 1) {
+                L += __shfl_xor(L, x);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (x0 + per * i >= c.parts || saw_nothing(ml[i])) continue;
-                const float w = weight(ml[i]);
-                L = fmaf(ml[i].y, w, L);
-                o[0] += form_weighed(a[i].x, w);
-                o[1] += form_weighed(a[i].y, w);
-                o[2] += form_weighed(a[i].z, w);
-                o[3] += form_weighed(a[i].w, w);
+                for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x);
             }
-        }
-        for (int x = gl; x < 64; x <<= 1) {
-            L += __shfl_xor(L, x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x);
-        }
+        };
+        join(std::false_type{});
+        const float sum = (o[0] + o[1]) + (o[2] + o[3]);
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum != sum && L == L) != 0, 0)) join(std::true_type{});
         if (sub) return;
         const float inv = L == 0.f ? 0.f : 1.f / L;
         if (p.act == QR_DTYPE_F32) {

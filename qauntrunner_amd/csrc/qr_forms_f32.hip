@@ -310,11 +310,17 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
         for (int x = 0; x < NG / 4; ++x) {
             const int i = wave * (NG / 4) + x, d = 16 * PE * (i >> 2) + PE * (4 * Q + (i & 3));
             few o{};
+            float sum = 0.f;
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                const few a = xa[((y * RT + t) * NG + i) * 64 + lane];
+            for (int y = 0; y < 4; ++y) o += xa[((y * RT + t) * NG + i) * 64 + lane] * c[y];
 #pragma unroll
-                for (int z = 0; z < PE; ++z) o[z] += form_weighed(a[z], c[y]);
+            for (int z = 0; z < PE; ++z) sum += o[z];
+            if (__builtin_expect(sum != sum && L == L, 0)) {
+                o = few{};
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+#pragma unroll
+                    for (int z = 0; z < PE; ++z) o[z] += form_weighed(xa[((y * RT + t) * NG + i) * 64 + lane][z], c[y]);
             }
             if (!whole) {
                 *reinterpret_cast<few*>(p.part_acc + slot * D + d) = o;

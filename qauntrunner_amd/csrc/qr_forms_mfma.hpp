@@ -370,12 +370,14 @@ struct FormTile {
     // stride, ... below step1 were the wave's.  (8 bits hold no infinity.)
     __device__ __forceinline__ void settle(const FormsK& p, const FormItem& it, int kvh, int step0, int step1, int stride) {
         if (E8) return;
-        float sum = 0.f;
+        f32x16_t all = acc[0];
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+        for (int d = 1; d < ND; ++d) all += acc[d];
+        float sum[4] = {all[0], all[1], all[2], all[3]};
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum += acc[d][r];
-        if (!__builtin_amdgcn_ballot_w64(sum != sum && l == l)) return;
+        for (int r = 4; r < 16; ++r) sum[r & 3] += all[r];
+        const float s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (__builtin_expect(!__builtin_amdgcn_ballot_w64(s != s && l == l), 1)) return;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -472,11 +474,22 @@ __device__ __forceinline__ void merge_waves(const FormsK& p, const FormItem& it,
             c[x] = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - M);
             L = fmaf(ml.y, c[x], L);
         }
+        f32x4_t all = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             out[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int x = 0; x < PW; ++x) out[i] += form_weighed(xa[((rw * PW + x) * NG + pw * NP + i) * 64 + w.lane], c[x]);
+            for (int x = 0; x < PW; ++x) out[i] += xa[((rw * PW + x) * NG + pw * NP + i) * 64 + w.lane] * c[x];
+            all += out[i];
+        }
+        const float sum = (all[0] + all[1]) + (all[2] + all[3]);
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum != sum && L == L) != 0, 0)) {  // (form_weighed throughout: 2 us of 33)
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                out[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int x = 0; x < PW; ++x) out[i] += form_weighed(xa[((rw * PW + x) * NG + pw * NP + i) * 64 + w.lane], c[x]);
+            }
         }
     }
     w.store(p, it, un, pw * NP, L, out);
