@@ -194,7 +194,7 @@ struct FormTile {
     // for each, but scores are mostly far below the cap, and tanh x / x on |x| <= 1/2 is a polynomial of x^2 (least squares at
     // Chebyshev's points, off by 6e-9; its last coefficient is positive).  Tiles with larger ones are capped in front, and the
     // coefficients become those of s.  Where they would leave fp32's range the launch takes kScoresBoth (per_weight).
-    static constexpr float kTanh[5] = {0.99999999f, -0.33333072f, 0.1332483f, -0.05298926f, 0.01714132f};
+    static constexpr float kTanh[5] = {0.99999999f, -0.33333071f, 0.1332483f, -0.05298926f, 0.01714132f};
     static constexpr bool PER_WEIGHT = SCORES == kScoresCap && !SPLIT;
     // What stands for a score that the row does not see; a polynomial of it is a large negative number or -infinity.
     static constexpr float kHidden = PER_WEIGHT ? -1e18f : -INFINITY;
