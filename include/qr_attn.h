@@ -267,7 +267,9 @@ typedef struct qr_attn_form {
 /* Attention of the chunks (appended before) in these forms:
  *   z_t = scale q.k_t, capped, less slope |P - t|;  out = sum softmax(z)_t v_t over the t the row sees:
  *   first <= t and (t <= P or t < full) and t > P - window.
- * A row that sees nothing gives zeros.  What stands at positions that a row does not see (NaN too) does not reach it.
+ * A row that sees nothing gives zeros.  What stands at positions that a row does not see (NaN too) does not reach it; with
+ * caps, scores beyond half the cap there or in other rows may change which of two roundings a row's weights take (2^-16 of a
+ * weight at most, queries of 16 bits).
  * Chunks that stand one after another (but for chunks without rows) and name the same prefix and length read it
  * together, up to 64 of them.  The prefix's sequence holds the same layer's K and V, rotated for positions from 0 on
  * (append the chunk's own rows with rope_pos0 = prefix_len + pos0).  Any cache type, fp32, fp16 or bf16 queries,

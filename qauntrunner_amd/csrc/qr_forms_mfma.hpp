@@ -192,8 +192,9 @@ struct FormTile {
     // Capped scores without slopes ascend with the products, so that the maximum is taken of these, and a product becomes its
     // capped score where it becomes a weight (PER_WEIGHT): 1 - 2 / (e^2x + 1) would be two more operations of a quarter of the rate
     // for each, but scores are mostly far below the cap, and tanh x / x on |x| <= 1/2 is a polynomial of x^2 (least squares at
-    // Chebyshev's points, off by 6e-9; its last coefficient is positive).  Tiles with larger ones are capped in front, and the
-    // coefficients become those of s.  Where they would leave fp32's range the launch takes kScoresBoth (per_weight).
+    // Chebyshev's points, off by 3e-8; its last coefficient is positive).  Tiles with larger ones, at positions that a row does not
+    // see and in other rows too, are capped in front, and the coefficients become those of s.  That quotient is off by up to 2^-22 of the
+    // cap for small scores, so that larger caps take kScoresBoth, as where the coefficients would leave fp32's range (per_weight).
     static constexpr float kTanh[5] = {0.99999999f, -0.33333071f, 0.1332483f, -0.05298926f, 0.01714132f};
     static constexpr bool PER_WEIGHT = SCORES == kScoresCap && !SPLIT;
     // What stands for a score that the row does not see; a polynomial of it is a large negative number or -infinity.
@@ -1054,7 +1055,10 @@ __global__ void __launch_bounds__(256, 2) forms_mfma_kernel(const FormsK p) {
 }
 template <int CT, int D, int PARTS> hipError_t form_launch_scores(const FormsK& k, int units, hipStream_t s) {
     const double in = std::fabs(k.qscale) / static_cast<double>(k.cap), last = k.cap * std::pow(in, 9.0) * 0.017;  // the last coefficient
-    const bool per_weight = in < 1e3 && last > 1e-36 && last < 1e30;
+    // Caps beyond 64 take the arithmetic that tells small scores from large ones: 2^-22 of a cap of 64 is 2^-16 of a weight, a 32nd of
+    // what fp16 rounds off; of a million it would be a quarter.  (2048 bf16 rows after 6144, 32 heads of 128 over 8 kv heads: 293 us
+    // with scores far below the cap and 362 about it per weight, 399 whatever the scores by kScoresBoth.)
+    const bool per_weight = k.cap <= 64.f * kLog2e && in < 1e3 && last > 1e-36 && last < 1e30;
     if (k.cap > 0.f && (k.slopes || !per_weight)) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresBoth>), dim3(units), dim3(256), 0, s, k);
     else if (k.cap > 0.f) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresCap>), dim3(units), dim3(256), 0, s, k);
     else if (k.slopes) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresSlope>), dim3(units), dim3(256), 0, s, k);
