@@ -10,6 +10,7 @@ enqueue on torch's current stream.
 from __future__ import annotations
 
 import ctypes
+import operator
 from array import array
 
 import numpy as np
@@ -108,6 +109,17 @@ def _ints(x, what):
         return array("i", x)
     except (TypeError, OverflowError) as e:
         raise ValueError(f"{what}: expected whole numbers of 32 bits ({e})") from None
+
+
+def _int(x, what):
+    """A whole number of 32 bits (ctypes would wrap others)."""
+    try:
+        n = operator.index(x)
+    except TypeError:
+        n = None
+    if n is None or not -(1 << 31) <= n < 1 << 31:
+        raise ValueError(f"{what}: expected a whole number of 32 bits, got {x!r}")
+    return n
 
 
 def _address(a):
@@ -458,7 +470,7 @@ class PagedKvCache:
         [head_dim], None: no norm), then the rotation of its first rotary_dim values (None: head_dim) by position
         rope_pos0[i] + j (None: pos0[i] + j).  q [rows, heads*head_dim], k and v [rows, kv_heads*head_dim], all of
         one dtype, may be slices of one tensor; q_out (contiguous) takes the queries, q and q_out None: none."""
-        ids, p, n, total = self._chunks(seq_ids, pos0, rows)
+        layer, (ids, p, n, total) = _int(layer, "layer"), self._chunks(seq_ids, pos0, rows)
         dev, qw, kw = self.Device, self.Heads * self.HeadDim, self.KvDim
         code = _torch_code(k, "k")
         ke, ks = _strided(k, total, kw, code, dev, "k")
@@ -476,9 +488,10 @@ class PagedKvCache:
         rp = None if rope_pos0 is None else _ints(rope_pos0, "rope_pos0")
         if rp is not None and len(rp) != len(ids):
             raise ValueError("rope_pos0 must agree with seq_ids")
+        rot = self.HeadDim if rotary_dim is None else _int(rotary_dim, "rotary_dim")
         check(self._lib.qr_kv_append_norm_rope_dev(
             self._h, len(ids), _address(ids), layer, _address(p), _address(n), _address(rp) if rp else None, qe[0], qs, ke[0], ks,
-            ve[0], vs, code, oe[0], qn, kn, eps, theta, self.HeadDim if rotary_dim is None else rotary_dim,
+            ve[0], vs, code, oe[0], qn, kn, eps, theta, rot,
             _stream_of(stream, dev)))
 
     def AttentionChunksDev(self, layer, seq_ids, pos0, rows, q, out, scale, weights=None, stream=None) -> None:
@@ -486,7 +499,7 @@ class PagedKvCache:
         positions 0..p of its sequence.  q and out [rows, heads*head_dim] of one dtype.  weights: float32
         [max_batch, kv_heads, max_seq] of this layer, to which each cached position's attention weight is added
         (summed over the chunk's rows and the kv head's query heads)."""
-        ids, p, n, total = self._chunks(seq_ids, pos0, rows)
+        layer, (ids, p, n, total) = _int(layer, "layer"), self._chunks(seq_ids, pos0, rows)
         dev, qw = self.Device, self.Heads * self.HeadDim
         code = _torch_code(q, "q")
         qe = _whole(q, total * qw, code, dev, "q")
@@ -508,7 +521,7 @@ class PagedKvCache:
         t < full[i] (lists of one entry per chunk, None: zeros); rows that see nothing give zeros.  prefix_ids[i] and
         prefix_len[i]: sequence and length of the prefix that stands before chunk i's own sequence (length 0: none),
         read together by chunks that stand one after another and share it; positions are counted from its start."""
-        ids, p, n, total = self._chunks(seq_ids, pos0, rows)
+        layer, (ids, p, n, total) = _int(layer, "layer"), self._chunks(seq_ids, pos0, rows)
         dev, qw = self.Device, self.Heads * self.HeadDim
         code = _torch_code(q, "q")
         qe = _whole(q, total * qw, code, dev, "q")
@@ -529,7 +542,7 @@ class PagedKvCache:
             if x is not None and len(x) != len(ids):
                 raise ValueError(f"{what} must agree with seq_ids")
             lists.append(x)
-        form = _lib.AttnForm(cap, se, window, *(_address(x) if x else None for x in lists))
+        form = _lib.AttnForm(cap, se, _int(window, "window"), *(_address(x) if x else None for x in lists))
         check(self._lib.qr_kv_attention_forms_dev(self._h, len(ids), _address(ids), layer, _address(p), _address(n), qe[0],
                                                   code, oe[0], scale, ctypes.byref(form), _stream_of(stream, dev)))
 
@@ -538,7 +551,7 @@ class PagedKvCache:
         `first`, the last `recent` and the `heavy` others of the largest weight, closed up in their order; kept
         (int32 [n, kv_heads, first+heavy+recent]) takes the positions kept (-1 past the length), kept_weights (None:
         weights itself) their weights and zeros up to the length.  Truncate when every layer is done."""
-        ids, ln = _ints(seq_ids, "seq_ids"), _ints(lengths, "lengths")
+        layer, ids, ln = _int(layer, "layer"), _ints(seq_ids, "seq_ids"), _ints(lengths, "lengths")
         if len(ids) != len(ln):
             raise ValueError("seq_ids and lengths must agree")
         dev = self.Device
@@ -548,6 +561,7 @@ class PagedKvCache:
             oe = self._weights(kept_weights, dev, "kept_weights")
             if oe != we and _overlap(oe, we):
                 raise ValueError("kept_weights overlaps weights")
+        first, heavy, recent = _int(first, "first"), _int(heavy, "heavy"), _int(recent, "recent")
         keep = first + heavy + recent
         if min(first, heavy, recent) < 0:
             raise ValueError("negative budget")
@@ -562,7 +576,7 @@ class PagedKvCache:
 
     def ReadDev(self, layer, seq_ids, pos0, rows, k_out, v_out, stream=None) -> None:
         """The chunks' cache rows as [rows, kv_dim] tensors of the cache's dtype (Read without the host)."""
-        ids, p, n, total = self._chunks(seq_ids, pos0, rows)
+        layer, (ids, p, n, total) = _int(layer, "layer"), self._chunks(seq_ids, pos0, rows)
         dev = self.Device
         if self.KvDtype == _lib.DTYPE_E4M3:
             raise ValueError("an 8-bit cache is read as values: ReadAsDev")
@@ -576,7 +590,7 @@ class PagedKvCache:
     def ReadAsDev(self, layer, seq_ids, pos0, rows, k_out, v_out, stream=None) -> None:
         """The chunks' cache rows as [rows, kv_dim] values of the tensors' dtype (float32, float16 or bfloat16), whatever
         the cache's: an 8-bit cache's are exact in float32 and bfloat16."""
-        ids, p, n, total = self._chunks(seq_ids, pos0, rows)
+        layer, (ids, p, n, total) = _int(layer, "layer"), self._chunks(seq_ids, pos0, rows)
         dev = self.Device
         code = _torch_code(k_out, "k_out")
         ke = _whole(k_out, total * self.KvDim, code, dev, "k_out")
