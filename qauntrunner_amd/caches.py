@@ -543,6 +543,8 @@ class PagedKvCache:
                 raise ValueError(f"{what} must agree with seq_ids")
             lists.append(x)
         form = _lib.AttnForm(cap, se, _int(window, "window"), *(_address(x) if x else None for x in lists))
+        if cap and not form.cap:
+            raise ValueError(f"cap: {cap} is zero in 32 bits")
         check(self._lib.qr_kv_attention_forms_dev(self._h, len(ids), _address(ids), layer, _address(p), _address(n), qe[0],
                                                   code, oe[0], scale, ctypes.byref(form), _stream_of(stream, dev)))
 

@@ -1,5 +1,5 @@
 """CPU tests: whole numbers that the calls over chunks of several sequences take one at a time (layer, window, dims, budgets) reach the
-library as they are or are refused: none is wrapped to 32 bits."""
+library as they are or are refused; none is wrapped to 32 bits, and no cap becomes the zero that stands for none."""
 import sys
 
 import pytest
@@ -72,3 +72,13 @@ def test_budgets(kv, what):  # noqa: F811
     for x in WRONG:
         with pytest.raises(ValueError):
             call(kv, "evict", **{what: x})
+
+
+def test_a_cap_too_small_for_32_bits_is_no_missing_cap(kv):  # noqa: F811
+    for x in (1e-50, -1e-50, 1e-46):
+        with pytest.raises(ValueError, match="cap"):
+            call(kv, "forms", cap=x)
+    kv._lib = Library()
+    for x in (0.0, -0.0, 0, 30.0, 1e-3):
+        with pytest.raises(Reached):
+            call(kv, "forms", cap=x)
