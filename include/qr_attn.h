@@ -271,13 +271,14 @@ typedef struct qr_attn_form {
  * caps, scores beyond half the cap there or in other rows may change which of two roundings a row's weights take (2^-16 of a
  * weight at most, queries of 16 bits).
  * Chunks that stand one after another (but for chunks without rows) and name the same prefix and length read it
- * together, up to 64 of them.  The prefix's sequence holds the same layer's K and V, rotated for positions from 0 on
+ * together, up to 64 of them and as many rows as a launch takes.  The prefix's sequence holds the same layer's K and V, rotated for positions from 0 on
  * (append the chunk's own rows with rope_pos0 = prefix_len + pos0).  Any cache type, fp32, fp16 or bf16 queries,
  * attn of the queries' type.  A sequence may stand in several chunks.  Positions are counted in slots: after an eviction
  * windows, slopes, first and full go by the slots that the kept positions moved to.  An infinite V makes its dim infinite
  * in every row that sees it, whatever its weight (NaN beside the other infinity).  Rows behind a prefix leave
- * 2 (4 head_dim + 8) bytes or more per head, and rows whose keys are split 4 head_dim + 8 per part, in the handle's workspace,
- * which grows as for attention_chunks_dev and must have its size before a capture. */
+ * 2 (4 head_dim + 8) bytes or more per head, and rows whose keys are split 4 head_dim + 8 per part, in the handle's workspace, up
+ * to 256 MB of a launch: a call of more rows behind prefixes runs in several (of 4032 rows with 32 heads of 128).  The workspace grows
+ * as for attention_chunks_dev and must have its size before a capture. */
 int qr_kv_attention_forms_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows,
                               const void* q_dev, int dtype, void* attn_dev, float scale, const qr_attn_form* form,
                               void* stream);

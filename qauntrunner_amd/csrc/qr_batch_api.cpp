@@ -83,25 +83,40 @@ int attend_forms(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos
     a.cap = f.cap;
     a.slopes = f.slopes_dev;
     a.window = f.window;
+    // rows behind prefixes of a launch, even shares of them all
+    long long all = 0;
+    for (int i = 0; i < n; ++i)
+        if (rows[i] && f.prefix_len && f.prefix_len[i]) all += rows[i];
+    const long long fit = form_rows_behind(kv->heads, kv->head_dim), launches = std::max(1LL, (all + fit - 1) / fit);
+    const int most = static_cast<int>((all + launches - 1) / launches);
     long long done = 0;
+    int taken = 0;  // rows of chunk i that earlier launches took
     for (int i = 0; i < n;) {
         a.n = a.rows = 0;
         const long long at = done * kv->heads * kv->head_dim * dtype_size(dtype);
         a.q = offset_bytes(q_dev, at);
         a.out = const_cast<char*>(offset_bytes(attn_dev, at));
-        for (; i < n && a.n < kBatch; ++i) {
-            if (!rows[i]) continue;
-            FormChunk& c = a.c[a.n++];
-            c = {};
-            c.pt_off = kv->store.pt_offset(seq_ids[i], layer);
-            c.pos0 = pos0[i];
-            c.rows = rows[i];
-            c.row0 = a.rows;
-            c.first = f.first ? f.first[i] : 0;
-            c.full = f.full ? f.full[i] : 0;
-            c.pre_len = f.prefix_len ? f.prefix_len[i] : 0;
-            if (c.pre_len) c.pre_off = kv->store.pt_offset(f.prefix_ids[i], layer);
-            a.rows += rows[i];
+        for (int behind = 0; i < n && a.n < kBatch;) {
+            const int len = f.prefix_len ? f.prefix_len[i] : 0;
+            const int take = len && rows[i] ? std::min(rows[i] - taken, most - behind) : rows[i];
+            if (take) {
+                FormChunk& c = a.c[a.n++];
+                c = {};
+                c.pt_off = kv->store.pt_offset(seq_ids[i], layer);
+                c.pos0 = pos0[i] + taken;
+                c.rows = take;
+                c.row0 = a.rows;
+                c.first = f.first ? f.first[i] : 0;
+                c.full = f.full ? f.full[i] : 0;
+                c.pre_len = len;
+                if (len) c.pre_off = kv->store.pt_offset(f.prefix_ids[i], layer);
+                if (len) behind += take;
+                a.rows += take;
+                taken += take;
+            }
+            if (taken < rows[i]) break;  // the rest is the next launch's
+            taken = 0;
+            ++i;
         }
         done += a.rows;
         if (!a.n) break;

@@ -152,7 +152,7 @@ struct Sample {
 // the CUs run at once, or some between and beyond.
 float best_part(const FormsArgs& a, const FormsPlan& p, const Sample* smp, int n) {
     const int kv = a.geom.kv_heads;
-    const float partial = (a.geom.head_dim * 4 + 8) * 0.5e-6f;  // written and read at 4 TB/s
+    const float partial = form_partial_bytes(a.geom.head_dim) * 0.5e-6f;  // written and read at 4 TB/s
     Shape shape[kFormKinds];
     for (int k = 0; k < kFormKinds; ++k) shape[k] = shape_of(a, k);
     float whole = 0.f, work = 0.f;
@@ -188,18 +188,22 @@ float best_part(const FormsArgs& a, const FormsPlan& p, const Sample* smp, int n
     const float even = work / kCus;
     for (const float f : {0.35f, 0.5f, 0.7f, 0.85f, 1.f, 1.04f, 1.08f, 1.15f, 1.25f, 1.4f, 1.7f, 2.f, 3.f})
         if (even * f < whole) consider(even * f);
-    // (the partials of a launch stay below 256 MB: 64 bf16 sequences of 8 rows behind 65536 positions)
+    // longer parts where the partials would pass their bytes
     for (;; best *= 1.25f) {
-        double bytes = 0;
+        int parts[kBatch] = {}, longest = 1;
         for (int i = 0; i < n;) {
             const FormItem& it = p.it[smp[i].item];
             const int per = per_of(shape[it.kind], best);
             int most = 1, j = i;
             for (; j < n && smp[j].item == smp[i].item; ++j) most = std::max(most, (smp[j].tiles + per - 1) / per);
-            if (most > 1) bytes += (a.geom.head_dim * 4.0 + 8) * it.rows * a.heads * most;
+            for (int c = 0; c < it.nc; ++c) parts[it.c0 + c] += most;
+            longest = std::max(longest, most);
             i = j;
         }
-        if (bytes <= (256 << 20)) return best;
+        long long bytes = 0;
+        for (int c = 0; c < a.n; ++c)
+            if (parts[c] > 1) bytes += form_partial_bytes(a.geom.head_dim) * a.c[c].rows * a.heads * parts[c];
+        if (longest == 1 || bytes <= kFormPartialBytes) return best;
     }
 }
 

@@ -41,6 +41,15 @@ struct FormsArgs {
     int window;
 };
 
+// Partials of a launch, at most (64 bf16 sequences of 8 rows behind 65536 positions would have more); a row alone may have more yet.
+constexpr long long kFormPartialBytes = 256LL << 20;
+__host__ __device__ constexpr long long form_partial_bytes(int head_dim) { return 4LL * head_dim + 8; }
+// Rows behind prefixes that a launch takes: one part of either list for each takes half of these bytes.
+constexpr int form_rows_behind(int heads, int head_dim) {
+    const long long n = kFormPartialBytes / 2 / (2 * form_partial_bytes(head_dim) * heads);
+    return n < 1 ? 1 : static_cast<int>(n);
+}
+
 // A chunk as the kernels see it.
 struct FormRows {
     int row0, rows;

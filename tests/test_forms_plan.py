@@ -1,0 +1,87 @@
+"""Host-side plans of attention in its other forms (CPU only): the workspace's bound and its layout, and what is launched."""
+import ctypes
+import os
+
+import pytest
+
+from qauntrunner_amd import _lib
+from tests.hosthip import run
+from tests.test_chunks_plan import BATCH, MB, Geom
+
+_i, _sz = ctypes.c_int, ctypes.c_size_t
+
+
+class Chunk(ctypes.Structure):  # FormChunk
+    _fields_ = [(f, _i) for f in ("pt_off", "pre_off", "pre_len", "pos0", "rows", "row0", "first", "full")]
+
+
+class Args(ctypes.Structure):  # FormsArgs
+    _fields_ = [("c", Chunk * BATCH), ("n", _i), ("rows", _i), ("pool", ctypes.c_void_p), ("page_table", ctypes.c_void_p), ("geom", Geom),
+                ("dtype", _i), ("act", _i), ("heads", _i), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("scale", ctypes.c_float),
+                ("cap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("window", _i)]
+
+
+class Rows(ctypes.Structure):  # FormRows
+    _fields_ = [(f, _i) for f in ("row0", "rows", "p0", "first", "full", "parts")] + [("slot0", ctypes.c_longlong)]
+
+
+class Item(ctypes.Structure):  # FormItem
+    _fields_ = [(f, _i) for f in ("pt_off", "c0", "nc", "row0", "rows", "base", "keys", "unit0", "blocks", "splits", "per", "part0", "kind")]
+
+
+class Plan(ctypes.Structure):  # FormsPlan
+    _fields_ = [("it", Item * (2 * BATCH)), ("us", ctypes.c_float * (2 * BATCH)), ("n", _i), ("c", Rows * BATCH), ("part_ml", _sz),
+                ("workspace_bytes", _sz), ("merge", ctypes.c_bool)]
+
+
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2, "e4m3": 16}
+
+
+def plan(dtype, heads, kv_heads, D, chunks, act=2, window=0, cap=0.0):
+    """chunks: (pos0, rows, prefix length, first visible position, prefix)"""
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    f = ctypes.CDLL(_lib.LIB_PATH)._ZN2qr10plan_formsERKNS_9FormsArgsE
+    f.restype, f.argtypes = Plan, [ctypes.POINTER(Args)]
+    a = Args()
+    tiles = dtype != "f32" and D in (64, 128)
+    a.geom.planes, a.geom.kv_heads, a.geom.head_dim, a.geom.mfma = 2, kv_heads, D, tiles | (2 if dtype == "e4m3" else 0)
+    a.dtype, a.act, a.heads, a.n, a.window, a.cap, a.scale = DTYPES[dtype], act, heads, len(chunks), window, cap, 1.0
+    for i, (pos0, rows, pre, first, of) in enumerate(chunks):
+        c = a.c[i]
+        c.pt_off, c.pre_off, c.pre_len, c.pos0, c.rows, c.row0, c.first = i, 1000 + of, pre, pos0, rows, a.rows, first
+        a.rows += rows
+    return f(ctypes.byref(a))
+
+
+BOUND = """
+FORMS = lambda kv, n, rows, pre, D: L.qr_kv_attention_forms_dev(kv._h, n, ints(*range(n)), 0, ints(*[0] * n), ints(*[rows] * n), ROWS, 2, ROWS, 1.0,
+    ctypes.byref(_lib.AttnForm(0.0, None, 0, None, None, ctypes.cast(ints(*[n] * n), ctypes.c_void_p), ctypes.cast(ints(*[pre] * n), ctypes.c_void_p))), None)
+for dtype, heads, kv_heads, D, n, rows, pre in (("bf16", 32, 8, 128, 64, 1000, 2048), ("e4m3", 64, 8, 128, 64, 500, 300), ("bf16", 64, 8, 128, 1, 16384, 5),
+                                                ("f32", 28, 4, 128, 3, 5001, 1), ("bf16", 5, 2, 40, 7, 9000, 700), ("e4m3", 32, 8, 128, 64, 8, 65536)):
+    kv = PagedKvCache(1, heads, kv_heads, D, max(rows, pre), dtype, n + 1)
+    assert append(kv, list(range(n + 1)), [0] * (n + 1), [rows] * n + [pre]) == 0, L.qr_last_error()
+    before = live.value
+    assert FORMS(kv, n, rows, pre, D) == 0, L.qr_last_error()
+    # (a buffer grows by doubling, so a launch that needs more than the last may leave up to twice what it needs)
+    assert live.value - before <= 2 * (256 << 20), (dtype, heads, D, n, rows, (live.value - before) / 2**20)
+    kv.close()
+"""
+
+
+def test_rows_behind_a_prefix_run_in_a_bounded_workspace(tmp_path):
+    """Two partials of every row behind a prefix pass any bound with the rows of a call: more launches then."""
+    run(tmp_path, BOUND)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("heads,kv_heads,D", [(32, 8, 128), (64, 8, 64), (28, 4, 128), (16, 1, 256), (5, 2, 40)])
+def test_partials_of_a_launch_are_bounded(dtype, heads, kv_heads, D):
+    """As many rows behind prefixes as a launch takes, long contexts of chunks without one, and both."""
+    most = 128 * MB // (2 * (4 * D + 8) * heads)
+    for n in (1, 7, 64):
+        for lens in ((100, 1), (16384, 2000), (1000000, 5)):
+            chunks = [(lens[1], most // n, lens[0], 0, i % 2) for i in range(n)]
+            assert plan(dtype, heads, kv_heads, D, chunks).workspace_bytes <= 256 * MB
+            assert plan(dtype, heads, kv_heads, D, chunks[:n // 2] + [(lens[0], 16, 0, 0, 0)] * (n - n // 2)).workspace_bytes <= 256 * MB
+    assert plan(dtype, 200000, 1, 512, [(0, 1, 5, 0, 0)]).workspace_bytes == 2 * 200000 * (4 * 512 + 8)  # (one row's own)
