@@ -295,7 +295,7 @@ FormsPlan plan_forms(const FormsArgs& a) {
         p.c[i].slot0 = slots;
         slots += static_cast<long long>(p.c[i].rows) * a.heads * p.c[i].parts;
     }
-    p.part_ml = static_cast<size_t>(slots) * a.geom.head_dim * 4;
+    p.part_ml = (static_cast<size_t>(slots) * a.geom.head_dim * 4 + 15) & ~static_cast<size_t>(15);
     p.workspace_bytes = p.part_ml + static_cast<size_t>(slots) * 8;
     return p;
 }

@@ -85,3 +85,17 @@ def test_partials_of_a_launch_are_bounded(dtype, heads, kv_heads, D):
             assert plan(dtype, heads, kv_heads, D, chunks).workspace_bytes <= 256 * MB
             assert plan(dtype, heads, kv_heads, D, chunks[:n // 2] + [(lens[0], 16, 0, 0, 0)] * (n - n // 2)).workspace_bytes <= 256 * MB
     assert plan(dtype, 200000, 1, 512, [(0, 1, 5, 0, 0)]).workspace_bytes == 2 * 200000 * (4 * 512 + 8)  # (one row's own)
+
+
+def test_the_partials_sums_are_aligned():
+    """(maximum, sum) pairs stand behind partials of D floats each: aligned for any number of them and any head size."""
+    odd = 0
+    for heads, kv_heads, D in ((3, 3, 1), (5, 1, 3), (3, 1, 33), (7, 7, 5), (32, 8, 128)):
+        for keys in (100, 1000, 5000, 20000, 100000):
+            for rows in (1, 2, 3):
+                p = plan("f32", heads, kv_heads, D, [(keys, rows, 0, 0, 0)], act=0)
+                parts = rows * heads * p.c[0].parts if p.merge else 0
+                odd += parts * D % 2
+                assert p.part_ml % 16 == 0 and p.part_ml >= parts * D * 4, (heads, D, keys, rows, p.part_ml)
+                assert p.workspace_bytes == p.part_ml + 8 * parts
+    assert odd
