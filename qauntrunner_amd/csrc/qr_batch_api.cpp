@@ -218,7 +218,7 @@ int qr_kv_append_norm_rope_dev(qr_kv* kv, int n, const int* seq_ids, int layer, 
         long long pages = kv->store.pages_used();
         for (int i = 0; i < n; ++i)
             if (rows[i])
-                pages += std::max(0, (pos0[i] + rows[i] + kPageTokens - 1) / kPageTokens - kv->store.pages_held(seq_ids[i], layer));
+                pages += std::max(0, pages_of(pos0[i] + rows[i]) - kv->store.pages_held(seq_ids[i], layer));
         if (pages > kv->store.capacity()) {
             QR_CHECK_ARG(pages < (1LL << 31), "%lld pages are too many", pages);
             QR_TRY(kv->store.reserve(static_cast<int>(pages)));  // (to twice the pool where that fits)

@@ -14,6 +14,7 @@ namespace qr {
 
 constexpr int kPageTokens = QR_PAGE_TOKENS;
 constexpr int kPageShift = 8;  // log2(kPageTokens)
+constexpr int pages_of(int tokens) { return (tokens >> kPageShift) + ((tokens & (kPageTokens - 1)) != 0); }
 
 // ---------------------------------------------------------------- errors
 // Thread-local message behind qr_last_error().

@@ -143,7 +143,7 @@ int qr_kv_create(qr_kv** out, int layers, int heads, int kv_heads, int head_dim,
     QR_CHECK_ARG(max_seq >= 1, "max_seq must be >= 1 (got %d)", max_seq);
     QR_CHECK_ARG(dtype_valid(kv_dtype) || kv_dtype == QR_DTYPE_E4M3, "unknown kv dtype %d", kv_dtype);
     QR_CHECK_ARG(max_batch >= 1, "max_batch must be >= 1 (got %d)", max_batch);
-    const long long pt_entries = static_cast<long long>(max_batch) * layers * ((max_seq + kPageTokens - 1) / kPageTokens);
+    const long long pt_entries = static_cast<long long>(max_batch) * layers * pages_of(max_seq);
     QR_CHECK_ARG(pt_entries < (1LL << 31), "page table of %lld entries is too large", pt_entries);
 
     qr_kv* kv = new (std::nothrow) qr_kv();

@@ -69,7 +69,7 @@ int PagedStore::init(const PageGeom& geom, int dtype, int layers, int seqs, int 
     dtype_ = dtype;
     layers_ = layers;
     seqs_ = seqs;
-    max_pages_ = (max_seq + kPageTokens - 1) / kPageTokens;
+    max_pages_ = pages_of(max_seq);
     const size_t entries = static_cast<size_t>(seqs) * layers * max_pages_;
     pt_host_.assign(entries, 0);
     held_.assign(static_cast<size_t>(seqs) * layers, 0);
@@ -151,7 +151,7 @@ int PagedStore::reserve(int pages) {
 }
 
 int PagedStore::ensure(int seq, int layer, int tokens, hipStream_t stream) {
-    const int need = (tokens + kPageTokens - 1) / kPageTokens;
+    const int need = pages_of(tokens);
     int& h = held_[static_cast<size_t>(seq) * layers_ + layer];
     if (need <= h) return QR_OK;
     const long long add = need - h;
