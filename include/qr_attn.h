@@ -248,7 +248,8 @@ int qr_kv_append_norm_rope_dev(qr_kv* kv, int n, const int* seq_ids, int layer, 
  *   weights[seq][kv head][t] += sum over the chunk's rows and the kv head's query heads of
  *                               softmax(...)[t],  t = 0 .. pos0 + rows - 1,
  * the same for every run with the same inputs (no atomics); other elements are left alone.  With
- * weights no sequence may stand twice.  An 8-bit cache takes no weights. */
+ * weights no sequence may stand twice.  An 8-bit cache takes no weights, and positions
+ * below 2^30. */
 int qr_kv_attention_chunks_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows,
                                const void* q_dev, int dtype, void* attn_dev, float* weights_dev, float scale, void* stream);
 /* What changes the scores of attention (a null pointer, or all members zero: nothing).  Positions are counted over a
@@ -270,15 +271,15 @@ typedef struct qr_attn_form {
  * A row that sees nothing gives zeros.  What stands at positions that a row does not see (NaN too) does not reach it; with
  * caps, scores beyond half the cap there or in other rows may change which of two roundings a row's weights take (2^-16 of a
  * weight at most, queries of 16 bits).
- * Chunks that stand one after another (but for chunks without rows) and name the same prefix and length read it
- * together, up to 64 of them and as many rows as a launch takes.  The prefix's sequence holds the same layer's K and V, rotated for positions from 0 on
- * (append the chunk's own rows with rope_pos0 = prefix_len + pos0).  Any cache type, fp32, fp16 or bf16 queries,
- * attn of the queries' type.  A sequence may stand in several chunks.  Positions are counted in slots: after an eviction
- * windows, slopes, first and full go by the slots that the kept positions moved to.  An infinite V makes its dim infinite
- * in every row that sees it, whatever its weight (NaN beside the other infinity).  Rows behind a prefix leave
- * 2 (4 head_dim + 8) bytes or more per head, and rows whose keys are split 4 head_dim + 8 per part, in the handle's workspace, up
- * to 256 MB of a launch: a call of more rows behind prefixes runs in several (of 4032 rows with 32 heads of 128).  The workspace grows
- * as for attention_chunks_dev and must have its size before a capture. */
+ * Chunks that stand one after another (but for chunks without rows) and name the same prefix and length read it together,
+ * up to 64 of them and as many rows as a launch takes.  The prefix's sequence holds the same layer's K and V, rotated for
+ * positions from 0 on (append the chunk's own rows with rope_pos0 = prefix_len + pos0).  Positions end at 2^30.  Any cache
+ * type, fp32, fp16 or bf16 queries, attn of the queries' type.  A sequence may stand in several chunks.  Positions are counted
+ * in slots: after an eviction windows, slopes, first and full go by the slots that the kept positions moved to.  An infinite V
+ * makes its dim infinite in every row that sees it, whatever its weight (NaN beside the other infinity).
+ * Rows behind a prefix leave 2 (4 head_dim + 8) bytes or more per head, and rows whose keys are split 4 head_dim + 8 per part,
+ * in the handle's workspace, up to 256 MB of a launch: a call of more rows behind prefixes runs in several (of 4032 rows with 32
+ * heads of 128).  The workspace grows as for attention_chunks_dev and must have its size before a capture. */
 int qr_kv_attention_forms_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows,
                               const void* q_dev, int dtype, void* attn_dev, float scale, const qr_attn_form* form,
                               void* stream);

@@ -67,6 +67,13 @@ int check_aligned(const void* p, size_t to, const char* what) {
     return QR_OK;
 }
 
+// The kernels of attend_forms count slots in 32 bits up to the tile behind a list's last.
+int check_near(int chunk, int prefix, int pos0, int rows) {
+    if (static_cast<long long>(prefix) + pos0 + rows <= 1 << 30) return QR_OK;
+    set_error("chunk %d: positions past 2^30", chunk);
+    return QR_ERR_OUT_OF_RANGE;
+}
+
 const char* offset_bytes(const void* p, long long bytes) { return p ? static_cast<const char*>(p) + bytes : nullptr; }
 
 // Attention of checked chunks (rows in all) in the forms of `f`.
@@ -281,6 +288,8 @@ int qr_kv_attention_chunks_dev(qr_kv* kv, int n, const int* seq_ids, int layer, 
         QR_CHECK_ARG(dtype_valid(dtype), "unknown q dtype %d", dtype);
         QR_CHECK_ARG(std::isfinite(scale), "scale must be a number");
         for (int i = 0; i < n; ++i)
+            if (rows[i] && kv->dtype == QR_DTYPE_E4M3) QR_TRY(check_near(i, 0, pos0[i], rows[i]));
+        for (int i = 0; i < n; ++i)
             if (rows[i]) QR_TRY(check_resident(kv, seq_ids[i], layer, pos0[i] + rows[i] - 1));
         if (total == 0) return QR_OK;
         QR_CHECK_ARG(q_dev && attn_dev, "null q/attn pointer");
@@ -404,12 +413,10 @@ int qr_kv_attention_forms_dev(qr_kv* kv, int n, const int* seq_ids, int layer, c
                 QR_TRY(check_pos(kv, len - 1));
                 QR_TRY(check_resident(kv, f.prefix_ids[i], layer, len - 1));
             }
-            if (static_cast<long long>(len) + pos0[i] + rows[i] > (1 << 30)) {
-                set_error("chunk %d: positions past 2^30", i);
-                return QR_ERR_OUT_OF_RANGE;
-            }
+            QR_TRY(check_near(i, len, pos0[i], rows[i]));
             const int first = f.first ? f.first[i] : 0, full = f.full ? f.full[i] : 0;
             QR_CHECK_ARG(first >= 0 && full >= 0, "chunk %d: negative first %d or full %d", i, first, full);
+            QR_TRY(check_near(i, 0, full, 0));
             const int last = std::max(pos0[i] + rows[i], full - len) - 1;  // of its own slots
             QR_TRY(check_pos(kv, last));
             QR_TRY(check_resident(kv, seq_ids[i], layer, last));

@@ -99,3 +99,21 @@ def test_the_partials_sums_are_aligned():
                 assert p.part_ml % 16 == 0 and p.part_ml >= parts * D * 4, (heads, D, keys, rows, p.part_ml)
                 assert p.workspace_bytes == p.part_ml + 8 * parts
     assert odd
+
+
+def test_positions_past_2_30_are_refused(tmp_path):
+    """Slots are counted in 32 bits up to the tile behind the last one, so both attention calls of an 8-bit cache end at 2^30 (seen
+    before whether the position is there)."""
+    run(tmp_path, """
+kv = PagedKvCache(1, 1, 1, 1, 2**31 - 1, "e4m3", 1)
+assert append(kv, [0], [0], [1]) == 0, L.qr_last_error()
+before = launches.value
+for p, n in ((2**30, 1), (2**31 - 2, 1), (2**30 - 5, 6)):
+    assert attend(kv, [0], [p], [n], weights=False) == _lib.QR_ERR_OUT_OF_RANGE, (p, L.qr_last_error())
+    assert L.qr_kv_attention_forms_dev(kv._h, 1, ints(0), 0, ints(p), ints(n), ROWS, 0, ROWS, 1.0, None, None) == _lib.QR_ERR_OUT_OF_RANGE
+full = _lib.AttnForm(0.0, None, 0, None, ctypes.cast(ints(2**30 + 1), ctypes.c_void_p), None, None)
+assert L.qr_kv_attention_forms_dev(kv._h, 1, ints(0), 0, ints(0), ints(1), ROWS, 0, ROWS, 1.0, ctypes.byref(full), None) == _lib.QR_ERR_OUT_OF_RANGE
+assert attend(kv, [0], [2**30 - 5], [5], weights=False) == _lib.QR_ERR_NOT_RESIDENT
+assert attend(kv, [0], [2**30], [0], weights=False) == 0 and launches.value == before
+assert attend(kv, [0], [0], [1], weights=False) == 0, L.qr_last_error()
+""")
