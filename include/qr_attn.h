@@ -277,7 +277,7 @@ typedef struct qr_attn_form {
  * type, fp32, fp16 or bf16 queries, attn of the queries' type.  A sequence may stand in several chunks.  Positions are counted
  * in slots: after an eviction windows, slopes, first and full go by the slots that the kept positions moved to.  An infinite V
  * makes its dim infinite in every row that sees it, whatever its weight (NaN beside the other infinity).
- * Rows behind a prefix leave 2 (4 head_dim + 8) bytes or more per head, and rows whose keys are split 4 head_dim + 8 per part,
+ * Rows behind a prefix that they see leave 2 (4 head_dim + 8) bytes or more per head, and rows whose keys are split 4 head_dim + 8 per part,
  * in the handle's workspace, up to 256 MB of a launch: a call of more rows behind prefixes runs in several (of 4032 rows with 32
  * heads of 128).  The workspace grows as for attention_chunks_dev and must have its size before a capture. */
 int qr_kv_attention_forms_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows,

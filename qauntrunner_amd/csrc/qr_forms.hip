@@ -229,15 +229,19 @@ FormsPlan plan_forms(const FormsArgs& a) {
         const FormChunk& c = a.c[i];
         p.c[i] = {c.row0, c.rows, c.pre_len + c.pos0, c.first, c.full, 0, 0};
     }
-    // the prefixes, then the chunks' own keys
+    // the prefixes that some row of a chunk sees (its first sees the most of them), then the chunks' own keys
+    auto sees = [&](int i) {
+        const FormSpan x = form_span(p.c[i], a.c[i].row0, a.window, 0, a.c[i].pre_len);
+        return x.lo <= x.hi;
+    };
     for (int i = 0; i < a.n;) {
         const FormChunk& c = a.c[i];
-        if (!c.pre_len) {
+        if (!sees(i)) {
             ++i;
             continue;
         }
         int j = i, rows = 0;
-        for (; j < a.n && a.c[j].pre_len == c.pre_len && a.c[j].pre_off == c.pre_off; ++j) rows += a.c[j].rows;
+        for (; j < a.n && a.c[j].pre_len == c.pre_len && a.c[j].pre_off == c.pre_off && sees(j); ++j) rows += a.c[j].rows;
         add(c.pre_off, i, j - i, rows, 0, c.pre_len);
         i = j;
     }

@@ -117,3 +117,19 @@ assert attend(kv, [0], [2**30 - 5], [5], weights=False) == _lib.QR_ERR_NOT_RESID
 assert attend(kv, [0], [2**30], [0], weights=False) == 0 and launches.value == before
 assert attend(kv, [0], [0], [1], weights=False) == 0, L.qr_last_error()
 """)
+
+
+def test_a_prefix_that_no_row_sees_takes_no_part():
+    """Windows and first positions behind the whole prefix: the chunk has its own keys alone, and writes its output without partials
+    where these are one part.  Chunks that see it share it beside others that do not."""
+    far, near = (2000, 5, 2048, 0, 0), (100, 5, 2048, 0, 0)
+    p = plan("bf16", 32, 8, 128, [far] * 3, window=500)
+    assert p.n == 3 and [p.it[i].nc for i in range(3)] == [1] * 3 and [p.it[i].base for i in range(3)] == [2048] * 3
+    assert [p.c[i].p0 for i in range(3)] == [4048] * 3
+    lone = plan("bf16", 32, 8, 128, [(30, 5, 64, 64, 0)])
+    assert lone.n == 1 and lone.c[0].parts == 1 and not lone.merge and lone.workspace_bytes == 0
+    p = plan("bf16", 32, 8, 128, [near, far, near, near], window=500)
+    assert [(p.it[i].c0, p.it[i].nc, p.it[i].base) for i in range(p.n)] == [(0, 1, 0), (2, 2, 0)] + [(i, 1, 2048) for i in range(4)]
+    # the first row of a chunk sees the prefix's last position; one further, none does
+    assert plan("bf16", 32, 8, 128, [(499, 9, 2048, 0, 0)], window=501).n == 2 and plan("bf16", 32, 8, 128, [(499, 9, 2048, 0, 0)], window=500).n == 1
+    assert plan("bf16", 32, 8, 128, [(0, 1, 300, 299, 0)]).n == 2 and plan("bf16", 32, 8, 128, [(0, 1, 300, 300, 0)]).n == 1
