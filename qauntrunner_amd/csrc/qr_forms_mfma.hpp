@@ -70,7 +70,7 @@ __device__ __forceinline__ bf16x8_t widen8(uint32_t lo, uint32_t hi, float scale
 // load that the compiler knows to write LDS it waits for memory before the next read of LDS, whichever bytes that reads, and
 // the tiles ahead would be awaited in every turn (three quarters of the time of a tile).  Nothing is written to registers;
 // wait_vmcnt and a barrier stand between a copy and the reads of its bytes.  (s_nop: a scalar that a vector instruction wrote is
-// read by a buffer load five wait states later at the earliest.  Nothing else here uses m0.)
+// read by a buffer load five wait states later at the earliest.)
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ u32x4_t dma_source(const char* base, int bytes) {
     const uint64_t b = reinterpret_cast<uint64_t>(base);
@@ -81,7 +81,7 @@ __device__ __forceinline__ uint32_t lds_address(const char* p) {
 }
 __device__ __forceinline__ void dma16(u32x4_t source, const char* to, uint32_t at, uint32_t from) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 : : "s"(lds_address(to)), "v"(at), "s"(source), "s"(from) : "memory");
+                 : : "s"(lds_address(to)), "v"(at), "s"(source), "s"(from) : "memory", "m0");
 }
 // One wave's 32 rows.
 template <int CT, int D, int PARTS, int SCORES>
