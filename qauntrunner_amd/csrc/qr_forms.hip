@@ -104,10 +104,10 @@ bool whole_queries(const FormsArgs& a) { return a.act == (a.dtype == QR_DTYPE_F1
 
 // What a unit of a kernel takes, in microseconds: a tile of it, its start and end, and its share of what runs at once on a CU.
 // Measured (D = 128): a tile of 64 slots 2.2 for 128 rows, 1.3 for 64 (8 bits, whose codes
-// become operands whatever the rows: 3.0 and 2.6), 1.4 times as long with capped scores and 2.2 times in parts; a
+// become operands whatever the rows: 3.0 and 2.5), 1.4 times as long with capped scores and 2.2 times in parts; a
 // streamed step of 32 slots by its bytes, 5 TB/s over all CUs; fp32 MFMAs' steps of 16 slots by their bytes for 16 rows, by their
 // MFMAs for 32.  (With 0.4 to 1.5 times the part that this gives, the cases it was tried on took 0 to 30% longer.  16 verify chunks of 64
-// heads behind two prefixes of 16001 positions, 8 bits: 129 us with the tiles of 16 bits, 114 with these.)
+// heads behind two prefixes of 16001 positions, 8 bits: 136 us with the tiles of 16 bits, 100 with these.)
 struct Shape {
     float tile, start, share;
     int least;  // tiles that a part has at least

@@ -4,7 +4,7 @@
 // some dims of every row.
 //
 // Bound by LDS reads, one for each product: with 32 heads of 96 over 8 kv heads, 16 bf16 sequences of 4096 positions took 412 us and
-// 512 rows after 3584 4650 us, where fp32 MFMAs take 59 and 267 (qr_forms_f32.hip).
+// 512 rows after 3584 4650 us, where fp32 MFMAs take 59 and 266 (qr_forms_f32.hip).
 //
 // A row never touches a position that it does not see, so that what such a slot holds (NaN too) does not matter.
 #include "qr_forms.hpp"

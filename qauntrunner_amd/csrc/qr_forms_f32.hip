@@ -14,7 +14,8 @@
 // of the 16-bit rate: 157 TFLOP/s), 16 by HBM.  Three prompts of 61 to 501 rows, 28 heads of 128 with slopes: 77 us for 4.3 GFLOP of
 // which a product would take 28; the rest is blocks that see part of their steps, the longest unit's end, and the operands
 // that come from L2 once for every 32 rows (64 rows per wave: registers).  With 32 heads of 96 over 8 kv heads, bf16: 16 sequences of 4096
-// positions 59 us (3.4 TB/s), 512 rows after 3584 267 us (91 TFLOP/s).
+// positions 54 to 59 us (3.4 to 3.7 TB/s), 512 rows after 3584 251 to 266 us (91 to 97 TFLOP/s); with heads of 256 149 us (3.6 TB/s)
+// and 1260 (51 TFLOP/s), 8 bits 140 and 833.
 #include "qr_forms.hpp"
 #include "qr_mfma.hpp"
 #include "qr_quant.hpp"
@@ -341,7 +342,7 @@ __device__ __forceinline__ void forms_f32(const FormsK& p, const FormItem& it, i
 }
 
 // (Head size 256: a row tile's queries, sums, K and V are 300 to 400 registers of a lane and 128 KB of LDS at the end: one workgroup
-// on a CU.)
+// on a CU, 64 to 320 bytes of a lane spilled but for 8 bits.)
 template <int CT, int D, int SCORES>
 __global__ void __launch_bounds__(kThreads, D > 128 ? 1 : 2) forms_f32_kernel(const FormsK p) {
     __shared__ __attribute__((aligned(16))) char lds[4 * 2 * (D / 4) * 4 * 64];

@@ -647,8 +647,10 @@ __device__ __forceinline__ void forms_stream(const FormsK& p, const FormItem& it
 // 16 bits: tiles are copied by buffer-load DMA as they lie in the page.  8 bits: a thread takes 16 bytes of K and V through
 // registers and writes them as bf16 operands, once for all waves.
 // Bound by MFMAs beside the exponentials, at the clock that the power limit leaves (1.7 to 2.1 of 2.4 GHz; a large product reaches
-// 1.2 to 1.27 PFLOP/s): 2048 rows after 6144, 32 heads of 128 over 8 kv heads, 240 GFLOP: bf16 242 us (993 TFLOP/s), fp16 256, 8 bits 265
-// to 272, with slopes 284, with capped scores 315, fp32 queries in three parts 600 (three times the MFMAs).
+// 1.2 to 1.27 PFLOP/s): 2048 rows after 6144, 32 heads of 128 over 8 kv heads, 240 GFLOP, on four cards: bf16 236 to 248 us (970 to
+// 1020 TFLOP/s), fp16 247 to 258, 8 bits 265 to 275, bf16 with slopes 279 to 289, with scores below a cap of 50 293 to 313 and
+// about it 360 to 372, with caps beyond 64 399 to 407, fp32 queries in three parts 577 to 606 (three times the MFMAs; they, and those
+// over 8 bits, spill 80 to 152 bytes of a lane at head size 128).
 template <int D> struct FormRings {
     static constexpr int KB = 128 * D;                       // bytes of a tile's operands of K (or V)
     static constexpr int NST = 2;                            // tiles of each

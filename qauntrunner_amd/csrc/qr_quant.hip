@@ -58,7 +58,7 @@ __device__ __forceinline__ void norm_rotate(T (&y)[NC], int lane, int D, const f
 }
 
 // Any head size: one workgroup per row, one wave per head, a lane every 64th value.  (The simple form, for caches without an operand
-// layout and rotations that split a run of 4: 512 rows of 32 + 8 + 8 heads of 96 take 21 us.)
+// layout and rotations that split a run of 4: 512 rows of 32 + 8 + 8 heads of 96 take 21 to 26 us.)
 __global__ void __launch_bounds__(kThreads) quant_any_kernel(const NormRopeArgs a) {
     __shared__ double csd[kMaxRopeHalf], snd[kMaxRopeHalf];
     __shared__ float cs[kMaxRopeHalf], sn[kMaxRopeHalf];
@@ -111,8 +111,9 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(const NormRopeArgs 
     }
 }
 
-// Rows back as values of a.act, any cache: a workgroup per row.  (8-bit rows of 8 heads of 96 as bf16: 302 MB in 182 us, bound by
-// single bytes; the operand layout's kernel below does without.)
+// Rows back as values of a.act, any cache: a workgroup per row.  (Single elements: 16 sequences of 4096 rows of 8 heads, 8-bit heads of 96
+// as bf16 302 MB in 182 to 194 us, bf16 heads of 128 as fp32 805 MB in 347, fp32 as bf16 in 329: 1.6 to 2.4 TB/s where the operand
+// layout's kernel below reaches 4.5.  The cache's own type goes by pieces of 16 bytes.)
 __global__ void __launch_bounds__(kThreads) read_as_any_kernel(const ReadArgs a) {
     const int row = blockIdx.x;
     const int e = batch_find(a.n, row, [&](int i) { return a.it[i].row0; });
