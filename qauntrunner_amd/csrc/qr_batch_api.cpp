@@ -90,10 +90,14 @@ int attend_forms(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos
     a.cap = f.cap;
     a.slopes = f.slopes_dev;
     a.window = f.window;
-    // rows behind prefixes of a launch, even shares of them all
+    // rows behind prefixes that they see of a launch, even shares of them all
+    auto sees = [&](int i, int row) {
+        const int len = f.prefix_len ? f.prefix_len[i] : 0;
+        return form_sees_prefix(len, len + pos0[i] + row, f.first ? f.first[i] : 0, f.window);
+    };
     long long all = 0;
     for (int i = 0; i < n; ++i)
-        if (rows[i] && f.prefix_len && f.prefix_len[i]) all += rows[i];
+        if (rows[i] && sees(i, 0)) all += rows[i];
     const long long fit = form_rows_behind(kv->heads, kv->head_dim), launches = std::max(1LL, (all + fit - 1) / fit);
     const int most = static_cast<int>((all + launches - 1) / launches);
     long long done = 0;
@@ -104,8 +108,8 @@ int attend_forms(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos
         a.q = offset_bytes(q_dev, at);
         a.out = const_cast<char*>(offset_bytes(attn_dev, at));
         for (int behind = 0; i < n && a.n < kBatch;) {
-            const int len = f.prefix_len ? f.prefix_len[i] : 0;
-            const int take = len && rows[i] ? std::min(rows[i] - taken, most - behind) : rows[i];
+            const bool shares = rows[i] && sees(i, taken);
+            const int take = shares ? std::min(rows[i] - taken, most - behind) : rows[i] - taken;
             if (take) {
                 FormChunk& c = a.c[a.n++];
                 c = {};
@@ -115,9 +119,9 @@ int attend_forms(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos
                 c.row0 = a.rows;
                 c.first = f.first ? f.first[i] : 0;
                 c.full = f.full ? f.full[i] : 0;
-                c.pre_len = len;
-                if (len) c.pre_off = kv->store.pt_offset(f.prefix_ids[i], layer);
-                if (len) behind += take;
+                c.pre_len = f.prefix_len ? f.prefix_len[i] : 0;
+                if (c.pre_len) c.pre_off = kv->store.pt_offset(f.prefix_ids[i], layer);
+                if (shares) behind += take;
                 a.rows += take;
                 taken += take;
             }

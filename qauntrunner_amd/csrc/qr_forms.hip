@@ -229,11 +229,8 @@ FormsPlan plan_forms(const FormsArgs& a) {
         const FormChunk& c = a.c[i];
         p.c[i] = {c.row0, c.rows, c.pre_len + c.pos0, c.first, c.full, 0, 0};
     }
-    // the prefixes that some row of a chunk sees (its first sees the most of them), then the chunks' own keys
-    auto sees = [&](int i) {
-        const FormSpan x = form_span(p.c[i], a.c[i].row0, a.window, 0, a.c[i].pre_len);
-        return x.lo <= x.hi;
-    };
+    // the prefixes that some row of a chunk sees, then the chunks' own keys
+    auto sees = [&](int i) { return form_sees_prefix(a.c[i].pre_len, p.c[i].p0, a.c[i].first, a.window); };
     for (int i = 0; i < a.n;) {
         const FormChunk& c = a.c[i];
         if (!sees(i)) {

@@ -8,6 +8,8 @@
 // parts over both lists: out = sum o e^(m - M) / sum l e^(m - M), M the largest m.
 #pragma once
 
+#include <algorithm>
+
 #include "qr_batch.hpp"
 
 namespace qr {
@@ -48,6 +50,11 @@ __host__ __device__ constexpr long long form_partial_bytes(int head_dim) { retur
 constexpr int form_rows_behind(int heads, int head_dim) {
     const long long n = kFormPartialBytes / 2 / (2 * form_partial_bytes(head_dim) * heads);
     return n < 1 ? 1 : static_cast<int>(n);
+}
+
+// Whether some row of a chunk sees its prefix: its first, at position p0, sees the most of it.
+inline bool form_sees_prefix(int pre_len, int p0, int first, int window) {
+    return pre_len > std::max(first, window ? p0 - window + 1 : 0);
 }
 
 // A chunk as the kernels see it.

@@ -74,6 +74,21 @@ def test_rows_behind_a_prefix_run_in_a_bounded_workspace(tmp_path):
     run(tmp_path, BOUND)
 
 
+def test_rows_that_see_no_prefix_are_not_counted(tmp_path):
+    """Behind a window they leave no second partial: one launch, as without a prefix (a merge beside it where keys are split)."""
+    run(tmp_path, """
+kv = PagedKvCache(1, 64, 8, 128, 4096, "bf16", 5)
+assert append(kv, list(range(5)), [0] * 5, [4096] * 5) == 0, L.qr_last_error()
+def launched(window, pre, n=4, rows=1000):
+    before = launches.value
+    form = _lib.AttnForm(0.0, None, window, None, None, ctypes.cast(ints(*[4] * n), ctypes.c_void_p), ctypes.cast(ints(*[pre] * n), ctypes.c_void_p))
+    assert L.qr_kv_attention_forms_dev(kv._h, n, ints(*range(n)), 0, ints(*[3000] * n), ints(*[rows] * n), ROWS, 2, ROWS, 1.0, ctypes.byref(form), None) == 0
+    return launches.value - before
+assert launched(3001, 2048) == launched(3001, 0) <= 2
+assert launched(3002, 2048) == 4  # the first rows see the prefix's last position: two launches and their merges
+""")
+
+
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("heads,kv_heads,D", [(32, 8, 128), (64, 8, 64), (28, 4, 128), (16, 1, 256), (5, 2, 40)])
 def test_partials_of_a_launch_are_bounded(dtype, heads, kv_heads, D):
