@@ -1059,8 +1059,9 @@ template <int CT, int D, int PARTS> hipError_t form_launch_scores(const FormsK& 
     const double in = std::fabs(k.qscale) / static_cast<double>(k.cap), last = k.cap * std::pow(in, 9.0) * 0.017;  // the last coefficient
     // Caps beyond 64 take the arithmetic that tells small scores from large ones: 2^-22 of a cap of 64 is 2^-16 of a weight, a 32nd of
     // what fp16 rounds off; of a million it would be a quarter.  (2048 bf16 rows after 6144, 32 heads of 128 over 8 kv heads: 293 us
-    // with scores far below the cap and 362 about it per weight, 399 whatever the scores by kScoresBoth.)
-    const bool per_weight = k.cap <= 64.f * kLog2e && in < 1e3 && last > 1e-36 && last < 1e30;
+    // with scores far below the cap and 362 about it per weight, 399 whatever the scores by kScoresBoth.)  Queries in
+    // parts are capped score by score in either; kScoresCap takes no slope off.
+    const bool per_weight = PARTS > 1 || (k.cap <= 64.f * kLog2e && in < 1e3 && last > 1e-36 && last < 1e30);
     if (k.cap > 0.f && (k.slopes || !per_weight)) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresBoth>), dim3(units), dim3(256), 0, s, k);
     else if (k.cap > 0.f) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresCap>), dim3(units), dim3(256), 0, s, k);
     else if (k.slopes) hipLaunchKernelGGL((forms_mfma_kernel<CT, D, PARTS, kScoresSlope>), dim3(units), dim3(256), 0, s, k);
