@@ -223,11 +223,10 @@ class PagedKvCache:
             self._h = None
 
     def __del__(self):
-        if _lib.finalizing():  # the exit hook closed what was open; the runtime may be gone
-            return
         try:
-            self.close()
-        except Exception:
+            if not _lib.finalizing():  # the exit hook closed what was open; the runtime may be gone
+                self.close()
+        except Exception:  # (the modules may be gone too)
             pass
 
     def __enter__(self):
@@ -653,11 +652,10 @@ class MlaLatentCache:
             self._h = None
 
     def __del__(self):
-        if _lib.finalizing():  # the exit hook closed what was open; the runtime may be gone
-            return
         try:
-            self.close()
-        except Exception:
+            if not _lib.finalizing():  # the exit hook closed what was open; the runtime may be gone
+                self.close()
+        except Exception:  # (the modules may be gone too)
             pass
 
     def __enter__(self):

@@ -123,11 +123,10 @@ class ModelStore:
         self.Dispose()
 
     def __del__(self):
-        if _lib.finalizing():  # the exit hook closed what was open; the runtime may be gone
-            return
         try:
-            self.Dispose()
-        except Exception:
+            if not _lib.finalizing():  # the exit hook closed what was open; the runtime may be gone
+                self.Dispose()
+        except Exception:  # (the modules may be gone too)
             pass
 
 

@@ -71,11 +71,10 @@ class Weight:
             self._h = None
 
     def __del__(self):
-        if _lib.finalizing():  # the exit hook closed what was open; the runtime may be gone
-            return
         try:
-            self.close()
-        except Exception:
+            if not _lib.finalizing():  # the exit hook closed what was open; the runtime may be gone
+                self.close()
+        except Exception:  # (the modules may be gone too)
             pass
 
 
