@@ -277,14 +277,14 @@ typedef struct qr_attn_form {
  * type, fp32, fp16 or bf16 queries, attn of the queries' type.  A sequence may stand in several chunks.  Positions are counted
  * in slots: after an eviction windows, slopes, first and full go by the slots that the kept positions moved to.  An infinite V
  * makes its dim infinite in every row that sees it, whatever its weight (NaN beside the other infinity).
- * 32 bits hold scores, softmax sums and outputs before their rounding.  On 16- and 8-bit caches of head size 64 and 128 with whole
- * groups of query heads, products run on MFMAs of 16 bits: fp16 queries over fp16 caches and bf16 ones over bf16 and 8-bit caches enter
- * as they are, and each weight is rounded once to that type (half a step, 2^-11 or 2^-8 of it; the sum that divides is of the
- * unrounded ones); queries of other types, and their weights, enter in parts of 22 bits or more together, and a key or query value that
- * is infinite gives no number there.  fp32 queries are the way to more bits over any cache.
- * Rows behind a prefix that they see leave 2 (4 head_dim + 8) bytes or more per head, and rows whose keys are split 4 head_dim + 8 per part,
- * in the handle's workspace, up to 256 MB of a launch: a call of more rows behind prefixes runs in several (of 4032 rows with 32
- * heads of 128).  The workspace grows as for attention_chunks_dev and must have its size before a capture. */
+ * 32 bits hold scores, softmax sums and outputs before their rounding.  On 16- and 8-bit caches of head size 64 and 128 with
+ * whole groups of query heads, products run on MFMAs of 16 bits: fp16 queries over fp16 caches and bf16 ones over bf16 and 8-bit
+ * caches enter as they are, and each weight is rounded once to that type (half a step, 2^-11 or 2^-8 of it; the sum that divides
+ * is of the unrounded ones); queries of other types, and their weights, enter in parts of 22 bits or more together, and a key or
+ * query value that is infinite gives no number there.  fp32 queries are the way to more bits over any cache.
+ * Rows behind a prefix that they see leave 2 (4 head_dim + 8) bytes or more per head, and rows whose keys are split
+ * 4 head_dim + 8 per part, in the handle's workspace, up to 256 MB of a launch: a call of more rows behind prefixes runs in several
+ * (of 4032 rows with 32 heads of 128).  The workspace grows as for attention_chunks_dev and must have its size before a capture. */
 int qr_kv_attention_forms_dev(qr_kv* kv, int n, const int* seq_ids, int layer, const int* pos0, const int* rows,
                               const void* q_dev, int dtype, void* attn_dev, float scale, const qr_attn_form* form,
                               void* stream);
